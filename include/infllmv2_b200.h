@@ -455,6 +455,76 @@ int ifv2_decode_prepared(const void* q, void* q_rotated, void* k_cache, void* v_
  * that share one (sequence, KV head), plan[1] = resident CTAs per SM of the kernel variant. */
 int ifv2_decode_plan(int batch, int heads_k, int32_t* plan);
 
+/* ---------------------------------------------------------------- rotary positions --------- */
+
+/* Rotary positions over up to four axes (time, height, width ...) for packed rows: pair i of rotary_dim / 2
+ * turns by the angle of the fp32 tables rotary_cos / rotary_sin (table_rows, rotary_dim / 2) at position
+ * positions[pair_axis[i] * axis_stride + t]; pair_axis: HOST array of rotary_dim / 2 axis numbers < axes, or
+ * null = axis 0 for every pair.  Pairs are features (2i, 2i+1) if interleaved != 0, else
+ * (i, i + rotary_dim / 2); features from rotary_dim on are copied.  q (tokens, heads_q, 128) and k (tokens,
+ * heads_k, 128) bf16 with the given strides (elements, multiples of 8); either may have 0 heads.  q_out and k_out are dense
+ * and may not alias the inputs.  backward != 0 turns by minus the angle: the gradients of q and k from those
+ * of the outputs.  Positions outside the tables take their first or last row.  rotary_dim: a positive multiple of 16.
+ * The reference rotates with one axis inside its decode only (csrc/flash_attn/src/rotary.h:20-150). */
+int ifv2_rotary_axes(const void* q, const void* k, void* q_out, void* k_out, const float* rotary_cos,
+                     const float* rotary_sin, const int32_t* positions, int64_t axis_stride,
+                     const uint8_t* pair_axis, int axes, int64_t tokens, int heads_q, int heads_k, int head_dim,
+                     int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride,
+                     int64_t k_head_stride, int rotary_dim, int64_t table_rows, int interleaved, int backward,
+                     void* stream);
+
+/* ---------------------------------------------------------------- cache in 8 bits ---------- */
+
+/* A cache in 8 bits: codes (slots, heads_k, length, 128), code 0 = e4m3, 1 = int8, and scale bytes (slots,
+ * heads_k, length); a row stands for code * 2^(byte - 127), byte 255 for NaN.  A slot is a sequence (`length` is
+ * its capacity) or, with a block_table (batch, block_table_stride) int32, a page of `length` positions: position
+ * p of sequence b then lives in page block_table[b][p / length].  The exponent of a row is the smallest >= -127
+ * with which its largest magnitude fits the codes (448 or 127); codes are rounded to nearest even.  A row with
+ * an infinity or a NaN is stored as NaN.  Writes to pages, slots or positions that the cache does not have are
+ * dropped; reads of them give NaN.  No counterpart in the reference, whose cache is bf16 or fp16.
+ *
+ * ifv2_q8_fill: packed rows k, v (total, heads_k, 128) bf16 with the given strides (elements, multiples of 8)
+ * of sequences cu_seqlens (batch + 1) go to positions start[b] + 0, 1, ... (start null = 0).  seqlens_out (may
+ * be null): min(start[b] + len_b, capacity).  Rows from cu_seqlens[batch] on are not read.
+ * ifv2_q8_read: the way back into dense k, v (total, heads_k, 128) bf16, exactly; rows from cu_seqlens[batch] on
+ * are set to 0.
+ * ifv2_q8_append: ifv2_decode_append for such a cache in slots; compressed keys are means of the keys as the
+ * cache holds them. */
+int ifv2_q8_fill(const void* k, const void* v, int64_t k_token_stride, int64_t k_head_stride,
+                 int64_t v_token_stride, int64_t v_head_stride, void* k_cache, void* v_cache, void* k_scale,
+                 void* v_scale, const int32_t* cu_seqlens, const int32_t* start, const int32_t* block_table,
+                 int block_table_stride, int32_t* seqlens_out, int64_t slots, int64_t length, int code, int batch,
+                 int64_t total, int heads_k, int head_dim, void* stream);
+int ifv2_q8_read(const void* k_cache, const void* v_cache, const void* k_scale, const void* v_scale, void* k,
+                 void* v, const int32_t* cu_seqlens, const int32_t* start, const int32_t* block_table,
+                 int block_table_stride, int64_t slots, int64_t length, int code, int batch, int64_t total,
+                 int heads_k, int head_dim, void* stream);
+int ifv2_q8_append(const void* k_new, const void* v_new, void* k_cache, void* v_cache, void* k_scale, void* v_scale,
+                   void* kc_cache, void* kc2_cache, int32_t* cache_seqlens, int32_t* positions, int32_t* n_comp,
+                   int32_t* n_comp2, int code, int batch, int64_t slots, int64_t capacity, int64_t c_capacity,
+                   int64_t c2_capacity, int heads_k, int head_dim, int kernel_size, int kernel_stride,
+                   int kernel2_size, int kernel2_stride, void* stream);
+
+/* Bytes of scratch ifv2_q8_decode needs. */
+int64_t ifv2_q8_decode_workspace_bytes(int batch, int heads_q, int head_dim);
+
+/* ifv2_decode_prepared over a cache in 8 bits: one query token per sequence, q / out (batch, heads_q, 128) bf16.
+ * k_new / v_new (batch, heads_k, 128) or null are first written at position cache_seqlens[b]; with rotary tables
+ * the new key and the query are rotated (as by ifv2_rotary_axes, but in fp32 without a rounding to bf16) at
+ * rotary_positions (axes rows of axis_stride, batch columns; null: cache_seqlens) before the key is quantised.
+ * topk_idx (batch, heads_k, topk) or null is packed into mask (batch, heads_k, mask_words); topk_idx null: mask is
+ * given, or null = all keys.  lse (batch, heads_q) fp32 or null.  Pages are a multiple of 16 positions.
+ * A sequence attends positions [0, min(cache_seqlens[b] + new, capacity)); a new token without room is neither
+ * written nor attended, a negative length attends nothing.  Sequences without keys get out = 0, lse = +inf. */
+int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void* k_scale, void* v_scale, const void* k_new,
+                   const void* v_new, const float* rotary_cos, const float* rotary_sin,
+                   const int32_t* rotary_positions, int64_t axis_stride, const uint8_t* pair_axis, int axes,
+                   int rotary_dim, int64_t table_rows, int interleaved, const int32_t* topk_idx, int topk,
+                   int64_t* mask, int mask_words, void* out, float* lse, const int32_t* cache_seqlens,
+                   const int32_t* cache_batch_idx, const int32_t* block_table, int block_table_stride,
+                   int64_t slots, int64_t length, int code, int batch, int heads_q, int heads_k, int head_dim,
+                   float softmax_scale, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------- self-tests -------------- */
 /* Test infrastructure shipped in the library so that a deployment can check the tensor-core
  * building blocks on its own GPU; not part of the attention path.  No counterpart in the

@@ -10,6 +10,8 @@ from .attention import (infllmv2_attn_varlen_func, infllmv2_attn_stage1,
                         infllmv2_attn_with_kvcache, infllmv2_stage1_block_scores,
                         infllmv2_stage1_decode_select,
                         check_device_status)
+from .rotary import rotary_axes
+from .quant_cache import q8_cache, cache_fill_q8, cache_read_q8, decode_append_q8, infllmv2_attn_with_kvcache_q8
 from .sparse_attention import SparseConfig, DecodeCache, SparseAttention
 
 __all__ = [
@@ -17,5 +19,6 @@ __all__ = [
     "max_pooling_1d_varlen", "infllmv2_attn_varlen_func", "infllmv2_attn_stage1",
     "infllmv2_attn_with_kvcache", "infllmv2_topk", "infllmv2_topk_mask", "infllmv2_stage1_block_scores", "infllmv2_stage1_decode_select", "transpose_blockmask", "check_device_status",
     "compress_keys", "compress_keys_append", "compressed_lengths", "cache_fill", "decode_append", "decode_select",
+    "rotary_axes", "q8_cache", "cache_fill_q8", "cache_read_q8", "decode_append_q8", "infllmv2_attn_with_kvcache_q8",
     "SparseConfig", "DecodeCache", "SparseAttention",
 ]

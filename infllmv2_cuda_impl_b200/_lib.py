@@ -16,6 +16,7 @@ _lib = None
 _lock = threading.Lock()
 
 c_void_p, c_int, c_int64, c_float = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
+c_char_p = ctypes.c_char_p
 
 # name -> argtypes, mirroring include/infllmv2_b200.h (every pointer is passed as an address)
 SIGNATURES = {
@@ -86,11 +87,20 @@ SIGNATURES = {
     "ifv2_decode_prepared": [c_void_p] * 8 + [c_int] * 3 + [c_void_p, c_int] + [c_void_p] * 3 +
                             [c_int, c_void_p, c_int, c_int, c_int, c_int, c_int64, c_int64, c_void_p, c_int, c_int,
                              c_void_p, c_void_p, c_float, c_void_p, c_int64, c_void_p],
+    "ifv2_rotary_axes": [c_void_p] * 7 + [c_int64, c_char_p, c_int, c_int64, c_int, c_int, c_int] + [c_int64] * 4 +
+                        [c_int, c_int64, c_int, c_int, c_void_p],
+    "ifv2_q8_fill": [c_void_p] * 2 + [c_int64] * 4 + [c_void_p] * 7 + [c_int, c_void_p, c_int64, c_int64, c_int, c_int,
+                                                                     c_int64, c_int, c_int, c_void_p],
+    "ifv2_q8_read": [c_void_p] * 9 + [c_int, c_int64, c_int64, c_int, c_int, c_int64, c_int, c_int, c_void_p],
+    "ifv2_q8_append": [c_void_p] * 12 + [c_int, c_int] + [c_int64] * 4 + [c_int] * 6 + [c_void_p],
+    "ifv2_q8_decode": [c_void_p] * 10 + [c_int64, c_char_p, c_int, c_int, c_int64, c_int, c_void_p, c_int, c_void_p, c_int] +
+                      [c_void_p] * 5 + [c_int, c_int64, c_int64] + [c_int] * 5 + [c_float, c_void_p, c_int64, c_void_p],
 }
 _INT64_RETURNS = {
     "ifv2_sparse_attn_bwd_workspace_bytes": [c_int64, c_int, c_int],
     "ifv2_decode_workspace_bytes": [c_int, c_int, c_int, c_int],
     "ifv2_stage1_decode_workspace_bytes": [c_int, c_int, c_int],
+    "ifv2_q8_decode_workspace_bytes": [c_int, c_int, c_int],
 }
 
 

@@ -1,0 +1,114 @@
+// Rows of a key-value cache in 8 bits: 128 codes (e4m3 or int8) and one power-of-two scale.
+//
+// For a row x with amax = max |x| the exponent e is the smallest integer >= -127 with amax 2^-e <= T, where T is
+// the type's largest code (448 or 127); code = round-to-nearest-even(x 2^-e), scale byte = e + 127 (e8m0).  With a
+// power of two the product is exact and so is code 2^e on the way back: a value is rounded once, its place in the
+// code alone decides how, and what is read back is a bf16 number that no further rounding touches.  For e4m3,
+// whose spacing is relative, the power of two costs nothing against amax / 448; int8 loses up to one bit.
+// A row that holds an infinity or a NaN gets scale byte 255 (NaN) and codes 0: it reads back as NaN.
+#pragma once
+#include <cuda_fp8.h>
+#include "common.cuh"
+
+namespace ifv2 {
+namespace q8 {
+
+constexpr int kE4m3 = 0, kInt8 = 1;
+constexpr int kNanByte = 255;
+
+// A product that keeps subnormal inputs and results (the build flushes them otherwise): a row whose largest
+// value is below 2^-118 has scale 2^-127 and elements that are subnormal numbers.
+__device__ __forceinline__ float mul_exact(float a, float b) {
+  float r;
+  asm("mul.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Scale byte of a row whose largest |x| has the bit pattern `amax`.
+template <int kCode>
+__device__ __forceinline__ int scale_byte(uint32_t amax) {
+  if (amax >= 0x7F800000u) return kNanByte;
+  // amax = 1.f 2^(k - 127); 448 = 1.75 2^8, 127 = 1.984375 2^6
+  const int k = (int)(amax >> 23), over = (amax & 0x7FFFFFu) > (kCode == kE4m3 ? 0x600000u : 0x7E0000u);
+  return max(k - (kCode == kE4m3 ? 8 : 6) + over, 0);
+}
+// 2^-e; a NaN row is multiplied by 0 ... its codes are set to 0 by encode4.
+__device__ __forceinline__ float inverse_scale(int byte) { return __uint_as_float((uint32_t)(254 - min(byte, 253)) << 23); }
+// 2^e, or NaN
+__device__ __forceinline__ float scale_value(int byte) {
+  return __uint_as_float(byte == kNanByte ? 0x7FC00000u : byte == 0 ? 0x00400000u : (uint32_t)byte << 23);
+}
+
+// Four values (times 2^-e) to four codes, the first in the low byte.
+template <int kCode>
+__device__ __forceinline__ uint32_t encode4(const float (&x)[4], int byte) {
+  if (byte == kNanByte) return 0u;
+  const float inv = inverse_scale(byte);
+  if (kCode == kE4m3) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(mul_exact(x[0], inv), mul_exact(x[1], inv)), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(mul_exact(x[2], inv), mul_exact(x[3], inv)), __NV_SATFINITE, __NV_E4M3);
+    return lo | hi << 16;
+  }
+  uint32_t r = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r |= ((uint32_t)__float2int_rn(mul_exact(x[i], inv)) & 0xFFu) << (8 * i);
+  return r;
+}
+
+// Four codes to numbers (without the scale); exact.
+template <int kCode>
+__device__ __forceinline__ void decode4(float (&x)[4], uint32_t c) {
+  if (kCode == kE4m3) {
+    const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(c & 0xFFFFu), __NV_E4M3);
+    const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(c >> 16), __NV_E4M3);
+    const float2 fa = __half22float2(__half2(a)), fb = __half22float2(__half2(b));
+    x[0] = fa.x; x[1] = fa.y; x[2] = fb.x; x[3] = fb.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = (float)(int8_t)(c >> (8 * i));
+  }
+}
+
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
+
+// A row of 128 values, four per lane, quantised by one warp.
+template <int kCode>
+__device__ __forceinline__ void store_row(const float (&x)[4], uint8_t* codes, uint8_t* scale, int lane) {
+  uint32_t amax = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) amax = max(amax, abs_bits(x[i]));
+  amax = __reduce_max_sync(0xFFFFFFFFu, amax);
+  const int byte = scale_byte<kCode>(amax);
+  reinterpret_cast<uint32_t*>(codes)[lane] = encode4<kCode>(x, byte);
+  if (lane == 0) *scale = (uint8_t)byte;
+}
+
+// Where position `pos` of sequence b lives: row ((slot * heads + h) * length + off) of the (rows, 128) codes and of
+// the (rows) scales.  A slot is a sequence (or the one that batch_idx names) or a page of the block table.
+struct Place {
+  const int32_t* block_table;    // (batch, bt_stride) or null
+  const int32_t* batch_idx;      // (batch) or null
+  int bt_stride, heads, length, slots;
+  // row of head 0, or -1 where there is no such row: a page or a slot that the cache does not have, a position
+  // past the table or below 0
+  __device__ __forceinline__ int64_t row0(int b, int64_t pos) const {
+    int slot, off;
+    if (pos < 0) return -1;
+    if (block_table != nullptr) {
+      const int64_t page = pos / length;
+      if (page >= bt_stride) return -1;
+      slot = __ldg(block_table + (int64_t)b * bt_stride + page);
+      off = (int)(pos - page * length);
+    } else {
+      if (pos >= length) return -1;
+      slot = batch_idx ? __ldg(batch_idx + b) : b;
+      off = (int)pos;
+    }
+    if (slot < 0 || slot >= slots) return -1;
+    return (int64_t)slot * heads * length + off;
+  }
+  __device__ __forceinline__ int64_t row(int64_t row0, int h) const { return row0 + (int64_t)h * length; }
+};
+
+}  // namespace q8
+}  // namespace ifv2

@@ -23,6 +23,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import ops
+from . import quant_cache
 from .attention import (infllmv2_attn_stage1, infllmv2_stage1_decode_select, infllmv2_attn_varlen_func, infllmv2_attn_with_kvcache,
                         infllmv2_stage1_block_scores, GROUP, HEAD_DIM)
 
@@ -51,14 +52,24 @@ class SparseConfig:
 class DecodeCache:
     """Per-sequence caches of keys, values and compressed keys at a fixed capacity, plus the
     small integer tensors a decode step needs (all device-resident; `max_len` is the only host
-    copy of the lengths and is an upper bound)."""
+    copy of the lengths and is an upper bound).
 
-    def __init__(self, batch: int, capacity: int, heads_k: int, config: SparseConfig, device="cuda"):
+    kv_dtype torch.float8_e4m3fn or torch.int8 keeps keys and values in 8 bits (quant_cache: k and v are
+    then (batch, heads_k, capacity, 128) codes with the scales k_scale and v_scale); half the memory, and half
+    the bytes a decode step reads.  Compressed keys stay bf16: those of a prefill are means of its exact keys,
+    those that decoding completes are means of the keys as the cache holds them."""
+
+    def __init__(self, batch: int, capacity: int, heads_k: int, config: SparseConfig, device="cuda",
+                 kv_dtype: torch.dtype = torch.bfloat16):
         dev = torch.device(device)
         self.config, self.batch, self.capacity, self.heads_k = config, batch, capacity, heads_k
-        shape = (batch, capacity, heads_k, HEAD_DIM)
-        self.k = torch.zeros(shape, dtype=torch.bfloat16, device=dev)
-        self.v = torch.zeros(shape, dtype=torch.bfloat16, device=dev)
+        self.k_scale = self.v_scale = None
+        if kv_dtype == torch.bfloat16:
+            shape = (batch, capacity, heads_k, HEAD_DIM)
+            self.k = torch.zeros(shape, dtype=torch.bfloat16, device=dev)
+            self.v = torch.zeros(shape, dtype=torch.bfloat16, device=dev)
+        else:
+            self.k, self.v, self.k_scale, self.v_scale = quant_cache.q8_cache(batch, capacity, heads_k, kv_dtype, dev)
         self.c_capacity = max(config.windows(capacity), 1)
         self.kc = torch.zeros(batch, self.c_capacity, heads_k, HEAD_DIM, dtype=torch.bfloat16, device=dev)
         self.kc2 = self.n_comp2 = self.cu_c2 = None
@@ -77,7 +88,12 @@ class DecodeCache:
 
     def fill(self, k, v, kc, cu_seqlens, cu_seqlens_c, max_seqlen, kc2=None, cu_seqlens_c2=None):
         """Load the caches from packed prefill tensors (rows past the capacity are dropped)."""
-        if k.shape == v.shape:
+        if self.k_scale is not None:
+            n = min(k.shape[0], v.shape[0])        # (rows of one tensor past the last sequence)
+            quant_cache.cache_fill_q8(k[:n], v[:n], self.k, self.v, self.k_scale, self.v_scale, cu_seqlens,
+                                      seqlens_out=self.seqlens)
+            ops.cache_fill(kc, self.kc, cu_seqlens_c, self.n_comp)
+        elif k.shape == v.shape:
             ops.cache_fill_kv(k, v, kc, self.k, self.v, self.kc, cu_seqlens, cu_seqlens_c, self.seqlens, self.n_comp)
         else:                                      # (rows of one tensor past the last sequence)
             ops.cache_fill(k, self.k, cu_seqlens, self.seqlens)
@@ -86,6 +102,13 @@ class DecodeCache:
         if self.kc2 is not None:
             ops.cache_fill(kc2, self.kc2, cu_seqlens_c2, self.n_comp2)
         self.max_len = min(int(max_seqlen), self.capacity)
+
+    def read(self, cu_seqlens, total: int, start: Optional[torch.Tensor] = None):
+        """Packed keys and values (total, heads_k, 128) bf16 of a cache in 8 bits, as it holds them: rows start[b]
+        (default 0) and on of every sequence, as many as cu_seqlens gives it (see cache_read_q8)."""
+        if self.k_scale is None:
+            raise NotImplementedError("DecodeCache.read: a bf16 cache is read as it is (k, v)")
+        return quant_cache.cache_read_q8(self.k, self.v, self.k_scale, self.v_scale, cu_seqlens, total, start)
 
 
 class SparseAttention:
@@ -166,10 +189,12 @@ class SparseAttention:
         if cache.max_len >= cache.capacity:
             raise RuntimeError("DecodeCache is full")
         q3 = q.reshape(b, hk * GROUP, HEAD_DIM)
-        ops.decode_append(k_new.reshape(b, hk, HEAD_DIM), v_new.reshape(b, hk, HEAD_DIM), cache.k, cache.v,
-                          cache.seqlens, cache.positions, cache.kc, cache.n_comp, c.kernel_size,
-                          c.kernel_stride, cache.kc2, cache.n_comp2, c.coarse_kernel_size,
-                          c.coarse_kernel_stride)
+        quant = cache.k_scale is not None
+        append, scales = (quant_cache.decode_append_q8, (cache.k_scale, cache.v_scale)) if quant else (ops.decode_append, ())
+        append(k_new.reshape(b, hk, HEAD_DIM), v_new.reshape(b, hk, HEAD_DIM), cache.k, cache.v, *scales,
+               cache.seqlens, cache.positions, cache.kc, cache.n_comp, c.kernel_size,
+               c.kernel_stride, cache.kc2, cache.n_comp2, c.coarse_kernel_size,
+               c.coarse_kernel_stride)
         cache.max_len += 1
         bound = cache.capacity if static_shapes else cache.max_len       # >= every sequence length
         max_c = c.windows(bound)
@@ -191,9 +216,9 @@ class SparseAttention:
                 mask = infllmv2_stage1_decode_select(q3, kc_flat, cache.cu_c, cache.positions, max_c,
                                                      cache.capacity, c.topk, c.local_blocks, c.init_blocks,
                                                      seqused_k=cache.n_comp, dense_len=c.dense_len)
-        return infllmv2_attn_with_kvcache(q3.view(b, 1, hk * GROUP, HEAD_DIM), cache.k, cache.v,
-                                          cache_seqlens=cache.seqlens, softmax_scale=softmax_scale,
-                                          block_mask=mask)
+        attend = quant_cache.infllmv2_attn_with_kvcache_q8 if quant else infllmv2_attn_with_kvcache
+        return attend(q3.view(b, 1, hk * GROUP, HEAD_DIM), cache.k, cache.v, *scales, cache_seqlens=cache.seqlens,
+                      softmax_scale=softmax_scale, block_mask=mask)
 
     def capture_decode(self, cache: DecodeCache, softmax_scale: Optional[float] = None):
         """Capture one decode step for `cache` in a CUDA graph.  Returns `step(q, k_new, v_new)`,
