@@ -17,6 +17,7 @@
 // cp.async requests per tile; other layouts use cp.async.  Both forms run at the same speed: what
 // held the step at half the HBM bandwidth was a launch of 1.15 waves, see the split count below.
 #include <string.h>
+#include "block_list.cuh"
 #include "mma_sync.cuh"
 #include "tc05.cuh"
 
@@ -86,69 +87,6 @@ __device__ __forceinline__ int64_t cache_row_offset(const int32_t* block_table, 
   return slot * batch_stride + pos * row_stride;
 }
 
-// The selected blocks of one (sequence, KV head), lowest first, looked up by a whole warp that takes
-// every kWarps-th of them: lane l fetches mask word 32 c + l of a chunk of words, a warp scan gives
-// the selected blocks before it, and lane i of the warp finds the i-th next block of the warp by two
-// short bisections, so that 32 look-ups cost one trip to memory.  (One thread walking the words paid a
-// chain of a load per word, 33 of them at 131072 tokens, for the count and again for every block.)
-// Every lane must make the calls and gets the same answers.
-struct BlockList {
-  const unsigned long long* words;   // null = every block below nblk
-  int nwords, nblk;
-  int cached;                        // lane i: block of look-up 32 n + i
-  __device__ unsigned long long word(int w) const {
-    if (w >= nwords) return 0ull;
-    unsigned long long x = __ldg(words + w);
-    const int first = w * 64;
-    if (nblk - first < 64) x &= (nblk > first) ? ((1ull << (nblk - first)) - 1ull) : 0ull;
-    return x;
-  }
-  __device__ int count(int lane) const {
-    if (words == nullptr) return nblk;
-    int n = 0;
-    for (int w = lane; w < nwords; w += 32) n += __popcll(word(w));
-    return __reduce_add_sync(0xFFFFFFFFu, n);
-  }
-  // blocks number j, j + kWarps, ... (0-based), one per lane; -1 past the end of the mask
-  __device__ void refill(int j, int lane) {
-    const int target = j + lane * kWarps;
-    cached = -1;
-    int before = 0;
-    for (int c = 0; c * 32 < nwords && before <= j + 31 * kWarps; ++c) {
-      const unsigned long long mine = word(c * 32 + lane);
-      const int cnt = __popcll(mine);
-      int incl = cnt;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int up = __shfl_up_sync(0xFFFFFFFFu, incl, d);
-        if (lane >= d) incl += up;
-      }
-      const int excl = incl - cnt, total = __shfl_sync(0xFFFFFFFFu, incl, 31);
-      const bool here = target >= before && target < before + total;
-      const int r = here ? target - before : 0;
-      int src = 0;                               // last word that starts at or below block r
-#pragma unroll
-      for (int d = 16; d >= 1; d >>= 1)
-        if (__shfl_sync(0xFFFFFFFFu, excl, src + d) <= r) src += d;
-      unsigned long long x = __shfl_sync(0xFFFFFFFFu, mine, src);
-      int rank = r - __shfl_sync(0xFFFFFFFFu, excl, src), pos = 0;
-#pragma unroll
-      for (int d = 32; d >= 1; d >>= 1) {        // position of the set bit with `rank` set bits below it
-        const int low = __popcll(x & ((1ull << d) - 1ull));
-        if (rank >= low) { rank -= low; pos += d; x >>= d; }
-      }
-      if (here) cached = (c * 32 + src) * 64 + pos;
-      before += total;
-    }
-  }
-  // the warp's look-up number i, of block j = first + i * kWarps; look-ups come in order
-  __device__ int nth(int i, int j, int lane) {
-    if (words == nullptr) return j;
-    if ((i & 31) == 0) refill(j, lane);
-    return __shfl_sync(0xFFFFFFFFu, cached, i & 31);
-  }
-};
-
 // kResident: CTAs per SM the kernel is compiled for (2: 236 registers, 3: 168 and a few bytes of spills)
 template <bool kTma, int kResident>
 __global__ void __launch_bounds__(kThreads, kResident)
@@ -179,7 +117,7 @@ decode_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   const int64_t end = min(max((int64_t)p.cache_seqlens[b], (int64_t)0) + p.new_tokens, p.capacity);
   const int len = (int)max(end - pad, (int64_t)0);
   const int slot = p.cache_batch_idx ? p.cache_batch_idx[b] : b;
-  BlockList list{p.mask ? p.mask + ((int64_t)b * p.heads_k + h) * p.mask_words : nullptr, p.mask_words,
+  BlockList<kWarps> list{p.mask ? p.mask + ((int64_t)b * p.heads_k + h) * p.mask_words : nullptr, p.mask_words,
                  (len + kBlockN - 1) / kBlockN, -1};
   const int n = list.count(lane);
   const int per_split = (n + p.splits - 1) / p.splits;

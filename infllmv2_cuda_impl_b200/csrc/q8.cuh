@@ -69,6 +69,26 @@ __device__ __forceinline__ void decode4(float (&x)[4], uint32_t c) {
   }
 }
 
+// Four codes as two fp16 pairs, codes (0, 1) and (2, 3); exact.  Integers go through 1024 + (code + 128), whose
+// fp16 numbers are 0x6400 + (code + 128).
+template <int kCode>
+__device__ __forceinline__ void decode_h2(uint32_t& lo, uint32_t& hi, uint32_t c) {
+  if (kCode == kE4m3) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi) : "r"(c));
+  } else {
+    c ^= 0x80808080u;
+    const uint32_t a = __byte_perm(c, 0x64646464u, 0x4140), b = __byte_perm(c, 0x64646464u, 0x4342);
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(a), "r"(0x64806480u));
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(b), "r"(0x64806480u));
+  }
+}
+// The same for codes (0, 2) and (1, 3): a transposed 16-bit load holds two tokens' codes of two features.
+template <int kCode>
+__device__ __forceinline__ void decode_h2_even_odd(uint32_t& even, uint32_t& odd, uint32_t c) {
+  decode_h2<kCode>(even, odd, __byte_perm(c, 0u, 0x3120));
+}
+
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
 
 // A row of 128 values, four per lane, quantised by one warp.
@@ -95,10 +115,10 @@ struct Place {
     int slot, off;
     if (pos < 0) return -1;
     if (block_table != nullptr) {
-      const int64_t page = pos / length;
-      if (page >= bt_stride) return -1;
+      if (pos >= (int64_t)bt_stride * length) return -1;
+      const uint32_t page = (uint32_t)pos / (uint32_t)length;      // (the host keeps positions below 2^31)
       slot = __ldg(block_table + (int64_t)b * bt_stride + page);
-      off = (int)(pos - page * length);
+      off = (int)((uint32_t)pos - page * (uint32_t)length);
     } else {
       if (pos >= length) return -1;
       slot = batch_idx ? __ldg(batch_idx + b) : b;

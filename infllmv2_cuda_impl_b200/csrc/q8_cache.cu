@@ -216,8 +216,9 @@ static int move_common(MoveParams& p, const char* what, void* k_cache, void* v_c
   IFV2_REQUIRE(block_table != nullptr || slots >= batch, IFV2_ERR_INVALID_ARG, "%s: fewer slots than sequences", what);
   IFV2_REQUIRE((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) % 16 == 0, IFV2_ERR_INVALID_ARG,
                "%s: tensors must be 16-byte aligned", what);
-  IFV2_REQUIRE(total <= INT32_MAX && length <= INT32_MAX && slots <= INT32_MAX && heads_k <= 65535, IFV2_ERR_TOO_LARGE,
-               "%s: a size is too large", what);
+  IFV2_REQUIRE(total <= INT32_MAX && length <= INT32_MAX && slots <= INT32_MAX && heads_k <= 65535 &&
+                   (block_table == nullptr || block_table_stride <= INT32_MAX / length),
+               IFV2_ERR_TOO_LARGE, "%s: a size is too large", what);
   p.codes[0] = static_cast<uint8_t*>(k_cache);
   p.codes[1] = static_cast<uint8_t*>(v_cache);
   p.scales[0] = static_cast<uint8_t*>(k_scale);

@@ -10,18 +10,28 @@
 // sizes are, and out = O 2^(M - m) / l.  (m and M differ by at most 127, the range of the exponents.)
 //
 // Launches: [prepare: block lists, append] -> split -> combine.
-#include "rotary.cuh"
+#include "block_list.cuh"
+#include "mma_sync.cuh"
 #include "q8.cuh"
+#include "rotary.cuh"
+#include "tc05.cuh"
 
 namespace ifv2 {
 namespace {
 
 using namespace q8;
 
-constexpr int kThreads = 128;
-constexpr int kUnit = 32;                        // keys handled at once
-constexpr int kMaxSplits = 16;
-constexpr int kPartialFloats = kHeadDim + 4;     // O row, m (log2 units), l, M, pad
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kResident = 3;                     // CTAs per SM
+constexpr int kUnit = 32;                        // keys that a warp handles at once
+constexpr int kStages = 2;                       // slots of a warp
+constexpr int kSlotBytes = 2 * kUnit * kHeadDim; // K and V codes of a unit
+constexpr int kSmemBytes = kWarps * kStages * kSlotBytes + 1024;
+constexpr int kMaxSplits = 16;                   // CTAs that share the selected blocks of a (sequence, KV head)
+constexpr int kDealtCtas = kResident * kNumSMs;  // CTAs that share all blocks where there is no mask
+constexpr long long kWaitLimit = 1ll << 28;      // clocks; a copy takes microseconds
+constexpr int kPartialFloats = kHeadDim + 4;     // O row, m (log2 units), l, exponent of O's units, pad
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -39,7 +49,7 @@ struct Q8DecodeParams {
   int batch, heads_k, new_tokens, splits, rotate;
   RotaryParams rotary;
   float scale_log2;
-  float* partial;                  // (batch, heads_k, splits, 16, kPartialFloats)
+  float* partial;                  // (batch, heads_k, splits | 2 per CTA, 16, kPartialFloats)
   __nv_bfloat16* out;
   float* lse;                      // (batch, heads_q) or null
 };
@@ -114,132 +124,503 @@ __global__ void __launch_bounds__(kThreads) q8_prepare_kernel(const Q8PreparePar
   }
 }
 
-// One split of one (sequence, KV head): eight threads per query head.
-template <int kCode>
-__global__ void __launch_bounds__(kThreads) q8_split_kernel(const Q8DecodeParams p) {
-  __shared__ float qs[kGroup][kHeadDim], ks[kUnit][kHeadDim + 1], vs[kUnit][kHeadDim], ps[kGroup][kUnit], ek[kUnit], ev[kUnit];
-  const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = tid / 8, c = tid % 8;
-  const int64_t pair = (int64_t)b * p.heads_k + h;
-  const int len = keys_of(p, b);
-  const int n_blocks = (len + kBlockN - 1) / kBlockN;
-  for (int i = warp; i < kGroup; i += kThreads / 32) {
-    float x[4];
-    load_rotated(x, p.q + (pair * kGroup + i) * kHeadDim, p.rotary, p.rotate, b, lane);
+// Blocks of 64 keys that one sequence's head attends without a mask.
+__device__ __forceinline__ int blocks_of(const Q8DecodeParams& p, int b) { return (keys_of(p, b) + kBlockN - 1) / kBlockN; }
+
+// Without a mask the blocks of all sequences and heads are one row of `total` blocks, sequence by sequence, head by
+// head, and CTA c of `ctas` takes those from c total / ctas on: every CTA reads the same number of bytes whatever the
+// lengths are (16 sequences of 1000 .. 32000 tokens in equal splits wait for the longest one).  Every warp finds its
+// place by itself, a sequence per lane.
+struct Deal {
+  int64_t total;
+  int ctas;
+  __device__ Deal(const Q8DecodeParams& p, int grid, int lane) {
+    int64_t n = 0;
+    for (int b = lane; b < p.batch; b += 32) n += blocks_of(p, b);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) qs[i][4 * lane + j] = x[j];
+    for (int d = 16; d >= 1; d >>= 1) n += __shfl_xor_sync(0xFFFFFFFFu, n, d);
+    total = n * p.heads_k;
+    // two blocks are one 32-key unit for each of the four warps
+    ctas = (int)max((int64_t)1, min((int64_t)grid, (total + 1) / 2));
   }
-  float o[16], m = -INFINITY, mv = -INFINITY, l = 0.f;
+  __device__ int64_t first(int c) const { return (int64_t)c * total / ctas; }
+  __device__ int cta_of(int64_t block) const { return (int)(((block + 1) * ctas - 1) / total); }
+};
+
+// Sequence that holds block `at` of the row, and the row's blocks before it.
+__device__ __forceinline__ int find_block(const Q8DecodeParams& p, int64_t at, int64_t& before, int lane) {
+  before = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += 32) {
+    const int64_t n = b0 + lane < p.batch ? (int64_t)blocks_of(p, b0 + lane) * p.heads_k : 0;
+    int64_t incl = n;
 #pragma unroll
-  for (int j = 0; j < 16; ++j) o[j] = 0.f;
-  for (int blk = split; blk < n_blocks; blk += p.splits) {
-    if (p.mask != nullptr && (blk / 64 >= p.mask_words || !((p.mask[pair * p.mask_words + blk / 64] >> (blk & 63)) & 1ull)))
-      continue;
-    for (int key0 = blk * kBlockN; key0 < min(len, (blk + 1) * kBlockN); key0 += kUnit) {
-      __syncthreads();
-      for (int i = warp; i < kUnit; i += kThreads / 32) {
-        const bool in = key0 + i < len;
-        const int64_t row0 = in ? p.place.row0(b, key0 + i) : -1;
-        float xk[4] = {0.f, 0.f, 0.f, 0.f}, xv[4] = {0.f, 0.f, 0.f, 0.f};
-        int bk = in ? kNanByte : 0, bv = bk;     // (a page that the cache does not have: the result is NaN)
-        if (row0 >= 0) {
-          const int64_t row = p.place.row(row0, h);
-          bk = p.k_scale[row];
-          bv = p.v_scale[row];
-          decode4<kCode>(xk, reinterpret_cast<const uint32_t*>(p.k_codes + row * kHeadDim)[lane]);
-          decode4<kCode>(xv, reinterpret_cast<const uint32_t*>(p.v_codes + row * kHeadDim)[lane]);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          ks[i][4 * lane + j] = xk[j];
-          vs[i][4 * lane + j] = xv[j];
-        }
-        if (lane == 0) {
-          ek[i] = scale_value(bk);
-          ev[i] = bv == kNanByte ? scale_value(bv) : (float)(bv - 127);
-        }
-      }
-      __syncthreads();
-      float s[4], z[4], mx = m, mz = mv;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int t = c + 8 * u;
-        float acc = 0.f;
-        for (int j = 0; j < kHeadDim; ++j) acc = fmaf(qs[r][j], ks[t][j], acc);
-        const bool in = key0 + t < len;
-        s[u] = in ? mul_exact(acc, ek[t]) * p.scale_log2 : -INFINITY;
-        z[u] = in ? s[u] + ev[t] : -INFINITY;
-        mx = fmaxf(mx, s[u]);
-        mz = fmaxf(mz, z[u]);
-      }
-#pragma unroll
-      for (int d = 1; d < 8; d <<= 1) {
-        mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, d));
-        mz = fmaxf(mz, __shfl_xor_sync(0xFFFFFFFFu, mz, d));
-      }
-      const float f = mx == -INFINITY ? 1.f : exp2f(m - mx), sub = mx == -INFINITY ? 0.f : mx;
-      const float fv = mz == -INFINITY ? 1.f : exp2f(mv - mz), subv = mz == -INFINITY ? 0.f : mz;
-      m = mx;
-      mv = mz;
-      l *= f;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        l += exp2f(s[u] - sub);
-        ps[r][c + 8 * u] = exp2f(z[u] - subv);
-      }
-      __syncwarp();
-#pragma unroll
-      for (int j = 0; j < 16; ++j) o[j] *= fv;
-      for (int t = 0; t < kUnit; ++t) {
-        const float e = ps[r][t];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) o[j] = fmaf(e, vs[t][c + 8 * j], o[j]);
-      }
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t up = __shfl_up_sync(0xFFFFFFFFu, incl, d);
+      if (lane >= d) incl += up;
     }
+    const uint32_t past = __ballot_sync(0xFFFFFFFFu, before + incl > at);
+    if (past) {
+      const int src = __ffs(past) - 1;
+      before += __shfl_sync(0xFFFFFFFFu, incl - n, src);
+      return b0 + src;
+    }
+    before += __shfl_sync(0xFFFFFFFFu, incl, 31);
   }
-#pragma unroll
-  for (int d = 1; d < 8; d <<= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, d);
-  float* dst = p.partial + ((pair * p.splits + split) * kGroup + r) * kPartialFloats;
-#pragma unroll
-  for (int j = 0; j < 16; ++j) dst[c + 8 * j] = o[j];
-  if (c == 0) {
-    dst[kHeadDim] = m;
-    dst[kHeadDim + 1] = l;
-    dst[kHeadDim + 2] = mv;
-  }
+  return p.batch;
 }
 
 // A partial sum in units of 2^m as one in units of 2^top.  Without a finite m it is 0, or NaN and stays so.
-__device__ __forceinline__ float join(float m, float top, float x) { return m == -INFINITY ? x : x * exp2f(m - top); }
+__device__ __forceinline__ float join_weight(float m, float top) { return m == -INFINITY ? 1.f : exp2f(m - top); }
 
-// x 2^d, |d| <= 127, in two steps so that neither factor leaves the normal numbers.
+// x 2^d, |d| <= 150, in two steps so that neither factor leaves the normal numbers.
 __device__ __forceinline__ float times_exp2(float x, float d) {
   const float f = exp2f(0.5f * d);
   return mul_exact(mul_exact(x, f), f);
 }
 
-// Joins the splits: one CTA per (sequence, KV head), one thread per feature.
-__global__ void __launch_bounds__(kThreads) q8_combine_kernel(const Q8DecodeParams p) {
-  const int h = blockIdx.x, b = blockIdx.y, d = threadIdx.x;
-  const int64_t pair = (int64_t)b * p.heads_k + h;
-  for (int r = 0; r < kGroup; ++r) {
-    const float* src = p.partial + (pair * p.splits * kGroup + r) * kPartialFloats;
-    float m = -INFINITY, mv = -INFINITY;
-    for (int s = 0; s < p.splits; ++s) {
-      m = fmaxf(m, src[(int64_t)s * kGroup * kPartialFloats + kHeadDim]);
-      mv = fmaxf(mv, src[(int64_t)s * kGroup * kPartialFloats + kHeadDim + 2]);
-    }
-    float acc = 0.f, l = 0.f;
-    for (int s = 0; s < p.splits; ++s) {
-      const float* part = src + (int64_t)s * kGroup * kPartialFloats;
-      l += join(part[kHeadDim], m, part[kHeadDim + 1]);
-      acc += join(part[kHeadDim + 2], mv, part[d]);
-    }
-    const bool none = l == 0.f;
-    const int64_t row = pair * kGroup + r;
-    p.out[row * kHeadDim + d] = __float2bfloat16_rn(none ? 0.f : times_exp2(acc / l, mv - m));
-    if (p.lse != nullptr && d == 0) p.lse[row] = none ? INFINITY : (m + log2f(l)) * kLn2;
+__device__ __forceinline__ void store_out(const Q8DecodeParams& p, int64_t qrow, int d0, const float (&acc)[4], float m, float l,
+                                          float unit) {
+  // l == 0: no key; NaN: a NaN among them
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  float x[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = l == 0.f ? 0.f : times_exp2(acc[i] * inv, unit - m);
+  *reinterpret_cast<uint2*>(p.out + qrow * kHeadDim + d0) = make_uint2(mmasync::pack2(x[0], x[1]), mmasync::pack2(x[2], x[3]));
+  if (p.lse != nullptr && d0 == 0) p.lse[qrow] = l == 0.f ? INFINITY : (m + log2f(l)) * kLn2;
+}
+
+// A CTA's blocks of one (sequence, KV head) at a time; each of its four warps streams 32-key units through its own
+// two slots of shared memory (K 4 KB, V 4 KB, 128-byte swizzle, filled by TMA), so that one unit is in flight while
+// another is worked on.  The 16 query heads are one M tile of mma.sync m16n8k16 in fp16, fp32 sums: codes become fp16
+// numbers exactly, a query row is scaled by a power of two into fp16's range (exact but for elements below 2^-39 of
+// its largest; a rotated one, which has 24 bits, becomes a sum of two fp16 rows), scales are applied to the scores and, as exponents, to the weights.  A weight is rounded to fp16 at
+// 2^15 times its value, 2^-12 relative down to 2^-29 of the largest weight and 2^-40 of that below.
+//
+// The contraction order over the 128 features is free, so codes 4t .. 4t + 3 of a 16-feature chunk, one 32-bit word
+// of ldmatrix, serve as k = 2t, 2t + 1, 2t + 8, 2t + 9; the query is read in the same order.  V comes through the
+// transposing 16-bit ldmatrix, a word of which holds two tokens' codes of two neighbouring features: even features
+// and odd features of a chunk are the columns of two products.
+template <int kCode, int kBox, bool kRotate>
+__global__ void __launch_bounds__(kThreads, kResident)
+q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Q8DecodeParams p) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  __shared__ uint64_t bars[kWarps][kStages];
+  __shared__ __align__(16) __half qs[kGroup][kHeadDim + 8];
+  __shared__ __align__(16) __half q_lo[kRotate ? kGroup : 1][kHeadDim + 8];
+  __shared__ float q_factor[kGroup];               // 2^x that undoes a row's scaling
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  uint8_t* slots = smem + warp * kStages * kSlotBytes;
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) tc::mbar_init(&bars[warp][i], 1);
+    tc::fence_barrier_init();
   }
+  __syncwarp();
+  uint32_t phases = 0;                             // bit i: parity of the next completion of slot i
+  bool expired = false;                            // a bounded wait ran out: the result is poisoned
+
+  // the CTA's share: blocks [at, end) of the row of all blocks, or split `split` of a mask's blocks
+  const bool dealt = p.mask == nullptr;
+  int b = 0, h = 0, split = 0;
+  int64_t at = 0, end = 0, before = 0;
+  if (dealt) {
+    const Deal deal(p, gridDim.x, lane);
+    if (deal.total == 0 || blockIdx.x >= deal.ctas) return;
+    at = deal.first(blockIdx.x);
+    end = deal.first(blockIdx.x + 1);
+    b = find_block(p, at, before, lane);
+  } else {
+    split = blockIdx.x % p.splits;
+    const int pair = blockIdx.x / p.splits;
+    b = pair / p.heads_k;
+    h = pair % p.heads_k;
+  }
+
+  while (true) {
+    const int len = keys_of(p, b);
+    int n = (len + kBlockN - 1) / kBlockN, j0, j1;
+    BlockList<2> list{dealt ? nullptr : p.mask + ((int64_t)b * p.heads_k + h) * p.mask_words, p.mask_words, n, -1};
+    if (dealt) {
+      h = (int)((at - before) / n);
+      j0 = (int)(at - before - (int64_t)h * n);
+      j1 = (int)min((int64_t)n, j0 + end - at);
+    } else {
+      n = list.count(lane);
+      const int per = (n + p.splits - 1) / p.splits;
+      j0 = split * per;
+      j1 = min(n, j0 + per);
+    }
+    const int64_t pair = (int64_t)b * p.heads_k + h;
+
+    // this warp's units: half (warp & 1) of blocks j0 + (warp >> 1), + 2, ...
+    int j = j0 + (warp >> 1), lookups = 0;
+    auto next_key = [&]() -> int {                 // first key of the next unit, or -1
+      while (j < j1) {
+        const int blk = list.nth(lookups++, j, lane);
+        j += 2;
+        const int key0 = blk * kBlockN + (warp & 1) * kUnit;
+        if (blk >= 0 && key0 < len) return key0;
+      }
+      return -1;
+    };
+    // starts the copies of a unit into slot i; returns the scale bytes of this lane's key (K low, V high)
+    auto fetch = [&](int i, int key0) -> uint32_t {
+      tc::fence_proxy_async_smem();                // the slot was read, and its tail zeroed, by ordinary accesses
+      __syncwarp();
+      uint32_t bytes = 0;
+      int row = -1;
+      if (key0 + lane < len) {
+        const int64_t row0 = p.place.row0(b, key0 + lane);
+        bytes = kNanByte << 8;                     // a page that the cache does not have: NaN
+        if (row0 >= 0) {
+          row = (int)p.place.row(row0, h);
+          bytes = (uint32_t)__ldg(p.k_scale + row) | (uint32_t)__ldg(p.v_scale + row) << 8;
+        }
+      }
+      const bool boxed = lane % kBox == 0 && row >= 0;
+      const int boxes = __popc(__ballot_sync(0xFFFFFFFFu, boxed));
+      uint64_t* bar = &bars[warp][i];
+      if (lane == 0) tc::mbar_expect_tx(bar, boxes * 2 * kBox * kHeadDim);
+      __syncwarp();
+      if (boxed) {
+        uint8_t* dst = slots + i * kSlotBytes + lane * kHeadDim;
+        tc::tma_load_2d(dst, &map_k, bar, 0, row);
+        tc::tma_load_2d(dst + kUnit * kHeadDim, &map_v, bar, 0, row);
+      }
+      return bytes;
+    };
+
+    int keys[kStages];                             // units in the slots, the next one first (it sits in slot `slot`)
+    uint32_t bytes[kStages];
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) {
+      keys[i] = next_key();
+      bytes[i] = keys[i] >= 0 ? fetch(i, keys[i]) : 0u;
+    }
+
+    // the query rows, rotated, as fp16 with a power of two taken out
+    for (int i = warp; i < kGroup; i += kWarps) {
+      float x[4];
+      load_rotated(x, p.q + (pair * kGroup + i) * kHeadDim, p.rotary, kRotate, b, lane);
+      uint32_t amax = 0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) amax = max(amax, abs_bits(x[u]));
+      const int e = min(max((int)(__reduce_max_sync(0xFFFFFFFFu, amax) >> 23), 15), 254);      // largest -> [2^14, 2^15)
+      const float f = __uint_as_float((uint32_t)(268 - e) << 23);
+#pragma unroll
+      for (int u = 0; u < 4; u += 2) {
+        const float y0 = mul_exact(x[u], f), y1 = mul_exact(x[u + 1], f);
+        const __half2 y = __floats2half2_rn(y0, y1);
+        *reinterpret_cast<__half2*>(&qs[i][4 * lane + u]) = y;
+        if (kRotate) {
+          const float2 z = __half22float2(y);
+          *reinterpret_cast<__half2*>(&q_lo[i][4 * lane + u]) = __floats2half2_rn(y0 - z.x, y1 - z.y);
+        }
+      }
+      if (lane == 0) q_factor[i] = __uint_as_float((uint32_t)(e - 14) << 23);
+    }
+    __syncthreads();
+    uint32_t qf[8][4];
+    auto q_fragment = [&](uint32_t (&f)[4], const __half (*rows)[kHeadDim + 8], int ks) {
+      const uint2 a = *reinterpret_cast<const uint2*>(&rows[g][16 * ks + 4 * t]), c = *reinterpret_cast<const uint2*>(&rows[g + 8][16 * ks + 4 * t]);
+      f[0] = a.x;
+      f[1] = c.x;
+      f[2] = a.y;
+      f[3] = c.y;
+    };
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) q_fragment(qf[ks], qs, ks);
+    const float c0 = q_factor[g] * p.scale_log2, c1 = q_factor[g + 8] * p.scale_log2;
+
+    float o[16][4];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    // rows g and g + 8: m, l and M; O's units are 2^(M - 15)
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, u0 = -INFINITY, u1 = -INFINITY;
+
+    for (int slot = 0; keys[0] >= 0; slot = slot + 1 == kStages ? 0 : slot + 1) {
+      const int key0 = keys[0];
+      const uint32_t by = bytes[0];
+      uint64_t* bar = &bars[warp][slot];
+      uint8_t* kt = slots + slot * kSlotBytes;
+      uint8_t* vt = kt + kUnit * kHeadDim;
+      if (!tc::mbar_try_wait(bar, (phases >> slot) & 1u)) {
+        const long long start = clock64();
+        while (!tc::mbar_try_wait_hint(bar, (phases >> slot) & 1u, 1000)) {
+          if (clock64() - start > kWaitLimit) {
+            expired = true;
+            break;
+          }
+        }
+      }
+      phases ^= 1u << slot;
+      __syncwarp();
+
+      // ---- S = Q . K^T (16 x 32)
+      float s[kUnit / 8][4];
+#pragma unroll
+      for (int nt = 0; nt < kUnit / 8; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+      for (int kp = 0; kp < 2; ++kp) {
+        uint32_t w[kUnit / 8][4];
+#pragma unroll
+        for (int nt = 0; nt < kUnit / 8; ++nt) {
+          const int row = nt * 8 + (lane & 7);
+          mmasync::ldmatrix_x4(w[nt], kt + row * kHeadDim + (((kp * 4 + (lane >> 3)) ^ (row & 7)) << 4));
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          uint32_t ql[4];
+          if (kRotate) q_fragment(ql, q_lo, kp * 4 + u);
+#pragma unroll
+          for (int nt = 0; nt < kUnit / 8; ++nt) {
+            uint32_t f0, f1;
+            decode_h2<kCode>(f0, f1, w[nt][u]);
+            mmasync::mma_f16(s[nt], qf[kp * 4 + u], f0, f1);
+            if (kRotate) mmasync::mma_f16(s[nt], ql, f0, f1);
+          }
+        }
+      }
+
+      // ---- scores, and scores with the exponent of the value, in log2 units
+      float z[kUnit / 8][4], mx0 = m0, mx1 = m1, mz0 = u0, mz1 = u1;
+#pragma unroll
+      for (int nt = 0; nt < kUnit / 8; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int key = nt * 8 + 2 * t + e;
+          const uint32_t w = __shfl_sync(0xFFFFFFFFu, by, key);
+          const bool in = key0 + key < len;
+          const float ks = __uint_as_float(max((w & 0xFFu) << 23, 0x00400000u));      // (NaN's byte: inf, times codes 0)
+          const int vb = (int)(w >> 8);
+          const float ev = vb == kNanByte ? __uint_as_float(0x7FC00000u) : (float)(vb - 127);
+          s[nt][e] = in ? mul_exact(s[nt][e], ks) * c0 : -INFINITY;
+          s[nt][2 + e] = in ? mul_exact(s[nt][2 + e], ks) * c1 : -INFINITY;
+          z[nt][e] = in ? s[nt][e] + ev : -INFINITY;
+          z[nt][2 + e] = in ? s[nt][2 + e] + ev : -INFINITY;
+          mx0 = fmaxf(mx0, s[nt][e]);
+          mx1 = fmaxf(mx1, s[nt][2 + e]);
+          mz0 = fmaxf(mz0, z[nt][e]);
+          mz1 = fmaxf(mz1, z[nt][2 + e]);
+        }
+      }
+#pragma unroll
+      for (int d = 1; d < 4; d <<= 1) {
+        mx0 = fmaxf(mx0, __shfl_xor_sync(0xFFFFFFFFu, mx0, d));
+        mx1 = fmaxf(mx1, __shfl_xor_sync(0xFFFFFFFFu, mx1, d));
+        mz0 = fmaxf(mz0, __shfl_xor_sync(0xFFFFFFFFu, mz0, d));
+        mz1 = fmaxf(mz1, __shfl_xor_sync(0xFFFFFFFFu, mz1, d));
+      }
+      const float f0 = mx0 == -INFINITY ? 1.f : exp2f(m0 - mx0), f1 = mx1 == -INFINITY ? 1.f : exp2f(m1 - mx1);
+      const float fu0 = mz0 == -INFINITY ? 1.f : exp2f(u0 - mz0), fu1 = mz1 == -INFINITY ? 1.f : exp2f(u1 - mz1);
+      const float sm0 = mx0 == -INFINITY ? 0.f : mx0, sm1 = mx1 == -INFINITY ? 0.f : mx1;
+      const float su0 = mz0 == -INFINITY ? 0.f : mz0 - 15.f, su1 = mz1 == -INFINITY ? 0.f : mz1 - 15.f;      // the largest weight: 2^15
+      m0 = mx0;
+      m1 = mx1;
+      u0 = mz0;
+      u1 = mz1;
+      float sum0 = 0.f, sum1 = 0.f;
+      uint32_t pf[kUnit / 16][4];                  // weights as A fragments of the second product
+#pragma unroll
+      for (int nt = 0; nt < kUnit / 8; ++nt) {
+        sum0 += exp2f(s[nt][0] - sm0) + exp2f(s[nt][1] - sm0);
+        sum1 += exp2f(s[nt][2] - sm1) + exp2f(s[nt][3] - sm1);
+        const __half2 w0 = __floats2half2_rn(exp2f(z[nt][0] - su0), exp2f(z[nt][1] - su0));
+        const __half2 w1 = __floats2half2_rn(exp2f(z[nt][2] - su1), exp2f(z[nt][3] - su1));
+        pf[nt >> 1][(nt & 1) * 2] = *reinterpret_cast<const uint32_t*>(&w0);
+        pf[nt >> 1][(nt & 1) * 2 + 1] = *reinterpret_cast<const uint32_t*>(&w1);
+      }
+      l0 = l0 * f0 + sum0;                         // per lane; added up over the quad at the end
+      l1 = l1 * f1 + sum1;
+      if (__any_sync(0xFFFFFFFFu, fu0 != 1.f || fu1 != 1.f)) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          o[k][0] *= fu0;
+          o[k][1] *= fu0;
+          o[k][2] *= fu1;
+          o[k][3] *= fu1;
+        }
+      }
+
+      // ---- O += P . V (16 x 128); rows past the last key have weight 0, but their bytes can be NaN codes
+      if (key0 + kUnit > len) {
+        for (int k = lane; k < kUnit * 8; k += 32)
+          if (key0 + (k >> 3) >= len) *reinterpret_cast<uint4*>(vt + k * 16) = make_uint4(0u, 0u, 0u, 0u);
+        __syncwarp();
+      }
+#pragma unroll
+      for (int kk = 0; kk < kUnit / 16; ++kk) {
+#pragma unroll
+        for (int np = 0; np < 4; ++np) {           // two chunks of 16 features
+          uint32_t w[4];
+          const int row = kk * 16 + (lane & 15), chunk = np * 2 + (lane >> 4);
+          mmasync::ldmatrix_x4_trans(w, vt + row * kHeadDim + ((chunk ^ (row & 7)) << 4));
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            uint32_t e0, e1, d0, d1;
+            decode_h2_even_odd<kCode>(e0, d0, w[2 * u]);
+            decode_h2_even_odd<kCode>(e1, d1, w[2 * u + 1]);
+            mmasync::mma_f16(o[4 * np + 2 * u], pf[kk], e0, e1);
+            mmasync::mma_f16(o[4 * np + 2 * u + 1], pf[kk], d0, d1);
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i + 1 < kStages; ++i) {
+        keys[i] = keys[i + 1];
+        bytes[i] = bytes[i + 1];
+      }
+      keys[kStages - 1] = next_key();
+      bytes[kStages - 1] = keys[kStages - 1] >= 0 ? fetch(slot, keys[kStages - 1]) : 0u;
+    }
+    if (__any_sync(0xFFFFFFFFu, expired)) l0 = l1 = __uint_as_float(0x7FC00000u);      // NaN: visible, not silent
+    l0 += __shfl_xor_sync(0xFFFFFFFFu, l0, 1);
+    l0 += __shfl_xor_sync(0xFFFFFFFFu, l0, 2);
+    l1 += __shfl_xor_sync(0xFFFFFFFFu, l1, 1);
+    l1 += __shfl_xor_sync(0xFFFFFFFFu, l1, 2);
+
+    // ---- join the four warps through the slots' memory (all their copies have landed and been read)
+    __syncthreads();
+    float* stage = reinterpret_cast<float*>(smem);             // [warp][16][kPartialFloats]
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      float* w = stage + (warp * kGroup + g + 8 * half) * kPartialFloats;
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        *reinterpret_cast<float4*>(w + 16 * c + 4 * t) =
+            make_float4(o[2 * c][2 * half], o[2 * c + 1][2 * half], o[2 * c][2 * half + 1], o[2 * c + 1][2 * half + 1]);
+      if (t == 0) {
+        w[kHeadDim] = half ? m1 : m0;
+        w[kHeadDim + 1] = half ? l1 : l0;
+        w[kHeadDim + 2] = (half ? u1 : u0) - 15.f;
+      }
+    }
+    __syncthreads();
+    const bool whole = dealt ? j0 == 0 && j1 == n : p.splits == 1;
+    const int64_t part = dealt ? 2 * (int64_t)blockIdx.x + (j0 == 0) : (int64_t)blockIdx.x;
+    for (int r = warp; r < kGroup; r += kWarps) {              // a row per warp, four features per lane
+      const float* src = stage + r * kPartialFloats;
+      float m = -INFINITY, unit = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        m = fmaxf(m, src[w * kGroup * kPartialFloats + kHeadDim]);
+        unit = fmaxf(unit, src[w * kGroup * kPartialFloats + kHeadDim + 2]);
+      }
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float* sw = src + w * kGroup * kPartialFloats;
+        l += join_weight(sw[kHeadDim], m) * sw[kHeadDim + 1];
+        const float f = join_weight(sw[kHeadDim + 2], unit);
+        const float4 v = *reinterpret_cast<const float4*>(sw + 4 * lane);
+        acc[0] += f * v.x;
+        acc[1] += f * v.y;
+        acc[2] += f * v.z;
+        acc[3] += f * v.w;
+      }
+      if (whole) {
+        store_out(p, pair * kGroup + r, 4 * lane, acc, m, l, unit);
+      } else {
+        float* dst = p.partial + (part * kGroup + r) * kPartialFloats;
+        *reinterpret_cast<float4*>(dst + 4 * lane) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        if (lane == 0) *reinterpret_cast<float4*>(dst + kHeadDim) = make_float4(m, l, unit, 0.f);
+      }
+    }
+    if (!dealt) return;
+    at += j1 - j0;
+    if (at >= end) return;
+    while (at - before >= (int64_t)blocks_of(p, b) * p.heads_k) {      // the next sequence that has a block
+      before += (int64_t)blocks_of(p, b) * p.heads_k;
+      ++b;
+    }
+    tc::fence_proxy_async_smem();
+    __syncthreads();                               // the stage is read before the next segment's copies land in it
+  }
+}
+
+// Joins the partial sums of a (sequence, KV head).  kSplitWarps warps share a row's partials, a lane holds four
+// features; eight partials' loads are in flight at a time.
+template <int kSplitWarps>
+__global__ void __launch_bounds__(256) q8_combine_kernel(const Q8DecodeParams p, int split_grid) {
+  __shared__ float4 sums[8][32];
+  __shared__ float stats[8][3];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t pair = blockIdx.y;
+  const int b = (int)(pair / p.heads_k), h = (int)(pair % p.heads_k);
+  const int r = blockIdx.x * (8 / kSplitWarps) + warp / kSplitWarps, w0 = warp % kSplitWarps;
+  int64_t first = pair * p.splits;
+  int n = p.splits;
+  bool start_slot = false;                          // the first partial lies in its CTA's second place
+  if (p.mask == nullptr) {
+    const Deal deal(p, split_grid, lane);
+    const int blocks = blocks_of(p, b);
+    if (blocks == 0) {
+      n = 0;
+    } else {
+      int64_t before = 0;
+      for (int b1 = lane; b1 < b; b1 += 32) before += blocks_of(p, b1);
+#pragma unroll
+      for (int d = 16; d >= 1; d >>= 1) before += __shfl_xor_sync(0xFFFFFFFFu, before, d);
+      const int64_t at = before * p.heads_k + (int64_t)h * blocks;
+      first = deal.cta_of(at);
+      n = deal.cta_of(at + blocks - 1) - (int)first + 1;
+      if (n == 1) return;                           // one CTA had all of it and wrote the result
+      start_slot = true;
+    }
+  }
+  auto partial = [&](int s) -> const float* {
+    const int64_t slot = start_slot ? 2 * (first + s) + (s == 0) : first + s;
+    return p.partial + (slot * kGroup + r) * kPartialFloats;
+  };
+  float m = -INFINITY, unit = -INFINITY;
+  for (int s = lane; s < n; s += 32) {
+    const float4 st = *reinterpret_cast<const float4*>(partial(s) + kHeadDim);
+    m = fmaxf(m, st.x);
+    unit = fmaxf(unit, st.z);
+  }
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) {
+    m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+    unit = fmaxf(unit, __shfl_xor_sync(0xFFFFFFFFu, unit, d));
+  }
+  float acc[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
+  constexpr int kBatch = 8;
+  for (int s0 = w0; s0 < n; s0 += kBatch * kSplitWarps) {
+    float4 v[kBatch], st[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      if (s0 + k * kSplitWarps >= n) continue;
+      const float* src = partial(s0 + k * kSplitWarps);
+      v[k] = *reinterpret_cast<const float4*>(src + 4 * lane);
+      st[k] = *reinterpret_cast<const float4*>(src + kHeadDim);
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      if (s0 + k * kSplitWarps >= n) continue;
+      l += join_weight(st[k].x, m) * st[k].y;
+      const float f = join_weight(st[k].z, unit);
+      acc[0] += f * v[k].x;
+      acc[1] += f * v[k].y;
+      acc[2] += f * v[k].z;
+      acc[3] += f * v[k].w;
+    }
+  }
+  if (kSplitWarps > 1) {
+    sums[warp][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    if (lane == 0) stats[warp][0] = l;
+    __syncthreads();
+    if (w0 != 0) return;
+#pragma unroll
+    for (int w = 1; w < kSplitWarps; ++w) {
+      const float4 v = sums[warp + w][lane];
+      acc[0] += v.x;
+      acc[1] += v.y;
+      acc[2] += v.z;
+      acc[3] += v.w;
+      l += stats[warp + w][0];
+    }
+  }
+  store_out(p, pair * kGroup + r, 4 * lane, acc, m, l, unit);
 }
 
 }  // namespace
@@ -249,7 +630,10 @@ using namespace ifv2;
 
 extern "C" int64_t ifv2_q8_decode_workspace_bytes(int batch, int heads_q, int head_dim) {
   if (batch < 0 || heads_q < 0 || head_dim != kHeadDim) return 0;
-  return (int64_t)batch * heads_q * kMaxSplits * kPartialFloats * 4 + 256;
+  // masks: every split of every (sequence, KV head), at most kDealtCtas of them or one each; no mask: two per CTA
+  const int64_t pairs = (int64_t)batch * (heads_q / kGroup);
+  const int64_t parts = pairs > 2 * kDealtCtas ? pairs : 2 * kDealtCtas;
+  return parts * kGroup * kPartialFloats * 4;
 }
 
 extern "C" int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void* k_scale, void* v_scale, const void* k_new,
@@ -286,7 +670,8 @@ extern "C" int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void*
                "q8_decode: the cache has more than 2^31-1 rows");
   const int64_t capacity = block_table != nullptr ? (int64_t)block_table_stride * length : length;
   IFV2_REQUIRE(capacity <= INT32_MAX - kBlockN, IFV2_ERR_TOO_LARGE, "q8_decode: more than 2^31-1 positions");
-  IFV2_REQUIRE(batch <= 65535 && heads_k <= 65535, IFV2_ERR_TOO_LARGE, "q8_decode: batch or heads_k > 65535");
+  IFV2_REQUIRE(batch <= 65535 && heads_k <= 65535 && (int64_t)batch * heads_k <= 65535, IFV2_ERR_TOO_LARGE,
+               "q8_decode: more than 65535 sequences x KV heads");
   IFV2_REQUIRE(workspace_bytes >= ifv2_q8_decode_workspace_bytes(batch, heads_q, head_dim), IFV2_ERR_INVALID_ARG,
                "q8_decode: workspace too small");
   for (const void* ptr : {q, (const void*)k_cache, (const void*)v_cache, (const void*)workspace, (const void*)out, k_new, v_new})
@@ -315,7 +700,12 @@ extern "C" int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void*
   p.partial = static_cast<float*>(workspace);
   p.out = static_cast<__nv_bfloat16*>(out);
   p.lse = lse;
-  p.splits = kMaxSplits;
+  const int64_t pairs = (int64_t)batch * heads_k;
+  p.splits = 1;
+  if (mask != nullptr) {
+    const int64_t most = kDealtCtas / pairs;
+    p.splits = most < 1 ? 1 : most > kMaxSplits ? kMaxSplits : (int)most;
+  }
   cudaStream_t st = (cudaStream_t)stream;
   if (k_new != nullptr || topk_idx != nullptr) {
     const Q8PrepareParams a{static_cast<const __nv_bfloat16*>(k_new), static_cast<const __nv_bfloat16*>(v_new),
@@ -327,10 +717,32 @@ extern "C" int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void*
     int rc = check_launch("q8_prepare");
     if (rc) return rc;
   }
-  if (code == kE4m3) q8_split_kernel<kE4m3><<<dim3(p.splits, heads_k, batch), kThreads, 0, st>>>(p);
-  else q8_split_kernel<kInt8><<<dim3(p.splits, heads_k, batch), kThreads, 0, st>>>(p);
-  int rc = check_launch("q8_split");
+  // boxes of 32 rows where 32 consecutive positions are 32 consecutive rows, else of 16
+  const bool wide = block_table == nullptr || length % kUnit == 0;
+  CUtensorMap map_k, map_v;
+  const uint64_t rows = (uint64_t)slots * heads_k * length;
+  int rc = make_tensor_map_rows128(&map_k, k_cache, rows, wide ? 32 : 16);
+  if (rc == IFV2_OK) rc = make_tensor_map_rows128(&map_v, v_cache, rows, wide ? 32 : 16);
   if (rc) return rc;
-  q8_combine_kernel<<<dim3(heads_k, batch), kThreads, 0, st>>>(p);
+  auto kernel = rotate ? (code == kE4m3 ? (wide ? q8_split_kernel<kE4m3, 32, true> : q8_split_kernel<kE4m3, 16, true>)
+                                        : (wide ? q8_split_kernel<kInt8, 32, true> : q8_split_kernel<kInt8, 16, true>))
+                       : (code == kE4m3 ? (wide ? q8_split_kernel<kE4m3, 32, false> : q8_split_kernel<kE4m3, 16, false>)
+                                        : (wide ? q8_split_kernel<kInt8, 32, false> : q8_split_kernel<kInt8, 16, false>));
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+  if (e != cudaSuccess) return set_error((int)e, "q8_decode: %s", cudaGetErrorString(e));
+  int64_t grid = pairs * p.splits;
+  if (mask == nullptr) {
+    grid = pairs * ceil_div64(capacity, kBlockN);
+    if (grid > kDealtCtas) grid = kDealtCtas;
+  }
+  IFV2_REQUIRE(grid <= INT32_MAX, IFV2_ERR_TOO_LARGE, "q8_decode: too many sequences x heads");
+  kernel<<<(unsigned)grid, kThreads, kSmemBytes, st>>>(map_k, map_v, p);
+  rc = check_launch("q8_split");
+  if (rc) return rc;
+  if (mask != nullptr && p.splits == 1) return IFV2_OK;      // the split kernel wrote the results
+  const int64_t per_pair = mask != nullptr ? p.splits : ceil_div64(grid, pairs);
+  if (per_pair > 16) q8_combine_kernel<8><<<dim3(16, (unsigned)pairs), 256, 0, st>>>(p, (int)grid);
+  else if (per_pair > 4) q8_combine_kernel<4><<<dim3(8, (unsigned)pairs), 256, 0, st>>>(p, (int)grid);
+  else q8_combine_kernel<1><<<dim3(2, (unsigned)pairs), 256, 0, st>>>(p, (int)grid);
   return check_launch("q8_combine");
 }

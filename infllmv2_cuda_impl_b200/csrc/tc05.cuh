@@ -491,4 +491,7 @@ int make_tensor_map_bf16_3d(CUtensorMap* map, const void* base, uint64_t d0, uin
                             uint64_t d2, uint64_t stride1_bytes, uint64_t stride2_bytes,
                             uint32_t b0, uint32_t b1, uint32_t b2);
 
+// rank-2 map of (rows, 128) bytes with 128-byte swizzle, boxes of box_rows whole rows.
+int make_tensor_map_rows128(CUtensorMap* map, const void* base, uint64_t rows, uint32_t box_rows);
+
 }  // namespace ifv2

@@ -47,4 +47,21 @@ int make_tensor_map_bf16_3d(CUtensorMap* map, const void* base, uint64_t d0, uin
   return IFV2_OK;
 }
 
+int make_tensor_map_rows128(CUtensorMap* map, const void* base, uint64_t rows, uint32_t box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  IFV2_REQUIRE(fn != nullptr, IFV2_ERR_DRIVER, "cuTensorMapEncodeTiled is not available (no driver?)");
+  IFV2_REQUIRE(reinterpret_cast<uintptr_t>(base) % 16 == 0, IFV2_ERR_INVALID_ARG,
+               "tensor base address must be 16-byte aligned");
+  cuuint64_t dims[2] = {128, rows ? rows : 1};
+  cuuint64_t strides[1] = {128};
+  cuuint32_t box[2] = {128, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  IFV2_REQUIRE(r == CUDA_SUCCESS, IFV2_ERR_DRIVER, "cuTensorMapEncodeTiled failed with CUresult %d",
+               (int)r);
+  return IFV2_OK;
+}
+
 }  // namespace ifv2
