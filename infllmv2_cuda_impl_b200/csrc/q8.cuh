@@ -72,13 +72,13 @@ __device__ __forceinline__ void decode4(float (&x)[4], uint32_t c) {
 // Four codes as two fp16 pairs, codes (0, 1) and (2, 3); exact.  Integers go through 1024 + (code + 128), whose
 // fp16 numbers are 0x6400 + (code + 128).
 template <int kCode>
-__device__ __forceinline__ void decode_h2(uint32_t& lo, uint32_t& hi, uint32_t c) {
+__device__ __forceinline__ void decode_h2(uint32_t& lo, uint32_t& hi, uint32_t c, uint32_t lo_bytes = 0x4140, uint32_t hi_bytes = 0x4342) {
   if (kCode == kE4m3) {
     asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
         : "=r"(lo), "=r"(hi) : "r"(c));
   } else {
     c ^= 0x80808080u;
-    const uint32_t a = __byte_perm(c, 0x64646464u, 0x4140), b = __byte_perm(c, 0x64646464u, 0x4342);
+    const uint32_t a = __byte_perm(c, 0x64646464u, lo_bytes), b = __byte_perm(c, 0x64646464u, hi_bytes);
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(a), "r"(0x64806480u));
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(b), "r"(0x64806480u));
   }
@@ -86,7 +86,8 @@ __device__ __forceinline__ void decode_h2(uint32_t& lo, uint32_t& hi, uint32_t c
 // The same for codes (0, 2) and (1, 3): a transposed 16-bit load holds two tokens' codes of two features.
 template <int kCode>
 __device__ __forceinline__ void decode_h2_even_odd(uint32_t& even, uint32_t& odd, uint32_t c) {
-  decode_h2<kCode>(even, odd, __byte_perm(c, 0u, 0x3120));
+  if (kCode == kE4m3) decode_h2<kCode>(even, odd, __byte_perm(c, 0u, 0x3120));
+  else decode_h2<kCode>(even, odd, c, 0x4240, 0x4341);
 }
 
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }

@@ -5,11 +5,12 @@
 // over the positions of the sequence, or those of the 64-key blocks that its mask row selects.  The keys are shared
 // by 16 query heads, split over CTAs, and the partial (m, l, M, O) of the splits are joined by a second kernel.
 //
-// O is a sum over codes, O = sum 2^(z_t - M) V_t with z_t = log2(e) s_t + eV(t) and M = max z: the exponents of the
-// values take part in the weights, next to the scores, so no weight is above 1, the largest is 1 whatever the values'
-// sizes are, and out = O 2^(M - m) / l.  (m and M differ by at most 127, the range of the exponents.)
+// O is a sum over codes, O = sum 2^(z_t - M) V_t with z_t = log2(e) s_t + eV(t) and M about max z: the exponents of the
+// values take part in the weights, next to the scores, so that the largest weight is about 1 whatever the values' sizes
+// are, and out = O 2^(M - m) / l.  (m and M differ by little more than 127, the range of the exponents.)
 //
 // Launches: [prepare: block lists, append] -> split -> combine.
+#include <type_traits>
 #include "block_list.cuh"
 #include "mma_sync.cuh"
 #include "q8.cuh"
@@ -23,13 +24,16 @@ using namespace q8;
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kResident = 3;                     // CTAs per SM
+#ifndef RES
+#define RES 3
+#endif
+constexpr int kResident = RES, kResidentRotate = 3;      // CTAs per SM
 constexpr int kUnit = 32;                        // keys that a warp handles at once
-constexpr int kStages = 2;                       // slots of a warp
-constexpr int kSlotBytes = 2 * kUnit * kHeadDim; // K and V codes of a unit
-constexpr int kSmemBytes = kWarps * kStages * kSlotBytes + 1024;
+constexpr int kSlots = 3;                        // a warp's tiles in shared memory: K, V, next K, next V ... in turn
+constexpr int kTileBytes = kUnit * kHeadDim;
+constexpr int kSmemBytes = kWarps * kSlots * kTileBytes + 1024;
 constexpr int kMaxSplits = 16;                   // CTAs that share the selected blocks of a (sequence, KV head)
-constexpr int kDealtCtas = kResident * kNumSMs;  // CTAs that share all blocks where there is no mask
+constexpr int kMaxCtas = kResident * kNumSMs;    // CTAs that share all blocks where there is no mask
 constexpr long long kWaitLimit = 1ll << 28;      // clocks; a copy takes microseconds
 constexpr int kPartialFloats = kHeadDim + 4;     // O row, m (log2 units), l, exponent of O's units, pad
 constexpr float kLog2e = 1.4426950408889634f;
@@ -132,30 +136,30 @@ __device__ __forceinline__ int blocks_of(const Q8DecodeParams& p, int b) { retur
 // lengths are (16 sequences of 1000 .. 32000 tokens in equal splits wait for the longest one).  Every warp finds its
 // place by itself, a sequence per lane.
 struct Deal {
-  int64_t total;
-  int ctas;
-  __device__ Deal(const Q8DecodeParams& p, int grid, int lane) {
-    int64_t n = 0;
+  uint32_t total, ctas, each, rest;                // total = each * ctas + rest
+  __device__ Deal(const Q8DecodeParams& p, uint32_t grid, int lane) {
+    uint32_t n = 0;
     for (int b = lane; b < p.batch; b += 32) n += blocks_of(p, b);
-#pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) n += __shfl_xor_sync(0xFFFFFFFFu, n, d);
-    total = n * p.heads_k;
+    total = __reduce_add_sync(0xFFFFFFFFu, n) * p.heads_k;      // (the host keeps it below 2^31)
     // two blocks are one 32-key unit for each of the four warps
-    ctas = (int)max((int64_t)1, min((int64_t)grid, (total + 1) / 2));
+    ctas = max(1u, min(grid, (total + 1) / 2));
+    each = total / ctas;
+    rest = total - each * ctas;
   }
-  __device__ int64_t first(int c) const { return (int64_t)c * total / ctas; }
-  __device__ int cta_of(int64_t block) const { return (int)(((block + 1) * ctas - 1) / total); }
+  __device__ uint32_t first(uint32_t c) const { return c * each + c * rest / ctas; }      // c total / ctas
+  // the last c with first(c) <= block: each c + floor(c rest / ctas) <= block
+  __device__ uint32_t cta_of(uint32_t block) const { return (uint32_t)((((uint64_t)block + 1) * ctas - 1) / total); }
 };
 
 // Sequence that holds block `at` of the row, and the row's blocks before it.
-__device__ __forceinline__ int find_block(const Q8DecodeParams& p, int64_t at, int64_t& before, int lane) {
+__device__ __forceinline__ int find_block(const Q8DecodeParams& p, uint32_t at, uint32_t& before, int lane) {
   before = 0;
   for (int b0 = 0; b0 < p.batch; b0 += 32) {
-    const int64_t n = b0 + lane < p.batch ? (int64_t)blocks_of(p, b0 + lane) * p.heads_k : 0;
-    int64_t incl = n;
+    const uint32_t n = b0 + lane < p.batch ? (uint32_t)(blocks_of(p, b0 + lane) * p.heads_k) : 0u;
+    uint32_t incl = n;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int64_t up = __shfl_up_sync(0xFFFFFFFFu, incl, d);
+      const uint32_t up = __shfl_up_sync(0xFFFFFFFFu, incl, d);
       if (lane >= d) incl += up;
     }
     const uint32_t past = __ballot_sync(0xFFFFFFFFu, before + incl > at);
@@ -189,31 +193,36 @@ __device__ __forceinline__ void store_out(const Q8DecodeParams& p, int64_t qrow,
   if (p.lse != nullptr && d0 == 0) p.lse[qrow] = l == 0.f ? INFINITY : (m + log2f(l)) * kLn2;
 }
 
-// A CTA's blocks of one (sequence, KV head) at a time; each of its four warps streams 32-key units through its own
-// two slots of shared memory (K 4 KB, V 4 KB, 128-byte swizzle, filled by TMA), so that one unit is in flight while
-// another is worked on.  The 16 query heads are one M tile of mma.sync m16n8k16 in fp16, fp32 sums: codes become fp16
+// A CTA's blocks of one (sequence, KV head) at a time; each of its four warps streams 32-key units, K and V in turn,
+// through its own three slots of shared memory (4 KB, 128-byte swizzle, filled by TMA), so that two tiles are in flight
+// while another is worked on.  The 16 query heads are one M tile of mma.sync m16n8k16 in fp16, fp32 sums: codes become fp16
 // numbers exactly, a query row is scaled by a power of two into fp16's range (exact but for elements below 2^-39 of
 // its largest; a rotated one, which has 24 bits, becomes a sum of two fp16 rows), scales are applied to the scores and, as exponents, to the weights.  A weight is rounded to fp16 at
-// 2^15 times its value, 2^-12 relative down to 2^-29 of the largest weight and 2^-40 of that below.
+// 2^8 to 2^15 times its share of the largest, 2^-12 relative down to 2^-22 of that and 2^-33 of it below.
 //
 // The contraction order over the 128 features is free, so codes 4t .. 4t + 3 of a 16-feature chunk, one 32-bit word
 // of ldmatrix, serve as k = 2t, 2t + 1, 2t + 8, 2t + 9; the query is read in the same order.  V comes through the
 // transposing 16-bit ldmatrix, a word of which holds two tokens' codes of two neighbouring features: even features
 // and odd features of a chunk are the columns of two products.
 template <int kCode, int kBox, bool kRotate>
-__global__ void __launch_bounds__(kThreads, kResident)
+__global__ void __launch_bounds__(kThreads, kRotate ? kResidentRotate : kResident)
 q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Q8DecodeParams p) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  __shared__ uint64_t bars[kWarps][kStages];
+  __shared__ uint64_t bars[kWarps][kSlots];
+  __shared__ __align__(16) float2 factors[kWarps][kUnit];        // of the unit at work: scale of a key, exponent of its value
   __shared__ __align__(16) __half qs[kGroup][kHeadDim + 8];
   __shared__ __align__(16) __half q_lo[kRotate ? kGroup : 1][kHeadDim + 8];
   __shared__ float q_factor[kGroup];               // 2^x that undoes a row's scaling
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  uint8_t* slots = smem + warp * kStages * kSlotBytes;
+  uint8_t* tiles = smem + warp * kSlots * kTileBytes;
   if (lane == 0) {
+    if (warp == 0) {
+      tc::prefetch_map(&map_k);
+      tc::prefetch_map(&map_v);
+    }
 #pragma unroll
-    for (int i = 0; i < kStages; ++i) tc::mbar_init(&bars[warp][i], 1);
+    for (int i = 0; i < kSlots; ++i) tc::mbar_init(&bars[warp][i], 1);
     tc::fence_barrier_init();
   }
   __syncwarp();
@@ -223,7 +232,7 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   // the CTA's share: blocks [at, end) of the row of all blocks, or split `split` of a mask's blocks
   const bool dealt = p.mask == nullptr;
   int b = 0, h = 0, split = 0;
-  int64_t at = 0, end = 0, before = 0;
+  uint32_t at = 0, end = 0, before = 0;
   if (dealt) {
     const Deal deal(p, gridDim.x, lane);
     if (deal.total == 0 || blockIdx.x >= deal.ctas) return;
@@ -242,9 +251,9 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     int n = (len + kBlockN - 1) / kBlockN, j0, j1;
     BlockList<2> list{dealt ? nullptr : p.mask + ((int64_t)b * p.heads_k + h) * p.mask_words, p.mask_words, n, -1};
     if (dealt) {
-      h = (int)((at - before) / n);
-      j0 = (int)(at - before - (int64_t)h * n);
-      j1 = (int)min((int64_t)n, j0 + end - at);
+      h = (int)((at - before) / (uint32_t)n);
+      j0 = (int)(at - before - (uint32_t)(h * n));
+      j1 = (int)min((uint32_t)n, j0 + end - at);
     } else {
       n = list.count(lane);
       const int per = (n + p.splits - 1) / p.splits;
@@ -264,39 +273,55 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       }
       return -1;
     };
-    // starts the copies of a unit into slot i; returns the scale bytes of this lane's key (K low, V high)
-    auto fetch = [&](int i, int key0) -> uint32_t {
-      tc::fence_proxy_async_smem();                // the slot was read, and its tail zeroed, by ordinary accesses
-      __syncwarp();
-      uint32_t bytes = 0;
-      int row = -1;
+    // where the key of this lane is (-1: nowhere), and its scale bytes (K low, V high)
+    auto locate = [&](int key0, int& row) -> uint32_t {
+      row = -1;
+      uint32_t kb = 0, vb = kNanByte;              // (a page that the cache does not have: NaN)
       if (key0 + lane < len) {
         const int64_t row0 = p.place.row0(b, key0 + lane);
-        bytes = kNanByte << 8;                     // a page that the cache does not have: NaN
         if (row0 >= 0) {
           row = (int)p.place.row(row0, h);
-          bytes = (uint32_t)__ldg(p.k_scale + row) | (uint32_t)__ldg(p.v_scale + row) << 8;
+          kb = __ldg(p.k_scale + row);
+          vb = __ldg(p.v_scale + row);
         }
       }
+      return kb | vb << 8;
+    };
+    // starts the copy of the tile whose keys' rows the lanes hold into slot i
+    auto fetch = [&](const CUtensorMap& map, int i, int row) {
+      tc::fence_proxy_async_smem();                // the slot was read, and its tail zeroed, by ordinary accesses
+      __syncwarp();
       const bool boxed = lane % kBox == 0 && row >= 0;
       const int boxes = __popc(__ballot_sync(0xFFFFFFFFu, boxed));
-      uint64_t* bar = &bars[warp][i];
-      if (lane == 0) tc::mbar_expect_tx(bar, boxes * 2 * kBox * kHeadDim);
+      if (lane == 0) tc::mbar_expect_tx(&bars[warp][i], boxes * kBox * kHeadDim);
       __syncwarp();
-      if (boxed) {
-        uint8_t* dst = slots + i * kSlotBytes + lane * kHeadDim;
-        tc::tma_load_2d(dst, &map_k, bar, 0, row);
-        tc::tma_load_2d(dst + kUnit * kHeadDim, &map_v, bar, 0, row);
+      if (boxed) tc::tma_load_2d(tiles + i * kTileBytes + lane * kHeadDim, &map, &bars[warp][i], 0, row);
+    };
+    auto arrived = [&](int i) {
+      if (!tc::mbar_try_wait(&bars[warp][i], (phases >> i) & 1u)) {
+        const long long start = clock64();
+        while (!tc::mbar_try_wait_hint(&bars[warp][i], (phases >> i) & 1u, 1000)) {
+          if (clock64() - start > kWaitLimit) {
+            expired = true;
+            break;
+          }
+        }
       }
-      return bytes;
+      phases ^= 1u << i;
     };
 
-    int keys[kStages];                             // units in the slots, the next one first (it sits in slot `slot`)
-    uint32_t bytes[kStages];
-#pragma unroll
-    for (int i = 0; i < kStages; ++i) {
-      keys[i] = next_key();
-      bytes[i] = keys[i] >= 0 ? fetch(i, keys[i]) : 0u;
+    // unit at work and the next one: first keys, rows, scale bytes; slots of K, V and the next K
+    int key0 = next_key(), key1 = -1, row, row1 = -1, slot_k = 0, slot_v = 1, slot_n = 2;
+    uint32_t by = 0, by1 = 0;
+    if (key0 >= 0) {
+      by = locate(key0, row);
+      fetch(map_k, slot_k, row);
+      fetch(map_v, slot_v, row);
+      key1 = next_key();
+      if (key1 >= 0) {
+        by1 = locate(key1, row1);
+        fetch(map_k, slot_n, row1);
+      }
     }
 
     // the query rows, rotated, as fp16 with a power of two taken out
@@ -321,7 +346,6 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       if (lane == 0) q_factor[i] = __uint_as_float((uint32_t)(e - 14) << 23);
     }
     __syncthreads();
-    uint32_t qf[8][4];
     auto q_fragment = [&](uint32_t (&f)[4], const __half (*rows)[kHeadDim + 8], int ks) {
       const uint2 a = *reinterpret_cast<const uint2*>(&rows[g][16 * ks + 4 * t]), c = *reinterpret_cast<const uint2*>(&rows[g + 8][16 * ks + 4 * t]);
       f[0] = a.x;
@@ -329,32 +353,21 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       f[2] = a.y;
       f[3] = c.y;
     };
-#pragma unroll
-    for (int ks = 0; ks < 8; ++ks) q_fragment(qf[ks], qs, ks);
     const float c0 = q_factor[g] * p.scale_log2, c1 = q_factor[g + 8] * p.scale_log2;
 
     float o[16][4];
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    // rows g and g + 8: m, l and M; O's units are 2^(M - 15)
+    bool fresh = true;                             // no unit yet: there are no references
+    // rows g and g + 8: reference m, l, and reference M; O's units are 2^(M - 8)
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, u0 = -INFINITY, u1 = -INFINITY;
 
-    for (int slot = 0; keys[0] >= 0; slot = slot + 1 == kStages ? 0 : slot + 1) {
-      const int key0 = keys[0];
-      const uint32_t by = bytes[0];
-      uint64_t* bar = &bars[warp][slot];
-      uint8_t* kt = slots + slot * kSlotBytes;
-      uint8_t* vt = kt + kUnit * kHeadDim;
-      if (!tc::mbar_try_wait(bar, (phases >> slot) & 1u)) {
-        const long long start = clock64();
-        while (!tc::mbar_try_wait_hint(bar, (phases >> slot) & 1u, 1000)) {
-          if (clock64() - start > kWaitLimit) {
-            expired = true;
-            break;
-          }
-        }
-      }
-      phases ^= 1u << slot;
+    while (key0 >= 0) {
+      const uint8_t* kt = tiles + slot_k * kTileBytes;
+      uint8_t* vt = tiles + slot_v * kTileBytes;
+      arrived(slot_k);
+      const int kb = by & 0xFF, vb = by >> 8;
+      factors[warp][lane] = make_float2(scale_value(kb), vb == kNanByte ? __uint_as_float(0x7FC00000u) : (float)(vb - 127));
       __syncwarp();
 
       // ---- S = Q . K^T (16 x 32)
@@ -371,79 +384,108 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          uint32_t ql[4];
+          uint32_t qh[4], ql[4];
+          q_fragment(qh, qs, kp * 4 + u);
           if (kRotate) q_fragment(ql, q_lo, kp * 4 + u);
 #pragma unroll
           for (int nt = 0; nt < kUnit / 8; ++nt) {
             uint32_t f0, f1;
             decode_h2<kCode>(f0, f1, w[nt][u]);
-            mmasync::mma_f16(s[nt], qf[kp * 4 + u], f0, f1);
+            mmasync::mma_f16(s[nt], qh, f0, f1);
             if (kRotate) mmasync::mma_f16(s[nt], ql, f0, f1);
           }
         }
       }
 
-      // ---- scores, and scores with the exponent of the value, in log2 units
-      float z[kUnit / 8][4], mx0 = m0, mx1 = m1, mz0 = u0, mz1 = u1;
+      if (key1 >= 0) fetch(map_v, slot_k, row1);
+
+      // ---- weights against reference maxima that move only when a weight would pass 2^15: the sum l against m, the
+      //      weights of the values against M - 8 (see the file's head).  A unit whose weights pass is done again.
+      float ev[kUnit / 8][2];                      // exponents of the values of keys 8 nt + 2t, + 1
 #pragma unroll
       for (int nt = 0; nt < kUnit / 8; ++nt) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int key = nt * 8 + 2 * t + e;
-          const uint32_t w = __shfl_sync(0xFFFFFFFFu, by, key);
-          const bool in = key0 + key < len;
-          const float ks = __uint_as_float(max((w & 0xFFu) << 23, 0x00400000u));      // (NaN's byte: inf, times codes 0)
-          const int vb = (int)(w >> 8);
-          const float ev = vb == kNanByte ? __uint_as_float(0x7FC00000u) : (float)(vb - 127);
-          s[nt][e] = in ? mul_exact(s[nt][e], ks) * c0 : -INFINITY;
-          s[nt][2 + e] = in ? mul_exact(s[nt][2 + e], ks) * c1 : -INFINITY;
-          z[nt][e] = in ? s[nt][e] + ev : -INFINITY;
-          z[nt][2 + e] = in ? s[nt][2 + e] + ev : -INFINITY;
-          mx0 = fmaxf(mx0, s[nt][e]);
-          mx1 = fmaxf(mx1, s[nt][2 + e]);
-          mz0 = fmaxf(mz0, z[nt][e]);
-          mz1 = fmaxf(mz1, z[nt][2 + e]);
-        }
+        const float4 f = *reinterpret_cast<const float4*>(&factors[warp][nt * 8 + 2 * t]);
+        ev[nt][0] = f.y;
+        ev[nt][1] = f.w;
+        s[nt][0] = mul_exact(s[nt][0], f.x);
+        s[nt][1] = mul_exact(s[nt][1], f.z);
+        s[nt][2] = mul_exact(s[nt][2], f.x);
+        s[nt][3] = mul_exact(s[nt][3], f.z);
       }
-#pragma unroll
-      for (int d = 1; d < 4; d <<= 1) {
-        mx0 = fmaxf(mx0, __shfl_xor_sync(0xFFFFFFFFu, mx0, d));
-        mx1 = fmaxf(mx1, __shfl_xor_sync(0xFFFFFFFFu, mx1, d));
-        mz0 = fmaxf(mz0, __shfl_xor_sync(0xFFFFFFFFu, mz0, d));
-        mz1 = fmaxf(mz1, __shfl_xor_sync(0xFFFFFFFFu, mz1, d));
-      }
-      const float f0 = mx0 == -INFINITY ? 1.f : exp2f(m0 - mx0), f1 = mx1 == -INFINITY ? 1.f : exp2f(m1 - mx1);
-      const float fu0 = mz0 == -INFINITY ? 1.f : exp2f(u0 - mz0), fu1 = mz1 == -INFINITY ? 1.f : exp2f(u1 - mz1);
-      const float sm0 = mx0 == -INFINITY ? 0.f : mx0, sm1 = mx1 == -INFINITY ? 0.f : mx1;
-      const float su0 = mz0 == -INFINITY ? 0.f : mz0 - 15.f, su1 = mz1 == -INFINITY ? 0.f : mz1 - 15.f;      // the largest weight: 2^15
-      m0 = mx0;
-      m1 = mx1;
-      u0 = mz0;
-      u1 = mz1;
-      float sum0 = 0.f, sum1 = 0.f;
+      float sum0, sum1;
       uint32_t pf[kUnit / 16][4];                  // weights as A fragments of the second product
+      auto weigh = [&](auto tail) -> bool {
+        constexpr bool kTail = decltype(tail)::value;
+        const float n0 = m0 == -INFINITY ? 0.f : -m0, n1 = m1 == -INFINITY ? 0.f : -m1;
+        const float w0 = u0 == -INFINITY ? 0.f : 8.f - u0, w1 = u1 == -INFINITY ? 0.f : 8.f - u1;
+        float top = -INFINITY;
+        sum0 = sum1 = 0.f;
 #pragma unroll
-      for (int nt = 0; nt < kUnit / 8; ++nt) {
-        sum0 += exp2f(s[nt][0] - sm0) + exp2f(s[nt][1] - sm0);
-        sum1 += exp2f(s[nt][2] - sm1) + exp2f(s[nt][3] - sm1);
-        const __half2 w0 = __floats2half2_rn(exp2f(z[nt][0] - su0), exp2f(z[nt][1] - su0));
-        const __half2 w1 = __floats2half2_rn(exp2f(z[nt][2] - su1), exp2f(z[nt][3] - su1));
-        pf[nt >> 1][(nt & 1) * 2] = *reinterpret_cast<const uint32_t*>(&w0);
-        pf[nt >> 1][(nt & 1) * 2 + 1] = *reinterpret_cast<const uint32_t*>(&w1);
-      }
-      l0 = l0 * f0 + sum0;                         // per lane; added up over the quad at the end
-      l1 = l1 * f1 + sum1;
-      if (__any_sync(0xFFFFFFFFu, fu0 != 1.f || fu1 != 1.f)) {
+        for (int nt = 0; nt < kUnit / 8; ++nt) {
+          float x[4];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const bool in = !kTail || key0 + nt * 8 + 2 * t + e < len;
+            const float a0 = fmaf(s[nt][e], c0, n0), a1 = fmaf(s[nt][2 + e], c1, n1);
+            sum0 += exp2f(in ? a0 : -INFINITY);
+            sum1 += exp2f(in ? a1 : -INFINITY);
+            x[e] = fmaf(s[nt][e], c0, w0) + ev[nt][e];
+            x[2 + e] = fmaf(s[nt][2 + e], c1, w1) + ev[nt][e];
+            if (!in) x[e] = x[2 + e] = -INFINITY;
+            top = fmaxf(top, fmaxf(x[e], x[2 + e]));
+          }
+          const __half2 y0 = __floats2half2_rn(exp2f(x[0]), exp2f(x[1])), y1 = __floats2half2_rn(exp2f(x[2]), exp2f(x[3]));
+          pf[nt >> 1][(nt & 1) * 2] = *reinterpret_cast<const uint32_t*>(&y0);
+          pf[nt >> 1][(nt & 1) * 2 + 1] = *reinterpret_cast<const uint32_t*>(&y1);
+        }
+        return top > 15.f || sum0 > 0x1p40f || sum1 > 0x1p40f;
+      };
+      bool again = fresh;
+      if (!fresh) again = key0 + kUnit > len ? weigh(std::true_type{}) : weigh(std::false_type{});
+      if (__any_sync(0xFFFFFFFFu, again)) {
+        float mx0 = m0, mx1 = m1, mu0 = u0, mu1 = u1;
+#pragma unroll
+        for (int nt = 0; nt < kUnit / 8; ++nt) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            if (key0 + nt * 8 + 2 * t + e >= len) continue;
+            const float a0 = s[nt][e] * c0, a1 = s[nt][2 + e] * c1;
+            mx0 = fmaxf(mx0, a0);
+            mx1 = fmaxf(mx1, a1);
+            mu0 = fmaxf(mu0, a0 + ev[nt][e]);
+            mu1 = fmaxf(mu1, a1 + ev[nt][e]);
+          }
+        }
+#pragma unroll
+        for (int d = 1; d < 4; d <<= 1) {
+          mx0 = fmaxf(mx0, __shfl_xor_sync(0xFFFFFFFFu, mx0, d));
+          mx1 = fmaxf(mx1, __shfl_xor_sync(0xFFFFFFFFu, mx1, d));
+          mu0 = fmaxf(mu0, __shfl_xor_sync(0xFFFFFFFFu, mu0, d));
+          mu1 = fmaxf(mu1, __shfl_xor_sync(0xFFFFFFFFu, mu1, d));
+        }
+        l0 *= mx0 == -INFINITY ? 1.f : exp2f(m0 - mx0);
+        l1 *= mx1 == -INFINITY ? 1.f : exp2f(m1 - mx1);
+        const float f0 = mu0 == -INFINITY ? 1.f : exp2f(u0 - mu0), f1 = mu1 == -INFINITY ? 1.f : exp2f(u1 - mu1);
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
-          o[k][0] *= fu0;
-          o[k][1] *= fu0;
-          o[k][2] *= fu1;
-          o[k][3] *= fu1;
+          o[k][0] *= f0;
+          o[k][1] *= f0;
+          o[k][2] *= f1;
+          o[k][3] *= f1;
         }
+        m0 = mx0;
+        m1 = mx1;
+        u0 = mu0;
+        u1 = mu1;
+        fresh = false;
+        weigh(std::true_type{});
       }
+      l0 += sum0;                                  // per lane; added up over the quad at the end
+      l1 += sum1;
 
       // ---- O += P . V (16 x 128); rows past the last key have weight 0, but their bytes can be NaN codes
+      arrived(slot_v);
+      __syncwarp();
       if (key0 + kUnit > len) {
         for (int k = lane; k < kUnit * 8; k += 32)
           if (key0 + (k >> 3) >= len) *reinterpret_cast<uint4*>(vt + k * 16) = make_uint4(0u, 0u, 0u, 0u);
@@ -466,13 +508,19 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
           }
         }
       }
-#pragma unroll
-      for (int i = 0; i + 1 < kStages; ++i) {
-        keys[i] = keys[i + 1];
-        bytes[i] = bytes[i + 1];
+      key0 = key1;
+      by = by1;
+      if (key1 >= 0) {
+        key1 = next_key();
+        if (key1 >= 0) {
+          by1 = locate(key1, row1);
+          fetch(map_k, slot_v, row1);
+        }
       }
-      keys[kStages - 1] = next_key();
-      bytes[kStages - 1] = keys[kStages - 1] >= 0 ? fetch(slot, keys[kStages - 1]) : 0u;
+      const int done = slot_k;
+      slot_k = slot_n;
+      slot_n = slot_v;
+      slot_v = done;
     }
     if (__any_sync(0xFFFFFFFFu, expired)) l0 = l1 = __uint_as_float(0x7FC00000u);      // NaN: visible, not silent
     l0 += __shfl_xor_sync(0xFFFFFFFFu, l0, 1);
@@ -493,7 +541,7 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       if (t == 0) {
         w[kHeadDim] = half ? m1 : m0;
         w[kHeadDim + 1] = half ? l1 : l0;
-        w[kHeadDim + 2] = (half ? u1 : u0) - 15.f;
+        w[kHeadDim + 2] = (half ? u1 : u0) - 8.f;
       }
     }
     __syncthreads();
@@ -529,8 +577,8 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     if (!dealt) return;
     at += j1 - j0;
     if (at >= end) return;
-    while (at - before >= (int64_t)blocks_of(p, b) * p.heads_k) {      // the next sequence that has a block
-      before += (int64_t)blocks_of(p, b) * p.heads_k;
+    while (at - before >= (uint32_t)(blocks_of(p, b) * p.heads_k)) {      // the next sequence that has a block
+      before += blocks_of(p, b) * p.heads_k;
       ++b;
     }
     tc::fence_proxy_async_smem();
@@ -543,12 +591,12 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 template <int kSplitWarps>
 __global__ void __launch_bounds__(256) q8_combine_kernel(const Q8DecodeParams p, int split_grid) {
   __shared__ float4 sums[8][32];
-  __shared__ float stats[8][3];
+  __shared__ float4 stats[8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t pair = blockIdx.y;
   const int b = (int)(pair / p.heads_k), h = (int)(pair % p.heads_k);
   const int r = blockIdx.x * (8 / kSplitWarps) + warp / kSplitWarps, w0 = warp % kSplitWarps;
-  int64_t first = pair * p.splits;
+  int64_t first = pair * p.splits;                  // (of partials)
   int n = p.splits;
   bool start_slot = false;                          // the first partial lies in its CTA's second place
   if (p.mask == nullptr) {
@@ -557,11 +605,9 @@ __global__ void __launch_bounds__(256) q8_combine_kernel(const Q8DecodeParams p,
     if (blocks == 0) {
       n = 0;
     } else {
-      int64_t before = 0;
+      uint32_t before = 0;
       for (int b1 = lane; b1 < b; b1 += 32) before += blocks_of(p, b1);
-#pragma unroll
-      for (int d = 16; d >= 1; d >>= 1) before += __shfl_xor_sync(0xFFFFFFFFu, before, d);
-      const int64_t at = before * p.heads_k + (int64_t)h * blocks;
+      const uint32_t at = __reduce_add_sync(0xFFFFFFFFu, before) * p.heads_k + h * blocks;
       first = deal.cta_of(at);
       n = deal.cta_of(at + blocks - 1) - (int)first + 1;
       if (n == 1) return;                           // one CTA had all of it and wrote the result
@@ -572,31 +618,33 @@ __global__ void __launch_bounds__(256) q8_combine_kernel(const Q8DecodeParams p,
     const int64_t slot = start_slot ? 2 * (first + s) + (s == 0) : first + s;
     return p.partial + (slot * kGroup + r) * kPartialFloats;
   };
-  float m = -INFINITY, unit = -INFINITY;
-  for (int s = lane; s < n; s += 32) {
-    const float4 st = *reinterpret_cast<const float4*>(partial(s) + kHeadDim);
-    m = fmaxf(m, st.x);
-    unit = fmaxf(unit, st.z);
-  }
-#pragma unroll
-  for (int d = 16; d >= 1; d >>= 1) {
-    m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
-    unit = fmaxf(unit, __shfl_xor_sync(0xFFFFFFFFu, unit, d));
-  }
-  float acc[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
+  float m = -INFINITY, unit = -INFINITY, acc[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
   constexpr int kBatch = 8;
   for (int s0 = w0; s0 < n; s0 += kBatch * kSplitWarps) {
     float4 v[kBatch], st[kBatch];
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
+      v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      st[k] = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
       if (s0 + k * kSplitWarps >= n) continue;
       const float* src = partial(s0 + k * kSplitWarps);
       v[k] = *reinterpret_cast<const float4*>(src + 4 * lane);
       st[k] = *reinterpret_cast<const float4*>(src + kHeadDim);
     }
+    float top = m, top_unit = unit;
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      if (s0 + k * kSplitWarps >= n) continue;
+      top = fmaxf(top, st[k].x);
+      top_unit = fmaxf(top_unit, st[k].z);
+    }
+    l *= join_weight(m, top);
+    const float f0 = join_weight(unit, top_unit);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] *= f0;
+    m = top;
+    unit = top_unit;
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
       l += join_weight(st[k].x, m) * st[k].y;
       const float f = join_weight(st[k].z, unit);
       acc[0] += f * v[k].x;
@@ -607,17 +655,27 @@ __global__ void __launch_bounds__(256) q8_combine_kernel(const Q8DecodeParams p,
   }
   if (kSplitWarps > 1) {
     sums[warp][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-    if (lane == 0) stats[warp][0] = l;
+    if (lane == 0) stats[warp] = make_float4(m, l, unit, 0.f);
     __syncthreads();
     if (w0 != 0) return;
 #pragma unroll
     for (int w = 1; w < kSplitWarps; ++w) {
-      const float4 v = sums[warp + w][lane];
-      acc[0] += v.x;
-      acc[1] += v.y;
-      acc[2] += v.z;
-      acc[3] += v.w;
-      l += stats[warp + w][0];
+      m = fmaxf(m, stats[warp + w].x);
+      unit = fmaxf(unit, stats[warp + w].z);
+    }
+    l *= join_weight(stats[warp].x, m);
+    const float f0 = join_weight(stats[warp].z, unit);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] *= f0;
+#pragma unroll
+    for (int w = 1; w < kSplitWarps; ++w) {
+      const float4 v = sums[warp + w][lane], st = stats[warp + w];
+      l += join_weight(st.x, m) * st.y;
+      const float f = join_weight(st.z, unit);
+      acc[0] += f * v.x;
+      acc[1] += f * v.y;
+      acc[2] += f * v.z;
+      acc[3] += f * v.w;
     }
   }
   store_out(p, pair * kGroup + r, 4 * lane, acc, m, l, unit);
@@ -630,9 +688,9 @@ using namespace ifv2;
 
 extern "C" int64_t ifv2_q8_decode_workspace_bytes(int batch, int heads_q, int head_dim) {
   if (batch < 0 || heads_q < 0 || head_dim != kHeadDim) return 0;
-  // masks: every split of every (sequence, KV head), at most kDealtCtas of them or one each; no mask: two per CTA
+  // masks: every split of every (sequence, KV head), at most kMaxCtas of them or one each; no mask: two per CTA
   const int64_t pairs = (int64_t)batch * (heads_q / kGroup);
-  const int64_t parts = pairs > 2 * kDealtCtas ? pairs : 2 * kDealtCtas;
+  const int64_t parts = pairs > 2 * kMaxCtas ? pairs : 2 * kMaxCtas;
   return parts * kGroup * kPartialFloats * 4;
 }
 
@@ -701,9 +759,10 @@ extern "C" int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void*
   p.out = static_cast<__nv_bfloat16*>(out);
   p.lse = lse;
   const int64_t pairs = (int64_t)batch * heads_k;
+  const int ctas = (rotate ? kResidentRotate : kResident) * kNumSMs;      // one wave
   p.splits = 1;
   if (mask != nullptr) {
-    const int64_t most = kDealtCtas / pairs;
+    const int64_t most = ctas / pairs;
     p.splits = most < 1 ? 1 : most > kMaxSplits ? kMaxSplits : (int)most;
   }
   cudaStream_t st = (cudaStream_t)stream;
@@ -733,9 +792,9 @@ extern "C" int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void*
   int64_t grid = pairs * p.splits;
   if (mask == nullptr) {
     grid = pairs * ceil_div64(capacity, kBlockN);
-    if (grid > kDealtCtas) grid = kDealtCtas;
+    IFV2_REQUIRE(grid <= INT32_MAX, IFV2_ERR_TOO_LARGE, "q8_decode: more than 2^31-1 blocks of 64 keys");
+    if (grid > ctas) grid = ctas;
   }
-  IFV2_REQUIRE(grid <= INT32_MAX, IFV2_ERR_TOO_LARGE, "q8_decode: too many sequences x heads");
   kernel<<<(unsigned)grid, kThreads, kSmemBytes, st>>>(map_k, map_v, p);
   rc = check_launch("q8_split");
   if (rc) return rc;
