@@ -24,6 +24,12 @@ __device__ __forceinline__ float mul_exact(float a, float b) {
   return r;
 }
 
+__device__ __forceinline__ uint64_t mul_exact2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // Scale byte of a row whose largest |x| has the bit pattern `amax`.
 template <int kCode>
 __device__ __forceinline__ int scale_byte(uint32_t amax) {

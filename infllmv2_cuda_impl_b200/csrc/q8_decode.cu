@@ -210,9 +210,9 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   __shared__ uint64_t bars[kWarps][kSlots];
-  __shared__ __align__(16) float2 factors[kWarps][kUnit];        // of the unit at work: scale of a key, exponent of its value
-  __shared__ __align__(16) __half qs[kGroup][kHeadDim + 8];
-  __shared__ __align__(16) __half q_lo[kRotate ? kGroup : 1][kHeadDim + 8];
+  __shared__ __align__(16) float factors[kWarps][2][kUnit];      // of the unit at work: scales of the keys, exponents of the values
+  // the query as A fragments: [high and low part][16-feature chunk][lane]
+  __shared__ uint4 q_frag[kRotate ? 2 : 1][kHeadDim / 16][32];
   __shared__ float q_factor[kGroup];               // 2^x that undoes a row's scaling
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   uint8_t* tiles = smem + warp * kSlots * kTileBytes;
@@ -226,6 +226,13 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     tc::fence_barrier_init();
   }
   __syncwarp();
+  // a lane's places in a tile: 16-byte chunk c of row r lies at chunk c ^ (r & 7)
+  const uint32_t tiles32 = tc::smem_u32(tiles);
+  uint32_t k_lane[2], v_lane[4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) k_lane[i] = (lane & 7) * kHeadDim + (((i * 4 + (lane >> 3)) ^ (lane & 7)) << 4);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v_lane[i] = (lane & 15) * kHeadDim + (((i * 2 + (lane >> 4)) ^ (lane & 7)) << 4);
   uint32_t phases = 0;                             // bit i: parity of the next completion of slot i
   bool expired = false;                            // a bounded wait ran out: the result is poisoned
 
@@ -273,29 +280,43 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       }
       return -1;
     };
-    // where the key of this lane is (-1: nowhere), and its scale bytes (K low, V high)
-    auto locate = [&](int key0, int& row) -> uint32_t {
+    // where the key of this lane is (-1: nowhere), and its scale bytes.  (The cache has fewer than 2^31 rows.)
+    int slot0 = 0;                                 // row of the head's first position, where slots are sequences
+    if (p.place.block_table == nullptr) {
+      const int slot = p.place.batch_idx ? __ldg(p.place.batch_idx + b) : b;
+      slot0 = slot >= 0 && slot < p.place.slots ? (slot * p.place.heads + h) * p.place.length : -1;
+    }
+    // The bytes are not touched before the unit's turn: whatever uses them waits for their loads.
+    auto locate = [&](int key0, int& row, uint32_t& kb, uint32_t& vb) {
       row = -1;
-      uint32_t kb = 0, vb = kNanByte;              // (a page that the cache does not have: NaN)
-      if (key0 + lane < len) {
-        const int64_t row0 = p.place.row0(b, key0 + lane);
-        if (row0 >= 0) {
-          row = (int)p.place.row(row0, h);
+      kb = 0;
+      vb = kNanByte;                               // (a page that the cache does not have: NaN)
+      const int key = key0 + lane;
+      if (key < len) {
+        if (p.place.block_table != nullptr) {
+          const int page = (int)((uint32_t)key / (uint32_t)p.place.length);
+          const int slot = __ldg(p.place.block_table + (int64_t)b * p.place.bt_stride + page);
+          if (slot >= 0 && slot < p.place.slots) row = (slot * p.place.heads + h) * p.place.length + key - page * p.place.length;
+        } else if (slot0 >= 0) {
+          row = slot0 + key;
+        }
+        if (row >= 0) {
           kb = __ldg(p.k_scale + row);
           vb = __ldg(p.v_scale + row);
         }
       }
-      return kb | vb << 8;
     };
-    // starts the copy of the tile whose keys' rows the lanes hold into slot i
+    // starts the copy of the tile whose keys' rows the lanes hold into slot i, which the warp is done reading (what is
+    // written there by ordinary stores, the zeros of a tail and the join, is fenced off at the end of a segment)
     auto fetch = [&](const CUtensorMap& map, int i, int row) {
-      tc::fence_proxy_async_smem();                // the slot was read, and its tail zeroed, by ordinary accesses
+      const int row16 = kBox == 16 ? __shfl_sync(0xFFFFFFFFu, row, 16) : -1;
       __syncwarp();
-      const bool boxed = lane % kBox == 0 && row >= 0;
-      const int boxes = __popc(__ballot_sync(0xFFFFFFFFu, boxed));
-      if (lane == 0) tc::mbar_expect_tx(&bars[warp][i], boxes * kBox * kHeadDim);
-      __syncwarp();
-      if (boxed) tc::tma_load_2d(tiles + i * kTileBytes + lane * kHeadDim, &map, &bars[warp][i], 0, row);
+      if (lane == 0) {
+        uint64_t* bar = &bars[warp][i];
+        tc::mbar_expect_tx(bar, ((row >= 0) + (row16 >= 0)) * kBox * kHeadDim);
+        if (row >= 0) tc::tma_load_2d(tiles + i * kTileBytes, &map, bar, 0, row);
+        if (row16 >= 0) tc::tma_load_2d(tiles + i * kTileBytes + 16 * kHeadDim, &map, bar, 0, row16);
+      }
     };
     auto arrived = [&](int i) {
       if (!tc::mbar_try_wait(&bars[warp][i], (phases >> i) & 1u)) {
@@ -312,14 +333,14 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 
     // unit at work and the next one: first keys, rows, scale bytes; slots of K, V and the next K
     int key0 = next_key(), key1 = -1, row, row1 = -1, slot_k = 0, slot_v = 1, slot_n = 2;
-    uint32_t by = 0, by1 = 0;
+    uint32_t kb = 0, vb = 0, kb1 = 0, vb1 = 0;
     if (key0 >= 0) {
-      by = locate(key0, row);
+      locate(key0, row, kb, vb);
       fetch(map_k, slot_k, row);
       fetch(map_v, slot_v, row);
       key1 = next_key();
       if (key1 >= 0) {
-        by1 = locate(key1, row1);
+        locate(key1, row1, kb1, vb1);
         fetch(map_k, slot_n, row1);
       }
     }
@@ -337,22 +358,17 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       for (int u = 0; u < 4; u += 2) {
         const float y0 = mul_exact(x[u], f), y1 = mul_exact(x[u + 1], f);
         const __half2 y = __floats2half2_rn(y0, y1);
-        *reinterpret_cast<__half2*>(&qs[i][4 * lane + u]) = y;
+        // features 4 lane + u, + 1 of row i: word (i / 8) + u of fragment lane 4 (i % 8) + lane % 4
+        const int at = (i & 7) * 4 + (lane & 3), word = (i >> 3) + u;
+        reinterpret_cast<__half2*>(&q_frag[0][lane >> 2][at])[word] = y;
         if (kRotate) {
           const float2 z = __half22float2(y);
-          *reinterpret_cast<__half2*>(&q_lo[i][4 * lane + u]) = __floats2half2_rn(y0 - z.x, y1 - z.y);
+          reinterpret_cast<__half2*>(&q_frag[kRotate ? 1 : 0][lane >> 2][at])[word] = __floats2half2_rn(y0 - z.x, y1 - z.y);
         }
       }
       if (lane == 0) q_factor[i] = __uint_as_float((uint32_t)(e - 14) << 23);
     }
     __syncthreads();
-    auto q_fragment = [&](uint32_t (&f)[4], const __half (*rows)[kHeadDim + 8], int ks) {
-      const uint2 a = *reinterpret_cast<const uint2*>(&rows[g][16 * ks + 4 * t]), c = *reinterpret_cast<const uint2*>(&rows[g + 8][16 * ks + 4 * t]);
-      f[0] = a.x;
-      f[1] = c.x;
-      f[2] = a.y;
-      f[3] = c.y;
-    };
     const float c0 = q_factor[g] * p.scale_log2, c1 = q_factor[g + 8] * p.scale_log2;
 
     float o[16][4];
@@ -363,11 +379,10 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, u0 = -INFINITY, u1 = -INFINITY;
 
     while (key0 >= 0) {
-      const uint8_t* kt = tiles + slot_k * kTileBytes;
-      uint8_t* vt = tiles + slot_v * kTileBytes;
+      const uint32_t kt = tiles32 + slot_k * kTileBytes, vt = tiles32 + slot_v * kTileBytes;
       arrived(slot_k);
-      const int kb = by & 0xFF, vb = by >> 8;
-      factors[warp][lane] = make_float2(scale_value(kb), vb == kNanByte ? __uint_as_float(0x7FC00000u) : (float)(vb - 127));
+      factors[warp][0][lane] = scale_value(kb);
+      factors[warp][1][lane] = vb == kNanByte ? __uint_as_float(0x7FC00000u) : (float)((int)vb - 127);
       __syncwarp();
 
       // ---- S = Q . K^T (16 x 32)
@@ -378,15 +393,11 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       for (int kp = 0; kp < 2; ++kp) {
         uint32_t w[kUnit / 8][4];
 #pragma unroll
-        for (int nt = 0; nt < kUnit / 8; ++nt) {
-          const int row = nt * 8 + (lane & 7);
-          mmasync::ldmatrix_x4(w[nt], kt + row * kHeadDim + (((kp * 4 + (lane >> 3)) ^ (row & 7)) << 4));
-        }
+        for (int nt = 0; nt < kUnit / 8; ++nt) mmasync::ldmatrix_x4(w[nt], kt + k_lane[kp] + nt * 8 * kHeadDim);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          uint32_t qh[4], ql[4];
-          q_fragment(qh, qs, kp * 4 + u);
-          if (kRotate) q_fragment(ql, q_lo, kp * 4 + u);
+          const uint4 hi4 = q_frag[0][kp * 4 + u][lane], lo4 = q_frag[kRotate ? 1 : 0][kp * 4 + u][lane];
+          const uint32_t qh[4] = {hi4.x, hi4.y, hi4.z, hi4.w}, ql[4] = {lo4.x, lo4.y, lo4.z, lo4.w};
 #pragma unroll
           for (int nt = 0; nt < kUnit / 8; ++nt) {
             uint32_t f0, f1;
@@ -401,44 +412,45 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 
       // ---- weights against reference maxima that move only when a weight would pass 2^15: the sum l against m, the
       //      weights of the values against M - 8 (see the file's head).  A unit whose weights pass is done again.
-      float ev[kUnit / 8][2];                      // exponents of the values of keys 8 nt + 2t, + 1
+      uint64_t ev[kUnit / 8], sp[kUnit / 8][2];    // pairs for keys 8 nt + 2t, + 1: exponents of values, q . K 2^e of two rows
 #pragma unroll
       for (int nt = 0; nt < kUnit / 8; ++nt) {
-        const float4 f = *reinterpret_cast<const float4*>(&factors[warp][nt * 8 + 2 * t]);
-        ev[nt][0] = f.y;
-        ev[nt][1] = f.w;
-        s[nt][0] = mul_exact(s[nt][0], f.x);
-        s[nt][1] = mul_exact(s[nt][1], f.z);
-        s[nt][2] = mul_exact(s[nt][2], f.x);
-        s[nt][3] = mul_exact(s[nt][3], f.z);
+        const uint64_t ks = *reinterpret_cast<const uint64_t*>(&factors[warp][0][nt * 8 + 2 * t]);
+        ev[nt] = *reinterpret_cast<const uint64_t*>(&factors[warp][1][nt * 8 + 2 * t]);
+        sp[nt][0] = mul_exact2(tc::pack_f32x2(s[nt][0], s[nt][1]), ks);
+        sp[nt][1] = mul_exact2(tc::pack_f32x2(s[nt][2], s[nt][3]), ks);
       }
-      float sum0, sum1;
+      float sum[2];
       uint32_t pf[kUnit / 16][4];                  // weights as A fragments of the second product
       auto weigh = [&](auto tail) -> bool {
         constexpr bool kTail = decltype(tail)::value;
-        const float n0 = m0 == -INFINITY ? 0.f : -m0, n1 = m1 == -INFINITY ? 0.f : -m1;
-        const float w0 = u0 == -INFINITY ? 0.f : 8.f - u0, w1 = u1 == -INFINITY ? 0.f : 8.f - u1;
-        float top = -INFINITY;
-        sum0 = sum1 = 0.f;
+        __half2 top;
 #pragma unroll
-        for (int nt = 0; nt < kUnit / 8; ++nt) {
-          float x[4];
+        for (int r = 0; r < 2; ++r) {
+          const float c = r ? c1 : c0, m = r ? m1 : m0, u = r ? u1 : u0;
+          const float n = m == -INFINITY ? 0.f : -m, w = u == -INFINITY ? 0.f : 8.f - u;
+          const uint64_t cc = tc::pack_f32x2(c, c), nn = tc::pack_f32x2(n, n), ww = tc::pack_f32x2(w, w);
+          uint64_t total = 0;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const bool in = !kTail || key0 + nt * 8 + 2 * t + e < len;
-            const float a0 = fmaf(s[nt][e], c0, n0), a1 = fmaf(s[nt][2 + e], c1, n1);
-            sum0 += exp2f(in ? a0 : -INFINITY);
-            sum1 += exp2f(in ? a1 : -INFINITY);
-            x[e] = fmaf(s[nt][e], c0, w0) + ev[nt][e];
-            x[2 + e] = fmaf(s[nt][2 + e], c1, w1) + ev[nt][e];
-            if (!in) x[e] = x[2 + e] = -INFINITY;
-            top = fmaxf(top, fmaxf(x[e], x[2 + e]));
+          for (int nt = 0; nt < kUnit / 8; ++nt) {
+            float a0, a1, x0, x1;
+            tc::unpack_f32x2(tc::fma_f32x2(sp[nt][r], cc, nn), a0, a1);
+            tc::unpack_f32x2(tc::add_f32x2(tc::fma_f32x2(sp[nt][r], cc, ww), ev[nt]), x0, x1);
+            if (kTail) {
+              if (key0 + nt * 8 + 2 * t >= len) a0 = x0 = -INFINITY;
+              if (key0 + nt * 8 + 2 * t + 1 >= len) a1 = x1 = -INFINITY;
+            }
+            total = tc::add_f32x2(total, tc::pack_f32x2(exp2f(a0), exp2f(a1)));
+            const __half2 y = __floats2half2_rn(exp2f(x0), exp2f(x1));
+            top = r == 0 && nt == 0 ? y : __hmax2(top, y);
+            pf[nt >> 1][(nt & 1) * 2 + r] = *reinterpret_cast<const uint32_t*>(&y);
           }
-          const __half2 y0 = __floats2half2_rn(exp2f(x[0]), exp2f(x[1])), y1 = __floats2half2_rn(exp2f(x[2]), exp2f(x[3]));
-          pf[nt >> 1][(nt & 1) * 2] = *reinterpret_cast<const uint32_t*>(&y0);
-          pf[nt >> 1][(nt & 1) * 2 + 1] = *reinterpret_cast<const uint32_t*>(&y1);
+          float a0, a1;
+          tc::unpack_f32x2(total, a0, a1);
+          sum[r] = a0 + a1;
         }
-        return top > 15.f || sum0 > 0x1p40f || sum1 > 0x1p40f;
+        const float2 y = __half22float2(top);
+        return fmaxf(y.x, y.y) > 0x1p15f || fmaxf(sum[0], sum[1]) > 0x1p40f;
       };
       bool again = fresh;
       if (!fresh) again = key0 + kUnit > len ? weigh(std::true_type{}) : weigh(std::false_type{});
@@ -449,11 +461,14 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             if (key0 + nt * 8 + 2 * t + e >= len) continue;
-            const float a0 = s[nt][e] * c0, a1 = s[nt][2 + e] * c1;
-            mx0 = fmaxf(mx0, a0);
-            mx1 = fmaxf(mx1, a1);
-            mu0 = fmaxf(mu0, a0 + ev[nt][e]);
-            mu1 = fmaxf(mu1, a1 + ev[nt][e]);
+            float a[2], b2[2], ex[2];
+            tc::unpack_f32x2(sp[nt][0], a[0], a[1]);
+            tc::unpack_f32x2(sp[nt][1], b2[0], b2[1]);
+            tc::unpack_f32x2(ev[nt], ex[0], ex[1]);
+            mx0 = fmaxf(mx0, a[e] * c0);
+            mx1 = fmaxf(mx1, b2[e] * c1);
+            mu0 = fmaxf(mu0, a[e] * c0 + ex[e]);
+            mu1 = fmaxf(mu1, b2[e] * c1 + ex[e]);
           }
         }
 #pragma unroll
@@ -480,15 +495,15 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         fresh = false;
         weigh(std::true_type{});
       }
-      l0 += sum0;                                  // per lane; added up over the quad at the end
-      l1 += sum1;
+      l0 += sum[0];                                // per lane; added up over the quad at the end
+      l1 += sum[1];
 
       // ---- O += P . V (16 x 128); rows past the last key have weight 0, but their bytes can be NaN codes
       arrived(slot_v);
       __syncwarp();
       if (key0 + kUnit > len) {
         for (int k = lane; k < kUnit * 8; k += 32)
-          if (key0 + (k >> 3) >= len) *reinterpret_cast<uint4*>(vt + k * 16) = make_uint4(0u, 0u, 0u, 0u);
+          if (key0 + (k >> 3) >= len) *reinterpret_cast<uint4*>(tiles + slot_v * kTileBytes + k * 16) = make_uint4(0u, 0u, 0u, 0u);
         __syncwarp();
       }
 #pragma unroll
@@ -496,8 +511,7 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 #pragma unroll
         for (int np = 0; np < 4; ++np) {           // two chunks of 16 features
           uint32_t w[4];
-          const int row = kk * 16 + (lane & 15), chunk = np * 2 + (lane >> 4);
-          mmasync::ldmatrix_x4_trans(w, vt + row * kHeadDim + ((chunk ^ (row & 7)) << 4));
+          mmasync::ldmatrix_x4_trans(w, vt + v_lane[np] + kk * 16 * kHeadDim);
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             uint32_t e0, e1, d0, d1;
@@ -509,11 +523,12 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         }
       }
       key0 = key1;
-      by = by1;
+      kb = kb1;
+      vb = vb1;
       if (key1 >= 0) {
         key1 = next_key();
         if (key1 >= 0) {
-          by1 = locate(key1, row1);
+          locate(key1, row1, kb1, vb1);
           fetch(map_k, slot_v, row1);
         }
       }
