@@ -77,25 +77,58 @@ __device__ __forceinline__ int keys_of(const Q8DecodeParams& p, int b) {
   return len < 0 ? 0 : (int)min(len + p.new_tokens, p.capacity);
 }
 
-// Four consecutive features (4 lane ..) of row `src`, rotated for token t.
-__device__ __forceinline__ void load_rotated(float (&x)[4], const __nv_bfloat16* src, const RotaryParams& r, bool rotate,
-                                             int64_t t, int lane) {
-  auto at = [&](int i) { return __bfloat162float(ldg16(src + i)); };
-  const int half = r.dim / 2;
+// Rows of a token in a warp, features 4 lane .. 4 lane + 3 in each lane: the lane's angles, loaded once for all rows, and
+// a row's own and partner features as they come from memory.
+struct Angles {
+  float c[4], s[4];
+  int mate;                        // where the partner's four features are (halves), 0: in the lane itself (neighbours)
+  bool on, second;                 // the lane's features turn; they are the second of their pairs (halves)
+  __device__ __forceinline__ void load(const RotaryParams& r, int64_t t, int lane) {
+    const int half = r.dim / 2, f = 4 * lane;
+    on = f < r.dim;
+    second = !r.interleaved && f >= half;
+    mate = r.interleaved || !on ? 0 : second ? -half : half;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int f = 4 * lane + i;
-    x[i] = at(f);
-    if (!rotate || f >= r.dim) continue;
-    const int pair = r.interleaved ? f / 2 : f % half;
-    const bool second = r.interleaved ? f & 1 : f >= half;
-    const int other = r.interleaved ? f ^ 1 : second ? f - half : f + half;
-    float x0 = second ? at(other) : x[i], x1 = second ? x[i] : at(other);
-    const int64_t e = r.table_row(t, pair) * half + pair;
-    rotate2(x0, x1, __ldg(r.cos_t + e), __ldg(r.sin_t + e));
-    x[i] = second ? x1 : x0;
+    for (int i = 0; i < 4; ++i) {
+      if (!on || (r.interleaved && i >= 2)) continue;
+      const int pair = r.interleaved ? 2 * lane + i : second ? f - half + i : f + i;
+      const int64_t e = r.table_row(t, pair) * half + pair;
+      c[i] = __ldg(r.cos_t + e);
+      s[i] = __ldg(r.sin_t + e);
+    }
   }
-}
+};
+struct RowPart {
+  uint2 own, mate;
+  __device__ __forceinline__ void load(const __nv_bfloat16* row, int lane, int mate_at) {
+    own = __ldg(reinterpret_cast<const uint2*>(row) + lane);
+    if (mate_at != 0) mate = __ldg(reinterpret_cast<const uint2*>(row + 4 * lane + mate_at));
+  }
+  static __device__ __forceinline__ void widen(float (&x)[4], const uint2& v) {
+    x[0] = __uint_as_float(v.x << 16);
+    x[1] = __uint_as_float(v.x & 0xFFFF0000u);
+    x[2] = __uint_as_float(v.y << 16);
+    x[3] = __uint_as_float(v.y & 0xFFFF0000u);
+  }
+  __device__ __forceinline__ void plain(float (&x)[4]) const { widen(x, own); }
+  __device__ __forceinline__ void turned(float (&x)[4], const Angles& a) const {
+    widen(x, own);
+    if (!a.on) return;
+    if (a.mate == 0) {
+      rotate2(x[0], x[1], a.c[0], a.s[0]);
+      rotate2(x[2], x[3], a.c[1], a.s[1]);
+      return;
+    }
+    float y[4];
+    widen(y, mate);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float x0 = a.second ? y[i] : x[i], x1 = a.second ? x[i] : y[i];
+      rotate2(x0, x1, a.c[i], a.s[i]);
+      x[i] = a.second ? x1 : x0;
+    }
+  }
+};
 
 // One CTA per (sequence, KV head): block lists -> mask row; the new key (rotated) and value -> their row.
 template <int kCode>
@@ -117,8 +150,14 @@ __global__ void __launch_bounds__(kThreads) q8_prepare_kernel(const Q8PreparePar
     if (row0 >= 0) {
       const int64_t row = p.place.row(row0, h);
       const bool is_v = tid >= 32;
+      Angles angles;
+      angles.mate = 0;
+      angles.on = false;
+      if (p.rotate && !is_v) angles.load(p.rotary, b, lane);
+      RowPart part;
+      part.load((is_v ? a.v_new : a.k_new) + pair * kHeadDim, lane, angles.mate);
       float x[4];
-      load_rotated(x, (is_v ? a.v_new : a.k_new) + pair * kHeadDim, p.rotary, p.rotate && !is_v, b, lane);
+      part.turned(x, angles);
       store_row<kCode>(x, (is_v ? a.v_codes : a.k_codes) + row * kHeadDim, (is_v ? a.v_scale : a.k_scale) + row, lane);
     }
   }
@@ -269,6 +308,14 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     }
     const int64_t pair = (int64_t)b * p.heads_k + h;
 
+    // the warp's rows of the query, on their way while the first tiles are asked for
+    Angles angles;
+    angles.mate = 0;
+    if (kRotate) angles.load(p.rotary, b, lane);
+    RowPart q_part[kGroup / kWarps];
+#pragma unroll
+    for (int i = 0; i < kGroup / kWarps; ++i) q_part[i].load(p.q + (pair * kGroup + warp + kWarps * i) * kHeadDim, lane, angles.mate);
+
     // this warp's units: half (warp & 1) of blocks j0 + (warp >> 1), + 2, ...
     int j = j0 + (warp >> 1), lookups = 0;
     auto next_key = [&]() -> int {                 // first key of the next unit, or -1
@@ -346,9 +393,12 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     }
 
     // the query rows, rotated, as fp16 with a power of two taken out
-    for (int i = warp; i < kGroup; i += kWarps) {
+#pragma unroll
+    for (int n4 = 0; n4 < kGroup / kWarps; ++n4) {
+      const int i = warp + kWarps * n4;
       float x[4];
-      load_rotated(x, p.q + (pair * kGroup + i) * kHeadDim, p.rotary, kRotate, b, lane);
+      if (kRotate) q_part[n4].turned(x, angles);
+      else q_part[n4].plain(x);
       uint32_t amax = 0;
 #pragma unroll
       for (int u = 0; u < 4; ++u) amax = max(amax, abs_bits(x[u]));
