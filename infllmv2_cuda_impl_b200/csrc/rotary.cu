@@ -40,7 +40,11 @@ struct RotaryKernelParams {
   int back;
 };
 
-__global__ void __launch_bounds__(kThreads) rotary_axes_kernel(const RotaryKernelParams p) {
+// A warp takes up to 36 rows of one token, four at a time.  Four CTAs per SM with one row per thread under way: two or
+// three rows loaded ahead cost the registers of a CTA and were slower (32768 tokens of 34 heads: 98 us, 92 % of the copy
+// bandwidth; 110 with two rows, 127 with three, 103 with five CTAs, whose registers spill, 108 with 18 rows per warp).
+template <bool kInterleaved>
+__global__ void __launch_bounds__(kThreads, 4) rotary_axes_kernel(const RotaryKernelParams p) {
   const int64_t w = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 5;
   const int64_t t = w / p.chunks;
   if (t >= p.tokens) return;
@@ -48,50 +52,76 @@ __global__ void __launch_bounds__(kThreads) rotary_axes_kernel(const RotaryKerne
   const int lane = threadIdx.x & 31, l = lane % kLanes;
   const bool turn = 8 * l < p.r.dim / 2;
   // vectors of the thread's 16 features: a neighbouring pair of vectors, or one in each half
-  const int a = !turn || p.r.interleaved ? 2 * l : l, b = !turn || p.r.interleaved ? 2 * l + 1 : l + p.r.dim / 16;
+  const int a = !turn || kInterleaved ? 2 * l : l, b = !turn || kInterleaved ? 2 * l + 1 : l + p.r.dim / 16;
+  const uint4 *src_q = p.src[0] + t * p.token_stride[0], *src_k = p.src[1] + t * p.token_stride[1];
+  uint4 *dst_q = p.dst[0] + t * p.heads[0] * (kHeadDim / 8), *dst_k = p.dst[1] + t * p.heads[1] * (kHeadDim / 8);
+  auto load = [&](int row, uint4& va, uint4& vb) {
+    const int h = row - p.heads[0];
+    const uint4* s = h < 0 ? src_q + row * p.head_stride[0] : src_k + h * p.head_stride[1];
+    va = __ldg(s + a);
+    vb = __ldg(s + b);
+  };
+  // the first row's loads and the angles, which wait for the positions, travel together
+  int row = first + lane / kLanes;
+  uint4 va, vb;
+  if (row < last) load(row, va, vb);
   float c[8], s[8];
   if (turn) {
+    const uint32_t axes = (p.r.axis_map[l >> 1] >> (16 * (l & 1))) & 0xFFFFu;
+    if (axes == (axes & 3) * 0x5555u) {          // all eight pairs on one axis: they are neighbours in the tables
+      const int64_t at = p.r.table_row(t, 8 * l) * (p.r.dim / 2) + 8 * l;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int64_t at = p.r.table_row(t, 8 * l + i) * (p.r.dim / 2) + 8 * l + i;
-      c[i] = __ldg(p.r.cos_t + at);
-      s[i] = p.back ? -__ldg(p.r.sin_t + at) : __ldg(p.r.sin_t + at);
-    }
-  }
-  for (int row = first + lane / kLanes; row < last; row += kRows) {
-    const int i = row < p.heads[0] ? 0 : 1, h = i ? row - p.heads[0] : row;
-    const uint4* src = p.src[i] + t * p.token_stride[i] + h * p.head_stride[i];
-    uint4* dst = p.dst[i] + (t * p.heads[i] + h) * (kHeadDim / 8);
-    const uint4 va = __ldg(src + a), vb = __ldg(src + b);
-    if (!turn) {
-      dst[a] = va;
-      dst[b] = vb;
-      continue;
-    }
-    uint32_t x[8] = {va.x, va.y, va.z, va.w, vb.x, vb.y, vb.z, vb.w};
-    float lo[8], hi[8];                          // first and second feature of pairs 0 .. 7
+      for (int i = 0; i < 2; ++i) {
+        const float4 fc = __ldg(reinterpret_cast<const float4*>(p.r.cos_t + at) + i);
+        const float4 fs = __ldg(reinterpret_cast<const float4*>(p.r.sin_t + at) + i);
+        c[4 * i] = fc.x; c[4 * i + 1] = fc.y; c[4 * i + 2] = fc.z; c[4 * i + 3] = fc.w;
+        s[4 * i] = fs.x; s[4 * i + 1] = fs.y; s[4 * i + 2] = fs.z; s[4 * i + 3] = fs.w;
+      }
+    } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float f0 = __uint_as_float(x[j] << 16), f1 = __uint_as_float(x[j] & 0xFFFF0000u);
-      if (p.r.interleaved) {
-        lo[j] = f0;
-        hi[j] = f1;
-      } else {                                   // words 0 .. 3: first features of pairs 2j, 2j + 1
-        (j < 4 ? lo : hi)[2 * (j & 3)] = f0;
-        (j < 4 ? lo : hi)[2 * (j & 3) + 1] = f1;
+      for (int i = 0; i < 8; ++i) {
+        const int64_t at = p.r.table_row(t, 8 * l + i) * (p.r.dim / 2) + 8 * l + i;
+        c[i] = __ldg(p.r.cos_t + at);
+        s[i] = __ldg(p.r.sin_t + at);
       }
     }
+    if (p.back) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) rotate2(lo[j], hi[j], c[j], s[j]);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const __nv_bfloat162 v = p.r.interleaved ? __floats2bfloat162_rn(lo[j], hi[j])
-                               : j < 4         ? __floats2bfloat162_rn(lo[2 * (j & 3)], lo[2 * (j & 3) + 1])
-                                               : __floats2bfloat162_rn(hi[2 * (j & 3)], hi[2 * (j & 3) + 1]);
-      x[j] = *reinterpret_cast<const uint32_t*>(&v);
+      for (int i = 0; i < 8; ++i) s[i] = -s[i];
     }
-    dst[a] = make_uint4(x[0], x[1], x[2], x[3]);
-    dst[b] = make_uint4(x[4], x[5], x[6], x[7]);
+  }
+  while (row < last) {
+    uint4* d = row < p.heads[0] ? dst_q + row * (kHeadDim / 8) : dst_k + (row - p.heads[0]) * (kHeadDim / 8);
+    if (turn) {
+      uint32_t x[8] = {va.x, va.y, va.z, va.w, vb.x, vb.y, vb.z, vb.w};
+      float lo[8], hi[8];                        // first and second feature of pairs 0 .. 7
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float f0 = __uint_as_float(x[j] << 16), f1 = __uint_as_float(x[j] & 0xFFFF0000u);
+        if (kInterleaved) {
+          lo[j] = f0;
+          hi[j] = f1;
+        } else {                                 // words 0 .. 3: first features of pairs 2j, 2j + 1
+          (j < 4 ? lo : hi)[2 * (j & 3)] = f0;
+          (j < 4 ? lo : hi)[2 * (j & 3) + 1] = f1;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) rotate2(lo[j], hi[j], c[j], s[j]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const __nv_bfloat162 v = kInterleaved ? __floats2bfloat162_rn(lo[j], hi[j])
+                                 : j < 4      ? __floats2bfloat162_rn(lo[2 * (j & 3)], lo[2 * (j & 3) + 1])
+                                              : __floats2bfloat162_rn(hi[2 * (j & 3)], hi[2 * (j & 3) + 1]);
+        x[j] = *reinterpret_cast<const uint32_t*>(&v);
+      }
+      va = make_uint4(x[0], x[1], x[2], x[3]);
+      vb = make_uint4(x[4], x[5], x[6], x[7]);
+    }
+    d[a] = va;
+    d[b] = vb;
+    row += kRows;
+    if (row < last) load(row, va, vb);
   }
 }
 
@@ -130,11 +160,15 @@ extern "C" int ifv2_rotary_axes(const void* q, const void* k, void* q_out, void*
   p.heads[0] = heads_q;
   p.heads[1] = heads_k;
   p.tokens = tokens;
-  p.chunks = ceil_div(heads_q + heads_k, 16);
-  p.chunk = ceil_div(heads_q + heads_k, p.chunks);
+  // rows per warp: many where there are many tokens, so that a token's angles are fetched by few warps; few where there
+  // are few, so that all SMs have work (64 tokens of 34 heads in a graph: 2.3 us with 4 rows, 2.7 with 12)
+  const int rows = heads_q + heads_k;
+  p.chunks = ceil_div(rows, tokens >= kNumSMs * 16 ? 36 : tokens >= kNumSMs ? 12 : 4);
+  p.chunk = ceil_div(rows, p.chunks);
   p.back = backward ? 1 : 0;
   const int64_t blocks = ceil_div64(tokens * p.chunks, kThreads / 32);
   IFV2_REQUIRE(blocks <= INT32_MAX, IFV2_ERR_TOO_LARGE, "rotary_axes: too many tokens x heads");
-  rotary_axes_kernel<<<(unsigned)blocks, kThreads, 0, (cudaStream_t)stream>>>(p);
+  if (interleaved) rotary_axes_kernel<true><<<(unsigned)blocks, kThreads, 0, (cudaStream_t)stream>>>(p);
+  else rotary_axes_kernel<false><<<(unsigned)blocks, kThreads, 0, (cudaStream_t)stream>>>(p);
   return check_launch("rotary_axes");
 }

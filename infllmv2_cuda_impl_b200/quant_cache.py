@@ -32,37 +32,38 @@ def q8_cache(slots: int, length: int, heads_k: int, dtype: torch.dtype = torch.f
 
 
 def _check_cache(what, k_cache, v_cache, k_scale, v_scale):
-    """(slots, heads_k, length, code) of a cache."""
+    """(slots, heads_k, length, code, device) of a cache."""
     _require_cuda(k_cache, "k_cache")
-    code = _CODES.get(k_cache.dtype)
-    if code is None or v_cache.dtype != k_cache.dtype or k_scale.dtype != torch.float8_e8m0fnu or v_scale.dtype != torch.float8_e8m0fnu:
+    dtype, shape, dev = k_cache.dtype, k_cache.shape, k_cache.device
+    code = _CODES.get(dtype)
+    if code is None or v_cache.dtype is not dtype or k_scale.dtype is not torch.float8_e8m0fnu or v_scale.dtype is not torch.float8_e8m0fnu:
         raise ValueError(f"{what}: the caches must be float8_e4m3fn or int8, their scales float8_e8m0fnu")
-    if k_cache.dim() != 4 or k_cache.shape[3] != HEAD_DIM or v_cache.shape != k_cache.shape or \
-            k_scale.shape != k_cache.shape[:3] or v_scale.shape != k_cache.shape[:3]:
+    rows = shape[:3]
+    if len(shape) != 4 or shape[3] != HEAD_DIM or v_cache.shape != shape or k_scale.shape != rows or v_scale.shape != rows:
         raise ValueError(f"{what}: caches must be (slots, heads_k, length, {HEAD_DIM}), their scales (slots, heads_k, length)")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
         raise ValueError(f"{what}: caches and scales must be contiguous")
-    dev = k_cache.device
     if v_cache.device != dev or k_scale.device != dev or v_scale.device != dev:
         raise ValueError(f"{what}: caches and scales must be on one device")
-    return k_cache.shape[0], k_cache.shape[1], k_cache.shape[2], code
+    return shape[0], shape[1], shape[2], code, dev
 
 
 def _ints(what, name, t, shape, dev):
     """An int32 tensor of the given shape on dev, contiguous."""
     if t is None:
         return None
-    if t.dtype != torch.int32 or t.device != dev or tuple(t.shape) != shape:
+    if t.dtype is not torch.int32 or t.shape != shape or t.device != dev:
         raise ValueError(f"{what}: {name} must be {shape} int32 on {dev}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _table(what, block_table, batch, dev):
     if block_table is None:
         return None, 0
-    if block_table.dim() != 2 or block_table.shape[1] < 1:
+    shape = block_table.shape
+    if len(shape) != 2 or shape[1] < 1:
         raise ValueError(f"{what}: block_table must be (batch, max_pages) int32")
-    return _ints(what, "block_table", block_table, (batch, block_table.shape[1]), dev), block_table.shape[1]
+    return _ints(what, "block_table", block_table, (batch, shape[1]), dev), shape[1]
 
 
 def _ptr(t):
@@ -70,9 +71,10 @@ def _ptr(t):
 
 
 def _cu(what, cu_seqlens, dev):
-    if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 or cu_seqlens.device != dev:
+    shape = cu_seqlens.shape
+    if cu_seqlens.dtype is not torch.int32 or len(shape) != 1 or shape[0] < 2 or cu_seqlens.device != dev:
         raise ValueError(f"{what}: cu_seqlens must be (batch + 1,) int32 on {dev}")
-    return cu_seqlens.contiguous(), cu_seqlens.numel() - 1
+    return cu_seqlens if cu_seqlens.is_contiguous() else cu_seqlens.contiguous(), shape[0] - 1
 
 
 def cache_fill_q8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -82,13 +84,13 @@ def cache_fill_q8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cac
     into positions start[b], start[b] + 1, ... of its slot or pages, in place.  start (batch,) int32, default 0;
     seqlens_out (batch,) int32, optional: min(start[b] + len_b, capacity).  One launch."""
     what = "cache_fill_q8"
-    slots, hk, length, code = _check_cache(what, k_cache, v_cache, k_scale, v_scale)
-    dev = k_cache.device
-    for name, t in (("k", k), ("v", v)):
-        if t.dtype != torch.bfloat16 or t.dim() != 3 or t.shape != k.shape or t.shape[1:] != (hk, HEAD_DIM) or t.device != dev:
-            raise ValueError(f"{what}: {name} must be (total, {hk}, {HEAD_DIM}) bf16 on {dev}")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise NotImplementedError(f"{what}: nothing flows back from a cache (pass {name}.detach())")
+    slots, hk, length, code, dev = _check_cache(what, k_cache, v_cache, k_scale, v_scale)
+    shape = k.shape
+    if (k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16 or len(shape) != 3 or shape[1] != hk or shape[2] != HEAD_DIM
+            or v.shape != shape or k.device != dev or v.device != dev):
+        raise ValueError(f"{what}: k and v must be (total, {hk}, {HEAD_DIM}) bf16 on {dev}")
+    if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+        raise NotImplementedError(f"{what}: nothing flows back from a cache (pass k.detach() and v.detach())")
     cu_seqlens, batch = _cu(what, cu_seqlens, dev)
     block_table, pages = _table(what, block_table, batch, dev)
     if block_table is None and slots < batch:
@@ -97,11 +99,11 @@ def cache_fill_q8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cac
     if seqlens_out is not None and (_ints(what, "seqlens_out", seqlens_out, (batch,), dev) is not seqlens_out
                                     or (start is not None and seqlens_out.data_ptr() == start.data_ptr())):
         raise ValueError(f"{what}: seqlens_out must be contiguous and not start itself")
-    k, v = _rows(k), _rows(v)
+    (k, k_token, k_head), (v, v_token, v_head) = _rows(k), _rows(v)
     with _on(dev):
-        _lib.call("ifv2_q8_fill", k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+        _lib.call("ifv2_q8_fill", k.data_ptr(), v.data_ptr(), k_token, k_head, v_token, v_head,
                   k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), cu_seqlens.data_ptr(),
-                  _ptr(start), _ptr(block_table), pages, _ptr(seqlens_out), slots, length, code, batch, k.shape[0], hk,
+                  _ptr(start), _ptr(block_table), pages, _ptr(seqlens_out), slots, length, code, batch, shape[0], hk,
                   HEAD_DIM, _stream(dev))
 
 
@@ -112,8 +114,7 @@ def cache_read_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.T
     cu_seqlens[b] rows of every sequence from position start[b] (default 0) on.  total: their number (rows past
     cu_seqlens[-1] are zeros).  What the next chunk of a prompt attends through infllmv2_attn_varlen_func."""
     what = "cache_read_q8"
-    slots, hk, length, code = _check_cache(what, k_cache, v_cache, k_scale, v_scale)
-    dev = k_cache.device
+    slots, hk, length, code, dev = _check_cache(what, k_cache, v_cache, k_scale, v_scale)
     cu_seqlens, batch = _cu(what, cu_seqlens, dev)
     block_table, pages = _table(what, block_table, batch, dev)
     if block_table is None and slots < batch:
@@ -140,8 +141,8 @@ def decode_append_q8(k_new: torch.Tensor, v_new: torch.Tensor, k_cache: torch.Te
     position cache_seqlens[b], completed windows of compressed keys become the mean of the keys as the cache holds
     them (kc_cache (batch, c_capacity, nheads_k, 128) bf16), lengths advance in place.  One launch."""
     what = "decode_append_q8"
-    slots, hk, cap, code = _check_cache(what, k_cache, v_cache, k_scale, v_scale)
-    dev, b = k_cache.device, cache_seqlens.numel()
+    slots, hk, cap, code, dev = _check_cache(what, k_cache, v_cache, k_scale, v_scale)
+    b = cache_seqlens.numel()
     for name, t in (("k_new", k_new), ("v_new", v_new)):
         if t.dtype != torch.bfloat16 or t.device != dev or not t.is_contiguous() or t.numel() != b * hk * HEAD_DIM:
             raise ValueError(f"{what}: {name} must be contiguous ({b}, {hk}, {HEAD_DIM}) bf16 on {dev}")
@@ -184,71 +185,76 @@ def infllmv2_attn_with_kvcache_q8(
     A new token without room in the cache is neither written nor attended.  A sequence without keys gets 0.
     Returns out (batch, 1, nheads, 128) [, softmax_lse (batch, nheads, 1) fp32].  Forward only."""
     what = "infllmv2_attn_with_kvcache_q8"
-    _require_cuda(q, "q")
-    slots, hk, length, code = _check_cache(what, k_cache, v_cache, k_scale, v_scale)
-    dev = q.device
-    if q.dtype != torch.bfloat16 or q.dim() != 4 or q.shape[1:] != (1, hk * GROUP, HEAD_DIM) or k_cache.device != dev:
-        raise ValueError(f"{what}: q must be (batch, 1, {hk * GROUP}, {HEAD_DIM}) bf16 ({GROUP} heads per KV head) on the "
+    slots, hk, length, code, dev = _check_cache(what, k_cache, v_cache, k_scale, v_scale)
+    shape = q.shape
+    batch, heads = shape[0], hk * GROUP
+    if q.dtype is not torch.bfloat16 or shape != (batch, 1, heads, HEAD_DIM) or q.device != dev:
+        raise ValueError(f"{what}: q must be (batch, 1, {heads}, {HEAD_DIM}) bf16 ({GROUP} heads per KV head) on the "
                          "cache's device")
-    batch = q.shape[0]
     if q.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError(f"{what}: forward only, as infllmv2_attn_with_kvcache")
-    if (k is None) != (v is None):
+    k_ptr = v_ptr = None
+    if k is not None and v is not None:
+        new = (batch, 1, hk, HEAD_DIM)
+        if (k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16 or k.shape != new or v.shape != new
+                or k.device != dev or v.device != dev):
+            raise ValueError(f"{what}: k and v must be {new} bf16 on {dev}")
+        k, v = k.contiguous(), v.contiguous()
+        k_ptr, v_ptr = k.data_ptr(), v.data_ptr()
+    elif k is not None or v is not None:
         raise ValueError(f"{what}: pass both k and v, or neither")
-    for t in (k, v):
-        if t is not None and (t.dtype != torch.bfloat16 or t.device != dev or t.shape != (batch, 1, hk, HEAD_DIM)):
-            raise ValueError(f"{what}: k and v must be ({batch}, 1, {hk}, {HEAD_DIM}) bf16 on {dev}")
     if (rotary_cos is None) != (rotary_sin is None):
         raise ValueError(f"{what}: pass both rotary_cos and rotary_sin, or neither")
-    block_table, pages = _table(what, block_table, batch, dev)
+    pages, cap = 0, length
     if block_table is not None:
+        block_table, pages = _table(what, block_table, batch, dev)
         if cache_batch_idx is not None:
             raise NotImplementedError(f"{what}: a paged cache takes no cache_batch_idx")
         if length % 16 != 0:
             raise NotImplementedError(f"{what}: page size must be a multiple of 16")
         cap = pages * length
-    else:
-        if cache_batch_idx is None and slots < batch:
-            raise ValueError(f"{what}: {batch} sequences need as many slots, or cache_batch_idx")
-        cap = length
+    elif cache_batch_idx is not None:
+        cache_batch_idx = _ints(what, "cache_batch_idx", cache_batch_idx, (batch,), dev)
+    elif slots < batch:
+        raise ValueError(f"{what}: {batch} sequences need as many slots, or cache_batch_idx")
     if cache_seqlens is None:
         cache_seqlens = cap
     if isinstance(cache_seqlens, int):
         cache_seqlens = torch.full((batch,), cache_seqlens, dtype=torch.int32, device=dev)
     cache_seqlens = _ints(what, "cache_seqlens", cache_seqlens, (batch,), dev)
-    cache_batch_idx = _ints(what, "cache_batch_idx", cache_batch_idx, (batch,), dev)
-    words = ((cap + BLOCK_N - 1) // BLOCK_N + 63) // 64
-    mask = None
+    mask_ptr, idx_ptr, words, topk = None, None, 0, 0
     if block_mask is not None:
-        if topk_idx is not None or block_mask.dtype != torch.int64 or block_mask.device != dev \
+        words = (cap + 64 * BLOCK_N - 1) // (64 * BLOCK_N)
+        if topk_idx is not None or block_mask.dtype is not torch.int64 or block_mask.device != dev \
                 or block_mask.numel() != batch * hk * words:
             raise ValueError(f"{what}: block_mask must be ({batch}, {hk}, 1, {words}) int64 on {dev} and excludes topk_idx")
-        mask = block_mask.contiguous()
+        block_mask = block_mask.contiguous()
+        mask_ptr = block_mask.data_ptr()
     elif topk_idx is not None:
-        if topk_idx.dtype != torch.int32 or topk_idx.device != dev or topk_idx.dim() not in (3, 4) \
+        words = (cap + 64 * BLOCK_N - 1) // (64 * BLOCK_N)
+        if topk_idx.dtype is not torch.int32 or topk_idx.device != dev or topk_idx.dim() not in (3, 4) \
                 or topk_idx.numel() != batch * hk * topk_idx.shape[-1]:
             raise ValueError(f"{what}: topk_idx must be ({batch}, {hk}, 1, topk) int32 on {dev}")
-        topk_idx = topk_idx.contiguous()
-        mask = torch.empty(batch, hk, 1, words, dtype=torch.int64, device=dev)
+        topk_idx, topk = topk_idx.contiguous(), topk_idx.shape[-1]
+        block_mask = torch.empty(batch, hk, 1, words, dtype=torch.int64, device=dev)
+        mask_ptr, idx_ptr = block_mask.data_ptr(), topk_idx.data_ptr()
     rotary = (None, None, None, 0, None, 0, 0, 0)
-    held = None
     if rotary_cos is not None and k is not None:
-        at = cache_seqlens if rotary_positions is None else rotary_positions
-        sections = None if rotary_sections is None else tuple(int(n) for n in rotary_sections)
-        held = cos, sin, at, axis_stride, pair_axis, axes = _tables(what, rotary_cos, rotary_sin, at, sections, batch, dev)
-        rotary = (cos.data_ptr(), sin.data_ptr(), at.data_ptr(), axis_stride, pair_axis, axes, 2 * cos.shape[1], cos.shape[0])
-    if softmax_scale is None:
-        softmax_scale = HEAD_DIM ** (-0.5)
-    q, k, v = [x.contiguous() if x is not None else None for x in (q, k, v)]
+        if rotary_sections is not None and type(rotary_sections) is not tuple:
+            rotary_sections = tuple(rotary_sections)
+        cos, sin, at, axis_stride, pair_axis, axes, rows, pairs = _tables(
+            what, rotary_cos, rotary_sin, cache_seqlens if rotary_positions is None else rotary_positions, rotary_sections,
+            batch, dev)
+        rotary = (cos.data_ptr(), sin.data_ptr(), at.data_ptr(), axis_stride, pair_axis, axes, 2 * pairs, rows)
+    q = q.contiguous()
     out = torch.empty_like(q)
-    lse = torch.empty(batch, hk * GROUP, 1, dtype=torch.float32, device=dev) if return_softmax_lse else None
-    ws_bytes = int(_lib.load().ifv2_q8_decode_workspace_bytes(batch, hk * GROUP, HEAD_DIM))
+    lse = torch.empty(batch, heads, 1, dtype=torch.float32, device=dev) if return_softmax_lse else None
+    ws_bytes = int(_lib.load().ifv2_q8_decode_workspace_bytes(batch, heads, HEAD_DIM))
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     with _on(dev):
         _lib.call("ifv2_q8_decode", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
-                  v_scale.data_ptr(), _ptr(k), _ptr(v), *rotary, int(bool(rotary_interleaved)), _ptr(topk_idx),
-                  topk_idx.shape[-1] if topk_idx is not None else 0, _ptr(mask), words if mask is not None else 0,
+                  v_scale.data_ptr(), k_ptr, v_ptr, *rotary, 1 if rotary_interleaved else 0, idx_ptr, topk, mask_ptr, words,
                   out.data_ptr(), _ptr(lse), cache_seqlens.data_ptr(), _ptr(cache_batch_idx), _ptr(block_table), pages,
-                  slots, length, code, batch, hk * GROUP, hk, HEAD_DIM, float(softmax_scale), ws.data_ptr(), ws_bytes,
-                  _stream(dev))
+                  slots, length, code, batch, heads, hk, HEAD_DIM, HEAD_DIM ** (-0.5) if softmax_scale is None else float(softmax_scale),
+                  ws.data_ptr(), ws_bytes, _stream(dev))
     return (out, lse) if return_softmax_lse else out

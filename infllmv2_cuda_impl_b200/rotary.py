@@ -11,6 +11,7 @@ import torch
 from . import _lib
 from .ops import _on, _plain_eager, _require_cuda, _stream
 
+_profiled = torch.autograd._profiler_enabled
 HEAD_DIM = 128
 MAX_AXES = 4
 
@@ -22,58 +23,70 @@ def _pair_axis(sections, pairs: int, axes: int) -> Optional[bytes]:
         if axes != 1:
             raise ValueError("rotary: positions on several axes need sections")
         return None
-    if len(sections) != axes or sum(sections) != pairs or min(sections) < 0:
+    if len(sections) != axes or sum(sections) != pairs or min(sections) < 0 or any(type(n) is not int for n in sections):
         raise ValueError(f"rotary: sections must be {axes} counts (one per axis of positions) that sum up to {pairs} pairs, "
-                         f"got {tuple(sections)}")
+                         f"got {sections}")
     return b"".join(bytes([a]) * n for a, n in enumerate(sections))
 
 
 def _tables(what, rotary_cos, rotary_sin, positions, sections, tokens, device):
-    """Checks of the arguments that every rotating call takes; (cos, sin, positions, axis_stride, pair_axis, axes)."""
-    for name, t in (("rotary_cos", rotary_cos), ("rotary_sin", rotary_sin)):
-        if t.dtype != torch.float32 or t.dim() != 2 or t.shape != rotary_cos.shape or t.device != device:
-            raise ValueError(f"{what}: {name} must be (positions, rotary_dim / 2) fp32 on {device}, as the other table")
-        if t.requires_grad:
-            raise NotImplementedError(f"{what}: the tables get no gradient")
-    pairs = rotary_cos.shape[1]
-    if pairs < 8 or pairs > HEAD_DIM // 2 or pairs % 8 != 0 or rotary_cos.shape[0] < 1:
+    """Checks of the arguments that every rotating call takes; (cos, sin, positions, axis_stride, pair_axis, axes, rows,
+    pairs).  (These calls are bound by their host time where tokens are few, so a check costs one attribute.)"""
+    shape, at = rotary_cos.shape, positions.shape
+    if (rotary_cos.dtype is not torch.float32 or rotary_sin.dtype is not torch.float32 or len(shape) != 2
+            or rotary_sin.shape != shape or rotary_cos.device != device or rotary_sin.device != device):
+        raise ValueError(f"{what}: rotary_cos and rotary_sin must be (positions, rotary_dim / 2) fp32 on {device}, of one shape")
+    if rotary_cos.requires_grad or rotary_sin.requires_grad:
+        raise NotImplementedError(f"{what}: the tables get no gradient")
+    rows, pairs = shape
+    if pairs < 8 or pairs > HEAD_DIM // 2 or pairs % 8 != 0 or rows < 1:
         raise ValueError(f"{what}: rotary_dim must be a positive multiple of 16 up to {HEAD_DIM}, and the tables hold a position")
-    if positions.dtype != torch.int32 or positions.device != device or positions.dim() not in (1, 2) or positions.shape[-1] != tokens:
+    if positions.dtype is not torch.int32 or len(at) not in (1, 2) or at[-1] != tokens or positions.device != device:
         raise ValueError(f"{what}: positions must be ({tokens},) or (axes, {tokens}) int32 on {device}")
-    axes = positions.shape[0] if positions.dim() == 2 else 1
-    if not 1 <= axes <= MAX_AXES:
-        raise ValueError(f"{what}: 1 to {MAX_AXES} axes, got {axes}")
-    if positions.stride(-1) != 1 and tokens > 1:
+    axes, axis_stride = 1, 0
+    if len(at) == 2:
+        axes = at[0]
+        if not 1 <= axes <= MAX_AXES:
+            raise ValueError(f"{what}: 1 to {MAX_AXES} axes, got {axes}")
+        strides = positions.stride()
+        if strides[1] != 1 and tokens > 1:
+            positions = positions.contiguous()
+            strides = positions.stride()
+        axis_stride = strides[0]
+    elif not positions.is_contiguous():
         positions = positions.contiguous()
-    pair_axis = _pair_axis(None if sections is None else tuple(sections), pairs, axes)
-    return (rotary_cos.contiguous(), rotary_sin.contiguous(), positions, positions.stride(0) if positions.dim() == 2 else 0,
-            pair_axis, axes)
+    return (rotary_cos.contiguous(), rotary_sin.contiguous(), positions, axis_stride, _pair_axis(tuple(sections) if type(sections) is list else sections, pairs, axes), axes, rows,
+            pairs)
 
 
 def _rows(x):
-    """x with unit stride in the features and rows on 16-byte boundaries; copied only where it has to be."""
-    if x.stride(-1) == 1 and (x.stride(0) | x.stride(1)) % 8 == 0 and x.data_ptr() % 16 == 0:
-        return x
-    return x.contiguous() if not x.is_contiguous() else x.clone()
+    """(x, its first two strides) with unit stride in the features and rows on 16-byte boundaries; copied only where it
+    has to be."""
+    a, b, c = x.stride()
+    if c != 1 or (a | b) & 7 or x.data_ptr() & 15:
+        x = x.clone(memory_format=torch.contiguous_format)
+        a, b, c = x.stride()
+    return x, a, b
 
 
 def _rotate(q, k, rotary_cos, rotary_sin, positions, sections, interleaved, back):
     """Returns (q, k) rotated, dense; k may be None."""
-    tokens, dev = q.shape[0], q.device
-    cos, sin, positions, axis_stride, pair_axis, axes = _tables("rotary_axes", rotary_cos, rotary_sin, positions, sections, tokens, dev)
-    q = _rows(q)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    k_out = None
-    k_args = (None, None, 0, 0, 0)
+    shape, dev = q.shape, q.device
+    cos, sin, positions, axis_stride, pair_axis, axes, rows, pairs = _tables("rotary_axes", rotary_cos, rotary_sin, positions,
+                                                                             sections, shape[0], dev)
+    q, q_token, q_head = _rows(q)
+    q_out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+    k_out = k_ptr = k_out_ptr = None
+    heads_k = k_token = k_head = 0
     if k is not None:
-        k = _rows(k)
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=dev)
-        k_args = (k.data_ptr(), k_out.data_ptr(), k.shape[1], k.stride(0), k.stride(1))
+        k, k_token, k_head = _rows(k)
+        heads_k = k.shape[1]
+        k_out = torch.empty(k.shape, dtype=torch.bfloat16, device=dev)
+        k_ptr, k_out_ptr = k.data_ptr(), k_out.data_ptr()
     with _on(dev):
-        _lib.call("ifv2_rotary_axes", q.data_ptr(), k_args[0], q_out.data_ptr(), k_args[1], cos.data_ptr(), sin.data_ptr(),
-                  positions.data_ptr(), axis_stride, pair_axis, axes, tokens, q.shape[1], k_args[2], HEAD_DIM, q.stride(0),
-                  q.stride(1), k_args[3], k_args[4], 2 * cos.shape[1], cos.shape[0], int(bool(interleaved)), int(bool(back)),
-                  _stream(dev))
+        _lib.call("ifv2_rotary_axes", q.data_ptr(), k_ptr, q_out.data_ptr(), k_out_ptr, cos.data_ptr(), sin.data_ptr(),
+                  positions.data_ptr(), axis_stride, pair_axis, axes, shape[0], shape[1], heads_k, HEAD_DIM, q_token, q_head,
+                  k_token, k_head, 2 * pairs, rows, interleaved, back, _stream(dev))
     return q_out, k_out
 
 
@@ -93,7 +106,7 @@ def _(q, k, rotary_cos, rotary_sin, positions, sections, interleaved, back):
 
 def _call(q, k, rotary_cos, rotary_sin, positions, sections, interleaved, back):
     """The body where nothing watches operators, the registered operator elsewhere."""
-    if not torch.compiler.is_compiling() and not torch.autograd._profiler_enabled() and _plain_eager(q, k, rotary_cos, rotary_sin, positions):
+    if not torch.compiler.is_compiling() and not _profiled() and _plain_eager(q, k, rotary_cos, rotary_sin, positions):
         return _rotate(q, k, rotary_cos, rotary_sin, positions, sections, interleaved, back)
     q, k_out = _rotary_axes(q, k, rotary_cos, rotary_sin, positions, None if sections is None else list(sections), interleaved, back)
     return q, k_out if k is not None else None
@@ -121,7 +134,7 @@ class RotaryAxesFunc(torch.autograd.Function):
 
 
 def _rotary_maybe_grad(q, k, *args):
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if (q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled():
         return RotaryAxesFunc.apply(q, k, *args)
     return _call(q, k, *args)
 
@@ -137,13 +150,14 @@ def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], rotary_cos: torch.Te
     (2i, 2i+1) if interleaved, else (i, i + rotary_dim / 2); features from rotary_dim on pass through.  The
     arithmetic is fp32, the results are rounded once.  A position outside the tables takes their first or last row.
     Returns (q, k) rotated (k None without one), dense."""
-    for name, t in (("q", q), ("k", k)):
-        if t is None and name == "k":
-            continue
-        _require_cuda(t, name)
-        if t.dtype != torch.bfloat16 or t.dim() != 3 or t.shape[-1] != HEAD_DIM:
-            raise ValueError(f"rotary_axes: {name} must be (tokens, heads, {HEAD_DIM}) bf16")
-    if k is not None and (k.shape[0] != q.shape[0] or k.device != q.device):
-        raise ValueError("rotary_axes: q and k must have the same tokens, on one device")
-    sections = None if sections is None else tuple(int(n) for n in sections)
+    shape = q.shape
+    if q.dtype is not torch.bfloat16 or len(shape) != 3 or shape[2] != HEAD_DIM:
+        raise ValueError(f"rotary_axes: q must be (tokens, nheads, {HEAD_DIM}) bf16")
+    _require_cuda(q, "q")
+    if k is not None:
+        other = k.shape
+        if k.dtype is not torch.bfloat16 or len(other) != 3 or other[2] != HEAD_DIM or other[0] != shape[0] or k.device != q.device:
+            raise ValueError(f"rotary_axes: k must be (tokens, nheads_k, {HEAD_DIM}) bf16, with the tokens and on the device of q")
+    if sections is not None and type(sections) is not tuple:
+        sections = tuple(sections)
     return _rotary_maybe_grad(q, k, rotary_cos, rotary_sin, positions, sections, bool(interleaved), False)
