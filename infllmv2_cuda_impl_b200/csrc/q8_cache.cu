@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(kThreads) q8_fill_kernel(const MoveParams p) {
   }
 }
 
-// The way back: one head of kTile tokens, eight threads per row with 16 codes each.  A row that the cache does not
+// The way back: one head of kTile tokens, eight threads per row; two 8-byte loads leave as vectors l and l + 8.  A row that the cache does not
 // have reads as NaN; rows behind the last sequence are zeros.
 template <int kCode>
 __global__ void __launch_bounds__(kThreads) q8_read_kernel(const MoveParams p) {
@@ -94,35 +94,36 @@ __global__ void __launch_bounds__(kThreads) q8_read_kernel(const MoveParams p) {
   if (t >= p.total) return;
   const int64_t row0 = token_row(p, t);
   const int64_t row = row0 >= 0 ? p.place.row(row0, h) : 0;
-  uint4 raw[2];
+  uint2 raw[2][2];
   int byte[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    raw[i] = make_uint4(0u, 0u, 0u, 0u);
+    raw[i][0] = raw[i][1] = make_uint2(0u, 0u);
     byte[i] = row0 == -2 ? 0 : kNanByte;
     if (row0 >= 0) {
-      raw[i] = __ldg(reinterpret_cast<const uint4*>(p.codes[i] + row * kHeadDim) + l);
+      const uint2* src = reinterpret_cast<const uint2*>(p.codes[i] + row * kHeadDim) + l;
+      raw[i][0] = __ldg(src);
+      raw[i][1] = __ldg(src + kLanes);
       byte[i] = __ldg(p.scales[i] + row);
     }
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const float s = scale_value(byte[i]);
-    const uint32_t c[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-    uint32_t w[8];
+    uint4* out = p.dst[i] + (t * p.place.heads + h) * (kHeadDim / 8) + l;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float x[4];
-      decode4<kCode>(x, c[j]);
+    for (int v = 0; v < 2; ++v) {
+      float x[8];
+      uint32_t w[4];
+      decode4<kCode>(*reinterpret_cast<float(*)[4]>(x), raw[i][v].x);
+      decode4<kCode>(*reinterpret_cast<float(*)[4]>(x + 4), raw[i][v].y);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const __nv_bfloat162 v = __floats2bfloat162_rn(mul_exact(x[2 * u], s), mul_exact(x[2 * u + 1], s));
-        w[2 * j + u] = *reinterpret_cast<const uint32_t*>(&v);
+      for (int u = 0; u < 4; ++u) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(mul_exact(x[2 * u], s), mul_exact(x[2 * u + 1], s));
+        w[u] = *reinterpret_cast<const uint32_t*>(&b);
       }
+      out[v * kLanes] = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    uint4* out = p.dst[i] + (t * p.place.heads + h) * (kHeadDim / 8) + 2 * l;
-    out[0] = make_uint4(w[0], w[1], w[2], w[3]);
-    out[1] = make_uint4(w[4], w[5], w[6], w[7]);
   }
 }
 
