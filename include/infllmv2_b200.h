@@ -485,7 +485,7 @@ int ifv2_rotary_axes(const void* q, const void* k, void* q_out, void* k_out, con
  *
  * ifv2_q8_fill: packed rows k, v (total, heads_k, 128) bf16 with the given strides (elements, multiples of 8)
  * of sequences cu_seqlens (batch + 1) go to positions start[b] + 0, 1, ... (start null = 0).  seqlens_out (may
- * be null): min(start[b] + len_b, capacity).  Rows from cu_seqlens[batch] on are not read.
+ * be null): min(start[b] + len_b, capacity).  Rows from cu_seqlens[batch] on go nowhere.
  * ifv2_q8_read: the way back into dense k, v (total, heads_k, 128) bf16, exactly; rows from cu_seqlens[batch] on
  * are set to 0.
  * ifv2_q8_append: ifv2_decode_append for such a cache in slots; compressed keys are means of the keys as the

@@ -51,15 +51,15 @@ __global__ void __launch_bounds__(kThreads) q8_fill_kernel(const MoveParams p) {
   if (p.seqlens_out != nullptr && h == 0)
     for (int64_t b = (int64_t)blockIdx.x * kThreads + threadIdx.x; b < p.batch; b += (int64_t)gridDim.x * kThreads)
       p.seqlens_out[b] = (int32_t)min((int64_t)max(p.cu[b + 1] - p.cu[b] + (p.start ? p.start[b] : 0), 0), p.capacity);
-  const int64_t row0 = token_row(p, t);
-  const bool on = row0 >= 0;
-  uint4 raw[2][2];
+  uint4 raw[2][2];                               // (on their way while the row's place is looked up)
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const uint4* src = p.src[i] + t * p.token_stride[i] + h * p.head_stride[i] + l;
-    raw[i][0] = on ? __ldg(src) : make_uint4(0u, 0u, 0u, 0u);
-    raw[i][1] = on ? __ldg(src + kLanes) : make_uint4(0u, 0u, 0u, 0u);
+    raw[i][0] = t < p.total ? __ldg(src) : make_uint4(0u, 0u, 0u, 0u);
+    raw[i][1] = t < p.total ? __ldg(src + kLanes) : make_uint4(0u, 0u, 0u, 0u);
   }
+  const int64_t row0 = token_row(p, t);
+  const bool on = row0 >= 0;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     float x[16];
