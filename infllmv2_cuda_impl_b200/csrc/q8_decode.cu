@@ -9,7 +9,7 @@
 // values take part in the weights, next to the scores, so that the largest weight is about 1 whatever the values' sizes
 // are, and out = O 2^(M - m) / l.  (m and M differ by little more than 127, the range of the exponents.)
 //
-// Launches: [prepare: block lists, append] -> split -> combine.
+// Launches: [prepare: block lists, append where sequences may share rows] -> split -> combine.
 #include <type_traits>
 #include "block_list.cuh"
 #include "mma_sync.cuh"
@@ -41,10 +41,12 @@ constexpr float kLn2 = 0.6931471805599453f;
 
 struct Q8DecodeParams {
   const __nv_bfloat16* q;          // (batch, heads_q, 128)
-  const uint8_t* k_codes;
-  const uint8_t* v_codes;
-  const uint8_t* k_scale;
-  const uint8_t* v_scale;
+  uint8_t* k_codes;
+  uint8_t* v_codes;
+  uint8_t* k_scale;
+  uint8_t* v_scale;
+  const __nv_bfloat16* k_new;      // (batch, heads_k, 128) new rows that the split kernel appends, or null
+  const __nv_bfloat16* v_new;
   const unsigned long long* mask;  // (batch, heads_k, mask_words) or null = all positions
   int mask_words;
   const int32_t* cache_seqlens;
@@ -316,6 +318,31 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 #pragma unroll
     for (int i = 0; i < kGroup / kWarps; ++i) q_part[i].load(p.q + (pair * kGroup + warp + kWarps * i) * kHeadDim, lane, angles.mate);
 
+    // the new token's row, by the warp whose unit it belongs to (no CTA attends it: by the first warp of split 0)
+    if (p.k_new != nullptr) {
+      const int pos = p.cache_seqlens[b];
+      if (pos >= 0 && pos < p.capacity) {
+        const int blk = pos / kBlockN;
+        const bool attended = dealt || (blk / 64 < p.mask_words && ((__ldg(list.words + blk / 64) >> (blk & 63)) & 1ull));
+        const int owner = attended ? (((n - 1 - j0) & 1) << 1) | ((pos / kUnit) & 1) : 0;
+        if ((attended ? j0 < j1 && j1 == n : split == 0) && warp == owner) {
+          const int64_t row = ((int64_t)b * p.heads_k + h) * p.place.length + pos;
+          RowPart k_part, v_part;
+          k_part.load(p.k_new + pair * kHeadDim, lane, angles.mate);
+          v_part.load(p.v_new + pair * kHeadDim, lane, 0);
+          float x[4];
+          if (kRotate) k_part.turned(x, angles);
+          else k_part.plain(x);
+          store_row<kCode>(x, p.k_codes + row * kHeadDim, p.k_scale + row, lane);
+          v_part.plain(x);
+          store_row<kCode>(x, p.v_codes + row * kHeadDim, p.v_scale + row, lane);
+          __threadfence();
+          tc::fence_proxy_async_global();
+          __syncwarp();
+        }
+      }
+    }
+
     // this warp's units: half (warp & 1) of blocks j0 + (warp >> 1), + 2, ...
     int j = j0 + (warp >> 1), lookups = 0;
     auto next_key = [&]() -> int {                 // first key of the next unit, or -1
@@ -348,8 +375,8 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
           row = slot0 + key;
         }
         if (row >= 0) {
-          kb = __ldg(p.k_scale + row);
-          vb = __ldg(p.v_scale + row);
+          kb = __ldcg(p.k_scale + row);            // (not through L1: the newest may have been written by this warp)
+          vb = __ldcg(p.v_scale + row);
         }
       }
     };
@@ -807,10 +834,17 @@ extern "C" int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void*
   }
   p.rotate = rotate;
   p.q = static_cast<const __nv_bfloat16*>(q);
-  p.k_codes = static_cast<const uint8_t*>(k_cache);
-  p.v_codes = static_cast<const uint8_t*>(v_cache);
-  p.k_scale = static_cast<const uint8_t*>(k_scale);
-  p.v_scale = static_cast<const uint8_t*>(v_scale);
+  p.k_codes = static_cast<uint8_t*>(k_cache);
+  p.v_codes = static_cast<uint8_t*>(v_cache);
+  p.k_scale = static_cast<uint8_t*>(k_scale);
+  p.v_scale = static_cast<uint8_t*>(v_scale);
+  // Where sequences may share rows (pages, slots by index) the new rows are all written before any is attended; slots
+  // that belong to one sequence each get them from the CTA that attends the new token's block.
+  const bool shared_rows = block_table != nullptr || cache_batch_idx != nullptr;
+  if (!shared_rows) {
+    p.k_new = static_cast<const __nv_bfloat16*>(k_new);
+    p.v_new = static_cast<const __nv_bfloat16*>(v_new);
+  }
   p.mask = reinterpret_cast<const unsigned long long*>(mask);
   p.mask_words = mask_words;
   p.cache_seqlens = cache_seqlens;
@@ -831,8 +865,8 @@ extern "C" int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void*
     p.splits = most < 1 ? 1 : most > kMaxSplits ? kMaxSplits : (int)most;
   }
   cudaStream_t st = (cudaStream_t)stream;
-  if (k_new != nullptr || topk_idx != nullptr) {
-    const Q8PrepareParams a{static_cast<const __nv_bfloat16*>(k_new), static_cast<const __nv_bfloat16*>(v_new),
+  if ((k_new != nullptr && shared_rows) || topk_idx != nullptr) {
+    const Q8PrepareParams a{shared_rows ? static_cast<const __nv_bfloat16*>(k_new) : nullptr, static_cast<const __nv_bfloat16*>(v_new),
                             static_cast<uint8_t*>(k_cache), static_cast<uint8_t*>(v_cache), static_cast<uint8_t*>(k_scale),
                             static_cast<uint8_t*>(v_scale), topk_idx, reinterpret_cast<unsigned long long*>(mask), topk, mask_words};
     const size_t smem = topk_idx ? (size_t)mask_words * 8 : 0;

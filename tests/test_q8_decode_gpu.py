@@ -181,6 +181,52 @@ def test_append_and_rotation(dtype, page, axes, interleaved, dim):
     _check(out, lse, q_rot, grown, [min(n + 1, cap) for n in lens], table)
 
 
+@pytest.mark.parametrize("dtype", [E4M3, INT8])
+@pytest.mark.parametrize("page", [0, 64])
+def test_append_with_block_lists(dtype, page):
+    """The new row is written whether its block is selected or not, and attended only if it is."""
+    hk, lens, cap = 2, [0, 63, 64, 500, 511, 130], 512
+    batch = len(lens)
+    table = _table(batch, cap // 64, batch * cap // 64, 4) if page else None
+    cache = _cache(batch * cap // 64, 64, hk, dtype, 3) if page else _cache(batch, cap, hk, dtype, 3)
+    q, k, v = det_tensor((batch, 1, hk * 16, 128), 7, 1.5), det_tensor((batch, 1, hk, 128), 8, 2.0), det_tensor((batch, 1, hk, 128), 9)
+    idx = _lists([n + 1 for n in lens], hk, 3, 5)
+    idx[3, 0, 0] = torch.tensor([0, 2, 7])          # 500 is in block 7
+    idx[3, 1, 0] = torch.tensor([0, 2, 6])
+    idx[4, 0, 0] = torch.tensor([-1, -1, -1])
+    idx[5, 1, 0] = torch.tensor([2, -1, -1])        # 130 is in block 2: one key and the new one
+    dev = _to_gpu(cache)
+    out, lse = infllm_v2.infllmv2_attn_with_kvcache_q8(
+        q.to(DEV), *dev, k=k.to(DEV), v=v.to(DEV), cache_seqlens=torch.tensor(lens, dtype=torch.int32, device=DEV),
+        block_table=None if table is None else table.to(DEV), topk_idx=idx.to(DEV), return_softmax_lse=True)
+    grown = [t.clone() for t in cache]
+    for b, n in enumerate(lens):
+        slot, off = (b, n) if table is None else (int(table[b, n // 64]), n % 64)
+        for j, x in ((0, k), (1, v)):
+            grown[j][slot, :, off], grown[j + 2][slot, :, off] = quantise(x[b, 0], dtype)
+    for got, want in zip(dev, grown):
+        if got.dtype == E4M3:
+            assert torch.equal(got.float().cpu(), want.float())              # (a zero may have either sign)
+        else:
+            assert torch.equal(got.view(torch.uint8).cpu(), want.view(torch.uint8))
+    _check(out, lse, q, grown, [n + 1 for n in lens], table, topk_idx=idx)
+
+
+def test_sequences_that_share_a_slot_are_appended_before_any_attends():
+    cache = _cache(2, 200, 1, E4M3, 3)
+    dev = _to_gpu(cache)
+    q, k = det_tensor((2, 1, 16, 128), 7), det_tensor((2, 1, 1, 128), 8)
+    slot = torch.tensor([1, 1], dtype=torch.int32)
+    lens = [150, 151]
+    out = infllm_v2.infllmv2_attn_with_kvcache_q8(q.to(DEV), *dev, k=k.to(DEV), v=k.to(DEV), cache_batch_idx=slot.to(DEV),
+                                                  cache_seqlens=torch.tensor(lens, dtype=torch.int32, device=DEV))
+    grown = [t.clone() for t in cache]
+    for b, n in enumerate(lens):
+        for j in (0, 1):
+            grown[j][1, :, n], grown[j + 2][1, :, n] = quantise(k[b, 0], E4M3)
+    _check(out, None, q, grown, [151, 152], batch_idx=slot)
+
+
 def test_lengths_past_the_capacity_and_below_zero():
     cache = _cache(3, 70, 1, E4M3, 3)
     q, k = det_tensor((3, 1, 16, 128), 7), det_tensor((3, 1, 1, 128), 8)
