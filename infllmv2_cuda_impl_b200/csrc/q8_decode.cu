@@ -178,18 +178,22 @@ __device__ __forceinline__ int blocks_of(const Q8DecodeParams& p, int b) { retur
 // place by itself, a sequence per lane.
 struct Deal {
   uint32_t total, ctas, each, rest;                // total = each * ctas + rest
-  __device__ Deal(const Q8DecodeParams& p, uint32_t grid, int lane) {
-    uint32_t n = 0;
-    for (int b = lane; b < p.batch; b += 32) n += blocks_of(p, b);
-    total = __reduce_add_sync(0xFFFFFFFFu, n) * p.heads_k;      // (the host keeps it below 2^31)
+  // blocks: of all sequences, for one KV head (the host keeps the total below 2^31)
+  __device__ Deal(uint32_t blocks, int heads_k, uint32_t grid) {
+    total = blocks * heads_k;
     // two blocks are one 32-key unit for each of the four warps
     ctas = max(1u, min(grid, (total + 1) / 2));
     each = total / ctas;
     rest = total - each * ctas;
   }
   __device__ uint32_t first(uint32_t c) const { return c * each + c * rest / ctas; }      // c total / ctas
-  // the last c with first(c) <= block: each c + floor(c rest / ctas) <= block
-  __device__ uint32_t cta_of(uint32_t block) const { return (uint32_t)((((uint64_t)block + 1) * ctas - 1) / total); }
+  // the last c with first(c) <= block, from an estimate that is off by one at most
+  __device__ uint32_t cta_of(uint32_t block) const {
+    uint32_t c = min((uint32_t)((float)block * ((float)ctas / (float)total)), ctas - 1);
+    while (c + 1 < ctas && first(c + 1) <= block) ++c;
+    while (first(c) > block) --c;
+    return c;
+  }
 };
 
 // Sequence that holds block `at` of the row, and the row's blocks before it.
@@ -282,7 +286,9 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   int b = 0, h = 0, split = 0;
   uint32_t at = 0, end = 0, before = 0;
   if (dealt) {
-    const Deal deal(p, gridDim.x, lane);
+    uint32_t blocks = 0;
+    for (int i = lane; i < p.batch; i += 32) blocks += blocks_of(p, i);
+    const Deal deal(__reduce_add_sync(0xFFFFFFFFu, blocks), p.heads_k, gridDim.x);
     if (deal.total == 0 || blockIdx.x >= deal.ctas) return;
     at = deal.first(blockIdx.x);
     end = deal.first(blockIdx.x + 1);
@@ -475,12 +481,15 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         for (int u = 0; u < 4; ++u) {
           const uint4 hi4 = q_frag[0][kp * 4 + u][lane], lo4 = q_frag[kRotate ? 1 : 0][kp * 4 + u][lane];
           const uint32_t qh[4] = {hi4.x, hi4.y, hi4.z, hi4.w}, ql[4] = {lo4.x, lo4.y, lo4.z, lo4.w};
+          uint32_t f[kUnit / 8][2];
 #pragma unroll
           for (int nt = 0; nt < kUnit / 8; ++nt) {
-            uint32_t f0, f1;
-            decode_h2<kCode>(f0, f1, w[nt][u]);
-            mmasync::mma_f16(s[nt], qh, f0, f1);
-            if (kRotate) mmasync::mma_f16(s[nt], ql, f0, f1);
+            decode_h2<kCode>(f[nt][0], f[nt][1], w[nt][u]);
+            mmasync::mma_f16(s[nt], qh, f[nt][0], f[nt][1]);
+          }
+          if (kRotate) {                           // (after the four others: a sum waits for its last product)
+#pragma unroll
+            for (int nt = 0; nt < kUnit / 8; ++nt) mmasync::mma_f16(s[nt], ql, f[nt][0], f[nt][1]);
           }
         }
       }
@@ -692,13 +701,18 @@ __global__ void __launch_bounds__(256) q8_combine_kernel(const Q8DecodeParams p,
   int n = p.splits;
   bool start_slot = false;                          // the first partial lies in its CTA's second place
   if (p.mask == nullptr) {
-    const Deal deal(p, split_grid, lane);
-    const int blocks = blocks_of(p, b);
+    uint32_t all = 0, before = 0, own = 0;          // blocks of all sequences, of those before b, of b
+    for (int i = lane; i < p.batch; i += 32) {
+      const uint32_t v = blocks_of(p, i);
+      all += v;
+      if (i < b) before += v;
+      if (i == b) own = v;
+    }
+    const Deal deal(__reduce_add_sync(0xFFFFFFFFu, all), p.heads_k, split_grid);
+    const uint32_t blocks = __reduce_add_sync(0xFFFFFFFFu, own);
     if (blocks == 0) {
       n = 0;
     } else {
-      uint32_t before = 0;
-      for (int b1 = lane; b1 < b; b1 += 32) before += blocks_of(p, b1);
       const uint32_t at = __reduce_add_sync(0xFFFFFFFFu, before) * p.heads_k + h * blocks;
       first = deal.cta_of(at);
       n = deal.cta_of(at + blocks - 1) - (int)first + 1;
@@ -900,7 +914,7 @@ extern "C" int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void*
   if (mask != nullptr && p.splits == 1) return IFV2_OK;      // the split kernel wrote the results
   const int64_t per_pair = mask != nullptr ? p.splits : ceil_div64(grid, pairs);
   if (per_pair > 16) q8_combine_kernel<8><<<dim3(16, (unsigned)pairs), 256, 0, st>>>(p, (int)grid);
-  else if (per_pair > 4) q8_combine_kernel<4><<<dim3(8, (unsigned)pairs), 256, 0, st>>>(p, (int)grid);
+  else if (per_pair > 6) q8_combine_kernel<4><<<dim3(8, (unsigned)pairs), 256, 0, st>>>(p, (int)grid);
   else q8_combine_kernel<1><<<dim3(2, (unsigned)pairs), 256, 0, st>>>(p, (int)grid);
   return check_launch("q8_combine");
 }
