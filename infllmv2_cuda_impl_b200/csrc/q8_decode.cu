@@ -132,12 +132,18 @@ struct RowPart {
   }
 };
 
+// A kernel that the next one of the call may start beside: that one reads what this one writes only after its wait,
+// which every thread of it makes before it ends, so that whatever comes after the call comes after both.
+__device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // One CTA per (sequence, KV head): block lists -> mask row; the new key (rotated) and value -> their row.
 template <int kCode>
 __global__ void __launch_bounds__(kThreads) q8_prepare_kernel(const Q8PrepareParams a, const Q8DecodeParams p) {
   extern __shared__ unsigned long long row_words[];
   const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
   const int64_t pair = (int64_t)b * p.heads_k + h;
+  allow_next();
   if (a.topk_idx != nullptr) {
     for (int w = tid; w < a.words; w += kThreads) row_words[w] = 0ull;
     __syncthreads();
@@ -252,6 +258,7 @@ __device__ __forceinline__ void store_out(const Q8DecodeParams& p, int64_t qrow,
 template <int kCode, int kBox, bool kRotate>
 __global__ void __launch_bounds__(kThreads, kRotate ? kResidentRotate : kResident)
 q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Q8DecodeParams p) {
+  allow_next();
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   __shared__ uint64_t bars[kWarps][kSlots];
@@ -289,7 +296,10 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     uint32_t blocks = 0;
     for (int i = lane; i < p.batch; i += 32) blocks += blocks_of(p, i);
     const Deal deal(__reduce_add_sync(0xFFFFFFFFu, blocks), p.heads_k, gridDim.x);
-    if (deal.total == 0 || blockIdx.x >= deal.ctas) return;
+    if (deal.total == 0 || blockIdx.x >= deal.ctas) {
+      wait_previous();
+      return;
+    }
     at = deal.first(blockIdx.x);
     end = deal.first(blockIdx.x + 1);
     b = find_block(p, at, before, lane);
@@ -303,9 +313,19 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   while (true) {
     const int len = keys_of(p, b);
     int n = (len + kBlockN - 1) / kBlockN, j0, j1;
+    if (dealt) h = (int)((at - before) / (uint32_t)n);
+    const int64_t pair = (int64_t)b * p.heads_k + h;
+    // the warp's rows of the query, on their way while the first tiles are asked for
+    Angles angles;
+    angles.mate = 0;
+    if (kRotate) angles.load(p.rotary, b, lane);
+    RowPart q_part[kGroup / kWarps];
+#pragma unroll
+    for (int i = 0; i < kGroup / kWarps; ++i) q_part[i].load(p.q + (pair * kGroup + warp + kWarps * i) * kHeadDim, lane, angles.mate);
+
+    wait_previous();                               // (the mask, or a new row of shared pages)
     BlockList<2> list{dealt ? nullptr : p.mask + ((int64_t)b * p.heads_k + h) * p.mask_words, p.mask_words, n, -1};
     if (dealt) {
-      h = (int)((at - before) / (uint32_t)n);
       j0 = (int)(at - before - (uint32_t)(h * n));
       j1 = (int)min((uint32_t)n, j0 + end - at);
     } else {
@@ -314,15 +334,6 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       j0 = split * per;
       j1 = min(n, j0 + per);
     }
-    const int64_t pair = (int64_t)b * p.heads_k + h;
-
-    // the warp's rows of the query, on their way while the first tiles are asked for
-    Angles angles;
-    angles.mate = 0;
-    if (kRotate) angles.load(p.rotary, b, lane);
-    RowPart q_part[kGroup / kWarps];
-#pragma unroll
-    for (int i = 0; i < kGroup / kWarps; ++i) q_part[i].load(p.q + (pair * kGroup + warp + kWarps * i) * kHeadDim, lane, angles.mate);
 
     // the new token's row, by the warp whose unit it belongs to (no CTA attends it: by the first warp of split 0)
     if (p.k_new != nullptr) {
@@ -716,10 +727,11 @@ __global__ void __launch_bounds__(256) q8_combine_kernel(const Q8DecodeParams p,
       const uint32_t at = __reduce_add_sync(0xFFFFFFFFu, before) * p.heads_k + h * blocks;
       first = deal.cta_of(at);
       n = deal.cta_of(at + blocks - 1) - (int)first + 1;
-      if (n == 1) return;                           // one CTA had all of it and wrote the result
       start_slot = true;
     }
   }
+  wait_previous();
+  if (start_slot && n == 1) return;                 // one CTA had all of it and wrote the result
   auto partial = [&](int s) -> const float* {
     const int64_t slot = start_slot ? 2 * (first + s) + (s == 0) : first + s;
     return p.partial + (slot * kGroup + r) * kPartialFloats;
@@ -791,6 +803,23 @@ __global__ void __launch_bounds__(256) q8_combine_kernel(const Q8DecodeParams p,
 }  // namespace ifv2
 
 using namespace ifv2;
+
+// beside: the kernel may start while the one before it in the stream still runs (see wait_previous).
+template <typename... Params, typename... Args>
+static cudaError_t launch(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream, bool beside,
+                          const Args&... args) {
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  config.attrs = &attribute;
+  config.numAttrs = beside ? 1 : 0;
+  return cudaLaunchKernelEx(&config, kernel, Params(args)...);
+}
 
 extern "C" int64_t ifv2_q8_decode_workspace_bytes(int batch, int heads_q, int head_dim) {
   if (batch < 0 || heads_q < 0 || head_dim != kHeadDim) return 0;
@@ -879,7 +908,8 @@ extern "C" int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void*
     p.splits = most < 1 ? 1 : most > kMaxSplits ? kMaxSplits : (int)most;
   }
   cudaStream_t st = (cudaStream_t)stream;
-  if ((k_new != nullptr && shared_rows) || topk_idx != nullptr) {
+  const bool prepared = (k_new != nullptr && shared_rows) || topk_idx != nullptr;
+  if (prepared) {
     const Q8PrepareParams a{shared_rows ? static_cast<const __nv_bfloat16*>(k_new) : nullptr, static_cast<const __nv_bfloat16*>(v_new),
                             static_cast<uint8_t*>(k_cache), static_cast<uint8_t*>(v_cache), static_cast<uint8_t*>(k_scale),
                             static_cast<uint8_t*>(v_scale), topk_idx, reinterpret_cast<unsigned long long*>(mask), topk, mask_words};
@@ -908,13 +938,13 @@ extern "C" int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void*
     IFV2_REQUIRE(grid <= INT32_MAX, IFV2_ERR_TOO_LARGE, "q8_decode: more than 2^31-1 blocks of 64 keys");
     if (grid > ctas) grid = ctas;
   }
-  kernel<<<(unsigned)grid, kThreads, kSmemBytes, st>>>(map_k, map_v, p);
-  rc = check_launch("q8_split");
-  if (rc) return rc;
+  e = launch(kernel, dim3((unsigned)grid), kThreads, kSmemBytes, st, prepared, map_k, map_v, p);
+  if (e != cudaSuccess) return set_error((int)e, "q8_split: launch failed: %s", cudaGetErrorString(e));
   if (mask != nullptr && p.splits == 1) return IFV2_OK;      // the split kernel wrote the results
   const int64_t per_pair = mask != nullptr ? p.splits : ceil_div64(grid, pairs);
-  if (per_pair > 16) q8_combine_kernel<8><<<dim3(16, (unsigned)pairs), 256, 0, st>>>(p, (int)grid);
-  else if (per_pair > 6) q8_combine_kernel<4><<<dim3(8, (unsigned)pairs), 256, 0, st>>>(p, (int)grid);
-  else q8_combine_kernel<1><<<dim3(2, (unsigned)pairs), 256, 0, st>>>(p, (int)grid);
-  return check_launch("q8_combine");
+  const int warps = per_pair > 16 ? 8 : per_pair > 6 ? 4 : 1;      // that share a row's partials
+  auto join = warps == 8 ? q8_combine_kernel<8> : warps == 4 ? q8_combine_kernel<4> : q8_combine_kernel<1>;
+  e = launch(join, dim3(2 * warps, (unsigned)pairs), 256, 0, st, true, p, (int)grid);
+  if (e != cudaSuccess) return set_error((int)e, "q8_combine: launch failed: %s", cudaGetErrorString(e));
+  return IFV2_OK;
 }
