@@ -24,16 +24,13 @@ using namespace q8;
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-#ifndef RES
-#define RES 3
-#endif
-constexpr int kResident = RES, kResidentRotate = 3;      // CTAs per SM
+constexpr int kResident = 3;                     // CTAs per SM
 constexpr int kUnit = 32;                        // keys that a warp handles at once
 constexpr int kSlots = 3;                        // a warp's tiles in shared memory: K, V, next K, next V ... in turn
 constexpr int kTileBytes = kUnit * kHeadDim;
 constexpr int kSmemBytes = kWarps * kSlots * kTileBytes + 1024;
-constexpr int kMaxSplits = 16;                   // CTAs that share the selected blocks of a (sequence, KV head)
-constexpr int kMaxCtas = kResident * kNumSMs;    // CTAs that share all blocks where there is no mask
+constexpr int kMaxSplits = 32;                   // CTAs that share the selected blocks of a (sequence, KV head)
+constexpr int kMaxCtas = kResident * kNumSMs;    // one wave: the CTAs that share all blocks where there is no mask
 constexpr long long kWaitLimit = 1ll << 28;      // clocks; a copy takes microseconds
 constexpr int kPartialFloats = kHeadDim + 4;     // O row, m (log2 units), l, exponent of O's units, pad
 constexpr float kLog2e = 1.4426950408889634f;
@@ -256,7 +253,7 @@ __device__ __forceinline__ void store_out(const Q8DecodeParams& p, int64_t qrow,
 // transposing 16-bit ldmatrix, a word of which holds two tokens' codes of two neighbouring features: even features
 // and odd features of a chunk are the columns of two products.
 template <int kCode, int kBox, bool kRotate>
-__global__ void __launch_bounds__(kThreads, kRotate ? kResidentRotate : kResident)
+__global__ void __launch_bounds__(kThreads, kResident)
 q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Q8DecodeParams p) {
   allow_next();
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -901,10 +898,9 @@ extern "C" int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void*
   p.out = static_cast<__nv_bfloat16*>(out);
   p.lse = lse;
   const int64_t pairs = (int64_t)batch * heads_k;
-  const int ctas = (rotate ? kResidentRotate : kResident) * kNumSMs;      // one wave
   p.splits = 1;
   if (mask != nullptr) {
-    const int64_t most = ctas / pairs;
+    const int64_t most = kMaxCtas / pairs;
     p.splits = most < 1 ? 1 : most > kMaxSplits ? kMaxSplits : (int)most;
   }
   cudaStream_t st = (cudaStream_t)stream;
@@ -936,7 +932,7 @@ extern "C" int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void*
   if (mask == nullptr) {
     grid = pairs * ceil_div64(capacity, kBlockN);
     IFV2_REQUIRE(grid <= INT32_MAX, IFV2_ERR_TOO_LARGE, "q8_decode: more than 2^31-1 blocks of 64 keys");
-    if (grid > ctas) grid = ctas;
+    if (grid > kMaxCtas) grid = kMaxCtas;
   }
   e = launch(kernel, dim3((unsigned)grid), kThreads, kSmemBytes, st, prepared, map_k, map_v, p);
   if (e != cudaSuccess) return set_error((int)e, "q8_split: launch failed: %s", cudaGetErrorString(e));
