@@ -10,6 +10,7 @@ A row's value is code * scale.  The scale is the smallest power of two (at least
 magnitude fits the codes (448 or 127), codes are rounded to nearest even, and reading back is exact.  A row with an
 infinity or a NaN reads back as NaN.  Writes to pages, slots or positions that the cache does not have are dropped,
 reads of them give NaN.  Two tokens of one call that go to the same row leave one of them."""
+import functools
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
@@ -64,6 +65,11 @@ def _table(what, block_table, batch, dev):
     if len(shape) != 2 or shape[1] < 1:
         raise ValueError(f"{what}: block_table must be (batch, max_pages) int32")
     return _ints(what, "block_table", block_table, (batch, shape[1]), dev), shape[1]
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(batch, heads):
+    return int(_lib.load().ifv2_q8_decode_workspace_bytes(batch, heads, HEAD_DIM))
 
 
 def _ptr(t):
@@ -122,7 +128,7 @@ def cache_read_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.T
     start = _ints(what, "start", start, (batch,), dev)
     if total < 0:
         raise ValueError(f"{what}: total must not be negative")
-    k = torch.empty(total, hk, HEAD_DIM, dtype=torch.bfloat16, device=dev)
+    k = torch.empty_strided((total, hk, HEAD_DIM), (hk * HEAD_DIM, HEAD_DIM, 1), dtype=torch.bfloat16, device=dev)
     v = torch.empty_like(k)
     with _on(dev):
         _lib.call("ifv2_q8_read", k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), k.data_ptr(),
@@ -248,8 +254,8 @@ def infllmv2_attn_with_kvcache_q8(
         rotary = (cos.data_ptr(), sin.data_ptr(), at.data_ptr(), axis_stride, pair_axis, axes, 2 * pairs, rows)
     q = q.contiguous()
     out = torch.empty_like(q)
-    lse = torch.empty(batch, heads, 1, dtype=torch.float32, device=dev) if return_softmax_lse else None
-    ws_bytes = int(_lib.load().ifv2_q8_decode_workspace_bytes(batch, heads, HEAD_DIM))
+    lse = torch.empty_strided((batch, heads, 1), (heads, 1, 1), dtype=torch.float32, device=dev) if return_softmax_lse else None
+    ws_bytes = _workspace_bytes(batch, heads)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     with _on(dev):
         _lib.call("ifv2_q8_decode", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),

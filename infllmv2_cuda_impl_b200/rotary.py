@@ -69,19 +69,24 @@ def _rows(x):
     return x, a, b
 
 
+def _dense_like(x):
+    """An empty (tokens, heads, 128) tensor of x's kind, dense in this order.  (torch.empty takes twice the time.)"""
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
 def _rotate(q, k, rotary_cos, rotary_sin, positions, sections, interleaved, back):
     """Returns (q, k) rotated, dense; k may be None."""
     shape, dev = q.shape, q.device
     cos, sin, positions, axis_stride, pair_axis, axes, rows, pairs = _tables("rotary_axes", rotary_cos, rotary_sin, positions,
                                                                              sections, shape[0], dev)
     q, q_token, q_head = _rows(q)
-    q_out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+    q_out = _dense_like(q)
     k_out = k_ptr = k_out_ptr = None
     heads_k = k_token = k_head = 0
     if k is not None:
         k, k_token, k_head = _rows(k)
         heads_k = k.shape[1]
-        k_out = torch.empty(k.shape, dtype=torch.bfloat16, device=dev)
+        k_out = _dense_like(k)
         k_ptr, k_out_ptr = k.data_ptr(), k_out.data_ptr()
     with _on(dev):
         _lib.call("ifv2_rotary_axes", q.data_ptr(), k_ptr, q_out.data_ptr(), k_out_ptr, cos.data_ptr(), sin.data_ptr(),
