@@ -30,7 +30,8 @@ struct MoveParams {
 __device__ __forceinline__ int64_t token_row(const MoveParams& p, int64_t t) {
   if (t >= p.total || t >= p.cu[p.batch]) return -2;
   const int b = find_sequence(p.cu, p.batch, (int)t);
-  return p.place.row0(b, t - p.cu[b] + (p.start ? p.start[b] : 0));
+  const int64_t at = t - p.cu[b];
+  return at < 0 ? -2 : p.place.row0(b, at + (p.start ? p.start[b] : 0));
 }
 
 __device__ __forceinline__ void to_float(float (&x)[16], const uint4& a, const uint4& b) {

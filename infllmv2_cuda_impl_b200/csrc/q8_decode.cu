@@ -244,9 +244,10 @@ __device__ __forceinline__ void store_out(const Q8DecodeParams& p, int64_t qrow,
 // A CTA's blocks of one (sequence, KV head) at a time; each of its four warps streams 32-key units, K and V in turn,
 // through its own three slots of shared memory (4 KB, 128-byte swizzle, filled by TMA), so that two tiles are in flight
 // while another is worked on.  The 16 query heads are one M tile of mma.sync m16n8k16 in fp16, fp32 sums: codes become fp16
-// numbers exactly, a query row is scaled by a power of two into fp16's range (exact but for elements below 2^-39 of
-// its largest; a rotated one, which has 24 bits, becomes a sum of two fp16 rows), scales are applied to the scores and, as exponents, to the weights.  A weight is rounded to fp16 at
-// 2^8 to 2^15 times its share of the largest, 2^-12 relative down to 2^-22 of that and 2^-33 of it below.
+// numbers exactly, a query row is scaled by a power of two so that its largest element is 1 to 2 (exact but for elements
+// below 2^-16 of that, which are off by 2^-25 of it at most; a rotated row, which has 24 bits, becomes a sum of two fp16
+// rows), scales are applied to the scores and, as exponents, to the weights.  A weight is rounded to fp16 at 2^8 to 2^15
+// times its share of the largest, 2^-12 relative down to 2^-22 of that and 2^-33 of it below.
 //
 // The contraction order over the 128 features is free, so codes 4t .. 4t + 3 of a 16-feature chunk, one 32-bit word
 // of ldmatrix, serve as k = 2t, 2t + 1, 2t + 8, 2t + 9; the query is read in the same order.  V comes through the
@@ -259,7 +260,8 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   __shared__ uint64_t bars[kWarps][kSlots];
-  __shared__ __align__(16) float factors[kWarps][2][kUnit];      // of the unit at work: scales of the keys, exponents of the values
+  // of the unit at work: scales of the keys in two factors, exponents of the values
+  __shared__ __align__(16) float factors[kWarps][3][kUnit];
   // the query as A fragments: [high and low part][16-feature chunk][lane]
   __shared__ uint4 q_frag[kRotate ? 2 : 1][kHeadDim / 16][32];
   __shared__ float q_factor[kGroup];               // 2^x that undoes a row's scaling
@@ -443,8 +445,8 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       uint32_t amax = 0;
 #pragma unroll
       for (int u = 0; u < 4; ++u) amax = max(amax, abs_bits(x[u]));
-      const int e = min(max((int)(__reduce_max_sync(0xFFFFFFFFu, amax) >> 23), 15), 254);      // largest -> [2^14, 2^15)
-      const float f = __uint_as_float((uint32_t)(268 - e) << 23);
+      const int e = min(max((int)(__reduce_max_sync(0xFFFFFFFFu, amax) >> 23), 1), 253);      // the largest becomes 1 .. 2
+      const float f = __uint_as_float((uint32_t)(254 - e) << 23);
 #pragma unroll
       for (int u = 0; u < 4; u += 2) {
         const float y0 = mul_exact(x[u], f), y1 = mul_exact(x[u + 1], f);
@@ -457,10 +459,10 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
           reinterpret_cast<__half2*>(&q_frag[kRotate ? 1 : 0][lane >> 2][at])[word] = __floats2half2_rn(y0 - z.x, y1 - z.y);
         }
       }
-      if (lane == 0) q_factor[i] = __uint_as_float((uint32_t)(e - 14) << 23);
+      if (lane == 0) q_factor[i] = __uint_as_float((uint32_t)e << 23);
     }
     __syncthreads();
-    const float c0 = q_factor[g] * p.scale_log2, c1 = q_factor[g + 8] * p.scale_log2;
+    const float c0 = mul_exact(q_factor[g], p.scale_log2), c1 = mul_exact(q_factor[g + 8], p.scale_log2);
 
     float o[16][4];
 #pragma unroll
@@ -472,8 +474,10 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     while (key0 >= 0) {
       const uint32_t kt = tiles32 + slot_k * kTileBytes, vt = tiles32 + slot_v * kTileBytes;
       arrived(slot_k);
-      factors[warp][0][lane] = scale_value(kb);
-      factors[warp][1][lane] = vb == kNanByte ? __uint_as_float(0x7FC00000u) : (float)((int)vb - 127);
+      // 2^(kb - 127) = 2^a 2^b: with the query's factor between the two no product leaves the range that the score is in
+      factors[warp][0][lane] = kb == kNanByte ? __uint_as_float(0x7FC00000u) : __uint_as_float((64 + kb / 2) << 23);
+      factors[warp][1][lane] = __uint_as_float((63 + (kb + 1) / 2) << 23);
+      factors[warp][2][lane] = vb == kNanByte ? __uint_as_float(0x7FC00000u) : (float)((int)vb - 127);
       __syncwarp();
 
       // ---- S = Q . K^T (16 x 32)
@@ -506,13 +510,16 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 
       // ---- weights against reference maxima that move only when a weight would pass 2^15: the sum l against m, the
       //      weights of the values against M - 8 (see the file's head).  A unit whose weights pass is done again.
-      uint64_t ev[kUnit / 8], sp[kUnit / 8][2];    // pairs for keys 8 nt + 2t, + 1: exponents of values, q . K 2^e of two rows
+      // pairs for keys 8 nt + 2t, + 1: exponents of values, second factors of keys, scores without it of two rows
+      uint64_t ev[kUnit / 8], kb2[kUnit / 8], sp[kUnit / 8][2];
+      const uint64_t cc0 = tc::pack_f32x2(c0, c0), cc1 = tc::pack_f32x2(c1, c1);
 #pragma unroll
       for (int nt = 0; nt < kUnit / 8; ++nt) {
         const uint64_t ks = *reinterpret_cast<const uint64_t*>(&factors[warp][0][nt * 8 + 2 * t]);
-        ev[nt] = *reinterpret_cast<const uint64_t*>(&factors[warp][1][nt * 8 + 2 * t]);
-        sp[nt][0] = mul_exact2(tc::pack_f32x2(s[nt][0], s[nt][1]), ks);
-        sp[nt][1] = mul_exact2(tc::pack_f32x2(s[nt][2], s[nt][3]), ks);
+        kb2[nt] = *reinterpret_cast<const uint64_t*>(&factors[warp][1][nt * 8 + 2 * t]);
+        ev[nt] = *reinterpret_cast<const uint64_t*>(&factors[warp][2][nt * 8 + 2 * t]);
+        sp[nt][0] = mul_exact2(mul_exact2(tc::pack_f32x2(s[nt][0], s[nt][1]), ks), cc0);
+        sp[nt][1] = mul_exact2(mul_exact2(tc::pack_f32x2(s[nt][2], s[nt][3]), ks), cc1);
       }
       float sum[2];
       uint32_t pf[kUnit / 16][4];                  // weights as A fragments of the second product
@@ -521,15 +528,15 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         __half2 top;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const float c = r ? c1 : c0, m = r ? m1 : m0, u = r ? u1 : u0;
+          const float m = r ? m1 : m0, u = r ? u1 : u0;
           const float n = m == -INFINITY ? 0.f : -m, w = u == -INFINITY ? 0.f : 8.f - u;
-          const uint64_t cc = tc::pack_f32x2(c, c), nn = tc::pack_f32x2(n, n), ww = tc::pack_f32x2(w, w);
+          const uint64_t nn = tc::pack_f32x2(n, n), ww = tc::pack_f32x2(w, w);
           uint64_t total = 0;
 #pragma unroll
           for (int nt = 0; nt < kUnit / 8; ++nt) {
             float a0, a1, x0, x1;
-            tc::unpack_f32x2(tc::fma_f32x2(sp[nt][r], cc, nn), a0, a1);
-            tc::unpack_f32x2(tc::add_f32x2(tc::fma_f32x2(sp[nt][r], cc, ww), ev[nt]), x0, x1);
+            tc::unpack_f32x2(tc::fma_f32x2(sp[nt][r], kb2[nt], nn), a0, a1);
+            tc::unpack_f32x2(tc::add_f32x2(tc::fma_f32x2(sp[nt][r], kb2[nt], ww), ev[nt]), x0, x1);
             if (kTail) {
               if (key0 + nt * 8 + 2 * t >= len) a0 = x0 = -INFINITY;
               if (key0 + nt * 8 + 2 * t + 1 >= len) a1 = x1 = -INFINITY;
@@ -556,13 +563,13 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
           for (int e = 0; e < 2; ++e) {
             if (key0 + nt * 8 + 2 * t + e >= len) continue;
             float a[2], b2[2], ex[2];
-            tc::unpack_f32x2(sp[nt][0], a[0], a[1]);
-            tc::unpack_f32x2(sp[nt][1], b2[0], b2[1]);
+            tc::unpack_f32x2(mul_exact2(sp[nt][0], kb2[nt]), a[0], a[1]);
+            tc::unpack_f32x2(mul_exact2(sp[nt][1], kb2[nt]), b2[0], b2[1]);
             tc::unpack_f32x2(ev[nt], ex[0], ex[1]);
-            mx0 = fmaxf(mx0, a[e] * c0);
-            mx1 = fmaxf(mx1, b2[e] * c1);
-            mu0 = fmaxf(mu0, a[e] * c0 + ex[e]);
-            mu1 = fmaxf(mu1, b2[e] * c1 + ex[e]);
+            mx0 = fmaxf(mx0, a[e]);
+            mx1 = fmaxf(mx1, b2[e]);
+            mu0 = fmaxf(mu0, a[e] + ex[e]);
+            mu1 = fmaxf(mu1, b2[e] + ex[e]);
           }
         }
 #pragma unroll

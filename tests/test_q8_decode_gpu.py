@@ -296,7 +296,8 @@ def test_nan_rows(dtype):
 
 
 @pytest.mark.parametrize("dtype", [E4M3, INT8])
-@pytest.mark.parametrize("kexp,vexp,qexp", [(0, -100, 0), (0, 110, 0), (-60, 0, 60), (40, 0, -40), (0, -125, 0)])
+@pytest.mark.parametrize("kexp,vexp,qexp", [(0, -100, 0), (0, 110, 0), (-60, 0, 60), (40, 0, -40), (0, -125, 0), (115, 0, -115), (-112, 0, 112), (100, -60, -100),
+                                            (0, 0, -120), (-126, 0, 60)])
 def test_extreme_sizes(dtype, kexp, vexp, qexp):
     """Scores and values of an ordinary kind from factors far from 1."""
     k, v = det_tensor((1, 1, 100, 128), 3, 1.0), det_tensor((1, 1, 100, 128), 4, 1.0)
@@ -313,6 +314,16 @@ def test_extreme_sizes(dtype, kexp, vexp, qexp):
         assert bool(((out.cpu().double()[:, 0] - want).abs() <= 2.0 ** -8 * want.abs() + avg * 2.0 ** -9 + 2.0 ** -126).all())
     else:
         _check(out, lse, q, cache, [100])
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.2])
+def test_scales_of_zero_and_below(scale):
+    cache = _cache(2, 130, 1, INT8, 3)
+    q = det_tensor((2, 1, 16, 128), 7, 1.5)
+    lens = [130, 77]
+    out, lse = infllm_v2.infllmv2_attn_with_kvcache_q8(q.to(DEV), *_to_gpu(cache), softmax_scale=scale, return_softmax_lse=True,
+                                                       cache_seqlens=torch.tensor(lens, dtype=torch.int32, device=DEV))
+    _check(out, lse, q, cache, lens, scale=scale)
 
 
 def test_values_that_differ_by_many_orders():
