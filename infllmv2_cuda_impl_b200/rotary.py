@@ -74,11 +74,10 @@ def _dense_like(x):
     return torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
-def _rotate(q, k, rotary_cos, rotary_sin, positions, sections, interleaved, back):
-    """Returns (q, k) rotated, dense; k may be None."""
-    shape, dev = q.shape, q.device
-    cos, sin, positions, axis_stride, pair_axis, axes, rows, pairs = _tables("rotary_axes", rotary_cos, rotary_sin, positions,
-                                                                             sections, shape[0], dev)
+def _turn(q, k, tables, interleaved, back):
+    """(q, k) rotated, dense; k may be None.  tables: what `_tables` returns."""
+    cos, sin, positions, axis_stride, pair_axis, axes, rows, pairs = tables
+    dev, (tokens, heads, _) = q.device, q.shape
     q, q_token, q_head = _rows(q)
     q_out = _dense_like(q)
     k_out = k_ptr = k_out_ptr = None
@@ -90,7 +89,7 @@ def _rotate(q, k, rotary_cos, rotary_sin, positions, sections, interleaved, back
         k_ptr, k_out_ptr = k.data_ptr(), k_out.data_ptr()
     with _on(dev):
         _lib.call("ifv2_rotary_axes", q.data_ptr(), k_ptr, q_out.data_ptr(), k_out_ptr, cos.data_ptr(), sin.data_ptr(),
-                  positions.data_ptr(), axis_stride, pair_axis, axes, shape[0], shape[1], heads_k, HEAD_DIM, q_token, q_head,
+                  positions.data_ptr(), axis_stride, pair_axis, axes, tokens, heads, heads_k, HEAD_DIM, q_token, q_head,
                   k_token, k_head, 2 * pairs, rows, interleaved, back, _stream(dev))
     return q_out, k_out
 
@@ -99,8 +98,10 @@ def _rotate(q, k, rotary_cos, rotary_sin, positions, sections, interleaved, back
 def _rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], rotary_cos: torch.Tensor, rotary_sin: torch.Tensor,
                  positions: torch.Tensor, sections: Optional[Sequence[int]], interleaved: bool,
                  back: bool) -> Tuple[torch.Tensor, torch.Tensor]:
-    """`_rotate` as a registered operator (an empty second result without k)."""
-    q_out, k_out = _rotate(q, k, rotary_cos, rotary_sin, positions, sections, interleaved, back)
+    """`_turn` as a registered operator (an empty second result without k)."""
+    tables = _tables("rotary_axes", rotary_cos, rotary_sin, positions, None if sections is None else tuple(sections), q.shape[0],
+                     q.device)
+    q_out, k_out = _turn(q, k, tables, interleaved, back)
     return q_out, k_out if k_out is not None else q_out.new_empty(0)
 
 
@@ -109,10 +110,12 @@ def _(q, k, rotary_cos, rotary_sin, positions, sections, interleaved, back):
     return q.new_empty(q.shape), k.new_empty(k.shape) if k is not None else q.new_empty(0)
 
 
-def _call(q, k, rotary_cos, rotary_sin, positions, sections, interleaved, back):
-    """The body where nothing watches operators, the registered operator elsewhere."""
-    if not torch.compiler.is_compiling() and not _profiled() and _plain_eager(q, k, rotary_cos, rotary_sin, positions):
-        return _rotate(q, k, rotary_cos, rotary_sin, positions, sections, interleaved, back)
+def _direct(*tensors) -> bool:
+    """True where nothing watches operators: the body is called then, the registered operator elsewhere."""
+    return not torch.compiler.is_compiling() and not _profiled() and _plain_eager(*tensors)
+
+
+def _registered(q, k, rotary_cos, rotary_sin, positions, sections, interleaved, back):
     q, k_out = _rotary_axes(q, k, rotary_cos, rotary_sin, positions, None if sections is None else list(sections), interleaved, back)
     return q, k_out if k is not None else None
 
@@ -122,26 +125,39 @@ class RotaryAxesFunc(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, rotary_cos, rotary_sin, positions, sections, interleaved, back):
-        ctx.save_for_backward(rotary_cos, rotary_sin, positions)
         ctx.sections, ctx.interleaved, ctx.back = sections, interleaved, back
         ctx.set_materialize_grads(False)
-        return _call(q, k, rotary_cos, rotary_sin, positions, sections, interleaved, back)
+        if _direct(q, k, rotary_cos, rotary_sin, positions):
+            tables = _tables("rotary_axes", rotary_cos, rotary_sin, positions, sections, q.shape[0], q.device)
+            ctx.save_for_backward(*tables[:3])
+            ctx.known = tables[3:]                      # (checked once: the backward pass is bound by its host time)
+            return _turn(q, k, tables, interleaved, back)
+        ctx.save_for_backward(rotary_cos, rotary_sin, positions)
+        ctx.known = None
+        return _registered(q, k, rotary_cos, rotary_sin, positions, sections, interleaved, back)
 
     @staticmethod
     def backward(ctx, dq, dk):
-        cos, sin, positions = ctx.saved_tensors
-        args = (cos, sin, positions, ctx.sections, ctx.interleaved, not ctx.back)
         dq = dq if ctx.needs_input_grad[0] else None
         dk = dk if ctx.needs_input_grad[1] else None
-        if dq is None:
-            return (None, _rotary_maybe_grad(dk, None, *args)[0] if dk is not None else None) + (None,) * 6
-        return _rotary_maybe_grad(dq, dk, *args) + (None,) * 6
+        one, other = (dk, None) if dq is None else (dq, dk)      # the body wants a first tensor
+        if one is None:
+            return (None,) * 8
+        tables = ctx.saved_tensors
+        if ctx.known is not None and not torch.is_grad_enabled() and _direct(one, other):
+            one, other = _turn(one, other, tables + ctx.known, ctx.interleaved, not ctx.back)
+        else:
+            one, other = _rotary_maybe_grad(one, other, *tables, ctx.sections, ctx.interleaved, not ctx.back)
+        return ((None, one) if dq is None else (one, other)) + (None,) * 6
 
 
-def _rotary_maybe_grad(q, k, *args):
+def _rotary_maybe_grad(q, k, rotary_cos, rotary_sin, positions, sections, interleaved, back):
     if (q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled():
-        return RotaryAxesFunc.apply(q, k, *args)
-    return _call(q, k, *args)
+        return RotaryAxesFunc.apply(q, k, rotary_cos, rotary_sin, positions, sections, interleaved, back)
+    if _direct(q, k, rotary_cos, rotary_sin, positions):
+        return _turn(q, k, _tables("rotary_axes", rotary_cos, rotary_sin, positions, sections, q.shape[0], q.device),
+                     interleaved, back)
+    return _registered(q, k, rotary_cos, rotary_sin, positions, sections, interleaved, back)
 
 
 def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], rotary_cos: torch.Tensor, rotary_sin: torch.Tensor,
