@@ -512,10 +512,11 @@ int64_t ifv2_q8_decode_workspace_bytes(int batch, int heads_q, int head_dim);
  * k_new / v_new (batch, heads_k, 128) or null are first written at position cache_seqlens[b]; with rotary tables
  * the new key and the query are rotated (as by ifv2_rotary_axes, but in fp32 without a rounding to bf16) at
  * rotary_positions (axes rows of axis_stride, batch columns; null: cache_seqlens) before the key is quantised.
- * topk_idx (batch, heads_k, topk) or null is packed into mask (batch, heads_k, mask_words); topk_idx null: mask is
- * given, or null = all keys.  lse (batch, heads_q) fp32 or null.  Pages are a multiple of 16 positions.
+ * topk_idx (batch, heads_k, topk) or null: 64-key blocks to attend; lists of more than 256 are packed into mask
+ * (batch, heads_k, mask_words; shorter ones leave it as it is, and it may be null).  topk_idx null: mask is given,
+ * or null = all keys.  lse (batch, heads_q) fp32 or null.  Pages are a multiple of 16 positions.
  * A sequence attends positions [0, min(cache_seqlens[b] + new, capacity)); a new token without room is neither
- * written nor attended, a negative length attends nothing.  Sequences without keys get out = 0, lse = +inf. */
+ * written nor attended, a negative length attends nothing.  Sequences without keys get out = 0, lse = +inf.  batch * heads_k <= 65535. */
 int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void* k_scale, void* v_scale, const void* k_new,
                    const void* v_new, const float* rotary_cos, const float* rotary_sin,
                    const int32_t* rotary_positions, int64_t axis_stride, const uint8_t* pair_axis, int axes,

@@ -9,7 +9,7 @@
 // values take part in the weights, next to the scores, so that the largest weight is about 1 whatever the values' sizes
 // are, and out = O 2^(M - m) / l.  (m and M differ by little more than 127, the range of the exponents.)
 //
-// Launches: [prepare: block lists, append where sequences may share rows] -> split -> combine.
+// Launches: [prepare: long block lists, append where sequences may share rows] -> split -> combine.
 #include <type_traits>
 #include "block_list.cuh"
 #include "mma_sync.cuh"
@@ -32,6 +32,7 @@ constexpr int kSmemBytes = kWarps * kSlots * kTileBytes + 1024;
 constexpr int kMaxSplits = 32;                   // CTAs that share the selected blocks of a (sequence, KV head)
 constexpr int kMaxCtas = kResident * kNumSMs;    // one wave: the CTAs that share all blocks where there is no mask
 constexpr uint32_t kStart = 4;              // blocks that the start of a head costs (see Deal)
+constexpr int kMaxList = 2 * kThreads;           // longest block list that the split kernel takes itself
 constexpr long long kWaitLimit = 1ll << 28;      // clocks; a copy takes microseconds
 constexpr int kPartialFloats = kHeadDim + 4;     // O row, m (log2 units), l, exponent of O's units, pad
 constexpr float kLog2e = 1.4426950408889634f;
@@ -47,6 +48,8 @@ struct Q8DecodeParams {
   const __nv_bfloat16* v_new;
   const unsigned long long* mask;  // (batch, heads_k, mask_words) or null = all positions
   int mask_words;
+  const int32_t* topk_idx;         // (batch, heads_k, topk <= kMaxList) block lists in place of a mask, or null
+  int topk;
   const int32_t* cache_seqlens;
   Place place;
   int64_t capacity;
@@ -227,6 +230,45 @@ __device__ __forceinline__ int find_block(const Q8DecodeParams& p, uint32_t at, 
   return p.batch;
 }
 
+// A block list as the split kernel walks it: the blocks below nblk, ascending, each once; returns their number.  Lists
+// come ascending with their unused entries last as a rule, which one look confirms; others are ranked entry by entry.
+__device__ __forceinline__ int sort_list(int* list, const int32_t* src, int topk, int nblk) {
+  constexpr int kNone = 0x7FFFFFFF;
+  const int tid = threadIdx.x;
+  int mine[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int i = tid + u * kThreads, x = i < topk ? __ldg(src + i) : -1;
+    mine[u] = x >= 0 && x < nblk ? x : kNone;
+    list[i] = mine[u];
+  }
+  int n = __syncthreads_count(mine[0] != kNone);
+  n += __syncthreads_count(mine[1] != kNone);
+  bool ascending = true;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int i = tid + u * kThreads, next = i + 1 < kMaxList ? list[i + 1] : kNone;
+    ascending &= mine[u] < next || next == kNone;
+  }
+  if (__syncthreads_and(ascending)) return n;
+  bool again[2] = {false, false};                 // an entry that stands before already
+  for (int u = 0; u < 2; ++u)
+    for (int j = 0; j < tid + u * kThreads && j < topk; ++j) again[u] |= list[j] == mine[u];
+  __syncthreads();
+  for (int u = 0; u < 2; ++u)
+    if (again[u]) list[tid + u * kThreads] = mine[u] = kNone;
+  n = __syncthreads_count(mine[0] != kNone);
+  n += __syncthreads_count(mine[1] != kNone);
+  int rank[2] = {0, 0};
+  for (int u = 0; u < 2; ++u)
+    for (int j = 0; j < topk; ++j) rank[u] += list[j] < mine[u];
+  __syncthreads();
+  for (int u = 0; u < 2; ++u)
+    if (mine[u] != kNone) list[rank[u]] = mine[u];
+  __syncthreads();
+  return n;
+}
+
 // A partial sum in units of 2^m as one in units of 2^top.  Without a finite m it is 0, or NaN and stays so.
 __device__ __forceinline__ float join_weight(float m, float top) { return m == -INFINITY ? 1.f : exp2f(m - top); }
 
@@ -271,6 +313,7 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   // the query as A fragments: [high and low part][16-feature chunk][lane]
   __shared__ uint4 q_frag[kRotate ? 2 : 1][kHeadDim / 16][32];
   __shared__ float q_factor[kGroup];               // 2^x that undoes a row's scaling
+  __shared__ int block_list[kMaxList];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   uint8_t* tiles = smem + warp * kSlots * kTileBytes;
   if (lane == 0) {
@@ -293,8 +336,8 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   uint32_t phases = 0;                             // bit i: parity of the next completion of slot i
   bool expired = false;                            // a bounded wait ran out: the result is poisoned
 
-  // the CTA's share: blocks [at, end) of the row of all blocks, or split `split` of a mask's blocks
-  const bool dealt = p.mask == nullptr;
+  // the CTA's share: blocks [at, end) of the row of all blocks, or split `split` of the selected blocks
+  const bool listed = p.topk_idx != nullptr, dealt = p.mask == nullptr && !listed;
   int b = 0, h = 0, split = 0;
   uint32_t at = 0, end = 0, before = 0;
   if (dealt) {
@@ -346,12 +389,12 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     for (int i = 0; i < kGroup / kWarps; ++i) q_part[i].load(p.q + (pair * kGroup + warp + kWarps * i) * kHeadDim, lane, angles.mate);
 
     wait_previous();                               // (the mask, or a new row of shared pages)
-    BlockList<2> list{dealt ? nullptr : p.mask + ((int64_t)b * p.heads_k + h) * p.mask_words, p.mask_words, n, -1};
+    BlockList<2> list{p.mask ? p.mask + pair * p.mask_words : nullptr, p.mask_words, n, -1};
     if (dealt) {
       j0 = (int)(max(v0, kStart) - kStart);
       j1 = (int)(v1 - kStart);
     } else {
-      n = list.count(lane);
+      n = listed ? sort_list(block_list, p.topk_idx + pair * p.topk, p.topk, n) : list.count(lane);
       const int per = (n + p.splits - 1) / p.splits;
       j0 = split * per;
       j1 = min(n, j0 + per);
@@ -362,7 +405,8 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       const int pos = p.cache_seqlens[b];
       if (pos >= 0 && pos < p.capacity) {
         const int blk = pos / kBlockN;
-        const bool attended = dealt || (blk / 64 < p.mask_words && ((__ldg(list.words + blk / 64) >> (blk & 63)) & 1ull));
+        const bool attended = dealt || (listed ? n > 0 && block_list[n - 1] == blk
+                                               : blk / 64 < p.mask_words && ((__ldg(list.words + blk / 64) >> (blk & 63)) & 1ull));
         const int owner = attended ? (((n - 1 - j0) & 1) << 1) | ((pos / kUnit) & 1) : 0;
         if ((attended ? j0 < j1 && j1 == n : split == 0) && warp == owner) {
           const int64_t row = ((int64_t)b * p.heads_k + h) * p.place.length + pos;
@@ -386,7 +430,7 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     int j = j0 + (warp >> 1), lookups = 0;
     auto next_key = [&]() -> int {                 // first key of the next unit, or -1
       while (j < j1) {
-        const int blk = list.nth(lookups++, j, lane);
+        const int blk = listed ? block_list[j] : list.nth(lookups++, j, lane);
         j += 2;
         const int key0 = blk * kBlockN + (warp & 1) * kUnit;
         if (blk >= 0 && key0 < len) return key0;
@@ -732,7 +776,7 @@ __global__ void __launch_bounds__(256) q8_combine_kernel(const Q8DecodeParams p,
   int64_t first = pair * p.splits;                  // (of partials)
   int n = p.splits;
   bool start_slot = false;                          // the first partial lies in its CTA's second place
-  if (p.mask == nullptr) {
+  if (p.mask == nullptr && p.topk_idx == nullptr) {
     uint32_t extents = 0, before = 0;               // of all sequences, of those before b
     for (int i = lane; i < p.batch; i += 32) {
       const uint32_t v = extent(blocks_of(p, i));
@@ -868,9 +912,12 @@ extern "C" int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void*
   const bool rotate = rotary_cos != nullptr;
   IFV2_REQUIRE(rotate == (rotary_sin != nullptr) && (!rotate || k_new), IFV2_ERR_INVALID_ARG,
                "q8_decode: rotation takes both tables and a new key");
-  IFV2_REQUIRE(topk_idx == nullptr || (mask != nullptr && topk >= 0), IFV2_ERR_INVALID_ARG, "q8_decode: block lists need a mask buffer");
+  const bool listed = topk_idx != nullptr && topk >= 0 && topk <= kMaxList;      // the split kernel takes short lists as they are
+  if (listed) mask = nullptr;
+  IFV2_REQUIRE(topk_idx == nullptr || listed || (mask != nullptr && topk >= 0), IFV2_ERR_INVALID_ARG,
+               "q8_decode: lists of more than %d blocks need a mask buffer", kMaxList);
   IFV2_REQUIRE(mask == nullptr || mask_words >= 1, IFV2_ERR_INVALID_ARG, "q8_decode: mask_words < 1");
-  IFV2_REQUIRE(topk_idx == nullptr || mask_words <= 4096, IFV2_ERR_TOO_LARGE, "q8_decode: more than 4096 mask words");
+  IFV2_REQUIRE(topk_idx == nullptr || listed || mask_words <= 4096, IFV2_ERR_TOO_LARGE, "q8_decode: more than 4096 mask words");
   if (block_table != nullptr) {
     IFV2_REQUIRE(length % 16 == 0 && block_table_stride >= 1, IFV2_ERR_INVALID_ARG,
                  "q8_decode: page size must be a positive multiple of 16");
@@ -909,6 +956,8 @@ extern "C" int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void*
   }
   p.mask = reinterpret_cast<const unsigned long long*>(mask);
   p.mask_words = mask_words;
+  p.topk_idx = listed ? topk_idx : nullptr;
+  p.topk = topk;
   p.cache_seqlens = cache_seqlens;
   p.place = Place{block_table, cache_batch_idx, block_table_stride, heads_k, (int)length, (int)slots};
   p.capacity = capacity;
@@ -920,18 +969,19 @@ extern "C" int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void*
   p.out = static_cast<__nv_bfloat16*>(out);
   p.lse = lse;
   const int64_t pairs = (int64_t)batch * heads_k;
+  const bool selected = listed || mask != nullptr;
   p.splits = 1;
-  if (mask != nullptr) {
+  if (selected) {
     const int64_t most = kMaxCtas / pairs;
     p.splits = most < 1 ? 1 : most > kMaxSplits ? kMaxSplits : (int)most;
   }
   cudaStream_t st = (cudaStream_t)stream;
-  const bool prepared = (k_new != nullptr && shared_rows) || topk_idx != nullptr;
+  const bool packed = topk_idx != nullptr && !listed, prepared = (k_new != nullptr && shared_rows) || packed;
   if (prepared) {
     const Q8PrepareParams a{shared_rows ? static_cast<const __nv_bfloat16*>(k_new) : nullptr, static_cast<const __nv_bfloat16*>(v_new),
                             static_cast<uint8_t*>(k_cache), static_cast<uint8_t*>(v_cache), static_cast<uint8_t*>(k_scale),
-                            static_cast<uint8_t*>(v_scale), topk_idx, reinterpret_cast<unsigned long long*>(mask), topk, mask_words};
-    const size_t smem = topk_idx ? (size_t)mask_words * 8 : 0;
+                            static_cast<uint8_t*>(v_scale), packed ? topk_idx : nullptr, reinterpret_cast<unsigned long long*>(mask), topk, mask_words};
+    const size_t smem = packed ? (size_t)mask_words * 8 : 0;
     if (code == kE4m3) q8_prepare_kernel<kE4m3><<<dim3(heads_k, batch), kThreads, smem, st>>>(a, p);
     else q8_prepare_kernel<kInt8><<<dim3(heads_k, batch), kThreads, smem, st>>>(a, p);
     int rc = check_launch("q8_prepare");
@@ -951,15 +1001,15 @@ extern "C" int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void*
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
   if (e != cudaSuccess) return set_error((int)e, "q8_decode: %s", cudaGetErrorString(e));
   int64_t grid = pairs * p.splits;
-  if (mask == nullptr) {
+  if (!selected) {
     grid = pairs * (ceil_div64(capacity, kBlockN) + kStart);
     IFV2_REQUIRE(grid <= INT32_MAX, IFV2_ERR_TOO_LARGE, "q8_decode: more than 2^31-1 blocks of 64 keys");
     if (grid > kMaxCtas) grid = kMaxCtas;
   }
   e = launch(kernel, dim3((unsigned)grid), kThreads, kSmemBytes, st, prepared, map_k, map_v, p);
   if (e != cudaSuccess) return set_error((int)e, "q8_split: launch failed: %s", cudaGetErrorString(e));
-  if (mask != nullptr && p.splits == 1) return IFV2_OK;      // the split kernel wrote the results
-  const int64_t per_pair = mask != nullptr ? p.splits : ceil_div64(grid, pairs);
+  if (selected && p.splits == 1) return IFV2_OK;      // the split kernel wrote the results
+  const int64_t per_pair = selected ? p.splits : ceil_div64(grid, pairs);
   const int warps = per_pair > 16 ? 8 : per_pair > 6 ? 4 : 1;      // that share a row's partials
   auto join = warps == 8 ? q8_combine_kernel<8> : warps == 4 ? q8_combine_kernel<4> : q8_combine_kernel<1>;
   e = launch(join, dim3(2 * warps, (unsigned)pairs), 256, 0, st, true, p, (int)grid);

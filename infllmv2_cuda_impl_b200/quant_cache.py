@@ -20,6 +20,7 @@ from .attention import BLOCK_N, GROUP, HEAD_DIM
 from .ops import _on, _require_cuda, _stream
 from .rotary import _rows, _tables
 
+_LIST = 256      # longest block list that the attention takes without a mask
 _CODES = {torch.float8_e4m3fn: 0, torch.int8: 1}
 
 
@@ -242,8 +243,10 @@ def infllmv2_attn_with_kvcache_q8(
                 or topk_idx.numel() != batch * hk * topk_idx.shape[-1]:
             raise ValueError(f"{what}: topk_idx must be ({batch}, {hk}, 1, topk) int32 on {dev}")
         topk_idx, topk = topk_idx.contiguous(), topk_idx.shape[-1]
-        block_mask = torch.empty(batch, hk, 1, words, dtype=torch.int64, device=dev)
-        mask_ptr, idx_ptr = block_mask.data_ptr(), topk_idx.data_ptr()
+        idx_ptr = topk_idx.data_ptr()
+        if topk > _LIST:                                 # (shorter lists are walked as they are)
+            block_mask = torch.empty(batch, hk, 1, words, dtype=torch.int64, device=dev)
+            mask_ptr = block_mask.data_ptr()
     rotary = (None, None, None, 0, None, 0, 0, 0)
     if rotary_cos is not None and k is not None:
         if rotary_sections is not None and type(rotary_sections) is not tuple:

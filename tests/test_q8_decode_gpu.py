@@ -88,7 +88,8 @@ def _lists(lens, hk, k, seed, dup=False):
 @pytest.mark.parametrize("lens,hk,page,topk", [
     ([1], 1, 0, 0), ([0, 1, 31, 32, 33, 63, 64, 65], 2, 0, 0), ([700, 0, 130], 2, 16, 0), ([513, 100, 1000], 1, 48, 0),
     ([300], 8, 64, 0), ([2000], 1, 256, 0), ([129, 1000, 64], 2, 0, 3), ([900, 1, 77, 0], 2, 16, 4), ([4097], 2, 64, 70),
-    ([90] * 40, 4, 0, 0), ([640] * 9, 16, 64, 5)])
+    ([90] * 40, 4, 0, 0), ([640] * 9, 16, 64, 5),
+    ([20011, 300], 1, 0, 300), ([16500], 1, 16, 256), ([700] * 30, 8, 0, 9)])
 def test_attention(dtype, lens, hk, page, topk):
     batch, most = len(lens), max(lens)
     table = None
@@ -112,6 +113,22 @@ def test_attention(dtype, lens, hk, page, topk):
         mask = infllm_v2.topk_to_uint64(idx.to(DEV), cap, 64)[0]
         got = infllm_v2.infllmv2_attn_with_kvcache_q8(q.to(DEV), *dev, block_mask=mask, **args)
         assert torch.equal(got[0], out) and torch.equal(got[1], lse)
+
+
+@pytest.mark.parametrize("dtype", [E4M3, INT8])
+def test_lists_in_any_order(dtype):
+    """Lists that are not ascending, hold entries twice, past the keys, or unused ones in between."""
+    cache = _cache(3, 2000, 2, dtype, 3)
+    q = det_tensor((3, 1, 32, 128), 7, 1.5)
+    lens = [2000, 900, 64]
+    idx = torch.tensor([[5, 3, 3, 31, 0, 40, -1, 7], [14, -1, 2, 13, 14, 0, -1, 2], [0, 0, -1, 1, 9, 0, 0, -1]], dtype=torch.int32)
+    idx = torch.stack([idx, idx.flip(1)], 1)[:, :, None].contiguous()
+    args = dict(cache_seqlens=torch.tensor(lens, dtype=torch.int32, device=DEV), return_softmax_lse=True)
+    out, lse = infllm_v2.infllmv2_attn_with_kvcache_q8(q.to(DEV), *_to_gpu(cache), topk_idx=idx.to(DEV), **args)
+    _check(out, lse, q, cache, lens, topk_idx=idx)
+    mask = infllm_v2.topk_to_uint64(idx.to(DEV), 2000, 64)[0]
+    got = infllm_v2.infllmv2_attn_with_kvcache_q8(q.to(DEV), *_to_gpu(cache), block_mask=mask, **args)
+    assert torch.equal(got[0], out) and torch.equal(got[1], lse)
 
 
 @pytest.mark.parametrize("dtype", [E4M3, INT8])

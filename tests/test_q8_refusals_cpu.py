@@ -226,8 +226,8 @@ def _decode_args(**kw):
 
 @pytest.mark.parametrize("change,code", [
     (dict(d=64), -2), (dict(hq=32), -2), (dict(code=7), -1), (dict(length=0), -1), (dict(q=None), -1), (dict(k=P), -1), (dict(cos=P, sin=P), -1),
-    (dict(k=P, v=P, cos=P), -1), (dict(k=P, v=P, cos=P, sin=P, dim=128, rows=4, axes=0), -1), (dict(idx=P, topk=4), -1), (dict(mask=P), -1),
-    (dict(idx=P, topk=4, mask=P, words=5000), -3), (dict(table=P, pages=2, length=24), -1), (dict(table=P, pages=2, bidx=P), -2),
+    (dict(k=P, v=P, cos=P), -1), (dict(k=P, v=P, cos=P, sin=P, dim=128, rows=4, axes=0), -1), (dict(idx=P, topk=257), -1), (dict(idx=P, topk=-1), -1), (dict(mask=P), -1),
+    (dict(idx=P, topk=300, mask=P, words=5000), -3), (dict(table=P, pages=2, length=24), -1), (dict(table=P, pages=2, bidx=P), -2),
     (dict(slots=1), -1), (dict(slots=1 << 20, length=1 << 20), -3), (dict(table=P, pages=1 << 30), -3), (dict(bytes=16), -1),
     (dict(q=P + 8), -1), (dict(batch=70000, slots=70000), -3)])
 def test_c_decode_refusals(lib, change, code):
