@@ -32,6 +32,7 @@ constexpr int kSmemBytes = kWarps * kSlots * kTileBytes + 1024;
 constexpr int kMaxSplits = 32;                   // CTAs that share the selected blocks of a (sequence, KV head)
 constexpr int kMaxCtas = kResident * kNumSMs;    // one wave: the CTAs that share all blocks where there is no mask
 constexpr uint32_t kStart = 4;              // blocks that the start of a head costs (see Deal)
+constexpr int kUsualBlocks = 64;                 // blocks that a mask row is taken to select
 constexpr int kMaxList = 2 * kThreads;           // longest block list that the split kernel takes itself
 constexpr long long kWaitLimit = 1ll << 28;      // clocks; a copy takes microseconds
 constexpr int kPartialFloats = kHeadDim + 4;     // O row, m (log2 units), l, exponent of O's units, pad
@@ -53,7 +54,9 @@ struct Q8DecodeParams {
   const int32_t* cache_seqlens;
   Place place;
   int64_t capacity;
-  int batch, heads_k, new_tokens, splits, rotate;
+  int batch, heads_k, new_tokens, rotate;
+  int splits;                      // CTAs that share a (sequence, KV head) each, or 0: the blocks are dealt (see Deal)
+  int most_blocks;                 // a head counts for so many blocks in the deal at most
   RotaryParams rotary;
   float scale_log2;
   float* partial;                  // (batch, heads_k, splits | 2 per CTA, 16, kPartialFloats)
@@ -176,8 +179,10 @@ __global__ void __launch_bounds__(kThreads) q8_prepare_kernel(const Q8PreparePar
   }
 }
 
-// Blocks of 64 keys that one sequence's head attends without a mask, and its length in the row below.
-__device__ __forceinline__ int blocks_of(const Q8DecodeParams& p, int b) { return (keys_of(p, b) + kBlockN - 1) / kBlockN; }
+// Blocks of 64 keys that one sequence's head counts for in the deal, and the length of its place there.
+__device__ __forceinline__ int blocks_of(const Q8DecodeParams& p, int b) {
+  return min((keys_of(p, b) + kBlockN - 1) / kBlockN, p.most_blocks);
+}
 __device__ __forceinline__ uint32_t extent(int blocks) { return blocks ? kStart + blocks : 0; }
 
 // Without a mask the blocks of all sequences and heads are one row of `total` blocks, sequence by sequence, head by
@@ -337,7 +342,7 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   bool expired = false;                            // a bounded wait ran out: the result is poisoned
 
   // the CTA's share: blocks [at, end) of the row of all blocks, or split `split` of the selected blocks
-  const bool listed = p.topk_idx != nullptr, dealt = p.mask == nullptr && !listed;
+  const bool listed = p.topk_idx != nullptr, selected = listed || p.mask != nullptr, dealt = p.splits == 0;
   int b = 0, h = 0, split = 0;
   uint32_t at = 0, end = 0, before = 0;
   if (dealt) {
@@ -366,18 +371,20 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   };
   while (true) {
     const int len = keys_of(p, b);
-    int n = (len + kBlockN - 1) / kBlockN, j0, j1;
-    uint32_t v0 = 0, v1 = 0;                       // the CTA's part of the head's place
+    uint32_t w0 = split, w1 = split + 1, nw = p.splits, used = 0;      // the CTA's share of the head: w0 .. w1 - 1 of nw
     if (dealt) {
-      const uint32_t nv = extent(n);
-      h = (int)((at - before) / nv);
-      v0 = at - before - h * nv;
-      v1 = min(nv, v0 + end - at);
-    }
-    if (dealt && v1 <= kStart) {                   // (nothing to do for this head)
-      wait_previous();
-      if (!advance(v1 - v0)) return;
-      continue;
+      nw = blocks_of(p, b);
+      const uint32_t place = kStart + nw;
+      h = (int)((at - before) / place);
+      const uint32_t v0 = at - before - h * place, v1 = min(place, v0 + end - at);
+      used = v1 - v0;
+      if (v1 <= kStart) {                          // (nothing to do for this head)
+        wait_previous();
+        if (!advance(used)) return;
+        continue;
+      }
+      w0 = max(v0, kStart) - kStart;
+      w1 = v1 - kStart;
     }
     const int64_t pair = (int64_t)b * p.heads_k + h;
     // the warp's rows of the query, on their way while the first tiles are asked for
@@ -389,26 +396,21 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     for (int i = 0; i < kGroup / kWarps; ++i) q_part[i].load(p.q + (pair * kGroup + warp + kWarps * i) * kHeadDim, lane, angles.mate);
 
     wait_previous();                               // (the mask, or a new row of shared pages)
-    BlockList<2> list{p.mask ? p.mask + pair * p.mask_words : nullptr, p.mask_words, n, -1};
-    if (dealt) {
-      j0 = (int)(max(v0, kStart) - kStart);
-      j1 = (int)(v1 - kStart);
-    } else {
-      n = listed ? sort_list(block_list, p.topk_idx + pair * p.topk, p.topk, n) : list.count(lane);
-      const int per = (n + p.splits - 1) / p.splits;
-      j0 = split * per;
-      j1 = min(n, j0 + per);
-    }
+    const int n_all = (len + kBlockN - 1) / kBlockN;
+    BlockList<2> list{p.mask ? p.mask + pair * p.mask_words : nullptr, p.mask_words, n_all, -1};
+    // blocks to attend, of which this CTA takes numbers j0 .. j1 - 1
+    const uint32_t n = listed ? sort_list(block_list, p.topk_idx + pair * p.topk, p.topk, n_all) : list.count(lane);
+    const int j0 = n == nw ? w0 : (int)((uint64_t)w0 * n / nw), j1 = n == nw ? w1 : (int)((uint64_t)w1 * n / nw);
 
-    // the new token's row, by the warp whose unit it belongs to (no CTA attends it: by the first warp of split 0)
+    // the new token's row, by the warp whose unit it belongs to (no CTA attends it: by the first warp of the first CTA)
     if (p.k_new != nullptr) {
       const int pos = p.cache_seqlens[b];
       if (pos >= 0 && pos < p.capacity) {
         const int blk = pos / kBlockN;
-        const bool attended = dealt || (listed ? n > 0 && block_list[n - 1] == blk
-                                               : blk / 64 < p.mask_words && ((__ldg(list.words + blk / 64) >> (blk & 63)) & 1ull));
+        const bool attended = !selected || (listed ? n > 0 && block_list[n - 1] == blk
+                                                   : blk / 64 < p.mask_words && ((__ldg(list.words + blk / 64) >> (blk & 63)) & 1ull));
         const int owner = attended ? (((n - 1 - j0) & 1) << 1) | ((pos / kUnit) & 1) : 0;
-        if ((attended ? j0 < j1 && j1 == n : split == 0) && warp == owner) {
+        if ((attended ? j0 < j1 && j1 == (int)n : w0 == 0) && warp == owner) {
           const int64_t row = ((int64_t)b * p.heads_k + h) * p.place.length + pos;
           RowPart k_part, v_part;
           k_part.load(p.k_new + pair * kHeadDim, lane, angles.mate);
@@ -728,8 +730,9 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       }
     }
     __syncthreads();
-    const bool whole = dealt ? j0 == 0 && j1 == n : p.splits == 1;
-    const int64_t part = dealt ? 2 * (int64_t)blockIdx.x + (j0 == 0) : (int64_t)blockIdx.x;
+    // all of the head: the result; in the deal the head's first blocks: the CTA's second place; otherwise its first
+    const bool whole = w0 == 0 && w1 == nw;
+    const int64_t part = dealt ? 2 * (int64_t)blockIdx.x + (w0 == 0) : (int64_t)blockIdx.x;
     for (int r = warp; r < kGroup; r += kWarps) {              // a row per warp, four features per lane
       const float* src = stage + r * kPartialFloats;
       float m = -INFINITY, unit = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
@@ -757,7 +760,7 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         if (lane == 0) *reinterpret_cast<float4*>(dst + kHeadDim) = make_float4(m, l, unit, 0.f);
       }
     }
-    if (!dealt || !advance(v1 - v0)) return;
+    if (!dealt || !advance(used)) return;
     tc::fence_proxy_async_smem();
     __syncthreads();                               // the stage is read before the next segment's copies land in it
   }
@@ -776,7 +779,7 @@ __global__ void __launch_bounds__(256) q8_combine_kernel(const Q8DecodeParams p,
   int64_t first = pair * p.splits;                  // (of partials)
   int n = p.splits;
   bool start_slot = false;                          // the first partial lies in its CTA's second place
-  if (p.mask == nullptr && p.topk_idx == nullptr) {
+  if (p.splits == 0) {
     uint32_t extents = 0, before = 0;               // of all sequences, of those before b
     for (int i = lane; i < p.batch; i += 32) {
       const uint32_t v = extent(blocks_of(p, i));
@@ -866,6 +869,18 @@ __global__ void __launch_bounds__(256) q8_combine_kernel(const Q8DecodeParams p,
 }  // namespace ifv2
 
 using namespace ifv2;
+
+// CTAs that share a (sequence, KV head) each, or 0: the blocks are dealt.  Without a selection they are.  Selected blocks
+// are shared by CTAs of their head alone, as many as fill one wave, because a CTA that goes on to another head starts over:
+// 64 of 64 blocks in 200 / 400 / 800 pairs 49 / 81 / 156 us, dealt 52 / 90 / 166; 16 blocks in 230 / 256 / 400 pairs 23 /
+// 24 / 28, dealt 29 / 30 / 41.  Long lists are dealt where the wave, or the last one, would be 70 % full or less: 64 blocks
+// in 150 / 256 / 460 / 600 pairs 45.6 / 70.9 / 133 / 147 us, dealt 42.1 / 60.7 / 103 / 128.
+static int plan_splits(int64_t pairs, int blocks) {
+  int64_t splits = kMaxCtas / pairs;
+  splits = splits < 1 ? 1 : splits > kMaxSplits ? kMaxSplits : splits;
+  const int64_t ctas = pairs * splits, waves = ceil_div64(ctas, kMaxCtas);
+  return splits < kMaxSplits && blocks >= 48 && 10 * ctas <= 7 * waves * kMaxCtas ? 0 : (int)splits;
+}
 
 // beside: the kernel may start while the one before it in the stream still runs (see wait_previous).
 template <typename... Params, typename... Args>
@@ -969,12 +984,11 @@ extern "C" int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void*
   p.out = static_cast<__nv_bfloat16*>(out);
   p.lse = lse;
   const int64_t pairs = (int64_t)batch * heads_k;
+  const int64_t n_blocks = ceil_div64(capacity, kBlockN);
+  IFV2_REQUIRE(pairs * (n_blocks + kStart) <= INT32_MAX, IFV2_ERR_TOO_LARGE, "q8_decode: more than 2^31-1 blocks of 64 keys");
   const bool selected = listed || mask != nullptr;
-  p.splits = 1;
-  if (selected) {
-    const int64_t most = kMaxCtas / pairs;
-    p.splits = most < 1 ? 1 : most > kMaxSplits ? kMaxSplits : (int)most;
-  }
+  p.most_blocks = !selected ? (int)n_blocks : topk_idx != nullptr && topk > 0 ? topk : kUsualBlocks;
+  p.splits = selected ? plan_splits(pairs, p.most_blocks) : 0;
   cudaStream_t st = (cudaStream_t)stream;
   const bool packed = topk_idx != nullptr && !listed, prepared = (k_new != nullptr && shared_rows) || packed;
   if (prepared) {
@@ -1001,15 +1015,14 @@ extern "C" int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void*
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
   if (e != cudaSuccess) return set_error((int)e, "q8_decode: %s", cudaGetErrorString(e));
   int64_t grid = pairs * p.splits;
-  if (!selected) {
-    grid = pairs * (ceil_div64(capacity, kBlockN) + kStart);
-    IFV2_REQUIRE(grid <= INT32_MAX, IFV2_ERR_TOO_LARGE, "q8_decode: more than 2^31-1 blocks of 64 keys");
+  if (p.splits == 0) {
+    grid = pairs * (kStart + (n_blocks < p.most_blocks ? n_blocks : p.most_blocks));
     if (grid > kMaxCtas) grid = kMaxCtas;
   }
   e = launch(kernel, dim3((unsigned)grid), kThreads, kSmemBytes, st, prepared, map_k, map_v, p);
   if (e != cudaSuccess) return set_error((int)e, "q8_split: launch failed: %s", cudaGetErrorString(e));
-  if (selected && p.splits == 1) return IFV2_OK;      // the split kernel wrote the results
-  const int64_t per_pair = selected ? p.splits : ceil_div64(grid, pairs);
+  if (p.splits == 1) return IFV2_OK;               // the split kernel wrote the results
+  const int64_t per_pair = p.splits ? p.splits : ceil_div64(grid, pairs);
   const int warps = per_pair > 16 ? 8 : per_pair > 6 ? 4 : 1;      // that share a row's partials
   auto join = warps == 8 ? q8_combine_kernel<8> : warps == 4 ? q8_combine_kernel<4> : q8_combine_kernel<1>;
   e = launch(join, dim3(2 * warps, (unsigned)pairs), 256, 0, st, true, p, (int)grid);

@@ -89,7 +89,8 @@ def _lists(lens, hk, k, seed, dup=False):
     ([1], 1, 0, 0), ([0, 1, 31, 32, 33, 63, 64, 65], 2, 0, 0), ([700, 0, 130], 2, 16, 0), ([513, 100, 1000], 1, 48, 0),
     ([300], 8, 64, 0), ([2000], 1, 256, 0), ([129, 1000, 64], 2, 0, 3), ([900, 1, 77, 0], 2, 16, 4), ([4097], 2, 64, 70),
     ([90] * 40, 4, 0, 0), ([640] * 9, 16, 64, 5),
-    ([20011, 300], 1, 0, 300), ([16500], 1, 16, 256), ([700] * 30, 8, 0, 9)])
+    ([20011, 300], 1, 0, 300), ([16500], 1, 16, 256), ([700] * 30, 8, 0, 9),
+    ([4200] * 5 + [64, 0, 700, 4097], 17, 0, 60), ([300] * 28, 8, 16, 50)])
 def test_attention(dtype, lens, hk, page, topk):
     batch, most = len(lens), max(lens)
     table = None
@@ -112,7 +113,9 @@ def test_attention(dtype, lens, hk, page, topk):
         cap = cache[0].shape[2] * (table.shape[1] if page else 1)
         mask = infllm_v2.topk_to_uint64(idx.to(DEV), cap, 64)[0]
         got = infllm_v2.infllmv2_attn_with_kvcache_q8(q.to(DEV), *dev, block_mask=mask, **args)
-        assert torch.equal(got[0], out) and torch.equal(got[1], lse)
+        if batch * hk <= 148:            # (shared by the same number of CTAs, whatever the mask selects)
+            assert torch.equal(got[0], out) and torch.equal(got[1], lse)
+        _check(*got, q, cache, lens, table, topk_idx=idx)
 
 
 @pytest.mark.parametrize("dtype", [E4M3, INT8])
