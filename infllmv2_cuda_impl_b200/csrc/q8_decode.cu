@@ -30,8 +30,8 @@ constexpr int kSlots = 3;                        // a warp's tiles in shared mem
 constexpr int kTileBytes = kUnit * kHeadDim;
 constexpr int kSmemBytes = kWarps * kSlots * kTileBytes + 1024;
 constexpr int kMaxSplits = 32;                   // CTAs that share the selected blocks of a (sequence, KV head)
-constexpr int kMaxCtas = kResident * kNumSMs;    // one wave: the CTAs that share all blocks where there is no mask
-constexpr uint32_t kStart = 4;              // blocks that the start of a head costs (see Deal)
+constexpr int kMaxCtas = kResident * kNumSMs;    // one wave
+constexpr uint32_t kStart = 4;                   // blocks that the start of a head costs (see Deal)
 constexpr int kUsualBlocks = 64;                 // blocks that a mask row is taken to select
 constexpr int kMaxList = 2 * kThreads;           // longest block list that the split kernel takes itself
 constexpr long long kWaitLimit = 1ll << 28;      // clocks; a copy takes microseconds
@@ -185,14 +185,18 @@ __device__ __forceinline__ int blocks_of(const Q8DecodeParams& p, int b) {
 }
 __device__ __forceinline__ uint32_t extent(int blocks) { return blocks ? kStart + blocks : 0; }
 
-// Without a mask the blocks of all sequences and heads are one row of `total` blocks, sequence by sequence, head by
-// head, and CTA c of `ctas` takes those from c total / ctas on: every CTA reads the same number of bytes whatever the
-// lengths are (16 sequences of 1000 .. 32000 tokens in equal splits wait for the longest one).  Every warp finds its
-// place by itself, a sequence per lane.
+// The blocks of all sequences and heads are one row, sequence by sequence, head by head, and CTA c of `ctas` takes those
+// from c total / ctas on: every CTA reads the same number of bytes whatever the lengths are (in equal splits, 16 sequences
+// of 1000 .. 32000 tokens wait for the longest one).  One wave of CTAs: with 1.5, 2 and 3 times as many, 64 sequences of
+// 4000 tokens took 53, 49 and 55 us instead of 37.  Every warp finds its place by itself, a sequence per lane.
+//
 // Where a CTA goes from one head to the next it starts over (query, first tiles, join), for about as long as it takes for
 // kStart blocks, so a head's place in the row begins with as many that are no work.  Without / with them: 16 sequences of
 // 1000 .. 32000 tokens 39.4 / 36.8 us, 12 of up to 30000 with 8 KV heads 108.5 / 100.3, 256 of 100 .. 1000 41.1 / 34.8; 3
 // or 5 in place of 4 make no difference beyond 1 %.
+//
+// Under a selection a head's place is as long as its list can be, and the CTAs that share it share the selected blocks in
+// proportion, so that the deal need not wait for their number.
 struct Deal {
   uint32_t total, ctas, each, rest;                // total = each * ctas + rest
   // extents: of all sequences, for one KV head (the host keeps the total below 2^31)
@@ -477,17 +481,16 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         if (row16 >= 0) tc::tma_load_2d(tiles + i * kTileBytes + 16 * kHeadDim, &map, bar, 0, row16);
       }
     };
-    auto arrived = [&](int i) {
-      if (!tc::mbar_try_wait(&bars[warp][i], (phases >> i) & 1u)) {
-        const long long start = clock64();
-        while (!tc::mbar_try_wait_hint(&bars[warp][i], (phases >> i) & 1u, 1000)) {
-          if (clock64() - start > kWaitLimit) {
-            expired = true;
-            break;
-          }
-        }
-      }
+    // waits for slot i's copy; the whole warp gets the same verdict
+    auto arrived = [&](int i) -> bool {
+      uint64_t* bar = &bars[warp][i];
+      const uint32_t parity = (phases >> i) & 1u;
       phases ^= 1u << i;
+      if (__all_sync(0xFFFFFFFFu, tc::mbar_try_wait(bar, parity))) return true;
+      const long long start = clock64();
+      while (!__all_sync(0xFFFFFFFFu, tc::mbar_try_wait_hint(bar, parity, 1000)))
+        if (__any_sync(0xFFFFFFFFu, clock64() - start > kWaitLimit)) return false;
+      return true;
     };
 
     // unit at work and the next one: first keys, rows, scale bytes; slots of K, V and the next K
@@ -542,7 +545,10 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 
     while (key0 >= 0) {
       const uint32_t kt = tiles32 + slot_k * kTileBytes, vt = tiles32 + slot_v * kTileBytes;
-      arrived(slot_k);
+      if (!arrived(slot_k)) {
+        expired = true;
+        break;
+      }
       // 2^(kb - 127) = 2^a 2^b: with the query's factor between the two no product leaves the range that the score is in
       factors[warp][0][lane] = kb == kNanByte ? __uint_as_float(0x7FC00000u) : __uint_as_float((64 + kb / 2) << 23);
       factors[warp][1][lane] = __uint_as_float((63 + (kb + 1) / 2) << 23);
@@ -669,8 +675,10 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       l1 += sum[1];
 
       // ---- O += P . V (16 x 128); rows past the last key have weight 0, but their bytes can be NaN codes
-      arrived(slot_v);
-      __syncwarp();
+      if (!arrived(slot_v)) {
+        expired = true;
+        break;
+      }
       if (key0 + kUnit > len) {
         for (int k = lane; k < kUnit * 8; k += 32)
           if (key0 + (k >> 3) >= len) *reinterpret_cast<uint4*>(tiles + slot_v * kTileBytes + k * 16) = make_uint4(0u, 0u, 0u, 0u);
@@ -707,7 +715,13 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       slot_n = slot_v;
       slot_v = done;
     }
-    if (__any_sync(0xFFFFFFFFu, expired)) l0 = l1 = __uint_as_float(0x7FC00000u);      // NaN: visible, not silent
+    if (expired) {                                 // NaN: visible, not silent; the other copies get their time to land
+      l0 = l1 = __uint_as_float(0x7FC00000u);
+      const long long start = clock64();
+      for (int i = 0; i < kSlots; ++i)
+        while (!tc::mbar_try_wait(&bars[warp][i], (phases >> i) & 1u) && clock64() - start < kWaitLimit >> 4) {}
+      __syncwarp();
+    }
     l0 += __shfl_xor_sync(0xFFFFFFFFu, l0, 1);
     l0 += __shfl_xor_sync(0xFFFFFFFFu, l0, 2);
     l1 += __shfl_xor_sync(0xFFFFFFFFu, l1, 1);
