@@ -263,6 +263,33 @@ def test_lengths_past_the_capacity_and_below_zero():
     _check(out, None, q, cache, [65, 65, 65], scale=0.3)
 
 
+@pytest.mark.parametrize("dtype", [E4M3, INT8])
+@pytest.mark.parametrize("page", [0, 16, 32])
+@pytest.mark.parametrize("at_k,at_v", [(0, 0), (1, 0), (7, 9), (15, 15), (16, 3), (0, 16)])
+def test_scales_at_every_alignment(dtype, page, at_k, at_v):
+    """Scale bytes at any address, rows of any number, the first and the last row of the cache attended, NaN around them."""
+    lens = [77, 33, 128] if page else [77, 33, 99]
+    length = page or 99
+    slots = 12 if page else 3
+    cache = _cache(slots, length, 2, dtype, 3)
+    q = det_tensor((3, 1, 32, 128), 7)
+    table = None
+    if page:                                                                     # (the first and the last page are used)
+        per = 128 // page
+        table = torch.arange(3 * per).flip(0).view(3, per).to(torch.int32) % slots
+    kc, vc, kb, vb = _to_gpu(cache)
+    args = dict(cache_seqlens=torch.tensor(lens, dtype=torch.int32, device=DEV), return_softmax_lse=True,
+                block_table=None if table is None else table.to(DEV))
+
+    def moved(scale, at):
+        buf = torch.full((scale.numel() + 64,), 255, dtype=torch.uint8, device=DEV)
+        buf[at:at + scale.numel()] = scale.view(torch.uint8).flatten()
+        return buf[at:at + scale.numel()].view(torch.float8_e8m0fnu).view(scale.shape)
+
+    out, lse = infllm_v2.infllmv2_attn_with_kvcache_q8(q.to(DEV), kc, vc, moved(kb, at_k), moved(vb, at_v), **args)
+    _check(out, lse, q, cache, lens, table)
+
+
 def test_slots_of_other_sequences():
     cache = _cache(5, 90, 2, INT8, 3)
     q = det_tensor((3, 1, 32, 128), 7)
