@@ -53,6 +53,8 @@ struct Q8DecodeParams {
   int topk;
   const int32_t* cache_seqlens;
   Place place;
+  uint32_t page_mul;               // a position's page: umulhi(position, page_mul) >> page_shift
+  int page_shift;
   int64_t capacity;
   int batch, heads_k, new_tokens, rotate;
   int splits;                      // CTAs that share a (sequence, KV head) each, or 0: the blocks are dealt (see Deal)
@@ -310,12 +312,14 @@ __device__ __forceinline__ void store_out(const Q8DecodeParams& p, int64_t qrow,
 // of ldmatrix, serve as k = 2t, 2t + 1, 2t + 8, 2t + 9; the query is read in the same order.  V comes through the
 // transposing 16-bit ldmatrix, a word of which holds two tokens' codes of two neighbouring features: even features
 // and odd features of a chunk are the columns of two products.
-// kCopied: scale bytes come with K's tile, by copies of 32 bytes, where every unit's begin at a multiple of 16 bytes.  As loads
-// of their own, the other way, they cost more than the 0.8 % that they are of the bytes: 64 sequences of 16000 tokens, two
-// heads, take 88.8 us against 95.5.
-template <int kCode, int kBox, bool kRotate, bool kCopied>
+// kPage: 0, slots are sequences; 32, pages of a multiple of 32 positions; 16, of 16, so that a tile comes in two boxes.
+// kCopied: scale bytes come with K's tile, by copies of their own, where a box's begin at a multiple of 16 bytes.  As loads
+// they cost more than the 0.8 % that they are of the bytes: 64 sequences of 16000 tokens, two heads, take 88.8 us against
+// 95.5.
+template <int kCode, int kPage, bool kRotate, bool kCopied>
 __global__ void __launch_bounds__(kThreads, kResident)
 q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Q8DecodeParams p) {
+  constexpr int kBox = kPage == 16 ? 16 : 32;      // rows that one copy takes
   allow_next();
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -335,7 +339,7 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       tc::prefetch_map(&map_v);
     }
 #pragma unroll
-    for (int i = 0; i < kSlots; ++i) tc::mbar_init(&bars[warp][i], 1);
+    for (int i = 0; i < kSlots; ++i) tc::mbar_init(&bars[warp][i], kUnit / kBox);
     tc::fence_barrier_init();
   }
   __syncwarp();
@@ -449,21 +453,26 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     };
     // where the key of this lane is (-1: nowhere), and its scale bytes.  (The cache has fewer than 2^31 rows.)
     int slot0 = 0;                                 // row of the head's first position, where slots are sequences
-    if (p.place.block_table == nullptr) {
+    if (kPage == 0) {
       const int slot = p.place.batch_idx ? __ldg(p.place.batch_idx + b) : b;
       slot0 = slot >= 0 && slot < p.place.slots ? (slot * p.place.heads + h) * p.place.length : -1;
     }
-    // The bytes are not touched before the unit's turn: whatever uses them waits for their loads.
-    auto locate = [&](int key0, int& row, uint32_t& kb, uint32_t& vb) {
+    // entry of the block table for it, read a unit ahead, because what uses it waits for the load (with the page by
+    // multiplication, and copied scale bytes: 64 sequences of 32000 tokens in pages of 16 189 us in place of 199)
+    auto page_of = [&](int key) -> int { return (int)(__umulhi((uint32_t)key, p.page_mul) >> p.page_shift); };
+    auto entry = [&](int key0) -> int {
+      const int key = key0 + lane;
+      return kPage != 0 && key0 >= 0 && key < len ? __ldg(p.place.block_table + (int64_t)b * p.place.bt_stride + page_of(key)) : -1;
+    };
+    // The bytes are not touched before the unit's turn either.
+    auto locate = [&](int key0, int slot, int& row, uint32_t& kb, uint32_t& vb) {
       row = -1;
       kb = 0;
       vb = kNanByte;                               // (a page that the cache does not have: NaN)
       const int key = key0 + lane;
       if (key < len) {
-        if (p.place.block_table != nullptr) {
-          const int page = (int)((uint32_t)key / (uint32_t)p.place.length);
-          const int slot = __ldg(p.place.block_table + (int64_t)b * p.place.bt_stride + page);
-          if (slot >= 0 && slot < p.place.slots) row = (slot * p.place.heads + h) * p.place.length + key - page * p.place.length;
+        if (kPage != 0) {
+          if (slot >= 0 && slot < p.place.slots) row = (slot * p.place.heads + h) * p.place.length + key - page_of(key) * p.place.length;
         } else if (slot0 >= 0) {
           row = slot0 + key;
         }
@@ -478,16 +487,16 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     int turn = 0;                                  // kCopied: which of its two places the next unit's scale bytes get
     auto fetch = [&](const CUtensorMap& map, int i, int row, auto with_scales) {
       constexpr bool kScales = kCopied && decltype(with_scales)::value;
-      const int row16 = kBox == 16 ? __shfl_sync(0xFFFFFFFFu, row, 16) : -1;
       __syncwarp();
-      if (lane == 0) {
+      if (lane % kBox == 0) {
         uint64_t* bar = &bars[warp][i];
-        tc::mbar_expect_tx(bar, ((row >= 0) + (row16 >= 0)) * kBox * kHeadDim + (kScales && row >= 0 ? 2 * kUnit : 0));
-        if (row >= 0) tc::tma_load_2d(tiles + i * kTileBytes, &map, bar, 0, row);
-        if (row16 >= 0) tc::tma_load_2d(tiles + i * kTileBytes + 16 * kHeadDim, &map, bar, 0, row16);
-        if (kScales && row >= 0) {
-          tc::bulk_load(scale_bytes[warp][turn][0], p.k_scale + row, kUnit, bar);
-          tc::bulk_load(scale_bytes[warp][turn][1], p.v_scale + row, kUnit, bar);
+        tc::mbar_expect_tx(bar, row >= 0 ? kBox * (kHeadDim + (kScales ? 2 : 0)) : 0);
+        if (row >= 0) {
+          tc::tma_load_2d(tiles + i * kTileBytes + lane * kHeadDim, &map, bar, 0, row);
+          if (kScales) {
+            tc::bulk_load(scale_bytes[warp][turn][0] + lane, p.k_scale + row, kBox, bar);
+            tc::bulk_load(scale_bytes[warp][turn][1] + lane, p.v_scale + row, kBox, bar);
+          }
         }
       }
       if (kScales) turn ^= 1;
@@ -504,17 +513,22 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       return true;
     };
 
-    // unit at work and the next one: first keys, rows, scale bytes; slots of K, V and the next K
-    int key0 = next_key(), key1 = -1, row = -1, row1 = -1, slot_k = 0, slot_v = 1, slot_n = 2;
+    // unit at work, the next one and that after it: first keys, rows, scale bytes; slots of K, V and the next K
+    int key0 = next_key(), key1 = key0 >= 0 ? next_key() : -1, key2 = -1, row = -1, row1 = -1, slot_k = 0, slot_v = 1, slot_n = 2;
+    int entry2 = -1;                               // of the block table
     uint32_t kb = 0, vb = 0, kb1 = 0, vb1 = 0;
     if (key0 >= 0) {
-      locate(key0, row, kb, vb);
+      const int entry0 = entry(key0), entry1 = entry(key1);
+      locate(key0, entry0, row, kb, vb);
       fetch(map_k, slot_k, row, std::true_type{});
       fetch(map_v, slot_v, row, std::false_type{});
-      key1 = next_key();
       if (key1 >= 0) {
-        locate(key1, row1, kb1, vb1);
+        locate(key1, entry1, row1, kb1, vb1);
         fetch(map_k, slot_n, row1, std::true_type{});
+        if (kPage != 0) {
+          key2 = next_key();
+          entry2 = entry(key2);
+        }
       }
     }
 
@@ -721,10 +735,14 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       kb = kb1;
       vb = vb1;
       if (key1 >= 0) {
-        key1 = next_key();
+        key1 = kPage != 0 ? key2 : next_key();
         if (key1 >= 0) {
-          locate(key1, row1, kb1, vb1);
+          locate(key1, entry2, row1, kb1, vb1);
           fetch(map_k, slot_v, row1, std::true_type{});
+          if (kPage != 0) {
+            key2 = next_key();
+            entry2 = entry(key2);
+          }
         }
       }
       const int done = slot_k;
@@ -914,9 +932,10 @@ static int plan_splits(int64_t pairs, int blocks) {
 }
 
 template <int kCode, bool kRotate>
-static auto split_kernel(bool wide, bool copied) {
-  return !wide ? q8_split_kernel<kCode, 16, kRotate, false>
-       : copied ? q8_split_kernel<kCode, 32, kRotate, true> : q8_split_kernel<kCode, 32, kRotate, false>;
+static auto split_kernel(int page, bool copied) {
+  return page == 32 ? q8_split_kernel<kCode, 32, kRotate, true>
+       : page == 16 ? (copied ? q8_split_kernel<kCode, 16, kRotate, true> : q8_split_kernel<kCode, 16, kRotate, false>)
+                    : (copied ? q8_split_kernel<kCode, 0, kRotate, true> : q8_split_kernel<kCode, 0, kRotate, false>);
 }
 
 // beside: the kernel may start while the one before it in the stream still runs (see wait_previous).
@@ -1013,6 +1032,14 @@ extern "C" int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void*
   p.cache_seqlens = cache_seqlens;
   p.place = Place{block_table, cache_batch_idx, block_table_stride, heads_k, (int)length, (int)slots};
   p.capacity = capacity;
+  // x / d for x < 2^31: with 2^(s - 1) < d <= 2^s and m = floor(2^(31 + s) / d) + 1 < 2^32, x m / 2^(31 + s) is past x / d by
+  // less than 2^-s <= 1 / d.  (d = length >= 16 where it is used)
+  if (block_table != nullptr) {
+    int s = 1;
+    while (((int64_t)1 << s) < length) ++s;
+    p.page_mul = (uint32_t)(((uint64_t)1 << (31 + s)) / (uint64_t)length + 1);
+    p.page_shift = s - 1;
+  }
   p.batch = batch;
   p.heads_k = heads_k;
   p.new_tokens = k_new != nullptr;
@@ -1038,17 +1065,17 @@ extern "C" int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void*
     int rc = check_launch("q8_prepare");
     if (rc) return rc;
   }
-  // boxes of 32 rows where 32 consecutive positions are 32 consecutive rows, else of 16
-  const bool wide = block_table == nullptr || length % kUnit == 0;
+  const bool aligned = ((reinterpret_cast<uintptr_t>(k_scale) | reinterpret_cast<uintptr_t>(v_scale)) & 15) == 0;
+  const bool whole = length % kUnit == 0;          // the 32 positions of a unit are in one slot
+  const int page = block_table == nullptr ? 0 : whole && aligned ? 32 : 16;
+  const bool copied = aligned && (whole || page != 0);
   CUtensorMap map_k, map_v;
   const uint64_t rows = (uint64_t)slots * heads_k * length;
-  int rc = make_tensor_map_rows128(&map_k, k_cache, rows, wide ? 32 : 16);
-  if (rc == IFV2_OK) rc = make_tensor_map_rows128(&map_v, v_cache, rows, wide ? 32 : 16);
+  int rc = make_tensor_map_rows128(&map_k, k_cache, rows, page == 16 ? 16 : 32);
+  if (rc == IFV2_OK) rc = make_tensor_map_rows128(&map_v, v_cache, rows, page == 16 ? 16 : 32);
   if (rc) return rc;
-  const bool copied = wide && length % kUnit == 0 &&
-                      ((reinterpret_cast<uintptr_t>(k_scale) | reinterpret_cast<uintptr_t>(v_scale)) & 15) == 0;
-  auto kernel = rotate ? (code == kE4m3 ? split_kernel<kE4m3, true>(wide, copied) : split_kernel<kInt8, true>(wide, copied))
-                       : (code == kE4m3 ? split_kernel<kE4m3, false>(wide, copied) : split_kernel<kInt8, false>(wide, copied));
+  auto kernel = rotate ? (code == kE4m3 ? split_kernel<kE4m3, true>(page, copied) : split_kernel<kInt8, true>(page, copied))
+                       : (code == kE4m3 ? split_kernel<kE4m3, false>(page, copied) : split_kernel<kInt8, false>(page, copied));
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
   if (e != cudaSuccess) return set_error((int)e, "q8_decode: %s", cudaGetErrorString(e));
   int64_t grid = pairs * p.splits;
