@@ -313,9 +313,9 @@ __device__ __forceinline__ void store_out(const Q8DecodeParams& p, int64_t qrow,
 // transposing 16-bit ldmatrix, a word of which holds two tokens' codes of two neighbouring features: even features
 // and odd features of a chunk are the columns of two products.
 // kPage: 0, slots are sequences; 32, pages of a multiple of 32 positions; 16, of 16, so that a tile comes in two boxes.
-// kCopied: scale bytes come with K's tile, by copies of their own, where a box's begin at a multiple of 16 bytes.  As loads
-// they cost more than the 0.8 % that they are of the bytes: 64 sequences of 16000 tokens, two heads, take 88.8 us against
-// 95.5.
+// kCopied: scale bytes come with K's tile, by copies of their own, where those of a unit are together and begin at a multiple
+// of 16 bytes.  As loads they cost more than the 0.8 % that they are of the bytes: 64 sequences of 16000 tokens, two heads,
+// take 88.8 us against 95.5.  In pages of 16 copies of 16 bytes cost more: 64 sequences of 32000 tokens 189 us against 184.
 template <int kCode, int kPage, bool kRotate, bool kCopied>
 __global__ void __launch_bounds__(kThreads, kResident)
 q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Q8DecodeParams p) {
@@ -458,7 +458,7 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       slot0 = slot >= 0 && slot < p.place.slots ? (slot * p.place.heads + h) * p.place.length : -1;
     }
     // entry of the block table for it, read a unit ahead, because what uses it waits for the load (with the page by
-    // multiplication, and copied scale bytes: 64 sequences of 32000 tokens in pages of 16 189 us in place of 199)
+    // multiplication: 64 sequences of 32000 tokens in pages of 16 184 us in place of 199)
     auto page_of = [&](int key) -> int { return (int)(__umulhi((uint32_t)key, p.page_mul) >> p.page_shift); };
     auto entry = [&](int key0) -> int {
       const int key = key0 + lane;
@@ -490,12 +490,12 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       __syncwarp();
       if (lane % kBox == 0) {
         uint64_t* bar = &bars[warp][i];
-        tc::mbar_expect_tx(bar, row >= 0 ? kBox * (kHeadDim + (kScales ? 2 : 0)) : 0);
+        tc::mbar_expect_tx(bar, row >= 0 ? kBox * kHeadDim + (kScales ? 2 * kUnit : 0) : 0);
         if (row >= 0) {
           tc::tma_load_2d(tiles + i * kTileBytes + lane * kHeadDim, &map, bar, 0, row);
           if (kScales) {
-            tc::bulk_load(scale_bytes[warp][turn][0] + lane, p.k_scale + row, kBox, bar);
-            tc::bulk_load(scale_bytes[warp][turn][1] + lane, p.v_scale + row, kBox, bar);
+            tc::bulk_load(scale_bytes[warp][turn][0], p.k_scale + row, kUnit, bar);
+            tc::bulk_load(scale_bytes[warp][turn][1], p.v_scale + row, kUnit, bar);
           }
         }
       }
@@ -934,8 +934,8 @@ static int plan_splits(int64_t pairs, int blocks) {
 template <int kCode, bool kRotate>
 static auto split_kernel(int page, bool copied) {
   return page == 32 ? q8_split_kernel<kCode, 32, kRotate, true>
-       : page == 16 ? (copied ? q8_split_kernel<kCode, 16, kRotate, true> : q8_split_kernel<kCode, 16, kRotate, false>)
-                    : (copied ? q8_split_kernel<kCode, 0, kRotate, true> : q8_split_kernel<kCode, 0, kRotate, false>);
+       : page == 16 ? q8_split_kernel<kCode, 16, kRotate, false>
+       : copied     ? q8_split_kernel<kCode, 0, kRotate, true> : q8_split_kernel<kCode, 0, kRotate, false>;
 }
 
 // beside: the kernel may start while the one before it in the stream still runs (see wait_previous).
@@ -1065,10 +1065,9 @@ extern "C" int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void*
     int rc = check_launch("q8_prepare");
     if (rc) return rc;
   }
-  const bool aligned = ((reinterpret_cast<uintptr_t>(k_scale) | reinterpret_cast<uintptr_t>(v_scale)) & 15) == 0;
-  const bool whole = length % kUnit == 0;          // the 32 positions of a unit are in one slot
-  const int page = block_table == nullptr ? 0 : whole && aligned ? 32 : 16;
-  const bool copied = aligned && (whole || page != 0);
+  // the scale bytes of a unit are together, at a multiple of 16 bytes
+  const bool copied = length % kUnit == 0 && ((reinterpret_cast<uintptr_t>(k_scale) | reinterpret_cast<uintptr_t>(v_scale)) & 15) == 0;
+  const int page = block_table == nullptr ? 0 : copied ? 32 : 16;
   CUtensorMap map_k, map_v;
   const uint64_t rows = (uint64_t)slots * heads_k * length;
   int rc = make_tensor_map_rows128(&map_k, k_cache, rows, page == 16 ? 16 : 32);
