@@ -244,8 +244,8 @@ def infllmv2_attn_with_kvcache_q8(
             raise ValueError(f"{what}: topk_idx must be ({batch}, {hk}, 1, topk) int32 on {dev}")
         topk_idx, topk = topk_idx.contiguous(), topk_idx.shape[-1]
         idx_ptr = topk_idx.data_ptr()
-        if topk > _LIST:                                 # (shorter lists are walked as they are)
-            block_mask = torch.empty(batch, hk, 1, words, dtype=torch.int64, device=dev)
+        if topk > _LIST or topk == 0:                    # (shorter lists are walked as they are; one of no entries has no address)
+            block_mask = (torch.zeros if topk == 0 else torch.empty)(batch, hk, 1, words, dtype=torch.int64, device=dev)
             mask_ptr = block_mask.data_ptr()
     rotary = (None, None, None, 0, None, 0, 0, 0)
     if rotary_cos is not None and k is not None:

@@ -363,6 +363,20 @@ def test_extreme_sizes(dtype, kexp, vexp, qexp):
         _check(out, lse, q, cache, [100])
 
 
+@pytest.mark.parametrize("append", [False, True])
+def test_lists_without_an_entry_attend_nothing(append):
+    cache = _to_gpu(_cache(2, 70, 1, INT8, 3))
+    q = det_tensor((2, 1, 16, 128), 7).to(DEV)
+    new = dict(k=det_tensor((2, 1, 1, 128), 8).to(DEV), v=det_tensor((2, 1, 1, 128), 9).to(DEV)) if append else {}
+    before = cache[1].clone()
+    idx = torch.empty(2, 1, 1, 0, dtype=torch.int32, device=DEV)
+    out, lse = infllm_v2.infllmv2_attn_with_kvcache_q8(
+        q, *cache, topk_idx=idx, cache_seqlens=torch.tensor([69, 5], dtype=torch.int32, device=DEV), return_softmax_lse=True, **new)
+    assert bool((out == 0).all()) and bool((lse == float("inf")).all())
+    changed = (cache[1] != before).any(dim=-1).nonzero().tolist()
+    assert changed == ([[0, 0, 69], [1, 0, 5]] if append else [])
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.2])
 def test_scales_of_zero_and_below(scale):
     cache = _cache(2, 130, 1, INT8, 3)
