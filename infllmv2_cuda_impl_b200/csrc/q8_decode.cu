@@ -190,12 +190,12 @@ __device__ __forceinline__ uint32_t extent(int blocks) { return blocks ? kStart 
 // The blocks of all sequences and heads are one row, sequence by sequence, head by head, and CTA c of `ctas` takes those
 // from c total / ctas on: every CTA reads the same number of bytes whatever the lengths are (in equal splits, 16 sequences
 // of 1000 .. 32000 tokens wait for the longest one).  One wave of CTAs: with 1.5, 2 and 3 times as many, 64 sequences of
-// 4000 tokens took 53, 49 and 55 us instead of 37.  Every warp finds its place by itself, a sequence per lane.
+// 4000 tokens take 42, 46 and 52 us instead of 32.  Every warp finds its place by itself, a sequence per lane.
 //
 // Where a CTA goes from one head to the next it starts over (query, first tiles, join), for about as long as it takes for
 // kStart blocks, so a head's place in the row begins with as many that are no work.  Without / with them: 16 sequences of
-// 1000 .. 32000 tokens 39.4 / 36.8 us, 12 of up to 30000 with 8 KV heads 108.5 / 100.3, 256 of 100 .. 1000 41.1 / 34.8; 3
-// or 5 in place of 4 make no difference beyond 1 %.
+// 1000 .. 32000 tokens 38.2 / 35.3 us, 12 of up to 30000 with 8 KV heads 107 / 98.8, 256 of 100 .. 1000 41.6 / 34.9; 3
+// or 5 in place of 4 made no difference beyond 1 %.
 //
 // Under a selection a head's place is as long as its list can be, and the CTAs that share it share the selected blocks in
 // proportion, so that the deal need not wait for their number.
@@ -312,6 +312,13 @@ __device__ __forceinline__ void store_out(const Q8DecodeParams& p, int64_t qrow,
 // of ldmatrix, serve as k = 2t, 2t + 1, 2t + 8, 2t + 9; the query is read in the same order.  V comes through the
 // transposing 16-bit ldmatrix, a word of which holds two tokens' codes of two neighbouring features: even features
 // and odd features of a chunk are the columns of two products.
+//
+// Bound by HBM where there is much to read, and by about 12 us of start (3 us to the first tile), uneven ends and join
+// elsewhere.  e4m3, two KV heads, 64 sequences of 4000 / 16000 / 32000 tokens: 32 / 88.8 / 164 us with the join, 63 / 91 /
+// 99 % of the copy bandwidth; without the copies the arithmetic alone takes 77 us at 16000.  Eight heads, 8 sequences of
+// 30000 tokens: e4m3 93 us, int8 100 (five instructions for four codes in place of two), with a rotated query 108 and 116
+// (three fp16 products for two).
+//
 // kPage: 0, slots are sequences; 32, pages of a multiple of 32 positions; 16, of 16, so that a tile comes in two boxes.
 // kCopied: scale bytes come with K's tile, by copies of their own, where those of a unit are together and begin at a multiple
 // of 16 bytes.  As loads they cost more than the 0.8 % that they are of the bytes: 64 sequences of 16000 tokens, two heads,
@@ -921,9 +928,9 @@ using namespace ifv2;
 
 // CTAs that share a (sequence, KV head) each, or 0: the blocks are dealt.  Without a selection they are.  Selected blocks
 // are shared by CTAs of their head alone, as many as fill one wave, because a CTA that goes on to another head starts over:
-// 64 of 64 blocks in 200 / 400 / 800 pairs 49 / 81 / 156 us, dealt 52 / 90 / 166; 16 blocks in 230 / 256 / 400 pairs 23 /
-// 24 / 28, dealt 29 / 30 / 41.  Long lists are dealt where the wave, or the last one, would be 70 % full or less: 64 blocks
-// in 150 / 256 / 460 / 600 pairs 45.6 / 70.9 / 133 / 147 us, dealt 42.1 / 60.7 / 103 / 128.
+// 64 blocks in 200 / 400 / 800 pairs 48 / 79 / 152 us, dealt 51 / 90 / 164; 16 blocks in 230 / 256 / 400 pairs 23 / 23 /
+// 27, dealt 27 / 28 / 40.  Long lists are dealt where the wave, or the last one, would be 70 % full or less: 64 blocks in
+// 150 / 256 / 460 / 600 pairs 44.6 / 68.9 / 129 / 142 us, dealt 41.1 / 60.6 / 102 / 127.
 static int plan_splits(int64_t pairs, int blocks) {
   int64_t splits = kMaxCtas / pairs;
   splits = splits < 1 ? 1 : splits > kMaxSplits ? kMaxSplits : splits;

@@ -1,7 +1,7 @@
 // Rotary positions over several axes (time, height, width of images and video) for packed queries and keys,
 // forward and backward (formulas: rotary.cuh).  The gradient of a rotation is the rotation by minus the angle.
 //
-// Bound by HBM: every row is read and written once (512 B); a token's angles are read once for a dozen rows.
+// Bound by HBM: every row is read and written once (512 B); a token's angles are read once for all of its rows.
 #include "rotary.cuh"
 
 namespace ifv2 {
