@@ -170,7 +170,10 @@ def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], rotary_cos: torch.Te
     several axes, how many of the rotary_dim / 2 pairs turn by the position on each (in order).  Pairs are features
     (2i, 2i+1) if interleaved, else (i, i + rotary_dim / 2); features from rotary_dim on pass through.  The
     arithmetic is fp32, the results are rounded once.  A position outside the tables takes their first or last row.
-    Returns (q, k) rotated (k None without one), dense."""
+    Returns (q, k) rotated (k None without one), dense.
+
+    A backward pass that is captured into a CUDA graph must not share its leaves with an eager graph that is still alive
+    (as for any operator: autograd would end the process)."""
     shape = q.shape
     if q.dtype is not torch.bfloat16 or len(shape) != 3 or shape[2] != HEAD_DIM:
         raise ValueError(f"rotary_axes: q must be (tokens, nheads, {HEAD_DIM}) bf16")
