@@ -342,8 +342,8 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   uint8_t* tiles = smem + warp * kSlots * kTileBytes;
   if (lane == 0) {
     if (warp == 0) {
-      tc::prefetch_map(&map_k);
-      tc::prefetch_map(&map_v);
+      tc::prefetch_tensormap(&map_k);
+      tc::prefetch_tensormap(&map_v);
     }
 #pragma unroll
     for (int i = 0; i < kSlots; ++i) tc::mbar_init(&bars[warp][i], kUnit / kBox);
