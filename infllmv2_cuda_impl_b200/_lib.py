@@ -140,12 +140,17 @@ def load():
     return _lib
 
 
+_entries = {}              # functions that `call` has looked up
+
+
 def call(name, *args):
     """Invoke an int-returning entry point and raise on a non-zero status."""
-    lib = load()
-    rc = getattr(lib, name)(*args)
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(load(), name)
+    rc = fn(*args)
     if rc != 0:
-        msg = lib.ifv2_last_error().decode(errors="replace")
+        msg = _lib.ifv2_last_error().decode(errors="replace")
         kind = {-1: ValueError, -2: NotImplementedError}.get(rc, Ifv2Error)
         raise kind(f"{name} failed (status {rc}): {msg}")
     return rc

@@ -19,21 +19,25 @@ def _stream(device) -> int:
 
 
 _AS_IT_IS = contextlib.nullcontext()
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
 
 
 def _on(device):
-    """Context in which `device` is the current one; nothing to switch (2-3 us of a call) if it is."""
-    return _AS_IT_IS if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    """Context in which `device`, that of a CUDA tensor, is the current one; nothing to switch (2-3 us of a call) if it is."""
+    return _AS_IT_IS if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 def _plain_eager(*tensors) -> bool:
     """True when nothing watches the operators that are called: no compilation or trace, no dispatch or
     function mode, no function transform, no tensor subclass.  Only then may a call that is made of
     operators go around them."""
-    return (not torch.compiler.is_compiling() and not torch.jit.is_tracing()
-            and torch._C._len_torch_dispatch_stack() == 0 and torch._C._len_torch_function_stack() == 0
-            and torch._C._functorch.peek_interpreter_stack() is None
-            and all(type(t) in (torch.Tensor, torch.nn.Parameter) for t in tensors if t is not None))
+    if (torch.compiler.is_compiling() or torch.jit.is_tracing() or torch._C._len_torch_dispatch_stack() != 0
+            or torch._C._len_torch_function_stack() != 0 or torch._C._functorch.peek_interpreter_stack() is not None):
+        return False
+    for t in tensors:                              # (a generator would take 0.6 us more)
+        if t is not None and type(t) not in _PLAIN:
+            return False
+    return True
 
 
 def _require_cuda(t: torch.Tensor, name: str):
