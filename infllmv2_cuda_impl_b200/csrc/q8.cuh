@@ -30,6 +30,17 @@ __device__ __forceinline__ uint64_t mul_exact2(uint64_t a, uint64_t b) {
   return r;
 }
 
+__device__ __forceinline__ uint64_t fma_exact2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // Scale byte of a row whose largest |x| has the bit pattern `amax`.
 template <int kCode>
 __device__ __forceinline__ int scale_byte(uint32_t amax) {
@@ -50,15 +61,20 @@ template <int kCode>
 __device__ __forceinline__ uint32_t encode4(const float (&x)[4], int byte) {
   if (byte == kNanByte) return 0u;
   const float inv = inverse_scale(byte);
+  const uint64_t inv2 = pair(inv, inv);
+  float2 a, b;
   if (kCode == kE4m3) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(mul_exact(x[0], inv), mul_exact(x[1], inv)), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(mul_exact(x[2], inv), mul_exact(x[3], inv)), __NV_SATFINITE, __NV_E4M3);
+    const uint64_t pa = mul_exact2(pair(x[0], x[1]), inv2), pb = mul_exact2(pair(x[2], x[3]), inv2);
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(pa));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(b.x), "=f"(b.y) : "l"(pb));
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, __NV_E4M3), hi = __nv_cvt_float2_to_fp8x2(b, __NV_SATFINITE, __NV_E4M3);
     return lo | hi << 16;
   }
-  uint32_t r = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) r |= ((uint32_t)__float2int_rn(mul_exact(x[i], inv)) & 0xFFu) << (8 * i);
-  return r;
+  // 1.5 2^23 + y has steps of 1, so that the sum is rounded to the integer, whose low byte is the number's
+  const uint64_t one = pair(0x1.8p23f, 0x1.8p23f);
+  const uint64_t pa = fma_exact2(pair(x[0], x[1]), inv2, one), pb = fma_exact2(pair(x[2], x[3]), inv2, one);
+  const uint32_t lo = __byte_perm((uint32_t)pa, (uint32_t)(pa >> 32), 0x0040), hi = __byte_perm((uint32_t)pb, (uint32_t)(pb >> 32), 0x0040);
+  return __byte_perm(lo, hi, 0x5410);
 }
 
 // Four codes to numbers (without the scale); exact.
