@@ -9,6 +9,7 @@
 #pragma once
 #include <cuda_fp8.h>
 #include "common.cuh"
+#include "tc05.cuh"
 
 namespace ifv2 {
 namespace q8 {
@@ -35,12 +36,6 @@ __device__ __forceinline__ uint64_t fma_exact2(uint64_t a, uint64_t b, uint64_t 
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-
 // Scale byte of a row whose largest |x| has the bit pattern `amax`.
 template <int kCode>
 __device__ __forceinline__ int scale_byte(uint32_t amax) {
@@ -61,18 +56,18 @@ template <int kCode>
 __device__ __forceinline__ uint32_t encode4(const float (&x)[4], int byte) {
   if (byte == kNanByte) return 0u;
   const float inv = inverse_scale(byte);
-  const uint64_t inv2 = pair(inv, inv);
+  const uint64_t inv2 = tc::pack_f32x2(inv, inv);
   float2 a, b;
   if (kCode == kE4m3) {
-    const uint64_t pa = mul_exact2(pair(x[0], x[1]), inv2), pb = mul_exact2(pair(x[2], x[3]), inv2);
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(pa));
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(b.x), "=f"(b.y) : "l"(pb));
+    const uint64_t pa = mul_exact2(tc::pack_f32x2(x[0], x[1]), inv2), pb = mul_exact2(tc::pack_f32x2(x[2], x[3]), inv2);
+    tc::unpack_f32x2(pa, a.x, a.y);
+    tc::unpack_f32x2(pb, b.x, b.y);
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, __NV_E4M3), hi = __nv_cvt_float2_to_fp8x2(b, __NV_SATFINITE, __NV_E4M3);
     return lo | hi << 16;
   }
   // 1.5 2^23 + y has steps of 1, so that the sum is rounded to the integer, whose low byte is the number's
-  const uint64_t one = pair(0x1.8p23f, 0x1.8p23f);
-  const uint64_t pa = fma_exact2(pair(x[0], x[1]), inv2, one), pb = fma_exact2(pair(x[2], x[3]), inv2, one);
+  const uint64_t one = tc::pack_f32x2(0x1.8p23f, 0x1.8p23f);
+  const uint64_t pa = fma_exact2(tc::pack_f32x2(x[0], x[1]), inv2, one), pb = fma_exact2(tc::pack_f32x2(x[2], x[3]), inv2, one);
   const uint32_t lo = __byte_perm((uint32_t)pa, (uint32_t)(pa >> 32), 0x0040), hi = __byte_perm((uint32_t)pb, (uint32_t)(pb >> 32), 0x0040);
   return __byte_perm(lo, hi, 0x5410);
 }
