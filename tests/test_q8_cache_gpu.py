@@ -89,6 +89,22 @@ def test_write_and_read_back(dtype, lens, hk, page, start):
 
 
 @pytest.mark.parametrize("dtype", [E4M3, INT8])
+def test_every_bf16_number_as_the_largest_of_a_row(dtype):
+    """65536 rows, one for each bit pattern, with random smaller numbers beside it: codes and scales are the oracle's."""
+    g = torch.Generator().manual_seed(1)
+    top = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
+    x = torch.randint(0, 65536, (65536, 1, 128), generator=g, dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
+    x = torch.where(x.abs().float() <= top.abs().float()[:, None, None], x, torch.zeros_like(x))   # (not below a NaN)
+    x[torch.arange(65536), 0, torch.randint(0, 128, (65536,), generator=g)] = top
+    kc, vc, ks, vs = infllm_v2.q8_cache(1, 65536, 1, dtype)
+    infllm_v2.cache_fill_q8(x.to(DEV), x.to(DEV), kc, vc, ks, vs, cu([65536], DEV))
+    codes, scales = quantise(x[:, 0], dtype)
+    assert torch.equal(ks.view(torch.uint8).cpu().flatten(), scales.view(torch.uint8).flatten())
+    assert torch.equal(kc.float().cpu().flatten(), codes.float().flatten())              # (a zero may have either sign)
+    assert torch.equal(kc.view(torch.uint8), vc.view(torch.uint8)) and torch.equal(ks.view(torch.uint8), vs.view(torch.uint8))
+
+
+@pytest.mark.parametrize("dtype", [E4M3, INT8])
 def test_infinities_and_nan_make_the_row_nan(dtype):
     k = det_tensor((4, 2, 128), 1)
     v = k.clone()
