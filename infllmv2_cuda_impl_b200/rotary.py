@@ -130,10 +130,8 @@ class RotaryAxesFunc(torch.autograd.Function):
         if _direct(q, k, rotary_cos, rotary_sin, positions):
             tables = _tables("rotary_axes", rotary_cos, rotary_sin, positions, sections, q.shape[0], q.device)
             ctx.save_for_backward(*tables[:3])
-            ctx.known = tables[3:]                      # (checked once: the backward pass is bound by its host time)
             return _turn(q, k, tables, interleaved, back)
         ctx.save_for_backward(rotary_cos, rotary_sin, positions)
-        ctx.known = None
         return _registered(q, k, rotary_cos, rotary_sin, positions, sections, interleaved, back)
 
     @staticmethod
@@ -143,11 +141,9 @@ class RotaryAxesFunc(torch.autograd.Function):
         one, other = (dk, None) if dq is None else (dq, dk)      # the body wants a first tensor
         if one is None:
             return (None,) * 8
-        tables = ctx.saved_tensors
-        if ctx.known is not None and not torch.is_grad_enabled() and _direct(one, other):
-            one, other = _turn(one, other, tables + ctx.known, ctx.interleaved, not ctx.back)
-        else:
-            one, other = _rotary_maybe_grad(one, other, *tables, ctx.sections, ctx.interleaved, not ctx.back)
+        # (a saved-tensor hook may give a saved tensor back with other strides: nothing that the forward pass knew of
+        # their layout holds here)
+        one, other = _rotary_maybe_grad(one, other, *ctx.saved_tensors, ctx.sections, ctx.interleaved, not ctx.back)
         return ((None, one) if dq is None else (one, other)) + (None,) * 6
 
 
