@@ -11,6 +11,7 @@ import torch
 from . import _lib
 from .ops import _on, _plain_eager, _require_cuda, _stream
 
+_forward_ad = torch.autograd.forward_ad
 _profiled = torch.autograd._profiler_enabled
 HEAD_DIM = 128
 MAX_AXES = 4
@@ -121,12 +122,16 @@ def _registered(q, k, rotary_cos, rotary_sin, positions, sections, interleaved, 
 
 
 class RotaryAxesFunc(torch.autograd.Function):
-    """A rotation is linear: its gradient is the rotation by minus the angle, and so on to any order."""
+    """A rotation is linear: its gradient is the rotation by minus the angle, and so on to any order; a tangent turns as
+    the rows do."""
 
     @staticmethod
     def forward(ctx, q, k, rotary_cos, rotary_sin, positions, sections, interleaved, back):
         ctx.sections, ctx.interleaved, ctx.back = sections, interleaved, back
         ctx.set_materialize_grads(False)
+        if _forward_ad._current_level >= 0:
+            ctx.save_for_forward(rotary_cos, rotary_sin, positions)
+            ctx.shapes = q.shape, None if k is None else k.shape
         if _direct(q, k, rotary_cos, rotary_sin, positions):
             tables = _tables("rotary_axes", rotary_cos, rotary_sin, positions, sections, q.shape[0], q.device)
             ctx.save_for_backward(*tables[:3])
@@ -146,9 +151,20 @@ class RotaryAxesFunc(torch.autograd.Function):
         one, other = _rotary_maybe_grad(one, other, *ctx.saved_tensors, ctx.sections, ctx.interleaved, not ctx.back)
         return ((None, one) if dq is None else (one, other)) + (None,) * 6
 
+    @staticmethod
+    def jvp(ctx, tq, tk, t_cos, t_sin, *_):
+        if t_cos is not None or t_sin is not None:
+            raise NotImplementedError("rotary_axes: the tables get no gradient")
+        one, other = (tk, None) if tq is None else (tq, tk)
+        turned, other = _rotary_maybe_grad(one, other, *ctx.saved_tensors, ctx.sections, ctx.interleaved, ctx.back)
+        both = (None, turned) if tq is None else (turned, other)
+        # (a result that is a tensor needs a tangent)
+        return tuple(turned.new_zeros(n) if t is None and n is not None else t for t, n in zip(both, ctx.shapes))
+
 
 def _rotary_maybe_grad(q, k, rotary_cos, rotary_sin, positions, sections, interleaved, back):
-    if (q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled():
+    if (((q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled())
+            or _forward_ad._current_level >= 0):       # (a tensor with a tangent need not require a gradient)
         return RotaryAxesFunc.apply(q, k, rotary_cos, rotary_sin, positions, sections, interleaved, back)
     if _direct(q, k, rotary_cos, rotary_sin, positions):
         return _turn(q, k, _tables("rotary_axes", rotary_cos, rotary_sin, positions, sections, q.shape[0], q.device),

@@ -56,3 +56,22 @@ def test_checkpointed_forward(reentrant):
         torch.autograd.backward(out, (q, k))
         grads.append((x.grad, y.grad))
     assert torch.equal(grads[0][0], grads[1][0]) and torch.equal(grads[0][1], grads[1][1])
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode(grad):
+    """A rotation is linear: the tangent of the result is the rotated tangent."""
+    from torch.autograd import forward_ad
+    q, k, cos, sin, pos, sections = _inputs(77, 3)
+    tq, tk = det_tensor(q.shape, 7).to(DEV), det_tensor(k.shape, 8).to(DEV)
+    want = infllm_v2.rotary_axes(tq, tk, cos, sin, pos, sections=sections)
+    x, y = q.clone().requires_grad_(grad), k.clone().requires_grad_(grad)
+    with forward_ad.dual_level():
+        out = infllm_v2.rotary_axes(forward_ad.make_dual(x, tq), forward_ad.make_dual(y, tk), cos, sin, pos, sections=sections)
+        out = [forward_ad.unpack_dual(t) for t in out]
+        alone = infllm_v2.rotary_axes(forward_ad.make_dual(x, tq), y, cos, sin, pos, sections=sections)
+        alone = [forward_ad.unpack_dual(t).tangent for t in alone]
+    plain = infllm_v2.rotary_axes(q, k, cos, sin, pos, sections=sections)
+    for i in range(2):
+        assert torch.equal(out[i].primal, plain[i]) and torch.equal(out[i].tangent, want[i])
+    assert torch.equal(alone[0], want[0]) and (alone[1] is None or not alone[1].any())

@@ -71,3 +71,70 @@ def test_saved_tensors_may_come_back_with_other_strides(launches, hook, axes):
             out = infllm_v2.rotary_axes(x, y, cos, sin, pos, sections=sections)
         grads.append(torch.autograd.grad(out, (x, y), (q, k)))
     assert torch.equal(grads[0][0], grads[1][0]) and torch.equal(grads[0][1], grads[1][1])
+
+
+def _rotated(x, cos, sin, pos, sections):
+    return infllm_v2.rotary_axes(x, None, cos, sin, pos, sections=sections)[0]
+
+
+@pytest.mark.parametrize("with_k", [None, "plain", "dual"])
+@pytest.mark.parametrize("q_dual", [True, False])
+def test_forward_mode_turns_the_tangents(launches, with_k, q_dual):
+    """A rotation is linear: the tangent of the result is the rotated tangent."""
+    from torch.autograd import forward_ad
+    if not q_dual and with_k != "dual":
+        return
+    q, k, cos, sin, wide = _inputs()
+    pos, sections = wide[:, 20:26], (20, 20, 24)
+    tq, tk = torch.randn(q.shape).to(BF), torch.randn(k.shape).to(BF)
+    for grad in (False, True):
+        x, y = q.clone().requires_grad_(grad), k.clone().requires_grad_(grad)
+        with forward_ad.dual_level():
+            a = forward_ad.make_dual(x, tq) if q_dual else x
+            b = None if with_k is None else forward_ad.make_dual(y, tk) if with_k == "dual" else y
+            out = infllm_v2.rotary_axes(a, b, cos, sin, pos, sections=sections)
+            (po, to), (pk, tk_out) = (forward_ad.unpack_dual(t) if t is not None else (None, None) for t in out)
+            assert torch.equal(po.detach(), _rotated(q, cos, sin, pos, sections))
+            for dual, got, tangent in ((q_dual, to, tq), (with_k == "dual", tk_out, tk)):
+                if dual:
+                    assert torch.equal(got.detach(), _rotated(tangent, cos, sin, pos, sections))
+                else:
+                    assert got is None or not got.any()
+
+
+def test_forward_over_reverse_and_reverse_over_forward(launches):
+    from torch.autograd import forward_ad
+    q, _, cos, sin, wide = _inputs()
+    pos, sections = wide[:, 20:26], (20, 20, 24)
+    g, tg, t = (torch.randn(q.shape).to(BF) for _ in range(3))
+    x = q.clone().requires_grad_(True)
+    with forward_ad.dual_level():
+        y = infllm_v2.rotary_axes(x, None, cos, sin, pos, sections=sections)[0]
+        dx = torch.autograd.grad(y, x, forward_ad.make_dual(g, tg))[0]
+        u = q.clone().requires_grad_(True)
+        want = torch.autograd.grad(infllm_v2.rotary_axes(u, None, cos, sin, pos, sections=sections)[0], u, tg)[0]
+        assert torch.equal(forward_ad.unpack_dual(dx).tangent, want)
+    t.requires_grad_(True)
+    with forward_ad.dual_level():
+        y = infllm_v2.rotary_axes(forward_ad.make_dual(q, t), None, cos, sin, pos, sections=sections)[0]
+        got = torch.autograd.grad(forward_ad.unpack_dual(y).tangent, t, tg)[0]
+    assert torch.equal(got, want)
+
+
+def test_tables_with_a_tangent_are_refused(launches):
+    from torch.autograd import forward_ad
+    q, _, cos, sin, wide = _inputs()
+    pos, sections = wide[:, 20:26], (20, 20, 24)
+    with forward_ad.dual_level():
+        for c, s in ((forward_ad.make_dual(cos, sin), sin), (cos, forward_ad.make_dual(sin, cos))):
+            with pytest.raises(NotImplementedError, match="tables"):
+                infllm_v2.rotary_axes(q, None, c, s, pos, sections=sections)
+
+
+def test_function_transforms_lose_no_derivative(launches):
+    """torch.func.jvp and vjp want more of an autograd.Function than this one has, and say so."""
+    q, _, cos, sin, wide = _inputs()
+    f = lambda x: _rotated(x, cos, sin, wide[:, 20:26], (20, 20, 24))
+    for call in (lambda: torch.func.jvp(f, (q,), (q,)), lambda: torch.func.vjp(f, q)):
+        with pytest.raises(RuntimeError, match="setup_context"):
+            call()
