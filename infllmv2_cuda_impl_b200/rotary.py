@@ -122,16 +122,12 @@ def _registered(q, k, rotary_cos, rotary_sin, positions, sections, interleaved, 
 
 
 class RotaryAxesFunc(torch.autograd.Function):
-    """A rotation is linear: its gradient is the rotation by minus the angle, and so on to any order; a tangent turns as
-    the rows do."""
+    """A rotation is linear: its gradient is the rotation by minus the angle, and so on to any order."""
 
     @staticmethod
     def forward(ctx, q, k, rotary_cos, rotary_sin, positions, sections, interleaved, back):
         ctx.sections, ctx.interleaved, ctx.back = sections, interleaved, back
         ctx.set_materialize_grads(False)
-        if _forward_ad._current_level >= 0:
-            ctx.save_for_forward(rotary_cos, rotary_sin, positions)
-            ctx.shapes = q.shape, None if k is None else k.shape
         if _direct(q, k, rotary_cos, rotary_sin, positions):
             tables = _tables("rotary_axes", rotary_cos, rotary_sin, positions, sections, q.shape[0], q.device)
             ctx.save_for_backward(*tables[:3])
@@ -151,6 +147,17 @@ class RotaryAxesFunc(torch.autograd.Function):
         one, other = _rotary_maybe_grad(one, other, *ctx.saved_tensors, ctx.sections, ctx.interleaved, not ctx.back)
         return ((None, one) if dq is None else (one, other)) + (None,) * 6
 
+
+class RotaryAxesDualFunc(RotaryAxesFunc):
+    """The same where a forward-mode level is open: a tangent turns as the rows do.  (Apart, because torch.compile takes
+    no Function with a jvp.)"""
+
+    @staticmethod
+    def forward(ctx, q, k, rotary_cos, rotary_sin, positions, sections, interleaved, back):
+        ctx.save_for_forward(rotary_cos, rotary_sin, positions)
+        ctx.shapes = q.shape, None if k is None else k.shape
+        return RotaryAxesFunc.forward(ctx, q, k, rotary_cos, rotary_sin, positions, sections, interleaved, back)
+
     @staticmethod
     def jvp(ctx, tq, tk, t_cos, t_sin, *_):
         if t_cos is not None or t_sin is not None:
@@ -163,8 +170,9 @@ class RotaryAxesFunc(torch.autograd.Function):
 
 
 def _rotary_maybe_grad(q, k, rotary_cos, rotary_sin, positions, sections, interleaved, back):
-    if (((q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled())
-            or _forward_ad._current_level >= 0):       # (a tensor with a tangent need not require a gradient)
+    if _forward_ad._current_level >= 0:                # (a tensor with a tangent need not require a gradient)
+        return RotaryAxesDualFunc.apply(q, k, rotary_cos, rotary_sin, positions, sections, interleaved, back)
+    if (q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled():
         return RotaryAxesFunc.apply(q, k, rotary_cos, rotary_sin, positions, sections, interleaved, back)
     if _direct(q, k, rotary_cos, rotary_sin, positions):
         return _turn(q, k, _tables("rotary_axes", rotary_cos, rotary_sin, positions, sections, q.shape[0], q.device),

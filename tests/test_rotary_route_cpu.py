@@ -138,3 +138,19 @@ def test_function_transforms_lose_no_derivative(launches):
     for call in (lambda: torch.func.jvp(f, (q,), (q,)), lambda: torch.func.vjp(f, q)):
         with pytest.raises(RuntimeError, match="setup_context"):
             call()
+
+
+def test_compilation_traces_the_differentiable_form(launches):
+    """In one piece (fullgraph); the compiled code itself, which would launch, is replaced."""
+    q, k, cos, sin, wide = _inputs()
+    pos, sections, graphs = wide[:, 20:26].contiguous(), (20, 20, 24), []
+
+    def backend(graph, inputs):
+        graphs.append(graph)
+        return lambda *args: (q * 2, k * 3)
+
+    f = torch.compile(lambda x, y: infllm_v2.rotary_axes(x, y, cos, sin, pos, sections=sections), backend=backend, fullgraph=True)
+    for grad in (False, True):
+        a, b = f(q.clone().requires_grad_(grad), k)
+        assert torch.equal(a, q * 2) and torch.equal(b, k * 3)
+    assert len(graphs) == 2 and not launches
