@@ -474,8 +474,7 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     // The bytes are not touched before the unit's turn either.
     auto locate = [&](int key0, int slot, int& row, uint32_t& kb, uint32_t& vb) {
       row = -1;
-      kb = 0;
-      vb = kNanByte;                               // (a page that the cache does not have: NaN)
+      kb = vb = kNanByte;                          // (a page that the cache does not have: NaN; no tile comes for it)
       const int key = key0 + lane;
       if (key < len) {
         if (kPage != 0) {
@@ -583,7 +582,7 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       }
       if (kCopied) {
         const int at = key1 >= 0 ? turn : turn ^ 1;          // (the places are given out in turn)
-        kb = row >= 0 ? scale_bytes[warp][at][0][lane] : 0;
+        kb = row >= 0 ? scale_bytes[warp][at][0][lane] : kNanByte;
         vb = row >= 0 ? scale_bytes[warp][at][1][lane] : kNanByte;
       }
       // 2^(kb - 127) = 2^a 2^b: with the query's factor between the two no product leaves the range that the score is in

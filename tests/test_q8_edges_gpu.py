@@ -1,0 +1,41 @@
+"""GPU: edges of the 8-bit cache and of the attention over it, next to the tests of each operator."""
+import pytest
+import torch
+
+import infllm_v2
+from oracle.q8 import attend, quantise
+from helpers import det_tensor, cu
+from test_q8_decode_gpu import DEV, E4M3, INT8, _cache, _check, _to_gpu
+
+pytestmark = pytest.mark.gpu
+
+
+def _ints(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+@pytest.mark.parametrize("dtype", [E4M3, INT8])
+@pytest.mark.parametrize("page,topk", [(0, False), (16, False), (32, False), (64, False), (16, True), (64, True)])
+def test_log_sum_exp_of_places_that_do_not_exist_is_nan(dtype, page, topk):
+    """Scores against rows that the cache does not have are NaN, whatever the SM's memory held before."""
+    q = det_tensor((3, 1, 32, 128), 7)
+    if page:
+        per = 192 // page
+        cache = _cache(3 * per, page, 2, dtype, 3)
+        table = torch.randperm(3 * per, generator=torch.Generator().manual_seed(1)).view(3, per).to(torch.int32)
+        table[1, 1], table[2, per - 1] = 3 * per, -1
+        lens, where = [192, 2 * page + 5, 192 - page], dict(block_table=table.to(DEV))       # the third does not reach its bad page
+    else:
+        cache = _cache(3, 190, 2, dtype, 3)
+        table = torch.tensor([0, 3, 2], dtype=torch.int32)
+        lens, where = [190, 77, 64], dict(cache_batch_idx=table.to(DEV))
+    idx = torch.arange(3, dtype=torch.int32).expand(3, 2, 1, 3).contiguous() if topk else None
+    junk = _to_gpu(_cache(64, 640, 2, dtype, 5))
+    for _ in range(3):
+        infllm_v2.infllmv2_attn_with_kvcache_q8(det_tensor((64, 1, 32, 128), 7).to(DEV), *junk)
+        out, lse = infllm_v2.infllmv2_attn_with_kvcache_q8(
+            q.to(DEV), *_to_gpu(cache), cache_seqlens=_ints(lens), topk_idx=None if idx is None else idx.to(DEV),
+            return_softmax_lse=True, **where)
+        assert bool(torch.isnan(out[1].float()).all()) and bool(torch.isnan(lse[1]).all())
+        assert not torch.isnan(lse[::2]).any()
+        _check(out[::2], lse[::2], q[::2], cache, lens[::2], table[::2] if page else None, None if page else table[::2])
