@@ -516,7 +516,7 @@ int64_t ifv2_q8_decode_workspace_bytes(int batch, int heads_q, int head_dim);
  * (batch, heads_k, mask_words; shorter ones leave it as it is, and it may be null).  topk_idx null: mask is given,
  * or null = all keys.  lse (batch, heads_q) fp32 or null.  Pages are a multiple of 16 positions.
  * A sequence attends positions [0, min(cache_seqlens[b] + new, capacity)); a new token without room is neither
- * written nor attended, a negative length attends nothing.  Sequences without keys get out = 0, lse = +inf; those with a key in a page or
+ * written nor attended, a negative length attends nothing.  Sequences without keys get out = 0, lse = +inf; those that attend a key in a page or
  * slot that the cache does not have out = lse = NaN.  batch * heads_k <= 65535. */
 int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void* k_scale, void* v_scale, const void* k_new,
                    const void* v_new, const float* rotary_cos, const float* rotary_sin,

@@ -10,14 +10,16 @@ namespace ifv2 {
 // short bisections, so that 32 look-ups cost one trip to memory.  (One thread walking the words paid a
 // chain of a load per word, 33 of them at 131072 tokens, for the count and again for every block.)
 // Every lane must make the calls and gets the same answers.
-template <int kStride>
+// kWritten: the words may be written while the kernel lives already, by one beside which it starts and for which it
+// waits before the first call; a read-only load (__ldg) is not for them, and may be moved in front of the wait.
+template <int kStride, bool kWritten = false>
 struct BlockList {
   const unsigned long long* words;   // null = every block below nblk
   int nwords, nblk;
   int cached;                        // lane i: block of look-up 32 n + i
   __device__ unsigned long long word(int w) const {
     if (w >= nwords) return 0ull;
-    unsigned long long x = __ldg(words + w);
+    unsigned long long x = kWritten ? words[w] : __ldg(words + w);
     const int first = w * 64;
     if (nblk - first < 64) x &= (nblk > first) ? ((1ull << (nblk - first)) - 1ull) : 0ull;
     return x;

@@ -416,7 +416,7 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 
     wait_previous();                               // (the mask, or a new row of shared pages)
     const int n_all = (len + kBlockN - 1) / kBlockN;
-    BlockList<2> list{p.mask ? p.mask + pair * p.mask_words : nullptr, p.mask_words, n_all, -1};
+    BlockList<2, true> list{p.mask ? p.mask + pair * p.mask_words : nullptr, p.mask_words, n_all, -1};
     // blocks to attend, of which this CTA takes numbers j0 .. j1 - 1
     const uint32_t n = listed ? sort_list(block_list, p.topk_idx + pair * p.topk, p.topk, n_all) : list.count(lane);
     const int j0 = n == nw ? w0 : (int)((uint64_t)w0 * n / nw), j1 = n == nw ? w1 : (int)((uint64_t)w1 * n / nw);
@@ -427,7 +427,7 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       if (pos >= 0 && pos < p.capacity) {
         const int blk = pos / kBlockN;
         const bool attended = !selected || (listed ? n > 0 && block_list[n - 1] == blk
-                                                   : blk / 64 < p.mask_words && ((__ldg(list.words + blk / 64) >> (blk & 63)) & 1ull));
+                                                   : blk / 64 < p.mask_words && ((list.words[blk / 64] >> (blk & 63)) & 1ull));
         const int owner = attended ? (((n - 1 - j0) & 1) << 1) | ((pos / kUnit) & 1) : 0;
         if ((attended ? j0 < j1 && j1 == (int)n : w0 == 0) && warp == owner) {
           const int64_t row = ((int64_t)b * p.heads_k + h) * p.place.length + pos;

@@ -190,7 +190,7 @@ def infllmv2_attn_with_kvcache_q8(
     does, at rotary_positions ((batch,) or (axes, batch) int32 with rotary_sections; default: cache_seqlens); without
     an append nothing is rotated.  The rotated rows are not rounded to bf16 in between.
     A new token without room in the cache is neither written nor attended.  A sequence without keys gets 0
-    (softmax_lse +inf), one with a key in a page or slot that the cache does not have NaN (softmax_lse too).
+    (softmax_lse +inf), one that attends a key in a page or slot that the cache does not have NaN (softmax_lse too).
     Returns out (batch, 1, nheads, 128) [, softmax_lse (batch, nheads, 1) fp32].  Forward only."""
     what = "infllmv2_attn_with_kvcache_q8"
     slots, hk, length, code, dev = _check_cache(what, k_cache, v_cache, k_scale, v_scale)

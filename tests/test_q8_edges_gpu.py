@@ -39,3 +39,31 @@ def test_log_sum_exp_of_places_that_do_not_exist_is_nan(dtype, page, topk):
         assert bool(torch.isnan(out[1].float()).all()) and bool(torch.isnan(lse[1]).all())
         assert not torch.isnan(lse[::2]).any()
         _check(out[::2], lse[::2], q[::2], cache, lens[::2], table[::2] if page else None, None if page else table[::2])
+
+
+@pytest.mark.parametrize("dtype", [E4M3, INT8])
+def test_long_lists_that_change_from_call_to_call(dtype):
+    """Lists of more than 256 entries are packed by a kernel beside which the attention starts: every call attends its own
+    list, although the packed words lie where those of the call before lay."""
+    n, k = 20000, 260
+    cache = _cache(1, n, 1, dtype, 3)
+    dev, q = _to_gpu(cache), det_tensor((1, 1, 16, 128), 7)
+    lists = []
+    for first in (0, 25, 50, 100, 0):
+        idx = torch.full((1, 1, 1, k), -1, dtype=torch.int32)
+        blocks = torch.arange(first, 313, 2 + first // 25)
+        idx[0, 0, 0, :len(blocks)] = blocks
+        lists.append(idx)
+    outs = [infllm_v2.infllmv2_attn_with_kvcache_q8(q.to(DEV), *dev, topk_idx=idx.to(DEV), return_softmax_lse=True)
+            for idx in lists]
+    for (out, lse), idx in zip(outs, lists):
+        _check(out, lse, q, cache, [n], topk_idx=idx)
+    graph, idx = torch.cuda.CUDAGraph(), lists[0].to(DEV)
+    qd = q.to(DEV)
+    with torch.cuda.graph(graph):
+        out, lse = infllm_v2.infllmv2_attn_with_kvcache_q8(qd, *dev, topk_idx=idx, return_softmax_lse=True)
+    for (want, want_lse), other in zip(outs, lists):
+        idx.copy_(other)
+        for _ in range(3):
+            graph.replay()
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
