@@ -483,8 +483,8 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
           row = slot0 + key;
         }
         if (!kCopied && row >= 0) {
-          kb = __ldcg(p.k_scale + row);            // (not through L1: the newest may have been written by this warp)
-          vb = __ldcg(p.v_scale + row);
+          kb = p.k_scale[row];                     // (ordinary loads: this warp or the kernel before wrote the newest)
+          vb = p.v_scale[row];
         }
       }
     };
