@@ -481,7 +481,8 @@ int ifv2_rotary_axes(const void* q, const void* k, void* q_out, void* k_out, con
  * p of sequence b then lives in page block_table[b][p / length].  The exponent of a row is the smallest >= -127
  * with which its largest magnitude fits the codes (448 or 127); codes are rounded to nearest even.  A row with
  * an infinity or a NaN is stored as NaN.  Writes to pages, slots or positions that the cache does not have are
- * dropped; reads of them give NaN.  No counterpart in the reference, whose cache is bf16 or fp16.
+ * dropped; reads of them give NaN.  A row that two tokens of one call go to is undefined (codes and scale may
+ * come from different tokens).  No counterpart in the reference, whose cache is bf16 or fp16.
  *
  * ifv2_q8_fill: packed rows k, v (total, heads_k, 128) bf16 with the given strides (elements, multiples of 8)
  * of sequences cu_seqlens (batch + 1) go to positions start[b] + 0, 1, ... (start null = 0).  seqlens_out (may

@@ -9,7 +9,9 @@ A slot is a sequence of up to `length` tokens, or with a block_table (batch, max
 A row's value is code * scale.  The scale is the smallest power of two (at least 2^-127) with which the row's largest
 magnitude fits the codes (448 or 127), codes are rounded to nearest even, and reading back is exact.  A row with an
 infinity or a NaN reads back as NaN.  Writes to pages, slots or positions that the cache does not have are dropped,
-reads of them give NaN.  Two tokens of one call that go to the same row leave one of them."""
+reads of them give NaN.  Where two tokens of one call go to the same row (a page twice in a block_table, sequences that
+share a slot at one length) that row is undefined: codes and scale may come from different tokens.  No other row is
+touched."""
 import functools
 from typing import Optional, Sequence, Tuple, Union
 

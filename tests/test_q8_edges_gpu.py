@@ -67,3 +67,42 @@ def test_long_lists_that_change_from_call_to_call(dtype):
         for _ in range(3):
             graph.replay()
         assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
+@pytest.mark.parametrize("dtype", [E4M3, INT8])
+def test_two_tokens_of_one_row_touch_no_other_row(dtype):
+    """Such a row is undefined; the rows around it, and what the other sequences attend, are not."""
+    hk, page, lens = 2, 16, [20, 36, 9]
+    table = torch.tensor([[0, 1, 2], [3, 1, 4], [5, 6, 7]], dtype=torch.int32)          # page 1 twice
+    k, v = det_tensor((sum(lens), hk, 128), 1), det_tensor((sum(lens), hk, 128), 2)
+    cache = infllm_v2.q8_cache(8, page, hk, dtype, DEV)
+    for t in cache:
+        t.view(torch.uint8).fill_(0xA5)
+    infllm_v2.cache_fill_q8(k.to(DEV), v.to(DEV), *cache, cu(lens, DEV), block_table=table.to(DEV))
+    new_k, new_v = det_tensor((3, 1, hk, 128), 3), det_tensor((3, 1, hk, 128), 4)
+    # the appends of the first two sequences: position 20 is in page 1 as well, offset 4, and so is 16 + 4 of the second
+    q = det_tensor((3, 1, 16 * hk, 128), 5)
+    out, lse = infllm_v2.infllmv2_attn_with_kvcache_q8(
+        q.to(DEV), *cache, k=new_k.to(DEV), v=new_v.to(DEV), cache_seqlens=_ints([20, 20, 9]), block_table=table.to(DEV),
+        return_softmax_lse=True)
+    want = [torch.full(t.shape, 0xA5, dtype=torch.uint8) for t in cache]
+    both = torch.zeros(8, page, dtype=torch.bool)
+    both[1, :5] = True
+    at = 0
+    for b, n in enumerate(lens):
+        for i in range(n):
+            p, o = int(table[b, i // page]), i % page
+            for x, j in ((k, 0), (v, 1)):
+                y, e = quantise(x[at + i], dtype)
+                want[j][p, :, o], want[j + 2][p, :, o] = y.view(torch.uint8), e
+        at += n
+    for x, j in ((new_k, 0), (new_v, 1)):
+        y, e = quantise(x[2, 0], dtype)
+        want[j][5, :, 9], want[j + 2][5, :, 9] = y.view(torch.uint8), e
+    for got, ref in zip(cache, want):
+        got, ref = got.view(torch.uint8).cpu().movedim(1, 2), ref.movedim(1, 2)
+        if got.dim() == 4 and dtype == E4M3:                                            # (a zero may have either sign)
+            got, ref = got.view(E4M3).float().nan_to_num(1000.0), ref.view(E4M3).float().nan_to_num(1000.0)
+        assert torch.equal(got[~both], ref[~both])
+    kc, vc, kb, vb = (t.cpu() for t in cache)
+    _check(out[2:], lse[2:], q[2:], (kc, vc, kb.view(torch.uint8), vb.view(torch.uint8)), [10], table[2:])
