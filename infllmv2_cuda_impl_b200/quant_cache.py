@@ -86,6 +86,11 @@ def _cu(what, cu_seqlens, dev):
     return cu_seqlens if cu_seqlens.is_contiguous() else cu_seqlens.contiguous(), shape[0] - 1
 
 
+def _no_gradient(what, k, v):
+    if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+        raise NotImplementedError(f"{what}: nothing flows back from a cache (pass k.detach() and v.detach())")
+
+
 def cache_fill_q8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
                   v_scale: torch.Tensor, cu_seqlens: torch.Tensor, start: Optional[torch.Tensor] = None,
                   block_table: Optional[torch.Tensor] = None, seqlens_out: Optional[torch.Tensor] = None) -> None:
@@ -98,8 +103,7 @@ def cache_fill_q8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cac
     if (k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16 or len(shape) != 3 or shape[1] != hk or shape[2] != HEAD_DIM
             or v.shape != shape or k.device != dev or v.device != dev):
         raise ValueError(f"{what}: k and v must be (total, {hk}, {HEAD_DIM}) bf16 on {dev}")
-    if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
-        raise NotImplementedError(f"{what}: nothing flows back from a cache (pass k.detach() and v.detach())")
+    _no_gradient(what, k, v)
     cu_seqlens, batch = _cu(what, cu_seqlens, dev)
     block_table, pages = _table(what, block_table, batch, dev)
     if block_table is None and slots < batch:
@@ -155,6 +159,7 @@ def decode_append_q8(k_new: torch.Tensor, v_new: torch.Tensor, k_cache: torch.Te
     for name, t in (("k_new", k_new), ("v_new", v_new)):
         if t.dtype != torch.bfloat16 or t.device != dev or not t.is_contiguous() or t.numel() != b * hk * HEAD_DIM:
             raise ValueError(f"{what}: {name} must be contiguous ({b}, {hk}, {HEAD_DIM}) bf16 on {dev}")
+    _no_gradient(what, k_new, v_new)
     if slots < b:
         raise ValueError(f"{what}: {b} sequences need as many slots")
     for name, t in (("cache_seqlens", cache_seqlens), ("positions", positions), ("n_comp", n_comp), ("n_comp2", n_comp2)):
@@ -209,6 +214,7 @@ def infllmv2_attn_with_kvcache_q8(
         if (k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16 or k.shape != new or v.shape != new
                 or k.device != dev or v.device != dev):
             raise ValueError(f"{what}: k and v must be {new} bf16 on {dev}")
+        _no_gradient(what, k, v)
         k, v = k.contiguous(), v.contiguous()
         k_ptr, v_ptr = k.data_ptr(), v.data_ptr()
     elif k is not None or v is not None:
