@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(kThreads) q8_fill_kernel(const MoveParams p) {
   const int64_t t = (int64_t)blockIdx.x * kTile + threadIdx.x / kLanes;
   if (p.seqlens_out != nullptr && h == 0)
     for (int64_t b = (int64_t)blockIdx.x * kThreads + threadIdx.x; b < p.batch; b += (int64_t)gridDim.x * kThreads)
-      p.seqlens_out[b] = (int32_t)min((int64_t)max(p.cu[b + 1] - p.cu[b] + (p.start ? p.start[b] : 0), 0), p.capacity);
+      p.seqlens_out[b] = (int32_t)min(max((int64_t)p.cu[b + 1] - p.cu[b] + (p.start ? p.start[b] : 0), (int64_t)0), p.capacity);
   uint4 raw[2][2];                               // (on their way while the row's place is looked up)
 #pragma unroll
   for (int i = 0; i < 2; ++i) {

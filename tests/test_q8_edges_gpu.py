@@ -106,3 +106,14 @@ def test_two_tokens_of_one_row_touch_no_other_row(dtype):
         assert torch.equal(got[~both], ref[~both])
     kc, vc, kb, vb = (t.cpu() for t in cache)
     _check(out[2:], lse[2:], q[2:], (kc, vc, kb.view(torch.uint8), vb.view(torch.uint8)), [10], table[2:])
+
+
+def test_lengths_next_to_the_border_of_32_bits():
+    """start + rows is a number of more than 32 bits: the length is the capacity, as for any start past it."""
+    cache = infllm_v2.q8_cache(3, 16, 1, INT8, DEV)
+    k = det_tensor((6, 1, 128), 1).to(DEV)
+    lens = torch.zeros(3, dtype=torch.int32, device=DEV)
+    infllm_v2.cache_fill_q8(k, k, *cache, cu([2, 2, 2], DEV), start=_ints([2 ** 31 - 1, -2 ** 31, 15]), seqlens_out=lens)
+    assert lens.tolist() == [16, 0, 16]
+    seen = cache[0].view(torch.uint8).any(-1).any(1).nonzero().tolist()
+    assert seen == [[2, 15]]
