@@ -38,6 +38,7 @@ constexpr long long kWaitLimit = 1ll << 28;      // clocks; a copy takes microse
 constexpr int kPartialFloats = kHeadDim + 4;     // O row, m (log2 units), l, exponent of O's units, pad
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kLowest = -0x1.fffffep127f;      // the lowest finite number
 
 struct Q8DecodeParams {
   const __nv_bfloat16* q;          // (batch, heads_q, 128)
@@ -640,7 +641,7 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const float m = r ? m1 : m0, u = r ? u1 : u0;
-          const float n = m == -INFINITY ? 0.f : -m, w = u == -INFINITY ? 0.f : 8.f - u;
+          const float n = -m, w = 8.f - u;
           const uint64_t nn = tc::pack_f32x2(n, n), ww = tc::pack_f32x2(w, w);
           uint64_t total = 0;
 #pragma unroll
@@ -667,7 +668,9 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       bool again = fresh;
       if (!fresh) again = key0 + kUnit > len ? weigh(std::true_type{}) : weigh(std::false_type{});
       if (__any_sync(0xFFFFFFFFu, again)) {
-        float mx0 = m0, mx1 = m1, mu0 = u0, mu1 = u1;
+        // (no reference is -inf: next to scores that are all -inf, or NaN, the first finite one weighs infinitely, and
+        // the references move)
+        float mx0 = fmaxf(m0, kLowest), mx1 = fmaxf(m1, kLowest), mu0 = fmaxf(u0, kLowest), mu1 = fmaxf(u1, kLowest);
 #pragma unroll
         for (int nt = 0; nt < kUnit / 8; ++nt) {
 #pragma unroll
@@ -690,9 +693,9 @@ q8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
           mu0 = fmaxf(mu0, __shfl_xor_sync(0xFFFFFFFFu, mu0, d));
           mu1 = fmaxf(mu1, __shfl_xor_sync(0xFFFFFFFFu, mu1, d));
         }
-        l0 *= mx0 == -INFINITY ? 1.f : exp2f(m0 - mx0);
-        l1 *= mx1 == -INFINITY ? 1.f : exp2f(m1 - mx1);
-        const float f0 = mu0 == -INFINITY ? 1.f : exp2f(u0 - mu0), f1 = mu1 == -INFINITY ? 1.f : exp2f(u1 - mu1);
+        l0 *= exp2f(m0 - mx0);
+        l1 *= exp2f(m1 - mx1);
+        const float f0 = exp2f(u0 - mu0), f1 = exp2f(u1 - mu1);
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
           o[k][0] *= f0;

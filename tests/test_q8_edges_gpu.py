@@ -117,3 +117,21 @@ def test_lengths_next_to_the_border_of_32_bits():
     assert lens.tolist() == [16, 0, 16]
     seen = cache[0].view(torch.uint8).any(-1).any(1).nonzero().tolist()
     assert seen == [[2, 15]]
+
+
+@pytest.mark.parametrize("dtype", [E4M3, INT8])
+def test_first_keys_whose_scores_leave_the_range(dtype):
+    """The first two blocks score -inf in 32 bits (-2^130), the others about -28: they alone have weight, and their weights
+    are held against their own maximum.  One CTA attends all of a head, so that every warp begins in such a block."""
+    batch, hk, n = 64, 8, 512
+    k, v = det_tensor((batch, hk, n, 128), 3, 1.0), det_tensor((batch, hk, n, 128), 4, 1.0)
+    q = (det_tensor((batch, 1, hk * 16, 128), 5, 1.0) * 8).round() / 8                   # (exact next to 2^10)
+    q[..., :8], q[..., 8] = -2.0 ** 10, 16.0
+    k[:, :, :128] = 0
+    k[:, :, :128, :8] = 2.0 ** 120
+    k[:, :, 128:, :8], k[:, :, 128:, 8] = 0, -20.0
+    (kc, kb), (vc, vb) = quantise(k, dtype), quantise(v, dtype)
+    idx = torch.arange(8, dtype=torch.int32, device=DEV).expand(batch, hk, 1, 8)
+    out, lse = infllm_v2.infllmv2_attn_with_kvcache_q8(q.to(DEV), *_to_gpu((kc, vc, kb, vb)), topk_idx=idx, return_softmax_lse=True)
+    rest = (kc[:, :, 128:], vc[:, :, 128:], kb[:, :, 128:], vb[:, :, 128:])
+    _check(out, lse, q, rest, [n - 128] * batch)
