@@ -486,11 +486,11 @@ int ifv2_rotary_axes(const void* q, const void* k, void* q_out, void* k_out, con
  *
  * ifv2_q8_fill: packed rows k, v (total, heads_k, 128) bf16 with the given strides (elements, multiples of 8)
  * of sequences cu_seqlens (batch + 1) go to positions start[b] + 0, 1, ... (start null = 0).  seqlens_out (may
- * be null): min(start[b] + len_b, capacity).  Rows from cu_seqlens[batch] on go nowhere.
+ * be null; overlaps neither start nor cu_seqlens): min(start[b] + len_b, capacity).  Rows from cu_seqlens[batch] on go nowhere.
  * ifv2_q8_read: the way back into dense k, v (total, heads_k, 128) bf16, exactly; rows from cu_seqlens[batch] on
  * are set to 0.
  * ifv2_q8_append: ifv2_decode_append for such a cache in slots; compressed keys are means of the keys as the
- * cache holds them. */
+ * cache holds them.  The lengths, positions and counts do not overlap. */
 int ifv2_q8_fill(const void* k, const void* v, int64_t k_token_stride, int64_t k_head_stride,
                  int64_t v_token_stride, int64_t v_head_stride, void* k_cache, void* v_cache, void* k_scale,
                  void* v_scale, const int32_t* cu_seqlens, const int32_t* start, const int32_t* block_table,

@@ -216,6 +216,12 @@ __global__ void __launch_bounds__(kThreads) q8_append_kernel(const AppendQ8Param
 
 using namespace ifv2;
 
+// Whether na and nb numbers from a and b on share memory (null: they do not).
+static bool overlap(const int32_t* a, int64_t na, const int32_t* b, int64_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a != nullptr && b != nullptr && x < y + 4 * (uintptr_t)nb && y < x + 4 * (uintptr_t)na;
+}
+
 static int move_common(MoveParams& p, const char* what, void* k_cache, void* v_cache, void* k_scale, void* v_scale,
                        const int32_t* cu_seqlens, const int32_t* start, const int32_t* block_table, int block_table_stride,
                        int64_t slots, int64_t length, int code, int batch, int64_t total, int heads_k, int head_dim) {
@@ -256,7 +262,8 @@ extern "C" int ifv2_q8_fill(const void* k, const void* v, int64_t k_token_stride
   IFV2_REQUIRE((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 == 0 &&
                    (k_token_stride | k_head_stride | v_token_stride | v_head_stride) % 8 == 0,
                IFV2_ERR_INVALID_ARG, "q8_fill: rows must be 16-byte aligned");
-  IFV2_REQUIRE(seqlens_out == nullptr || seqlens_out != start, IFV2_ERR_INVALID_ARG, "q8_fill: seqlens_out must not alias start");
+  IFV2_REQUIRE(!overlap(seqlens_out, batch, start, batch) && !overlap(seqlens_out, batch, cu_seqlens, (int64_t)batch + 1),
+               IFV2_ERR_INVALID_ARG, "q8_fill: seqlens_out must not overlap start or cu_seqlens");
   p.src[0] = static_cast<const uint4*>(k);
   p.src[1] = static_cast<const uint4*>(v);
   p.token_stride[0] = k_token_stride / 8;
@@ -303,7 +310,11 @@ extern "C" int ifv2_q8_append(const void* k_new, const void* v_new, void* k_cach
   IFV2_REQUIRE(batch >= 1 && slots >= batch && heads_k >= 1 && capacity >= 1, IFV2_ERR_INVALID_ARG, "q8_append: bad size");
   IFV2_REQUIRE(k_new && v_new && k_cache && v_cache && k_scale && v_scale && cache_seqlens, IFV2_ERR_INVALID_ARG,
                "q8_append: null pointer");
-  IFV2_REQUIRE(cache_seqlens != positions, IFV2_ERR_INVALID_ARG, "q8_append: positions must not alias cache_seqlens");
+  const int32_t* written[4] = {cache_seqlens, positions, n_comp, n_comp2};
+  for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < i; ++j)
+      IFV2_REQUIRE(!overlap(written[i], batch, written[j], batch), IFV2_ERR_INVALID_ARG,
+                   "q8_append: cache_seqlens, positions and the counts must not overlap");
   IFV2_REQUIRE(kc_cache == nullptr || (c_capacity >= 1 && kernel_size >= 1 && kernel_stride >= 1), IFV2_ERR_INVALID_ARG,
                "q8_append: bad compression arguments");
   IFV2_REQUIRE(kc2_cache == nullptr || (c2_capacity >= 1 && kernel2_size >= 1 && kernel2_stride >= 1), IFV2_ERR_INVALID_ARG,
