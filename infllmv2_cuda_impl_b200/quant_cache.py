@@ -20,7 +20,7 @@ import torch
 from . import _lib
 from .attention import BLOCK_N, GROUP, HEAD_DIM
 from .ops import _on, _require_cuda, _stream
-from .rotary import _rows, _tables
+from .rotary import _no_gradient as _no_table_gradient, _rows, _tables
 
 _LIST = 256      # longest block list that the attention takes without a mask
 _CODES = {torch.float8_e4m3fn: 0, torch.int8: 1}
@@ -258,6 +258,7 @@ def infllmv2_attn_with_kvcache_q8(
             mask_ptr = block_mask.data_ptr()
     rotary = (None, None, None, 0, None, 0, 0, 0)
     if rotary_cos is not None and k is not None:
+        _no_table_gradient(what, rotary_cos, rotary_sin)
         if rotary_sections is not None and type(rotary_sections) is not tuple:
             rotary_sections = tuple(rotary_sections)
         cos, sin, at, axis_stride, pair_axis, axes, rows, pairs = _tables(

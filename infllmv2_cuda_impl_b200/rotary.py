@@ -30,6 +30,12 @@ def _pair_axis(sections, pairs: int, axes: int) -> Optional[bytes]:
     return b"".join(bytes([a]) * n for a, n in enumerate(sections))
 
 
+def _no_gradient(what, rotary_cos, rotary_sin):
+    """(Of the caller's own tensors: below the registered operator, and where a compiler traces it, nobody would ask.)"""
+    if rotary_cos.requires_grad or rotary_sin.requires_grad:
+        raise NotImplementedError(f"{what}: the tables get no gradient")
+
+
 def _tables(what, rotary_cos, rotary_sin, positions, sections, tokens, device):
     """Checks of the arguments that every rotating call takes; (cos, sin, positions, axis_stride, pair_axis, axes, rows,
     pairs).  (These calls are bound by their host time where tokens are few, so a check costs one attribute.)"""
@@ -37,8 +43,6 @@ def _tables(what, rotary_cos, rotary_sin, positions, sections, tokens, device):
     if (rotary_cos.dtype is not torch.float32 or rotary_sin.dtype is not torch.float32 or len(shape) != 2
             or rotary_sin.shape != shape or rotary_cos.device != device or rotary_sin.device != device):
         raise ValueError(f"{what}: rotary_cos and rotary_sin must be (positions, rotary_dim / 2) fp32 on {device}, of one shape")
-    if rotary_cos.requires_grad or rotary_sin.requires_grad:
-        raise NotImplementedError(f"{what}: the tables get no gradient")
     rows, pairs = shape
     if pairs < 8 or pairs > HEAD_DIM // 2 or pairs % 8 != 0 or rows < 1:
         raise ValueError(f"{what}: rotary_dim must be a positive multiple of 16 up to {HEAD_DIM}, and the tables hold a position")
@@ -202,6 +206,7 @@ def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], rotary_cos: torch.Te
         other = k.shape
         if k.dtype is not torch.bfloat16 or len(other) != 3 or other[2] != HEAD_DIM or other[0] != shape[0] or k.device != q.device:
             raise ValueError(f"rotary_axes: k must be (tokens, nheads_k, {HEAD_DIM}) bf16, with the tokens and on the device of q")
+    _no_gradient("rotary_axes", rotary_cos, rotary_sin)
     if sections is not None and type(sections) is not tuple:
         sections = tuple(sections)
     return _rotary_maybe_grad(q, k, rotary_cos, rotary_sin, positions, sections, bool(interleaved), False)

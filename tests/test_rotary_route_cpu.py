@@ -154,3 +154,28 @@ def test_compilation_traces_the_differentiable_form(launches):
         a, b = f(q.clone().requires_grad_(grad), k)
         assert torch.equal(a, q * 2) and torch.equal(b, k * 3)
     assert len(graphs) == 2 and not launches
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_tables_that_require_a_gradient_are_refused_in_every_form(launches, grad):
+    q, k, cos, sin, wide = _inputs()
+    pos, sections = wide[:, 20:26].contiguous(), (20, 20, 24)
+    q.requires_grad_(grad)
+
+    class Pass(torch.overrides.TorchFunctionMode):
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    def call(c, s):
+        return infllm_v2.rotary_axes(q, k, c, s, pos, sections=sections)
+
+    def under_a_mode(c, s):
+        with Pass():
+            return call(c, s)
+
+    compiled = torch.compile(call, backend=lambda graph, inputs: lambda *args: (q * 2, k * 3))
+    for f in (call, under_a_mode, compiled):
+        for c, s in ((cos.clone().requires_grad_(True), sin), (cos, sin.clone().requires_grad_(True))):
+            with pytest.raises(NotImplementedError, match="tables"):
+                f(c, s)
+    assert not launches
