@@ -135,3 +135,20 @@ def test_first_keys_whose_scores_leave_the_range(dtype):
     out, lse = infllm_v2.infllmv2_attn_with_kvcache_q8(q.to(DEV), *_to_gpu((kc, vc, kb, vb)), topk_idx=idx, return_softmax_lse=True)
     rest = (kc[:, :, 128:], vc[:, :, 128:], kb[:, :, 128:], vb[:, :, 128:])
     _check(out, lse, q, rest, [n - 128] * batch)
+
+
+@pytest.mark.parametrize("dtype", [E4M3, INT8])
+@pytest.mark.parametrize("vexp", [-120, -125, -128])
+def test_results_among_the_subnormal_numbers(dtype, vexp):
+    """A bf16 number below 2^-126 has steps of 2^-133, so a rounding is off by 2^-134; 2^-133 leaves as much for fp32 sums of
+    subnormal numbers (2^-149 each).  Weights: 2^-11, and scores off by 130 * 2^-24 * sum |q k| / sqrt(128) < 2^-13."""
+    k, v, q = det_tensor((1, 1, 100, 128), 3, 1.0), det_tensor((1, 1, 100, 128), 4, 1.0), det_tensor((1, 1, 16, 128), 5, 1.0)
+    v = (v.double() * 2.0 ** vexp).to(torch.bfloat16)
+    v[0, 0, 7] = 0
+    (kc, kb), (vc, vb) = quantise(k, dtype), quantise(v, dtype)
+    out = infllm_v2.infllmv2_attn_with_kvcache_q8(q.to(DEV), *_to_gpu((kc, vc, kb, vb)), cache_seqlens=100).cpu().double()[:, 0]
+    want, _ = attend(q[:, 0], kc, vc, kb, vb, [100])
+    avg, _ = attend(q[:, 0], kc, vc.float().abs(), kb, vb, [100])
+    tol = 2.0 ** -8 * want.abs() + 2.0 ** -10 * avg + 2.0 ** -133
+    assert bool(((out - want).abs() <= tol).all())
+    assert float((out == 0).double().mean()) <= float((want.abs() <= 2.0 ** -134 + 2.0 ** -10 * avg).double().mean())
