@@ -192,7 +192,7 @@ def infllmv2_attn_with_kvcache_q8(
     into position cache_seqlens[b] first, in place.  cache_seqlens: int or (batch,) int32 (default: the whole
     capacity).  cache_batch_idx (batch,) int32: the slot each sequence uses.  block_table (batch, max_pages) int32:
     slots are pages, of a multiple of 16 positions.  topk_idx: int32 (batch, nheads_k, 1, topk) 64-token blocks to
-    attend (None = all), or block_mask: the same packed, int64 (batch, nheads_k, 1, words).
+    attend (None = all), or block_mask: the same packed, int64 (batch, nheads_k, 1, words); the 1 may be missing.
     rotary_cos / rotary_sin (positions, rotary_dim / 2) fp32 rotate the query and the appended key, as `rotary_axes`
     does, at rotary_positions ((batch,) or (axes, batch) int32 with rotary_sections; default: cache_seqlens); without
     an append nothing is rotated.  The rotated rows are not rounded to bf16 in between.
@@ -242,16 +242,17 @@ def infllmv2_attn_with_kvcache_q8(
     if block_mask is not None:
         words = (cap + 64 * BLOCK_N - 1) // (64 * BLOCK_N)
         if topk_idx is not None or block_mask.dtype is not torch.int64 or block_mask.device != dev \
-                or block_mask.numel() != batch * hk * words:
+                or block_mask.shape not in ((batch, hk, 1, words), (batch, hk, words)):
             raise ValueError(f"{what}: block_mask must be ({batch}, {hk}, 1, {words}) int64 on {dev} and excludes topk_idx")
         block_mask = block_mask.contiguous()
         mask_ptr = block_mask.data_ptr()
     elif topk_idx is not None:
         words = (cap + 64 * BLOCK_N - 1) // (64 * BLOCK_N)
-        if topk_idx.dtype is not torch.int32 or topk_idx.device != dev or topk_idx.dim() not in (3, 4) \
-                or topk_idx.numel() != batch * hk * topk_idx.shape[-1]:
+        shape = topk_idx.shape
+        if topk_idx.dtype is not torch.int32 or topk_idx.device != dev or len(shape) not in (3, 4) \
+                or shape[:-1] not in ((batch, hk, 1), (batch, hk)):
             raise ValueError(f"{what}: topk_idx must be ({batch}, {hk}, 1, topk) int32 on {dev}")
-        topk_idx, topk = topk_idx.contiguous(), topk_idx.shape[-1]
+        topk_idx, topk = topk_idx.contiguous(), shape[-1]
         idx_ptr = topk_idx.data_ptr()
         if topk > _LIST or topk == 0:                    # (shorter lists are walked as they are; one of no entries has no address)
             block_mask = (torch.zeros if topk == 0 else torch.empty)(batch, hk, 1, words, dtype=torch.int64, device=dev)
