@@ -1,5 +1,5 @@
-// Warp-level tile helpers shared by the decode-time kernels (one query token per sequence: the
-// 16 query heads of a KV head are exactly one mma.sync M tile, far too small for tcgen05):
+// Warp-level tile helpers shared by the decode-time kernels (one query token per sequence: the 16 query heads of a KV
+// head are exactly one mma.sync M tile, an eighth of a tcgen05 one; the keys as M and the heads as N were not tried):
 // cp.async tiles of 32 keys x 128 features in swizzled shared memory, ldmatrix fragments,
 // mma.sync m16n8k16 bf16 -> fp32.
 #pragma once

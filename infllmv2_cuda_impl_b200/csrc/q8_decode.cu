@@ -189,17 +189,18 @@ __device__ __forceinline__ int blocks_of(const Q8DecodeParams& p, int b) {
 __device__ __forceinline__ uint32_t extent(int blocks) { return blocks ? kStart + blocks : 0; }
 
 // The blocks of all sequences and heads are one row, sequence by sequence, head by head, and CTA c of `ctas` takes those
-// from c total / ctas on: every CTA reads the same number of bytes whatever the lengths are (in equal splits, 16 sequences
-// of 1000 .. 32000 tokens wait for the longest one).  One wave of CTAs: with 1.5, 2 and 3 times as many, 64 sequences of
-// 4000 tokens take 42, 46 and 52 us instead of 32.  Every warp finds its place by itself, a sequence per lane.
+// from c total / ctas on: shares of equal cost, blocks and starts of heads, whatever the lengths are (in equal splits, 16
+// sequences of 1000 .. 32000 tokens wait for the longest one).  One wave of CTAs: with 1.5, 2 and 3 times as many, 64
+// sequences of 4000 tokens take 42, 46 and 52 us instead of 32.  Every warp finds its place by itself, a sequence per lane.
 //
 // Where a CTA goes from one head to the next it starts over (query, first tiles, join), for about as long as it takes for
-// kStart blocks, so a head's place in the row begins with as many that are no work.  Without / with them: 16 sequences of
+// kStart blocks, so a head's place in the row begins with as many that are no work: CTAs whose shares hold more starts
+// read fewer bytes.  Without / with them: 16 sequences of
 // 1000 .. 32000 tokens 38.2 / 35.3 us, 12 of up to 30000 with 8 KV heads 107 / 98.8, 256 of 100 .. 1000 41.6 / 34.9; 3
 // or 5 in place of 4 made no difference beyond 1 %.
 //
-// Under a selection a head's place is as long as its list can be, and the CTAs that share it share the selected blocks in
-// proportion, so that the deal need not wait for their number.
+// Under a selection a head's place is as long as its list can be (a mask: as kUsualBlocks, whatever it selects), and the
+// CTAs that share it share the selected blocks in proportion, so that the deal need not wait for their number.
 struct Deal {
   uint32_t total, ctas, each, rest;                // total = each * ctas + rest
   // extents: of all sequences, for one KV head (the host keeps the total below 2^31)
