@@ -87,9 +87,9 @@ def test_forward_mode_turns_the_tangents(launches, with_k, q_dual):
     q, k, cos, sin, wide = _inputs()
     pos, sections = wide[:, 20:26], (20, 20, 24)
     tq, tk = torch.randn(q.shape).to(BF), torch.randn(k.shape).to(BF)
-    for grad in (False, True):
-        x, y = q.clone().requires_grad_(grad), k.clone().requires_grad_(grad)
-        with forward_ad.dual_level():
+    for grad in (None, False, True):                      # (None: without gradient mode, which forward mode does not ask)
+        x, y = q.clone().requires_grad_(bool(grad)), k.clone().requires_grad_(bool(grad))
+        with forward_ad.dual_level(), torch.set_grad_enabled(grad is not None):
             a = forward_ad.make_dual(x, tq) if q_dual else x
             b = None if with_k is None else forward_ad.make_dual(y, tk) if with_k == "dual" else y
             out = infllm_v2.rotary_axes(a, b, cos, sin, pos, sections=sections)
@@ -135,7 +135,8 @@ def test_function_transforms_lose_no_derivative(launches):
     """torch.func.jvp and vjp want more of an autograd.Function than this one has, and say so."""
     q, _, cos, sin, wide = _inputs()
     f = lambda x: _rotated(x, cos, sin, wide[:, 20:26], (20, 20, 24))
-    for call in (lambda: torch.func.jvp(f, (q,), (q,)), lambda: torch.func.vjp(f, q)):
+    for call in (lambda: torch.func.jvp(f, (q,), (q,)), lambda: torch.func.vjp(f, q),
+                 lambda: torch.func.grad(lambda x: f(x).float().sum())(q)):
         with pytest.raises(RuntimeError, match="setup_context"):
             call()
 
