@@ -528,6 +528,52 @@ int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void* k_scale, v
                    int64_t slots, int64_t length, int code, int batch, int heads_q, int heads_k, int head_dim,
                    float softmax_scale, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------- pages ------------------- */
+/* Tables and slots of a step over paged caches, and a cache in 8 bits with block scales.  No counterpart in the
+ * reference, whose callers bring tables and slots.
+ *
+ * ifv2_pages_resize: requests of seqlens[b] tokens become targets[b] long (both (batch) int32).  free_pages
+ * (num_pages) is a ring of page numbers, free_range = (place of the first free one, their number).  New pages are taken
+ * from its front in the order of the requests and written into block_table (batch rows of table_stride, `width` used);
+ * pages of shortened requests go behind its end.  Requests that need more than `width` pages, or more than are left
+ * for them and those before them, are refused: length kept, slots -1.  Written: seqlens_out (batch), free_range_out
+ * (2), cu_seqlens (batch + 1), positions (total) and slots (total, page * page_size + place, -1 in rows behind the last
+ * new token); none overlaps an input.  batch <= 16384, width * page_size and total below 2^31.
+ *
+ * ifv2_cache_write: rows k, v (total, heads_k, 128) bf16 with the given strides (elements, multiples of 8) to rows
+ * slots[t] of k_cache, v_cache (num_pages, page_size, heads_k, 128); slots that the cache does not have are skipped.
+ *
+ * The cache in 8 bits: codes (num_pages, heads_k, page_size, 128), code 0 e4m3, 1 e5m2, and a scale byte (e8m0, 255
+ * NaN) per 64 tokens and head, (num_pages, heads_k, page_size / 64).
+ * ifv2_b8_write: rows like ifv2_cache_write's (strides multiples of 4) quantised to their slots.  The rows of one
+ * block are consecutive tokens at consecutive slots; rows that begin a block set its scale, others may raise it, and
+ * the block's earlier codes are then rounded to the new scale.
+ * ifv2_b8_attn: q, out (total_q, heads_q, 128) bf16 of sequences cu_seqlens_q (batch + 1), none of more than
+ * max_seqlen_q tokens, over cache_seqlens[b] keys each; causal: aligned to the last one.  block_table (batch,
+ * block_table_stride) or null (sequence b is page b).  mask (heads_k, total_q, mask_words) or null: 64-key blocks that a
+ * token attends.  lse (total_q, heads_q) fp32 or null.  Tokens without keys and rows behind the last sequence get 0, lse
+ * +inf; tokens that see a NaN block or a page that the cache does not have get NaN.  Caches begin at a multiple of 16
+ * bytes. */
+int ifv2_pages_resize(const int32_t* seqlens, const int32_t* targets, int32_t* block_table, int64_t table_stride,
+                      int width, int32_t* free_pages, int num_pages, const int32_t* free_range,
+                      int32_t* seqlens_out, int32_t* free_range_out, int32_t* cu_seqlens, int32_t* positions,
+                      int64_t* slots, int batch, int page_size, int64_t total, void* stream);
+int ifv2_cache_write(const void* k, const void* v, int64_t k_token_stride, int64_t k_head_stride,
+                     int64_t v_token_stride, int64_t v_head_stride, void* k_cache, void* v_cache,
+                     const int64_t* slots, int64_t num_pages, int page_size, int64_t total, int heads_k,
+                     int head_dim, void* stream);
+int ifv2_b8_write(const void* k, const void* v, int64_t k_token_stride, int64_t k_head_stride,
+                  int64_t v_token_stride, int64_t v_head_stride, void* k_cache, void* v_cache, void* k_scale,
+                  void* v_scale, const int64_t* slots, int64_t num_pages, int page_size, int code, int64_t total,
+                  int heads_k, int head_dim, void* stream);
+int64_t ifv2_b8_attn_workspace_bytes(int64_t total_q, int batch, int heads_q, int head_dim, int max_seqlen_q);
+int ifv2_b8_attn(const void* q, const void* k_cache, const void* v_cache, const void* k_scale, const void* v_scale,
+                 void* out, float* lse, const int32_t* cu_seqlens_q, const int32_t* cache_seqlens,
+                 const int32_t* block_table, int block_table_stride, const int64_t* mask, int mask_words, int batch,
+                 int64_t total_q, int max_seqlen_q, int64_t num_pages, int64_t length, int code, int heads_q,
+                 int heads_k, int head_dim, float softmax_scale, int causal, void* workspace,
+                 int64_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------- self-tests -------------- */
 /* Test infrastructure shipped in the library so that a deployment can check the tensor-core
  * building blocks on its own GPU; not part of the attention path.  No counterpart in the

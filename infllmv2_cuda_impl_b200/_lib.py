@@ -95,12 +95,18 @@ SIGNATURES = {
     "ifv2_q8_append": [c_void_p] * 12 + [c_int, c_int] + [c_int64] * 4 + [c_int] * 6 + [c_void_p],
     "ifv2_q8_decode": [c_void_p] * 10 + [c_int64, c_char_p, c_int, c_int, c_int64, c_int, c_void_p, c_int, c_void_p, c_int] +
                       [c_void_p] * 5 + [c_int, c_int64, c_int64] + [c_int] * 5 + [c_float, c_void_p, c_int64, c_void_p],
+    "ifv2_pages_resize": [c_void_p] * 3 + [c_int64, c_int, c_void_p, c_int] + [c_void_p] * 6 + [c_int, c_int, c_int64, c_void_p],
+    "ifv2_cache_write": [c_void_p] * 2 + [c_int64] * 4 + [c_void_p] * 3 + [c_int64, c_int, c_int64, c_int, c_int, c_void_p],
+    "ifv2_b8_write": [c_void_p] * 2 + [c_int64] * 4 + [c_void_p] * 5 + [c_int64, c_int, c_int, c_int64, c_int, c_int, c_void_p],
+    "ifv2_b8_attn": [c_void_p] * 10 + [c_int, c_void_p, c_int, c_int, c_int64, c_int, c_int64, c_int64] + [c_int] * 4 +
+                    [c_float, c_int, c_void_p, c_int64, c_void_p],
 }
 _INT64_RETURNS = {
     "ifv2_sparse_attn_bwd_workspace_bytes": [c_int64, c_int, c_int],
     "ifv2_decode_workspace_bytes": [c_int, c_int, c_int, c_int],
     "ifv2_stage1_decode_workspace_bytes": [c_int, c_int, c_int],
     "ifv2_q8_decode_workspace_bytes": [c_int, c_int, c_int],
+    "ifv2_b8_attn_workspace_bytes": [c_int64, c_int, c_int, c_int, c_int],
 }
 
 
