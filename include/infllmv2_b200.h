@@ -580,7 +580,8 @@ int ifv2_b8_attn(const void* q, const void* k_cache, const void* v_cache, const 
  * reference.
  * ifv2_selftest_umma: one tile product through TMA + tcgen05 in the operand arrangement `mode`
  *   (0: Q.K^T shape, 1/2: P.V with P in shared memory / TMEM, 3: MN-major x MN-major,
- *   4/5: thread-written K-major tiles without / with the 32-byte swizzle); d receives fp32.
+ *   4/5: thread-written K-major tiles without / with the 32-byte swizzle, 6/7: 8-bit codes, K-major /
+ *   MN-major); d receives fp32.
  * ifv2_selftest_wait_timeout: makes a bounded wait run out on purpose, safely: a kernel waits at
  *   most limit_cycles (<= 2^24) SM clocks on a barrier that nothing arms, stores `site` in the
  *   status block, frees its tensor memory and returns; result: int32[3] = {abort flag seen by

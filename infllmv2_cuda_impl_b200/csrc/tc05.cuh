@@ -479,6 +479,33 @@ __device__ __forceinline__ void umma_commit_pred(uint64_t* bar, uint32_t leader)
       : "memory");
 }
 
+// ---- 8-bit operands (kind::f8f6f4, fp32 accumulators): K = 32 per MMA, a code is one byte.
+// A and B have a type each (0 = e4m3, 1 = e5m2); the fields stand where kind::f16 has its own.
+__host__ __device__ constexpr uint32_t umma_idesc_f8(int m, int n, int a_type, int b_type, bool a_mn_major, bool b_mn_major) {
+  return (1u << 4) | ((uint32_t)a_type << 7) | ((uint32_t)b_type << 10) | ((a_mn_major ? 1u : 0u) << 15) |
+         ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+// A K-major tile (rows of 128 codes, 128-byte swizzle) and an MN-major one (128 values of M or N per row, a row per K
+// index) have the descriptor of the 16-bit forms: both are laid out in bytes.  An MMA takes 32 bytes of each K-major row,
+// or 32 rows (4096 bytes) of an MN-major one.
+// MN-major without swizzle, written by threads: the 16 values of a group of 16 columns at one K index are 16 bytes, K
+// indices follow one another, and the groups are `group_bytes` apart.
+__device__ __forceinline__ uint64_t umma_desc_noswz_mn8(uint32_t smem_addr, uint32_t group_bytes) {
+  uint64_t d = 0;
+  d |= (uint64_t)((smem_addr >> 4) & 0x3FFFu);
+  d |= (uint64_t)(128u >> 4) << 16;                 // from 8 K indices to the next 8
+  d |= (uint64_t)(group_bytes >> 4) << 32;
+  d |= 1ull << 46;
+  return d;
+}
+__device__ __forceinline__ void umma_f8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
+
 // The mbarrier gets one arrival when every MMA issued so far by this thread has completed.
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(

@@ -15,6 +15,7 @@ struct SelfTestParams {
   float* d;                 // (128, n) fp32
   int mode;
   int32_t* status;
+  const uint8_t *a8, *b8;   // modes 6, 7: bytes of 8-bit codes
 };
 
 // mode 0: D(128x64)  = A(128x128, K-major) * B(64x128, K-major)^T      [the Q.K^T shape]
@@ -24,6 +25,8 @@ struct SelfTestParams {
 // mode 5: as mode 4 with the 32-byte swizzle
 // mode 4: D(128x64)  = A(128x16) * B(64x16)^T, both K-major WITHOUT swizzle, written by threads
 //                                                                        [the row-constant K step of stage 1]
+// mode 6: D(128x32)  = A(128x128) * B(32x128)^T, e4m3 codes, K-major with the 128-byte swizzle      [codes of keys * query]
+// mode 7: D(128x32)  = At(128x128, MN-major, e4m3)^T * Bt(128x32, MN-major without swizzle, e5m2)   [codes of values * weights]
 __global__ void __launch_bounds__(128)
 umma_selftest_kernel(const __grid_constant__ CUtensorMap map_a,
                      const __grid_constant__ CUtensorMap map_b, const SelfTestParams p) {
@@ -54,7 +57,7 @@ umma_selftest_kernel(const __grid_constant__ CUtensorMap map_a,
   const uint32_t tmem_d = tmem, tmem_a = tmem + 128;
   const int mode = p.mode;
   const bool sw32 = p.mode == 5;               // mode 5 = mode 4 with the 32-byte swizzle
-  const int n = (mode == 0 || mode == 3 || mode == 4 || mode == 5) ? 64 : 128;
+  const int n = mode >= 6 ? 32 : (mode == 0 || mode == 3 || mode == 4 || mode == 5) ? 64 : 128;
   if (sw32) {
     for (int i = threadIdx.x; i < 128 * 16; i += 128)
       *reinterpret_cast<__nv_bfloat16*>(sA + umma_sw32_off(i >> 4, i & 15)) = p.a[i];
@@ -67,6 +70,16 @@ umma_selftest_kernel(const __grid_constant__ CUtensorMap map_a,
       *reinterpret_cast<__nv_bfloat16*>(sA + umma_noswz16_off(i >> 4, i & 15)) = p.a[i];
     for (int i = threadIdx.x; i < 64 * 16; i += 128)
       *reinterpret_cast<__nv_bfloat16*>(sB + umma_noswz16_off(i >> 4, i & 15)) = p.b[i];
+    fence_proxy_async_smem();
+  }
+
+  if (mode == 6) {
+    for (int i = threadIdx.x; i < 32 * 128; i += 128)
+      sB[(i >> 7) * 128 + ((((i >> 4) & 7) ^ ((i >> 7) & 7)) << 4) + (i & 15)] = p.b8[i];
+    fence_proxy_async_smem();
+  }
+  if (mode == 7) {
+    for (int i = threadIdx.x; i < 128 * 32; i += 128) sB[((i >> 4) & 1) * 2048 + (i >> 5) * 16 + (i & 15)] = p.b8[i];
     fence_proxy_async_smem();
   }
 
@@ -85,6 +98,9 @@ umma_selftest_kernel(const __grid_constant__ CUtensorMap map_a,
     tc_fence_after();
     if (mode == 4 || mode == 5) {
       mbar_arrive(&bar_load);                                 // nothing to fetch
+    } else if (mode >= 6) {
+      mbar_expect_tx(&bar_load, 16384);
+      tma_load_2d(sA, &map_a, &bar_load, 0, 0);
     } else if (mode == 0) {
       mbar_expect_tx(&bar_load, 2 * 16384 + 2 * 8192);
       tma_load_3d(sA, &map_a, &bar_load, 0, 0, 0);
@@ -108,7 +124,18 @@ umma_selftest_kernel(const __grid_constant__ CUtensorMap map_a,
     }
     if (mbar_wait(&bar_load, 0, &abort_flag, p.status, 1)) {
       tc_fence_after();
-      if (mode == 5) {
+      if (mode >= 6) {
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          const uint32_t a = smem_u32(sA), b = smem_u32(sB);
+          if (mode == 6)
+            umma_f8_ss(tmem_d, umma_desc_sw128(a + kk * 32, 16, 1024), umma_desc_sw128(b + kk * 32, 16, 1024),
+                       umma_idesc_f8(128, 32, 0, 0, false, false), kk > 0);
+          else
+            umma_f8_ss(tmem_d, umma_desc_sw128(a + kk * 4096, 16, 1024), umma_desc_noswz_mn8(b + kk * 512, 2048),
+                       umma_idesc_f8(128, 32, 0, 1, true, true), kk > 0);
+        }
+      } else if (mode == 5) {
         umma_ss(tmem_d, umma_desc_sw32(smem_u32(sA)), umma_desc_sw32(smem_u32(sB)),
                 umma_idesc_bf16(128, 64, false), false);
       } else if (mode == 4) {
@@ -219,9 +246,11 @@ extern "C" int ifv2_selftest_wait_timeout(int32_t* status, int64_t limit_cycles,
 //   mode 0: a (128,128), b (64,128)  -> d (128,64);  modes 1, 2: a (128,64), b (64,128) -> d (128,128)
 //   mode 3: a (128,128) = At, b (128,64) = Bt -> d = At^T . Bt (128,64)
 //   mode 4: a (128,16), b (64,16) -> d = a . b^T (128,64)
+//   mode 6: a (128,128), b (32,128) e4m3 codes -> d = a . b^T (128,32)
+//   mode 7: a (128,128) = At e4m3, b (128,32) = Bt e5m2 -> d = At^T . Bt (128,32)
 extern "C" int ifv2_selftest_umma(int mode, const void* a, const void* b, float* d, int32_t* status,
                                   void* stream) {
-  IFV2_REQUIRE(mode >= 0 && mode <= 5, IFV2_ERR_INVALID_ARG, "selftest: mode must be 0..5");
+  IFV2_REQUIRE(mode >= 0 && mode <= 7, IFV2_ERR_INVALID_ARG, "selftest: mode must be 0..7");
   IFV2_REQUIRE(a && b && d && status, IFV2_ERR_INVALID_ARG, "selftest: null pointer");
   CUtensorMap map_a, map_b;
   int rc;
@@ -229,6 +258,10 @@ extern "C" int ifv2_selftest_umma(int mode, const void* a, const void* b, float*
     rc = make_tensor_map_bf16_3d(&map_a, a, 128, 128, 1, 256, 256 * 128, 64, 128, 1);
     if (rc) return rc;
     rc = make_tensor_map_bf16_3d(&map_b, b, 128, 64, 1, 256, 256 * 64, 64, 64, 1);
+  } else if (mode >= 6) {
+    rc = make_tensor_map_rows128(&map_a, a, 128, 128);
+    if (rc) return rc;
+    map_b = map_a;                           // (B is written by threads)
   } else if (mode == 4 || mode == 5) {       // operands are written by threads; the maps are not used
     rc = make_tensor_map_bf16_3d(&map_a, d, 64, 128, 1, 128, 128 * 128, 64, 128, 1);
     if (rc) return rc;
@@ -247,7 +280,7 @@ extern "C" int ifv2_selftest_umma(int mode, const void* a, const void* b, float*
                                           cudaFuncAttributeMaxDynamicSharedMemorySize, 50 * 1024);
   if (attr != cudaSuccess) return set_error((int)attr, "selftest: %s", cudaGetErrorString(attr));
   SelfTestParams p{static_cast<const __nv_bfloat16*>(a), static_cast<const __nv_bfloat16*>(b), d, mode,
-                   status};
+                   status, static_cast<const uint8_t*>(a), static_cast<const uint8_t*>(b)};
   umma_selftest_kernel<<<1, 128, 50 * 1024, (cudaStream_t)stream>>>(map_a, map_b, p);
   return check_launch("umma_selftest");
 }
