@@ -550,8 +550,9 @@ int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void* k_scale, v
  * the block's earlier codes are then rounded to the new scale.
  * ifv2_b8_attn: q, out (total_q, heads_q, 128) bf16 of sequences cu_seqlens_q (batch + 1), none of more than
  * max_seqlen_q tokens, over cache_seqlens[b] keys each; causal: aligned to the last one.  block_table (batch,
- * block_table_stride) or null (sequence b is page b).  mask (heads_k, total_q, mask_words) or null: 64-key blocks that a
- * token attends.  lse (total_q, heads_q) fp32 or null.  Tokens without keys and rows behind the last sequence get 0, lse
+ * block_table_stride) or null (sequence b is page b).  64-key blocks that a token attends: topk_idx (heads_k, total_q,
+ * topk), entries below 0 unused, or mask (heads_k, total_q, mask_words), a word per 64 blocks of a sequence's capacity, at
+ * most 524288 keys; both null: all.  lse (total_q, heads_q) fp32 or null.  Tokens without keys and rows behind the last sequence get 0, lse
  * +inf; tokens that see a NaN block or a page that the cache does not have get NaN.  Caches begin at a multiple of 16
  * bytes. */
 int ifv2_pages_resize(const int32_t* seqlens, const int32_t* targets, int32_t* block_table, int64_t table_stride,
@@ -569,10 +570,10 @@ int ifv2_b8_write(const void* k, const void* v, int64_t k_token_stride, int64_t 
 int64_t ifv2_b8_attn_workspace_bytes(int64_t total_q, int batch, int heads_q, int head_dim, int max_seqlen_q);
 int ifv2_b8_attn(const void* q, const void* k_cache, const void* v_cache, const void* k_scale, const void* v_scale,
                  void* out, float* lse, const int32_t* cu_seqlens_q, const int32_t* cache_seqlens,
-                 const int32_t* block_table, int block_table_stride, const int64_t* mask, int mask_words, int batch,
-                 int64_t total_q, int max_seqlen_q, int64_t num_pages, int64_t length, int code, int heads_q,
-                 int heads_k, int head_dim, float softmax_scale, int causal, void* workspace,
-                 int64_t workspace_bytes, void* stream);
+                 const int32_t* block_table, int block_table_stride, const int32_t* topk_idx, int topk,
+                 const int64_t* mask, int mask_words, int batch, int64_t total_q, int max_seqlen_q,
+                 int64_t num_pages, int64_t length, int code, int heads_q, int heads_k, int head_dim,
+                 float softmax_scale, int causal, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------- self-tests -------------- */
 /* Test infrastructure shipped in the library so that a deployment can check the tensor-core

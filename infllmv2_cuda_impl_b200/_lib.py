@@ -98,7 +98,7 @@ SIGNATURES = {
     "ifv2_pages_resize": [c_void_p] * 3 + [c_int64, c_int, c_void_p, c_int] + [c_void_p] * 6 + [c_int, c_int, c_int64, c_void_p],
     "ifv2_cache_write": [c_void_p] * 2 + [c_int64] * 4 + [c_void_p] * 3 + [c_int64, c_int, c_int64, c_int, c_int, c_void_p],
     "ifv2_b8_write": [c_void_p] * 2 + [c_int64] * 4 + [c_void_p] * 5 + [c_int64, c_int, c_int, c_int64, c_int, c_int, c_void_p],
-    "ifv2_b8_attn": [c_void_p] * 10 + [c_int, c_void_p, c_int, c_int, c_int64, c_int, c_int64, c_int64] + [c_int] * 4 +
+    "ifv2_b8_attn": [c_void_p] * 10 + [c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int64, c_int, c_int64, c_int64] + [c_int] * 4 +
                     [c_float, c_int, c_void_p, c_int64, c_void_p],
 }
 _INT64_RETURNS = {

@@ -1,0 +1,469 @@
+// What the kernels of the attention over 8-bit blocks share: how a call is dealt to CTAs, the warp that looks blocks up
+// and fetches them, and the numbers that the softmax hands to the tensor cores.
+//
+//   x_tk = log2(e) scale 2^eK(k) q_t . K_k,   out_t = sum_k 2^x_tk 2^eV(k) V_k / sum_k 2^x_tk
+//
+// over the keys that token t sees.  The codes go to the tensor cores as they lie in memory (kind::f8f6f4): the
+// other operand of each product is split into 8-bit numbers instead.
+//   * A query row, scaled by a power of two to a largest magnitude of 224..448, is the sum of two e4m3 numbers, to
+//     2^-10, that is 2^-18 of its largest element: for bf16 rows exact down to elements 2^-10 of the largest.
+//   * A weight is the sum of three e5m2 numbers, to 2^-9 of it (half a bf16 step).  e5m2 is the upper byte of an fp16
+//     number: a term is a byte, what it leaves over one subtraction.  Weights are 2^(x + eV - M) with M about 2^-10 of the
+//     largest so far, at most 2^15, and below 2^-16 they have the type's fixed spacing of 2^-16: 2^-27 of the largest.
+//     The values' exponents take part in M, so that contributions keep their size against one another whatever
+//     the sizes of the blocks' values are.  The sum of the softmax is held in units of 2^(M - E), E the largest eV so far.
+//
+// A tile is up to kT tokens of a sequence x the 16 query heads of a KV head.  A CTA takes an even share of the call's
+// cost, units of 128 keys plus kStart per tile, whatever the lengths are; pieces of a tile that shares cut go to a workspace
+// and are joined by a second kernel.  Where a sequence has one tile per head (a decode step, drafts) every CTA finds
+// its share by itself, from the lengths; otherwise a kernel in front lists the tiles.
+#pragma once
+#include "b8.cuh"
+
+namespace ifv2 {
+namespace b8 {
+
+using namespace tc;
+
+constexpr int kUnit = 2 * kBlockN;               // keys of a step: two blocks
+constexpr int kTileBytes = kUnit * kHeadDim;
+constexpr int kStart = 2;                        // units that the start of a tile costs
+constexpr int kMaxMaskWords = 128;               // 524288 keys
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kUnset = -1e30f;                 // reference of a row that has seen no key
+constexpr float kTop = 10.f, kRoom = 15.f;       // a new reference puts the largest weight at 2^kTop; past 2^kRoom it moves
+constexpr int kDeepest = -90;                    // eV - E that the sum's range has room for
+constexpr int kNoScale = -10000;                 // eV of no block
+
+struct AttnParams {
+  const __nv_bfloat16* q;
+  const uint8_t *k_scale, *v_scale;
+  __nv_bfloat16* out;
+  float* lse;
+  const int32_t *cu_q, *seqlens, *block_table;
+  const unsigned long long* mask;                // (heads_k, total_q, words) or null
+  const int32_t* lists;                          // (heads_k, total_q, topk) in place of a mask, or null
+  int bt_stride, words, topk, batch, heads_k, length, causal;
+  int usual;                                     // blocks that a token is taken to select, where it selects
+  uint32_t page_mul;                             // a block's page: umulhi(2 block, page_mul) >> page_shift
+  int page_shift;
+  int64_t total_q, capacity;
+  int pages;
+  float scale_log2;
+  int least_share;
+  // workspace
+  int4* join;                                    // per CTA: the cut tile that its share begins inside (see Item)
+  float *part_o, *part_lse;                      // two pieces per CTA: (2 grid, 16 kT, 128), (2 grid, 16 kT)
+  int most_chunks;                               // listed tiles of a head that the workspace has room for
+  int32_t* first_chunk;                          // (batch + 1) chunks of kT tokens before each sequence
+  int32_t* first_tile;                           // tile that a CTA begins with; behind these the number of tiles
+  int4* tiles;                                   // sequence, row of the first token, keys of the last one, tokens << 16 | head
+  int64_t* start;                                // (tiles + 1) cost before each tile
+};
+
+// Shares of a cost: CTA g has [begin(g), begin(g + 1)).
+struct Shares {
+  int64_t each, rest;
+  int grid;
+  __device__ __forceinline__ Shares(int64_t cost, int most, int least) {
+    if (cost >> 31 == 0) {                         // (a 64-bit division takes some hundred clocks)
+      const uint32_t c = (uint32_t)cost;
+      grid = (int)min(max(c / (uint32_t)least, 1u), (uint32_t)most);
+      each = c / (uint32_t)grid;
+      rest = c - (uint32_t)each * (uint32_t)grid;
+    } else {
+      grid = most;
+      each = cost / grid;
+      rest = cost - each * grid;
+    }
+  }
+  __device__ __forceinline__ int64_t begin(int g) const { return each * g + min((int64_t)g, rest); }
+};
+
+// Tokens of sequence b (cu_q is clamped to the rows there are).
+__device__ __forceinline__ int tokens_of(const AttnParams& p, int b, int& row0) {
+  row0 = (int)min(max((int64_t)p.cu_q[b], (int64_t)0), p.total_q);
+  return max((int)min((int64_t)p.cu_q[b + 1], p.total_q) - row0, 0);
+}
+__device__ __forceinline__ int keys_of(const AttnParams& p, int b) {
+  return (int)min((int64_t)max(p.seqlens[b], 0), p.capacity);
+}
+
+// Word w of the union of the masks of `tokens` rows; bits from block `blocks` on are not there.
+__device__ __forceinline__ unsigned long long below(unsigned long long word, int w, int blocks) {
+  const int left = blocks - w * 64;
+  return left >= 64 ? word : left <= 0 ? 0ull : word & ((1ull << left) - 1);
+}
+__device__ __forceinline__ unsigned long long union_word(const AttnParams& p, int head, int64_t row, int tokens, int w, int blocks) {
+  if (w * 64 >= blocks) return 0;
+  const unsigned long long* m = p.mask + ((int64_t)head * p.total_q + row) * p.words + w;
+  unsigned long long u = 0;
+  for (int t = 0; t < tokens; ++t) u |= __ldg(m + (int64_t)t * p.words);
+  return below(u, w, blocks);
+}
+
+// ------------------------------------------------------------------------ inside a CTA --
+// A block on its way through the CTA: written by the fetching warp, read by the softmax.
+struct __align__(16) Block {
+  float k_scale;                                   // 2^eK, or NaN
+  int e_v;                                         // eV, kNanByte: NaN block
+  int valid;                                       // keys (0: the block only fills a unit)
+  int pos;                                         // position of its first key
+  uint32_t tokens;                                 // tokens that attend it
+  uint32_t pad[3];
+};
+// A CTA's part of a tile.
+struct __align__(16) Item {
+  int row, head, tokens, reach;                    // first token, KV head, tokens, keys that the last one sees
+  int units;                                       // -1: no more items
+  int piece;                                       // -1: the whole tile, else the place of a partial result
+};
+
+__device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
+  if (mbar_try_wait(bar, parity)) return true;
+  if (*gave_up) return false;
+  return mbar_wait(bar, parity, gave_up, nullptr, 0);
+}
+// All lanes of a warp (the TMEM instructions behind it want them together).
+__device__ __forceinline__ bool bounded_wait_warp(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
+  return __all_sync(0xFFFFFFFFu, bounded_wait(bar, parity, gave_up));
+}
+
+template <int kThreads>
+__device__ __forceinline__ void named_sync() { asm volatile("barrier.cta.sync 1, %0;" ::"n"(kThreads) : "memory"); }
+template <int kThreads>
+__device__ __forceinline__ bool named_any(bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r) : "r"((uint32_t)x), "n"(kThreads) : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 2^e for any e (0 and inf outside the range)
+__device__ __forceinline__ float pow2i(int e) { return e < -126 ? 0.f : e > 127 ? INFINITY : __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// Four weights to their three terms, a byte each.  The first two are cut off, the last is rounded.
+__device__ __forceinline__ void split4(float a, float b, float c, float d, uint32_t& t0, uint32_t& t1, uint32_t& t2) {
+  uint32_t lo, hi;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(b), "f"(a));
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(d), "f"(c));
+  t0 = __byte_perm(lo, hi, 0x7531);
+  asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(lo) : "r"(lo & 0xFF00FF00u));
+  asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(hi) : "r"(hi & 0xFF00FF00u));
+  t1 = __byte_perm(lo, hi, 0x7531);
+  asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(lo) : "r"(lo & 0xFF00FF00u));
+  asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(hi) : "r"(hi & 0xFF00FF00u));
+  t2 = __byte_perm(lo + 0x00800080u, hi + 0x00800080u, 0x7531);
+}
+
+// 16 values of a query row, one of 8 neighbouring lanes' parts, to their two terms at `at` and `at + second` (128-byte-
+// swizzled rows); returns the factor that scores of the row get.
+__device__ __forceinline__ float write_query16(const uint4 (&x)[2], uint8_t* at, int second_at, float scale_log2) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(x);
+  uint32_t m2 = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) m2 = __vmaxu2(m2, w[j] & 0x7FFF7FFFu);
+  uint32_t amax = max(m2 & 0xFFFFu, m2 >> 16);
+#pragma unroll
+  for (int d = 1; d < 8; d <<= 1) amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, d));
+  const int byte = amax ? scale_byte<kE4m3>(amax << 16) : 127;
+  // (a negative scale turns the query round, so that larger products are larger scores)
+  const float inv = byte == kNanByte ? 0.f : scale_log2 < 0.f ? -q8::inverse_scale(byte) : q8::inverse_scale(byte);
+  uint32_t first[4], second[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float y[4] = {__uint_as_float(w[2 * j] << 16), __uint_as_float(w[2 * j] & 0xFFFF0000u),
+                  __uint_as_float(w[2 * j + 1] << 16), __uint_as_float(w[2 * j + 1] & 0xFFFF0000u)}, near[4];
+    if (byte == kNanByte) y[0] = y[1] = y[2] = y[3] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = q8::mul_exact(y[e], inv);
+    first[j] = encode4<kE4m3>(y, 1.f);
+    decode4<kE4m3>(near, first[j]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] -= near[e];
+    second[j] = encode4<kE4m3>(y, 1.f);
+  }
+  *reinterpret_cast<uint4*>(at) = make_uint4(first[0], first[1], first[2], first[3]);
+  *reinterpret_cast<uint4*>(at + second_at) = make_uint4(second[0], second[1], second[2], second[3]);
+  return fabsf(scale_log2) * q8::scale_value(byte);
+}
+
+// Barriers and records that the roles share.
+template <int kT, int kStages>
+struct Common {
+  uint64_t full[kStages], empty[kStages];          // K and V of a unit
+  uint64_t item_full[2], item_empty[2];
+  Block block[kStages][2];
+  Item item[2];
+  unsigned long long words[kT][kMaxMaskWords];     // block lists of the tile's tokens as masks
+  uint32_t tmem;
+  int gave_up;
+};
+
+// ---------------------------------------------------------------------- fetching warp --
+// All lanes run it.  kListed: tiles come from the kernel in front.
+template <int kT, int kStages, bool kListed>
+__device__ __forceinline__ void fetch(const AttnParams& p, const CUtensorMap* k_map, const CUtensorMap* v_map, Common<kT, kStages>& s,
+                                      uint8_t* ring) {
+  const int lane = threadIdx.x & 31;
+  volatile int* gave_up = &s.gave_up;
+  const bool selected = p.mask != nullptr || p.lists != nullptr;
+  int b = 0, head = 0, row = 0, tokens = 0, reach = 0, tile = 0, n_tiles = 0;
+  int64_t cost = 0, begin = 0, end = 0;            // of the call; of the tile
+  // cost of a head of sequence b, not listed
+  const auto cost_of = [&](int b, int& row, int& tokens, int& reach) {
+    tokens = min(tokens_of(p, b, row), kT);
+    if (tokens == 0) return 0;
+    reach = keys_of(p, b);
+    int n = ceil_div(reach, kUnit);
+    if (selected) n = min(n, ceil_div(p.usual * (3 + tokens), 8));
+    return kStart + n;
+  };
+  if (kListed) {
+    n_tiles = p.first_tile[gridDim.x];
+    cost = p.start[n_tiles];
+  } else {
+    for (int base = 0; base < p.batch; base += 32) {
+      int r, t, k;
+      if (base + lane < p.batch) cost += cost_of(base + lane, r, t, k);
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) cost += __shfl_xor_sync(0xFFFFFFFFu, cost, d);
+    cost *= p.heads_k;
+  }
+  const Shares shares(max(cost, (int64_t)1), gridDim.x, p.least_share);
+  const int me = blockIdx.x;
+  const int64_t lo = me < shares.grid ? shares.begin(me) : cost, hi = me < shares.grid ? shares.begin(me + 1) : cost;
+  int each = 0;                                    // cost of the sequence's heads
+  bool more = lo < hi && cost > 0;
+  if (more) {
+    if (kListed) {
+      tile = p.first_tile[me];
+    } else {
+      for (int base = 0;; base += 32) {            // the sequence that lo lies in
+        int r = 0, t = 0, k = 0, c = 0;
+        if (base + lane < p.batch) c = cost_of(base + lane, r, t, k);
+        int64_t upto = (int64_t)c * p.heads_k;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const int64_t o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+          if (lane >= d) upto += o;
+        }
+        const uint32_t past = __ballot_sync(0xFFFFFFFFu, begin + upto > lo);
+        if (past) {
+          const int src = __ffs(past) - 1;
+          b = base + src;
+          row = __shfl_sync(0xFFFFFFFFu, r, src);
+          tokens = __shfl_sync(0xFFFFFFFFu, t, src);
+          reach = __shfl_sync(0xFFFFFFFFu, k, src);
+          each = __shfl_sync(0xFFFFFFFFu, c, src);
+          begin += __shfl_sync(0xFFFFFFFFu, upto, src) - (int64_t)each * p.heads_k;
+          head = (int)((uint32_t)min(lo - begin, (int64_t)0x7FFFFFFF) / (uint32_t)each);
+          begin += (int64_t)head * each;
+          break;
+        }
+        begin += __shfl_sync(0xFFFFFFFFu, upto, 31);
+      }
+    }
+  }
+  int4 cut = make_int4(0, 0, 0, 0);
+  int n = 0, items = 0;                            // units, items so far
+  for (bool first = true; more && !*gave_up; first = false) {
+    if (kListed) {
+      const int4 t = p.tiles[tile];
+      b = t.x, row = t.y, reach = t.z, tokens = t.w >> 16, head = t.w & 0xFFFF;
+      begin = p.start[tile], end = p.start[tile + 1];
+    } else {
+      end = begin + each;
+    }
+    // the part of the tile that lies in this share, in units of the estimate
+    const int64_t s0 = begin + kStart;
+    const int est = (int)(end - s0);
+    const int est_a = (int)min(max(lo - s0, (int64_t)0), (int64_t)est), est_z = (int)min(max(hi - s0, (int64_t)est_a), (int64_t)est);
+    const int blocks = ceil_div(reach, kBlockN);
+    // the tile's blocks: all, or those that its tokens select, 4 words of their union per lane
+    unsigned long long u[4] = {0, 0, 0, 0};
+    int upto = 0, total = blocks;
+    if (selected) {
+      if (p.lists) {
+        __syncwarp();
+        for (int i = lane; i < tokens * kMaxMaskWords; i += 32) s.words[i / kMaxMaskWords][i % kMaxMaskWords] = 0;
+        __syncwarp();
+        for (int t = 0; t < tokens; ++t) {
+          const int32_t* list = p.lists + ((int64_t)head * p.total_q + row + t) * p.topk;
+          for (int i = lane; i < p.topk; i += 32) {
+            const int block = __ldg(list + i);
+            if (block >= 0 && block < blocks)
+              atomicOr(reinterpret_cast<uint32_t*>(s.words[t]) + (block >> 5), 1u << (block & 31));
+          }
+        }
+        __syncwarp();
+      }
+      int count = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int w = 4 * lane + i;
+        if (p.lists)
+          for (int t = 0; t < tokens; ++t) u[i] |= s.words[t][w];
+        else if (w < p.words)
+          u[i] = union_word(p, head, row, tokens, w, blocks);
+        count += __popcll(u[i]);
+      }
+      upto = count;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+        if (lane >= d) upto += o;
+      }
+      total = __shfl_sync(0xFFFFFFFFu, upto, 31);
+    }
+    const int units = ceil_div(total, 2);
+    // (a tile's cost is an estimate where blocks are selected: parts are in proportion)
+    const int a = est == units ? est_a : est ? (int)((int64_t)est_a * units / est) : 0;
+    const int z = est == units ? est_z : est ? (int)((int64_t)est_z * units / est) : 0;
+    const bool whole = lo <= begin && hi >= end;
+    if (first && me > 0 && begin < lo && begin >= shares.begin(me - 1)) {
+      int last = me;
+      while (last + 1 < shares.grid && shares.begin(last + 1) < end) ++last;
+      cut = make_int4(row, tokens << 16 | head, last, 1);
+    }
+    {
+      const int slot = items & 1;
+      if (!bounded_wait_warp(&s.item_empty[slot], ((items >> 1) & 1) ^ 1, gave_up)) break;
+      if (lane == 0) {
+        s.item[slot] = Item{row, head, tokens, reach, z - a, whole ? -1 : 2 * me + (lo <= begin ? 1 : 0)};
+        mbar_arrive(&s.item_full[slot]);
+      }
+      ++items;
+    }
+    const auto nth_block = [&](int k) {            // all lanes, each with its k
+      if (!selected) return k;
+      int at = 0;                                  // lane whose words hold it: the first with upto > k
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1)
+        if (__shfl_sync(0xFFFFFFFFu, upto, (at + d - 1) & 31) <= k) at += d;
+      at &= 31;
+      const int before = __shfl_sync(0xFFFFFFFFu, upto, (at + 31) & 31);
+      int left = k - (at ? before : 0), block = 256 * at;
+      unsigned long long word = 0;
+      bool found = false;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const unsigned long long w = __shfl_sync(0xFFFFFFFFu, u[i], at);
+        const int c = __popcll(w);
+        if (!found) {
+          if (left < c) found = true, word = w;
+          else left -= c, block += 64;
+        }
+      }
+#pragma unroll
+      for (int d = 32; d > 0; d >>= 1) {           // its left-th bit
+        const int c = __popcll(word & ((1ull << d) - 1));
+        if (left >= c) left -= c, word >>= d, block += d;
+      }
+      return block;
+    };
+    // 32 blocks at a time, one per lane; the next ones' pages are looked up while these are fetched, their scales behind that
+    int block = 0, page = 0;
+    const auto look = [&](int k0) {
+      block = nth_block(min(k0 + lane, total - 1));
+      const int in_table = (int)(__umulhi(2u * (uint32_t)block, p.page_mul) >> p.page_shift);
+      page = p.block_table ? __ldg(p.block_table + (int64_t)b * p.bt_stride + in_table) : b;
+    };
+    int row_of, kb, vb;
+    const auto scales = [&]() {
+      const bool bad = page < 0 || page >= p.pages;
+      const int in_table = p.block_table ? (int)(__umulhi(2u * (uint32_t)block, p.page_mul) >> p.page_shift) : 0;
+      const int place = block * kBlockN - in_table * p.length;
+      const int r = (int)(((int64_t)(bad ? 0 : page) * p.heads_k + head) * p.length) + place;
+      row_of = r;
+      kb = bad ? kNanByte : __ldg(p.k_scale + r / kBlockN);
+      vb = bad ? kNanByte : __ldg(p.v_scale + r / kBlockN);
+    };
+    if (z > a) {
+      look(2 * a);
+      scales();
+    }
+    for (int k0 = 2 * a; k0 < 2 * z; k0 += 32) {
+      Block r;
+      r.pos = block * kBlockN;
+      r.valid = k0 + lane < total ? min(kBlockN, reach - r.pos) : 0;
+      r.k_scale = q8::scale_value(kb);
+      r.e_v = vb == kNanByte ? kNanByte : vb - 127;
+      r.tokens = (1u << tokens) - 1;
+      if (selected && kT > 1) {
+        r.tokens = 0;
+        const unsigned long long* m = p.mask + ((int64_t)head * p.total_q + row) * p.words + (block >> 6);
+        for (int i = 0; i < tokens; ++i) {
+          const unsigned long long w = p.lists ? s.words[i][block >> 6] : __ldg(m + (int64_t)i * p.words);
+          r.tokens |= (uint32_t)((w >> (block & 63)) & 1) << i;
+        }
+      }
+      const int now = row_of, many = min(32, 2 * (z - a) - (k0 - 2 * a));
+      const bool next = k0 + 32 < 2 * z;
+      if (next) look(k0 + 32);
+      for (int j = 0; j < many; j += 2, ++n) {
+        const int stage = n % kStages;
+        if (!bounded_wait_warp(&s.empty[stage], ((n / kStages) & 1) ^ 1, gave_up)) break;
+        if ((lane & ~1) == j) s.block[stage][lane & 1] = r;
+        const int row0 = __shfl_sync(0xFFFFFFFFu, now, j), row1 = __shfl_sync(0xFFFFFFFFu, now, j + 1);
+        __syncwarp();
+        if (lane == 0) {
+          uint8_t* to = ring + stage * 2 * kTileBytes;
+          mbar_expect_tx(&s.full[stage], 2 * kTileBytes);
+          tma_load_2d(to, k_map, &s.full[stage], 0, row0);
+          tma_load_2d(to + kTileBytes / 2, k_map, &s.full[stage], 0, row1);
+          tma_load_2d(to + kTileBytes, v_map, &s.full[stage], 0, row0);
+          tma_load_2d(to + kTileBytes + kTileBytes / 2, v_map, &s.full[stage], 0, row1);
+        }
+        if (next && j == 8) scales();
+      }
+      if (*gave_up) break;
+    }
+    // the next tile
+    if (end >= hi) break;
+    if (kListed) {
+      ++tile;
+      more = tile < n_tiles;
+    } else {
+      begin = end;
+      if (++head == p.heads_k) {
+        head = 0;
+        do ++b; while (b < p.batch && (each = cost_of(b, row, tokens, reach)) == 0);
+        more = b < p.batch;
+      }
+    }
+  }
+  if (lane == 0) p.join[me] = cut;
+  const int slot = items & 1;
+  if (bounded_wait_warp(&s.item_empty[slot], ((items >> 1) & 1) ^ 1, gave_up) && lane == 0) {
+    s.item[slot].units = -1;
+    mbar_arrive(&s.item_full[slot]);
+  }
+  __syncwarp();
+  if (*gave_up)                                    // copies that are under way land before the CTA ends
+    for (int i = max(n - kStages, 0); i < n; ++i) mbar_wait_drain(&s.full[i % kStages], (i / kStages) & 1);
+}
+
+// The kernels that the parts of the call are: each may start beside the one before it.
+__device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+}  // namespace b8
+
+// b8_decode.cu, b8_chunk.cu: enqueue the attention kernel for tiles of at most 1, 2 or 8 tokens.
+int b8_launch_few(const CUtensorMap& k_map, const CUtensorMap& v_map, const b8::AttnParams& p, int tokens, int code, cudaStream_t stream);
+int b8_launch_chunk(const CUtensorMap& k_map, const CUtensorMap& v_map, const b8::AttnParams& p, bool listed, int code, cudaStream_t stream);
+constexpr int kB8FewGrid = 2 * kNumSMs, kB8ChunkGrid = kNumSMs;
+
+}  // namespace ifv2

@@ -1,0 +1,380 @@
+// Attention over 8-bit blocks for several new tokens per sequence: drafts and prompts' chunks (formulas, operands and
+// shares: b8_attn.cuh).
+//
+// Eight tokens x 16 heads are the M side:
+//     S (128 rows x 128 keys)      = [Q1 + Q2] . K^T         both K-major in shared memory, two products into one sum
+//     O (128 rows x 128 features) += [W1 + W2 + W3] . V      W in TMEM (four codes per word), V MN-major as it lies
+// Units go to two groups of four softmax warps in turn (thread = row).  Each group has a score buffer, its weights over
+// the scores, and sums of its own (M, l, O), so that neither waits for the other; the two are put together at the end
+// of the tile.  TMEM: two S and two O of 128 columns, all there is.  Warps: 0 looks blocks up and issues TMA, 1 issues
+// MMAs (in order: a group's next scores come behind the product that reads its weights), 2..5 and 6..9 are the groups.
+#include "b8_attn.cuh"
+
+namespace ifv2 {
+namespace {
+
+using namespace b8;
+
+constexpr int kT = 8, kRows = kT * kGroup;
+constexpr int kThreads = 320, kSoftmax = 256;
+constexpr int kStages = 5;
+constexpr int kQBytes = kRows * kHeadDim;         // one of two terms
+constexpr int kRing = 2 * kQBytes, kSmem = kRing + kStages * 2 * kTileBytes + 1024;
+
+template <int kCode, bool kListed>
+__global__ void __launch_bounds__(kThreads, 1)
+b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const AttnParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  __shared__ Common<kT, kStages> s;
+  __shared__ uint64_t bar_s[2], bar_p[2], bar_pv[2], bar_q, bar_drain;
+  __shared__ float s_c[kRows], s_top[2][kRows], s_lse[2][kRows];       // row's factor; a group's M and log2 of its sum
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  volatile int* gave_up = &s.gave_up;
+
+  if (tid == 0) {
+    s.gave_up = 0;
+    for (int i = 0; i < kStages; ++i) mbar_init(&s.full[i], 1), mbar_init(&s.empty[i], 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar_s[i], 1), mbar_init(&bar_p[i], 4), mbar_init(&bar_pv[i], 1);
+      mbar_init(&s.item_full[i], 1), mbar_init(&s.item_empty[i], 9);
+    }
+    mbar_init(&bar_q, 8);
+    mbar_init(&bar_drain, 1);
+    fence_barrier_init();
+    prefetch_tensormap(&k_map);
+    prefetch_tensormap(&v_map);
+  }
+  if (warp == 1) {
+    tmem_alloc(&s.tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  allow_next();
+  if (kListed) wait_previous();
+  const uint32_t tmem = s.tmem;                    // S of group g at 128 g, O at 256 + 128 g
+
+  if (warp == 0) {
+    fetch<kT, kStages, kListed>(p, &k_map, &v_map, s, smem + kRing);
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMAs
+    if (elect_one()) {
+      const uint32_t base = smem_u32(smem);
+      constexpr uint32_t kIdescS = umma_idesc_f8(128, 128, kE4m3, kCode, false, false);
+      constexpr uint32_t kIdescO = umma_idesc_f8(128, 128, kE5m2, kCode, false, true);
+      bool ok = true;
+      int n = 0, queries = 0;
+      const auto values = [&](int unit, bool first) {        // O += W V of a unit
+        const int stage = unit % kStages, g = unit & 1;
+        ok = ok && bounded_wait(&bar_p[g], (unit >> 1) & 1, gave_up);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t v = base + kRing + stage * 2 * kTileBytes + kTileBytes;
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            umma_f8_ts(tmem + 256 + 128 * g, tmem + 128 * g + 32 * i + 8 * kk, umma_desc_sw128(v + kk * 4096, 16, 1024), kIdescO,
+                       !first || i + kk > 0);
+        umma_commit(&s.empty[stage]);
+        umma_commit(&bar_pv[g]);
+      };
+      for (int item = 0; ok; ++item) {
+        ok = bounded_wait(&s.item_full[item & 1], (item >> 1) & 1, gave_up);
+        const int units = ok ? s.item[item & 1].units : -1;
+        if (units < 0) break;
+        mbar_arrive(&s.item_empty[item & 1]);
+        if (units == 0) continue;
+        ok = bounded_wait(&bar_q, queries++ & 1, gave_up);
+        for (int i = 0; ok && i < units; ++i, ++n) {
+          const int stage = n % kStages;
+          ok = bounded_wait(&s.full[stage], (n / kStages) & 1, gave_up);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t k = base + kRing + stage * 2 * kTileBytes;
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_f8_ss(tmem + 128 * (n & 1), umma_desc_sw128(base + j * kQBytes + kk * 32, 16, 1024), umma_desc_sw128(k + kk * 32, 16, 1024),
+                         kIdescS, j + kk > 0);
+          umma_commit(&bar_s[n & 1]);
+          if (i > 0) values(n - 1, i <= 2);
+        }
+        values(n - 1, units <= 2);
+      }
+      if (!ok) {
+        umma_commit(&bar_drain);
+        mbar_wait_drain(&bar_drain, 0);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------------------------------------------------------- softmax
+    // A wait that gave up only makes the results NaN: within an item every thread keeps to the same loops and barriers.
+    const int group = (warp - 2) >> 2, quad = warp & 3, r = quad * 32 + lane;
+    const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+    const uint32_t my_s = tmem + 128 * group + lanes, my_o = tmem + 256 + 128 * group + lanes;
+    const int stid = tid - 64;
+    const int heads = p.heads_k * kGroup;
+
+    // Query rows of an item: 8 threads per row, 16 values each.
+    const auto write_query = [&](const Item& t) {
+#pragma unroll
+      for (int i = 0; i < kRows * 8 / kSoftmax; ++i) {
+        const int row = i * (kSoftmax / 8) + (stid >> 3), c = stid & 7;
+        uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+        if (row / kGroup < t.tokens) {
+          const uint4* src = reinterpret_cast<const uint4*>(
+              p.q + ((int64_t)(t.row + row / kGroup) * heads + t.head * kGroup + row % kGroup) * kHeadDim + c * 16);
+          x[0] = __ldg(src);
+          x[1] = __ldg(src + 1);
+        }
+        const float f = write_query16(x, smem + row * kHeadDim + ((c ^ (row & 7)) << 4), kQBytes, p.scale_log2);
+        if (c == 0) s_c[row] = f;
+      }
+      fence_proxy_async_smem();
+      mbar_arrive_warp(&bar_q);
+    };
+    Item next;
+    const auto next_item = [&](int item) {
+      const bool ok = bounded_wait_warp(&s.item_full[item & 1], (item >> 1) & 1, gave_up);
+      if (named_any<kSoftmax>(!ok)) {
+        next.units = -1;
+        return;
+      }
+      next = s.item[item & 1];
+      mbar_arrive_warp(&s.item_empty[item & 1]);
+    };
+
+    int n0 = 0;                                    // units of earlier items
+    next_item(0);
+    if (next.units > 0) write_query(next);
+    named_sync<kSoftmax>();
+    for (int item = 0; next.units >= 0; ++item) {
+      const Item t = next;
+      const int tok = r / kGroup;
+      const int limit = tok < t.tokens ? (p.causal ? t.reach - (t.tokens - 1 - tok) : t.reach) : 0;      // keys that the row sees
+      const float c_row = s_c[r];
+      const bool c_nan = !(c_row == c_row);
+      float m = kUnset, l = 0.f;                   // M, the sum in units of 2^(M - E)
+      int e_ref = kNoScale, deepest = 0;           // E; least eV - E of the blocks so far
+      bool begun = false;                          // O holds something
+      for (int i = (n0 & 1) ^ group; i < t.units; i += 2) {
+        const int n = n0 + i, stage = n % kStages;
+        bounded_wait_warp(&s.full[stage], (n / kStages) & 1, gave_up);
+        const Block blk[2] = {s.block[stage][0], s.block[stage][1]};
+        int seen[2], e_blk[2];
+        float c[2], ev[2], dv[2];
+        int e_new = e_ref;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          seen[h] = (blk[h].tokens >> tok) & 1 ? max(min(limit - blk[h].pos, blk[h].valid), 0) : 0;
+          e_blk[h] = blk[h].valid > 0 && blk[h].e_v != kNanByte ? blk[h].e_v : kNoScale;
+          e_new = max(e_new, e_blk[h]);
+          c[h] = fmaxf(c_row * blk[h].k_scale, 1e-37f);        // (-inf of a masked key times 0 would be NaN)
+        }
+        if (e_new == kNoScale) e_new = 0;
+        float back = 1.f;                          // what the sums so far are multiplied with
+        if (e_new != e_ref && e_ref != kNoScale) {
+          const int delta = e_new - e_ref, bump = max(kDeepest - (deepest - delta), 0);
+          deepest = max(deepest - delta, kDeepest);
+          l *= pow2i(min(delta - bump, 127));
+          if (m != kUnset) m += (float)bump;
+          back = pow2i(-bump);
+        }
+        e_ref = e_new;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int d = e_blk[h] > kNoScale ? max(e_blk[h] - e_ref, kDeepest) : 0;
+          deepest = min(deepest, d);
+          dv[h] = (float)d;
+          ev[h] = (float)(e_ref + d);
+        }
+        bounded_wait_warp(&bar_s[group], (n >> 1) & 1, gave_up);
+        tc_fence_after();
+        uint32_t x[2][64];
+        tmem_ld64_wait(my_s, x[0]);
+        tmem_ld64_wait(my_s + 64, x[1]);
+        if (!__all_sync(0xFFFFFFFFu, seen[0] == kBlockN && seen[1] == kBlockN)) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 64; ++j)
+              if (j >= seen[h]) x[h][j] = 0xFF800000u;
+        }
+        float top = -INFINITY;
+        bool odd = false;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float a = __uint_as_float(x[h][0]), b = __uint_as_float(x[h][1]);
+#pragma unroll
+          for (int j = 2; j < 64; j += 4) {
+            a = fmaxf(fmaxf(a, __uint_as_float(x[h][j])), __uint_as_float(x[h][j + 1]));
+            if (j + 2 < 64) b = fmaxf(fmaxf(b, __uint_as_float(x[h][j + 2])), __uint_as_float(x[h][j + 3]));
+          }
+          const bool k_nan = !(blk[h].k_scale == blk[h].k_scale);
+          odd |= k_nan || c_nan || (seen[h] > 0 && (blk[h].e_v == kNanByte || e_blk[h] - e_ref < kDeepest));
+          if (!k_nan && !c_nan) top = fmaxf(top, fmaf(fmaxf(a, b), c[h], ev[h]));
+        }
+        const bool moves = top - m > kRoom;
+        __syncwarp();
+        if (__any_sync(0xFFFFFFFFu, moves || back != 1.f)) {
+          float f = back;
+          if (moves) {
+            f = m == kUnset ? 0.f : f * ex2(m - (top - kTop));
+            l = l > 0.f ? l * (m == kUnset ? 0.f : ex2(m - (top - kTop))) : l;
+            m = top - kTop;
+          }
+          __syncwarp();
+          if (begun) {
+            bounded_wait_warp(&bar_pv[group], ((n - 2) >> 1) & 1, gave_up);
+            tc_fence_after();
+#pragma unroll
+            for (int c0 = 0; c0 < kHeadDim; c0 += 16) {
+              uint32_t o[16];
+              tmem_ld16(my_o + c0, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+              tmem_st16(my_o + c0, o);
+            }
+          }
+        }
+        begun = true;
+        odd = __any_sync(0xFFFFFFFFu, odd);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float b = ev[h] - m;
+          const uint64_t b2 = pack_f32x2(b, b), c2 = pack_f32x2(c[h], c[h]);
+          uint64_t sum2 = 0, sum2b = 0;
+          uint32_t t0[16], t1[16], t2[16];
+          const bool nan_key = c_nan || !(blk[h].k_scale == blk[h].k_scale), nan_value = blk[h].e_v == kNanByte;
+          const bool none = !nan_value && e_blk[h] - e_ref < kDeepest;      // values too small to be seen beside the others'
+#pragma unroll
+          for (int j = 0; j < 64; j += 4) {
+            float w[4];
+            unpack_f32x2(fma_f32x2(pack_f32x2(x[h][j], x[h][j + 1]), c2, b2), w[0], w[1]);
+            unpack_f32x2(fma_f32x2(pack_f32x2(x[h][j + 2], x[h][j + 3]), c2, b2), w[2], w[3]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = ex2(w[e]);
+            if (odd) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (nan_key) w[e] = j + e < seen[h] ? NAN : 0.f;
+            }
+            sum2 = add_f32x2(sum2, pack_f32x2(w[0], w[1]));
+            sum2b = add_f32x2(sum2b, pack_f32x2(w[2], w[3]));
+            if (odd) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if (nan_value) w[e] = j + e < seen[h] ? NAN : 0.f;
+                if (none) w[e] = w[e] == w[e] ? 0.f : w[e];
+              }
+            }
+            split4(w[0], w[1], w[2], w[3], t0[j / 4], t1[j / 4], t2[j / 4]);
+          }
+          tmem_st16(my_s + 16 * h, t0);
+          tmem_st16(my_s + 32 + 16 * h, t1);
+          tmem_st16(my_s + 64 + 16 * h, t2);
+          float s0, s1;
+          unpack_f32x2(add_f32x2(sum2, sum2b), s0, s1);
+          l += (s0 + s1) * ex2(-dv[h]);
+        }
+        if ((r & 63) >= (r < kBlockN ? blk[0].valid : blk[1].valid)) {       // a value row that is no key may hold anything: 0 x NaN
+          uint4* row = reinterpret_cast<uint4*>(smem + kRing + stage * 2 * kTileBytes + kTileBytes + r * kHeadDim);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) row[j] = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive_warp(&bar_p[group]);
+      }
+      s_top[group][r] = m;
+      s_lse[group][r] = l == 0.f ? -INFINITY : m - (float)e_ref + lg2(l);
+      // the next item's query, while the last products run (every S of this item has been read)
+      next_item(item + 1);
+      if (next.units > 0) write_query(next);
+
+      // ---- the item's results: each group has half of the features
+      const int n1 = n0 + t.units;
+      for (int n = max(n1 - 2, n0); n < n1; ++n) bounded_wait_warp(&bar_pv[n & 1], (n >> 1) & 1, gave_up);
+      tc_fence_after();
+      const float lse0 = s_lse[0][r], lse1 = s_lse[1][r];
+      const float most = fmaxf(lse0, lse1), nan = lse0 != lse0 ? lse0 : lse1 != lse1 ? lse1 : 0.f;
+      const bool none = most == -INFINITY;
+      const float lse2 = none ? -INFINITY + nan : most + lg2(ex2(lse0 - most) + ex2(lse1 - most)) + nan;
+      const bool lost = *gave_up;
+      if (group == 0 && tok < t.tokens) {
+        if (t.piece >= 0) p.part_lse[(int64_t)t.piece * kRows + r] = lse2;
+        else if (p.lse) p.lse[(int64_t)(t.row + tok) * heads + t.head * kGroup + r % kGroup] = none && nan == 0.f ? INFINITY : lse2 * kLn2;
+      }
+      // 2^(M - lse) in two steps, so that neither leaves fp32's range
+      float f[2];
+      bool with[2];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        with[g] = t.units > (g ^ (n0 & 1));        // this group had a unit
+        f[g] = none ? nan : ex2(0.5f * (s_top[g][r] - lse2));
+        if (s_lse[g][r] == -INFINITY) f[g] = nan;
+      }
+      __nv_bfloat16* out = p.out + ((int64_t)(t.row + tok) * heads + t.head * kGroup + r % kGroup) * kHeadDim + 64 * group;
+      float* part = p.part_o + ((int64_t)max(t.piece, 0) * kRows + r) * kHeadDim + 64 * group;
+#pragma unroll
+      for (int c0 = 0; c0 < 64; c0 += 16) {
+        float y[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) y[j] = nan;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          if (!with[g]) continue;
+          uint32_t o[16];
+          __syncwarp();
+          tmem_ld16(tmem + 256 + 128 * g + lanes + 64 * group + c0, o);
+          tmem_wait_ld();
+          if (f[g] != 0.f) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) y[j] += q8::mul_exact(q8::mul_exact(__uint_as_float(o[j]), f[g]), f[g]);
+          }
+        }
+        if (lost) y[0] = y[4] = y[8] = y[12] = NAN;
+        if (tok < t.tokens && t.piece < 0) {
+          uint4 a, b;
+          a.x = pack_bf16(y[0], y[1]), a.y = pack_bf16(y[2], y[3]), a.z = pack_bf16(y[4], y[5]), a.w = pack_bf16(y[6], y[7]);
+          b.x = pack_bf16(y[8], y[9]), b.y = pack_bf16(y[10], y[11]), b.z = pack_bf16(y[12], y[13]), b.w = pack_bf16(y[14], y[15]);
+          reinterpret_cast<uint4*>(out + c0)[0] = a;
+          reinterpret_cast<uint4*>(out + c0)[1] = b;
+        } else if (tok < t.tokens) {
+#pragma unroll
+          for (int j = 0; j < 16; j += 4) *reinterpret_cast<float4*>(part + c0 + j) = make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]);
+        }
+      }
+      tc_fence_before();
+      named_sync<kSoftmax>();
+      n0 = n1;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(s.tmem, 512);
+}
+
+template <int kCode, bool kListed>
+int launch(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttnParams& p, cudaStream_t stream) {
+  const cudaError_t e = cudaFuncSetAttribute(b8_chunk_kernel<kCode, kListed>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  if (e != cudaSuccess) return set_error((int)e, "b8_attn: %s", cudaGetErrorString(e));
+  b8_chunk_kernel<kCode, kListed><<<kB8ChunkGrid, kThreads, kSmem, stream>>>(k_map, v_map, p);
+  return check_launch("b8_attn");
+}
+
+}  // namespace
+
+int b8_launch_chunk(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttnParams& p, bool listed, int code, cudaStream_t stream) {
+  if (listed) return code == kE4m3 ? launch<kE4m3, true>(k_map, v_map, p, stream) : launch<kE5m2, true>(k_map, v_map, p, stream);
+  return code == kE4m3 ? launch<kE4m3, false>(k_map, v_map, p, stream) : launch<kE5m2, false>(k_map, v_map, p, stream);
+}
+
+}  // namespace ifv2

@@ -1,0 +1,403 @@
+// Attention over 8-bit blocks for one or two new tokens per sequence (formulas, operands and shares: b8_attn.cuh).
+//
+// Keys are the M side of both products, so that few query rows cost few tensor clocks:
+//     S^T (128 keys x 2 x 16 kT)        = K . [Q1 Q2]^T     the query's two terms side by side, added by the softmax
+//     O^T (128 features x 3 x 16 kT)   += V^T . [W1 W2 W3]  V is MN-major as it lies; W is written [key][column]
+// A softmax thread has a key of its own, with the tile's columns in registers: a decode step's exponentials are spread
+// over all lanes.  One A operand then serves all terms of the other side (4 MMAs for each product of a unit; term by
+// term they were 8 and 12, and A is what they cost).  Warps: 0 looks blocks up and issues TMA, 1 issues MMAs, 2..5 are
+// the softmax (thread = key = feature).  Two CTAs per SM.
+#include "b8_attn.cuh"
+
+namespace ifv2 {
+namespace {
+
+using namespace b8;
+
+constexpr int kThreads = 192, kSoftmax = 128;
+
+template <int kT>
+struct Shape {
+  static constexpr int kN = kGroup * kT;           // columns
+  static constexpr int kStages = kT == 1 ? 3 : 2;
+  static constexpr int kQBytes = kN * kHeadDim;    // one of two terms
+  static constexpr int kPBytes = kN * kUnit;       // one of three terms
+  static constexpr int kQ = 0, kP = 2 * kQBytes, kRing = (kP + 3 * kPBytes + 1023) / 1024 * 1024;
+  static constexpr int kSmem = kRing + kStages * 2 * kTileBytes + 1024;
+  static constexpr int kO = 4 * kN;                // columns of O behind two S
+  static constexpr int kTmem = kT == 1 ? 128 : 256;
+};
+
+// Floats as integers of the same order, for redux.
+__device__ __forceinline__ int ordered(float x) {
+  const int i = __float_as_int(x);
+  return i ^ ((i >> 31) & 0x7FFFFFFF);
+}
+__device__ __forceinline__ float from_ordered(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7FFFFFFF)); }
+
+// Column sums over the 32 lanes: half the columns go to the other lane in each step.  Column `first` is in v[0] at the end.
+template <int kN>
+__device__ __forceinline__ int column_sums(float (&v)[kN], int lane) {
+  int first = 0;
+  int n = kN;
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) {
+    const bool up = lane & s;
+    if (n > 1) {
+      n >>= 1;
+#pragma unroll
+      for (int i = 0; i < kN / 2; ++i) {
+        if (i >= n) continue;
+        const float mine = up ? v[i + n] : v[i], other = up ? v[i] : v[i + n];
+        v[i] = mine + __shfl_xor_sync(0xFFFFFFFFu, other, s);
+      }
+      if (up) first += n;
+    } else {
+      v[0] += __shfl_xor_sync(0xFFFFFFFFu, v[0], s);
+    }
+  }
+  return first;
+}
+
+template <int kT, int kCode>
+__global__ void __launch_bounds__(kThreads, 2)
+b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const AttnParams p) {
+  using S = Shape<kT>;
+  constexpr int kN = S::kN, kStages = S::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  __shared__ Common<kT, kStages> s;
+  __shared__ uint64_t bar_s[2], bar_sfree[2], bar_p, bar_pv, bar_q, bar_drain;
+  __shared__ float s_c[kN], s_mu[kN], s_fl[kN], s_fo[kN], s_red[4][kN];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  volatile int* gave_up = &s.gave_up;
+
+  if (tid == 0) {
+    s.gave_up = 0;
+    for (int i = 0; i < kStages; ++i) mbar_init(&s.full[i], 1), mbar_init(&s.empty[i], 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar_s[i], 1), mbar_init(&bar_sfree[i], 4);
+      mbar_init(&s.item_full[i], 1), mbar_init(&s.item_empty[i], 5);
+    }
+    mbar_init(&bar_p, 4);
+    mbar_init(&bar_pv, 1);
+    mbar_init(&bar_q, 4);
+    mbar_init(&bar_drain, 1);
+    fence_barrier_init();
+    prefetch_tensormap(&k_map);
+    prefetch_tensormap(&v_map);
+  }
+  if (warp == 1) {
+    tmem_alloc(&s.tmem, S::kTmem);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  allow_next();
+  const uint32_t tmem_s = s.tmem, tmem_o = s.tmem + S::kO;
+
+  if (warp == 0) {
+    fetch<kT, kStages, false>(p, &k_map, &v_map, s, smem + S::kRing);
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMAs
+    if (elect_one()) {
+      const uint32_t base = smem_u32(smem);
+      constexpr uint32_t kIdescS = umma_idesc_f8(128, 2 * kN, kCode, kE4m3, false, false);
+      constexpr uint32_t kIdescO = umma_idesc_f8(128, 3 * kN, kCode, kE5m2, true, true);
+      bool ok = true;
+      int n = 0, queries = 0;
+      const auto values = [&](int unit, bool first) {        // O += W V of a unit
+        const int stage = unit % kStages;
+        ok = ok && bounded_wait(&bar_p, unit & 1, gave_up);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t v = base + S::kRing + stage * 2 * kTileBytes + kTileBytes;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          umma_f8_ss(tmem_o, umma_desc_sw128(v + kk * 4096, 16, 1024), umma_desc_noswz_mn8(base + S::kP + kk * 512, 16 * kUnit),
+                     kIdescO, !first || kk > 0);
+        umma_commit(&s.empty[stage]);
+        umma_commit(&bar_pv);
+      };
+      for (int item = 0; ok; ++item) {
+        ok = bounded_wait(&s.item_full[item & 1], (item >> 1) & 1, gave_up);
+        const int units = ok ? s.item[item & 1].units : -1;
+        if (units < 0) break;
+        mbar_arrive(&s.item_empty[item & 1]);
+        if (units == 0) continue;
+        ok = bounded_wait(&bar_q, queries++ & 1, gave_up);
+        for (int i = 0; ok && i < units; ++i, ++n) {
+          const int stage = n % kStages;
+          ok = bounded_wait(&s.full[stage], (n / kStages) & 1, gave_up) && bounded_wait(&bar_sfree[n & 1], ((n >> 1) & 1) ^ 1, gave_up);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t k = base + S::kRing + stage * 2 * kTileBytes;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            umma_f8_ss(tmem_s + (n & 1) * 2 * kN, umma_desc_sw128(k + kk * 32, 16, 1024), umma_desc_sw128(base + S::kQ + kk * 32, 16, 1024),
+                       kIdescS, kk > 0);
+          umma_commit(&bar_s[n & 1]);
+          if (i > 0) values(n - 1, i == 1);
+        }
+        values(n - 1, units == 1);
+      }
+      if (!ok) {
+        umma_commit(&bar_drain);
+        mbar_wait_drain(&bar_drain, 0);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------------------------------------------------------- softmax
+    // A wait that gave up only makes the results NaN: within an item every thread keeps to the same loops and barriers.
+    const int quad = warp & 3, r = quad * 32 + lane;
+    const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+    const int stid = tid - 64;
+    const int heads = p.heads_k * kGroup;
+
+    // Query rows of an item: 8 threads per row, 16 values each.
+    const auto write_query = [&](const Item& t) {
+#pragma unroll
+      for (int i = 0; i < kT; ++i) {
+        const int col = i * 16 + (stid >> 3), c = stid & 7;
+        uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+        if (i < t.tokens) {
+          const uint4* src = reinterpret_cast<const uint4*>(p.q + ((int64_t)(t.row + i) * heads + t.head * kGroup + (stid >> 3)) * kHeadDim + c * 16);
+          x[0] = __ldg(src);
+          x[1] = __ldg(src + 1);
+        }
+        const float f = write_query16(x, smem + S::kQ + col * kHeadDim + ((c ^ (col & 7)) << 4), S::kQBytes, p.scale_log2);
+        if (c == 0) s_c[col] = f;
+      }
+      fence_proxy_async_smem();
+      mbar_arrive_warp(&bar_q);
+      named_sync<kSoftmax>();
+    };
+    Item next;
+    const auto next_item = [&](int item) {
+      const bool ok = bounded_wait_warp(&s.item_full[item & 1], (item >> 1) & 1, gave_up);
+      if (named_any<kSoftmax>(!ok)) {
+        next.units = -1;
+        return;
+      }
+      next = s.item[item & 1];
+      mbar_arrive_warp(&s.item_empty[item & 1]);
+    };
+
+    int n = 0;
+    next_item(0);
+    if (next.units > 0) write_query(next);
+    for (int item = 0; next.units >= 0; ++item) {
+      const Item t = next;
+      float l[kN];
+#pragma unroll
+      for (int i = 0; i < kN; ++i) l[i] = 0.f;
+      if (stid < kN) s_mu[stid] = kUnset;
+      named_sync<kSoftmax>();
+      int e_ref = kNoScale, deepest = 0;           // E; least eV - E of the blocks so far
+      for (int i = 0; i < t.units; ++i, ++n) {
+        const int stage = n % kStages;
+        bounded_wait_warp(&s.full[stage], (n / kStages) & 1, gave_up);
+        bounded_wait_warp(&bar_s[n & 1], (n >> 1) & 1, gave_up);
+        tc_fence_after();
+        float x[kN];
+        {
+          uint32_t y[2 * kN];
+          if constexpr (kN == 16) tmem_ld32_wait(tmem_s + (n & 1) * 2 * kN + lanes, y);
+          else tmem_ld64_wait(tmem_s + (n & 1) * 2 * kN + lanes, y);
+#pragma unroll
+          for (int c = 0; c < kN; ++c) x[c] = __uint_as_float(y[c]) + __uint_as_float(y[kN + c]);
+        }
+        tc_fence_before();
+        mbar_arrive_warp(&bar_sfree[n & 1]);
+        const Block mine = s.block[stage][r >> 6], other = s.block[stage][(r >> 6) ^ 1];
+        const int e_mine = mine.valid > 0 && mine.e_v != kNanByte ? mine.e_v : kNoScale;
+        const int e_other = other.valid > 0 && other.e_v != kNanByte ? other.e_v : kNoScale;
+        int e_new = max(e_ref, max(e_mine, e_other));
+        if (e_new == kNoScale) e_new = 0;
+        const int in_block = r & 63;
+        const bool here = in_block < mine.valid;
+        // keys that token i sees end at position reach - (tokens - 1 - i) if causal, reach otherwise
+        const int left = t.reach - (mine.pos + in_block);      // > 0: the last token sees this key
+        const auto sees = [&](int tok) {
+          return here && ((mine.tokens >> tok) & 1) && (p.causal ? left > t.tokens - 1 - tok : left > 0);
+        };
+        const int dv = mine.e_v - e_new;                       // (of no interest without a key or in a NaN block)
+        const float v_scale = mine.e_v == kNanByte ? NAN : pow2i(dv), v_ref = pow2i(max(min(dv, 0), kDeepest));
+        float w[kN];
+        const auto weights = [&]() {
+          float most = 0.f;
+#pragma unroll
+          for (int tok = 0; tok < kT; ++tok) {
+            const bool see = sees(tok);
+#pragma unroll
+            for (int g = 0; g < kGroup; ++g) {
+              const int c = tok * kGroup + g;
+              const float y = ex2(fmaf(x[c], s_c[c] * mine.k_scale, -s_mu[c]));
+              w[c] = see ? y : 0.f;
+              most = fmaxf(most, w[c]);
+            }
+          }
+          return most;
+        };
+        bool moves = e_new != e_ref;
+        if (!moves) moves = named_any<kSoftmax>(weights() * v_ref > 32768.f);
+        if (moves) {
+          // new references: the largest x + eV of each column, and E
+          const int delta = e_ref == kNoScale ? 0 : e_new - e_ref;
+          const int bump = max(kDeepest - (deepest - delta), 0);
+          deepest = max(deepest - delta, kDeepest);
+          const float up = (float)max(min(dv, 0), kDeepest);
+#pragma unroll
+          for (int tok = 0; tok < kT; ++tok) {
+            const bool see = sees(tok);
+#pragma unroll
+            for (int g = 0; g < kGroup; ++g) {
+              const int c = tok * kGroup + g;
+              float y = fmaf(x[c], s_c[c] * mine.k_scale, up);
+              if (!see || !(y == y)) y = -INFINITY;
+              const int top = __reduce_max_sync(0xFFFFFFFFu, ordered(y));
+              if (lane == 0) s_red[quad][c] = from_ordered(top);
+            }
+          }
+          named_sync<kSoftmax>();
+          if (stid < kN) {
+            const float top = fmaxf(fmaxf(s_red[0][stid], s_red[1][stid]), fmaxf(s_red[2][stid], s_red[3][stid]));
+            const float mu = s_mu[stid];
+            float mu_new = mu, fl = 0.f, fo = 0.f;
+            if (mu == kUnset) {
+              if (top > -INFINITY) mu_new = top - kTop;
+            } else {
+              mu_new = mu + (float)(bump - delta);
+              if (top - mu_new > kRoom) mu_new = top - kTop;
+              fl = ex2(mu - mu_new);
+              fo = ex2(mu - mu_new - (float)delta);
+            }
+            s_mu[stid] = mu_new;
+            s_fl[stid] = fl;
+            s_fo[stid] = fo;
+          }
+          named_sync<kSoftmax>();
+#pragma unroll
+          for (int c = 0; c < kN; ++c) l[c] = l[c] > 0.f ? l[c] * s_fl[c] : l[c];
+          if (i > 0) {                             // what is in O so far
+            bounded_wait_warp(&bar_pv, (n - 1) & 1, gave_up);
+            tc_fence_after();
+#pragma unroll
+            for (int c0 = 0; c0 < 3 * kN; c0 += 16) {
+              uint32_t o[16];
+              tmem_ld16(tmem_o + lanes + c0, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * s_fo[c0 % kN + c]);
+              tmem_st16(tmem_o + lanes + c0, o);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+          }
+          e_ref = e_new;
+          weights();
+        }
+        if (e_mine > kNoScale) deepest = max(min(deepest, e_mine - e_ref), kDeepest);
+        if (e_other > kNoScale) deepest = max(min(deepest, e_other - e_ref), kDeepest);
+        // the one buffer of weights is free again when the product before has been made
+        if (n > 0) bounded_wait_warp(&bar_pv, (n - 1) & 1, gave_up);
+#pragma unroll
+        for (int tok = 0; tok < kT; ++tok) {
+          const bool see = sees(tok);
+          uint32_t out[3][4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int c = tok * kGroup + 4 * j + e;
+              l[c] += w[c];
+              y[e] = see ? w[c] * v_scale : 0.f;
+            }
+            split4(y[0], y[1], y[2], y[3], out[0][j], out[1][j], out[2][j]);
+          }
+#pragma unroll
+          for (int k = 0; k < 3; ++k)
+            *reinterpret_cast<uint4*>(smem + S::kP + k * S::kPBytes + tok * 16 * kUnit + r * 16) =
+                make_uint4(out[k][0], out[k][1], out[k][2], out[k][3]);
+        }
+        if (!here) {                               // a value row that is no key may hold anything: 0 x NaN
+          uint4* row = reinterpret_cast<uint4*>(smem + S::kRing + stage * 2 * kTileBytes + kTileBytes + r * kHeadDim);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) row[j] = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+        mbar_arrive_warp(&bar_p);
+      }
+      // the next item's query, while the last product runs (every S of this item has been read)
+      next_item(item + 1);
+      if (next.units > 0) write_query(next);
+
+      // ---- the item's results
+      const int first = column_sums<kN>(l, lane);
+      s_red[quad][first] = l[0];                   // (16 columns: two lanes, one value)
+      named_sync<kSoftmax>();
+      if (t.units > 0) bounded_wait_warp(&bar_pv, (n - 1) & 1, gave_up);
+      tc_fence_after();
+      if (stid < kN) {
+        const float sum = s_red[0][stid] + s_red[1][stid] + s_red[2][stid] + s_red[3][stid];
+        const bool none = sum == 0.f;
+        const float lse2 = none ? -INFINITY : s_mu[stid] + lg2(sum);
+        s_fl[stid] = none ? 0.f : 1.f / sum;
+        const int tok = stid / kGroup;
+        if (t.piece >= 0) p.part_lse[(int64_t)t.piece * kN + stid] = lse2;
+        else if (p.lse && tok < t.tokens)
+          p.lse[(int64_t)(t.row + tok) * heads + t.head * kGroup + stid % kGroup] = none ? INFINITY : lse2 * kLn2;
+      }
+      named_sync<kSoftmax>();
+      const float e_half = pow2i(e_ref > kNoScale ? e_ref / 2 : 0), e_rest = pow2i(e_ref > kNoScale ? e_ref - e_ref / 2 : 0);
+      const bool lost = *gave_up;
+#pragma unroll
+      for (int tok = 0; tok < kT; ++tok) {
+        if (tok >= t.tokens) continue;
+        uint32_t o[3][16];
+        if (t.units > 0) {
+#pragma unroll
+          for (int k = 0; k < 3; ++k) tmem_ld16(tmem_o + lanes + k * kN + tok * kGroup, o[k]);
+          tmem_wait_ld();
+        }
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+          const int col = tok * kGroup + c;
+          const float f = s_fl[col];
+          float y = 0.f;
+          if (t.units > 0 && f != 0.f)
+            y = q8::mul_exact(q8::mul_exact((__uint_as_float(o[0][c]) + __uint_as_float(o[1][c]) + __uint_as_float(o[2][c])) * f, e_half), e_rest);
+          if (lost) y = NAN;
+          if (t.piece < 0) p.out[((int64_t)(t.row + tok) * heads + t.head * kGroup + c) * kHeadDim + r] = __float2bfloat16(y);
+          else p.part_o[((int64_t)t.piece * kN + col) * kHeadDim + r] = y;
+        }
+      }
+      tc_fence_before();
+      named_sync<kSoftmax>();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(s.tmem, S::kTmem);
+}
+
+template <int kT, int kCode>
+int launch(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttnParams& p, cudaStream_t stream) {
+  constexpr int smem = Shape<kT>::kSmem;
+  const cudaError_t e = cudaFuncSetAttribute(b8_few_kernel<kT, kCode>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return set_error((int)e, "b8_attn: %s", cudaGetErrorString(e));
+  b8_few_kernel<kT, kCode><<<kB8FewGrid, kThreads, smem, stream>>>(k_map, v_map, p);
+  return check_launch("b8_attn");
+}
+
+}  // namespace
+
+int b8_launch_few(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttnParams& p, int tokens, int code, cudaStream_t stream) {
+  if (tokens == 1) return code == kE4m3 ? launch<1, kE4m3>(k_map, v_map, p, stream) : launch<1, kE5m2>(k_map, v_map, p, stream);
+  return code == kE4m3 ? launch<2, kE4m3>(k_map, v_map, p, stream) : launch<2, kE5m2>(k_map, v_map, p, stream);
+}
+
+}  // namespace ifv2

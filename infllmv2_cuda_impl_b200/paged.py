@@ -23,7 +23,7 @@ import torch
 
 from . import _lib
 from .attention import BLOCK_N, GROUP, HEAD_DIM
-from .ops import _on, _require_cuda, _stream, topk_to_uint64
+from .ops import _on, _require_cuda, _stream
 from .quant_cache import _cu, _ints, _no_gradient, _ptr, _table
 from .rotary import _rows
 
@@ -220,7 +220,9 @@ def infllmv2_attn_paged_b8(
     elif topk_idx is not None:
         if topk_idx.dtype is not torch.int32 or topk_idx.device != dev or topk_idx.dim() != 3 or topk_idx.shape[:2] != (hk, total):
             raise ValueError(f"{what}: topk_idx must be ({hk}, {total}, topk) int32 on {dev}")
-        block_mask = topk_to_uint64(topk_idx, cap, BLOCK_N)[0] if total else None
+        topk_idx = topk_idx.contiguous()
+        if topk_idx.shape[2] == 0:                     # (a list of no entries has no address)
+            topk_idx = torch.full((hk, total, 1), -1, dtype=torch.int32, device=dev)
     q = q.contiguous()
     out = torch.empty_like(q)
     lse = torch.empty(total, heads, dtype=torch.float32, device=dev) if return_softmax_lse else None
@@ -230,7 +232,8 @@ def infllmv2_attn_paged_b8(
         with _on(dev):
             _lib.call("ifv2_b8_attn", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                       out.data_ptr(), _ptr(lse), cu_seqlens_q.data_ptr(), cache_seqlens.data_ptr(), _ptr(block_table), width,
-                      _ptr(block_mask), words if block_mask is not None else 0, batch, total, max_seqlen_q, pages, length, code, heads,
+                      _ptr(topk_idx), topk_idx.shape[2] if topk_idx is not None else 0, _ptr(block_mask),
+                      words if block_mask is not None else 0, batch, total, max_seqlen_q, pages, length, code, heads,
                       hk, HEAD_DIM, HEAD_DIM ** -0.5 if softmax_scale is None else float(softmax_scale), 1 if causal else 0,
                       ws.data_ptr(), ws_bytes, _stream(dev))
     return (out, lse) if return_softmax_lse else out

@@ -135,8 +135,8 @@ def test_selected_blocks(dtype, lens, new, page):
     check(got, q, k, v, cu_q, lens, table, True, lists)
     cap = cache[0].shape[2] * (1 if table is None else table.shape[1])
     mask, _ = infllm_v2.topk_to_uint64(lists.to(DEV), cap, 64)
-    again = infllm_v2.infllmv2_attn_paged_b8(*args, block_mask=mask, **more)
-    assert all(torch.equal(a, b) for a, b in zip(got, again))
+    # (not bit for bit the same: a mask row counts for another cost than a list, so that tiles are cut elsewhere)
+    check(infllm_v2.infllmv2_attn_paged_b8(*args, block_mask=mask, **more), q, k, v, cu_q, lens, table, True, lists)
 
 
 @pytest.mark.parametrize("dtype", [E4M3, E5M2])
