@@ -567,7 +567,9 @@ int ifv2_b8_write(const void* k, const void* v, int64_t k_token_stride, int64_t 
                   int64_t v_token_stride, int64_t v_head_stride, void* k_cache, void* v_cache, void* k_scale,
                   void* v_scale, const int64_t* slots, int64_t num_pages, int page_size, int code, int64_t total,
                   int heads_k, int head_dim, void* stream);
-int64_t ifv2_b8_attn_workspace_bytes(int64_t total_q, int batch, int heads_q, int head_dim, int max_seqlen_q);
+/* capacity: keys that a sequence has room for (block_table_stride * length, or length). */
+int64_t ifv2_b8_attn_workspace_bytes(int64_t total_q, int batch, int heads_q, int head_dim, int max_seqlen_q,
+                                     int64_t capacity);
 int ifv2_b8_attn(const void* q, const void* k_cache, const void* v_cache, const void* k_scale, const void* v_scale,
                  void* out, float* lse, const int32_t* cu_seqlens_q, const int32_t* cache_seqlens,
                  const int32_t* block_table, int block_table_stride, const int32_t* topk_idx, int topk,

@@ -106,7 +106,7 @@ _INT64_RETURNS = {
     "ifv2_decode_workspace_bytes": [c_int, c_int, c_int, c_int],
     "ifv2_stage1_decode_workspace_bytes": [c_int, c_int, c_int],
     "ifv2_q8_decode_workspace_bytes": [c_int, c_int, c_int],
-    "ifv2_b8_attn_workspace_bytes": [c_int64, c_int, c_int, c_int, c_int],
+    "ifv2_b8_attn_workspace_bytes": [c_int64, c_int, c_int, c_int, c_int, c_int64],
 }
 
 

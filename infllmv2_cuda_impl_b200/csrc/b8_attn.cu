@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(kPlanThreads) b8_plan_kernel(const AttnParams 
     p.first_tile[grid_most] = tiles;
   }
   __syncthreads();
-  const Shares shares(max(before, (int64_t)1), grid_most, p.least_share);
+  const Shares<int64_t> shares(max(before, (int64_t)1), grid_most, p.least_share);
   for (int g = tid; g < grid_most; g += kPlanThreads) {
     const int64_t at = shares.begin(min(g, shares.grid - 1));
     int lo = 0, hi = tiles;                        // start[lo] <= at < start[hi]
@@ -198,11 +198,12 @@ struct Layout {
   int tokens, grid;                                // of a tile; CTAs
   bool listed;
   int64_t chunks, lse_at, o_at, tiles_at, start_at, chunk_at, first_at, bytes;
-  Layout(int64_t total_q, int batch, int heads_k, int max_seqlen_q) {
+  Layout(int64_t total_q, int batch, int heads_k, int max_seqlen_q, int64_t capacity) {
     const auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
-    tokens = max_seqlen_q <= 1 ? 1 : max_seqlen_q == 2 ? 2 : kTokensPerTile;
+    // (CTAs that find their share themselves add up costs in 32 bits)
+    listed = max_seqlen_q > kTokensPerTile || (int64_t)batch * heads_k * (capacity / kUnit + 1 + kStart) >= (1ll << 30);
+    tokens = listed ? kTokensPerTile : max_seqlen_q <= 1 ? 1 : max_seqlen_q == 2 ? 2 : kTokensPerTile;
     grid = tokens <= 2 ? kB8FewGrid : kB8ChunkGrid;
-    listed = max_seqlen_q > kTokensPerTile;
     chunks = listed ? ceil_div64(total_q, kTokensPerTile) + batch : 0;
     lse_at = up(16 * grid);
     o_at = up(lse_at + 4ll * 2 * grid * kGroup * tokens);
@@ -220,9 +221,10 @@ struct Layout {
 
 using namespace ifv2;
 
-extern "C" int64_t ifv2_b8_attn_workspace_bytes(int64_t total_q, int batch, int heads_q, int head_dim, int max_seqlen_q) {
-  if (total_q < 0 || batch < 0 || heads_q < 0 || head_dim != kHeadDim) return 0;
-  return Layout(total_q, batch, heads_q / kGroup, max_seqlen_q).bytes;
+extern "C" int64_t ifv2_b8_attn_workspace_bytes(int64_t total_q, int batch, int heads_q, int head_dim, int max_seqlen_q,
+                                                int64_t capacity) {
+  if (total_q < 0 || batch < 0 || heads_q < 0 || head_dim != kHeadDim || capacity < 0) return 0;
+  return Layout(total_q, batch, heads_q / kGroup, max_seqlen_q, capacity).bytes;
 }
 
 extern "C" int ifv2_b8_attn(const void* q, const void* k_cache, const void* v_cache, const void* k_scale, const void* v_scale,
@@ -249,7 +251,7 @@ extern "C" int ifv2_b8_attn(const void* q, const void* k_cache, const void* v_ca
                "b8_attn: mask rows must have a word per 64 blocks of the capacity");
   IFV2_REQUIRE((mask == nullptr && topk_idx == nullptr) || cap <= kMaxMaskWords * 64 * kBlockN, IFV2_ERR_TOO_LARGE,
                "b8_attn: blocks are selected among at most %d keys", kMaxMaskWords * 64 * kBlockN);
-  const Layout at(total_q, batch, heads_k, max_seqlen_q);
+  const Layout at(total_q, batch, heads_k, max_seqlen_q, cap);
   IFV2_REQUIRE(at.chunks * heads_k < (1ll << 31), IFV2_ERR_TOO_LARGE, "b8_attn: too many tiles");
   IFV2_REQUIRE(workspace_bytes >= at.bytes, IFV2_ERR_INVALID_ARG, "b8_attn: the workspace is too small");
   IFV2_REQUIRE(((reinterpret_cast<uintptr_t>(workspace) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) == 0,

@@ -18,6 +18,7 @@
 // and are joined by a second kernel.  Where a sequence has one tile per head (a decode step, drafts) every CTA finds
 // its share by itself, from the lengths; otherwise a kernel in front lists the tiles.
 #pragma once
+#include <type_traits>
 #include "b8.cuh"
 
 namespace ifv2 {
@@ -33,7 +34,7 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kUnset = -1e30f;                 // reference of a row that has seen no key
 constexpr float kTop = 10.f, kRoom = 15.f;       // a new reference puts the largest weight at 2^kTop; past 2^kRoom it moves
 constexpr int kDeepest = -90;                    // eV - E that the sum's range has room for
-constexpr int kNoScale = -10000;                 // eV of no block
+constexpr int kNoScale = -10000, kNanScale = 10000;      // eV of no block, of a NaN block
 
 struct AttnParams {
   const __nv_bfloat16* q;
@@ -61,23 +62,17 @@ struct AttnParams {
   int64_t* start;                                // (tiles + 1) cost before each tile
 };
 
-// Shares of a cost: CTA g has [begin(g), begin(g + 1)).
+// Shares of a cost: CTA g has [begin(g), begin(g + 1)).  Cost: int where the host knows that a call's fits.
+template <typename Cost>
 struct Shares {
-  int64_t each, rest;
+  Cost each, rest;
   int grid;
-  __device__ __forceinline__ Shares(int64_t cost, int most, int least) {
-    if (cost >> 31 == 0) {                         // (a 64-bit division takes some hundred clocks)
-      const uint32_t c = (uint32_t)cost;
-      grid = (int)min(max(c / (uint32_t)least, 1u), (uint32_t)most);
-      each = c / (uint32_t)grid;
-      rest = c - (uint32_t)each * (uint32_t)grid;
-    } else {
-      grid = most;
-      each = cost / grid;
-      rest = cost - each * grid;
-    }
+  __device__ __forceinline__ Shares(Cost cost, int most, int least) {
+    grid = cost >= (Cost)most * least ? most : (int)max((uint32_t)cost / (uint32_t)least, 1u);
+    each = sizeof(Cost) == 4 ? (Cost)((uint32_t)cost / (uint32_t)grid) : cost / grid;
+    rest = cost - each * grid;
   }
-  __device__ __forceinline__ int64_t begin(int g) const { return each * g + min((int64_t)g, rest); }
+  __device__ __forceinline__ Cost begin(int g) const { return each * g + min((Cost)g, rest); }
 };
 
 // Tokens of sequence b (cu_q is clamped to the rows there are).
@@ -106,11 +101,12 @@ __device__ __forceinline__ unsigned long long union_word(const AttnParams& p, in
 // A block on its way through the CTA: written by the fetching warp, read by the softmax.
 struct __align__(16) Block {
   float k_scale;                                   // 2^eK, or NaN
-  int e_v;                                         // eV, kNanByte: NaN block
+  int e_v;                                         // eV; kNoScale without keys, kNanScale: NaN block
   int valid;                                       // keys (0: the block only fills a unit)
+  int e_unit;                                      // largest (low half) and least (high) eV of the unit's two blocks
   int pos;                                         // position of its first key
   uint32_t tokens;                                 // tokens that attend it
-  uint32_t pad[3];
+  uint32_t pad[2];
 };
 // A CTA's part of a tile.
 struct __align__(16) Item {
@@ -119,10 +115,13 @@ struct __align__(16) Item {
   int piece;                                       // -1: the whole tile, else the place of a partial result
 };
 
-__device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
-  if (mbar_try_wait(bar, parity)) return true;
+// (the long form stands apart: what is taken every time has to stay in the instruction cache)
+static __device__ __noinline__ bool long_wait(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
   if (*gave_up) return false;
   return mbar_wait(bar, parity, gave_up, nullptr, 0);
+}
+__device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
+  return __builtin_expect(mbar_try_wait(bar, parity), 1) ? true : long_wait(bar, parity, gave_up);
 }
 // All lanes of a warp (the TMEM instructions behind it want them together).
 __device__ __forceinline__ bool bounded_wait_warp(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
@@ -212,40 +211,38 @@ struct Common {
 
 // ---------------------------------------------------------------------- fetching warp --
 // All lanes run it.  kListed: tiles come from the kernel in front.
-template <int kT, int kStages, bool kListed>
+template <int kT, int kStages, bool kListed, bool kSelected>
 __device__ __forceinline__ void fetch(const AttnParams& p, const CUtensorMap* k_map, const CUtensorMap* v_map, Common<kT, kStages>& s,
                                       uint8_t* ring) {
+  using Cost = typename std::conditional<kListed, int64_t, int>::type;
   const int lane = threadIdx.x & 31;
   volatile int* gave_up = &s.gave_up;
-  const bool selected = p.mask != nullptr || p.lists != nullptr;
   int b = 0, head = 0, row = 0, tokens = 0, reach = 0, tile = 0, n_tiles = 0;
-  int64_t cost = 0, begin = 0, end = 0;            // of the call; of the tile
+  Cost cost = 0, begin = 0, end = 0;               // of the call; of the tile
   // cost of a head of sequence b, not listed
   const auto cost_of = [&](int b, int& row, int& tokens, int& reach) {
     tokens = min(tokens_of(p, b, row), kT);
-    if (tokens == 0) return 0;
     reach = keys_of(p, b);
     int n = ceil_div(reach, kUnit);
-    if (selected) n = min(n, ceil_div(p.usual * (3 + tokens), 8));
-    return kStart + n;
+    if (kSelected) n = min(n, ceil_div(p.usual * (3 + tokens), 8));
+    return tokens ? kStart + n : 0;
   };
   if (kListed) {
     n_tiles = p.first_tile[gridDim.x];
-    cost = p.start[n_tiles];
+    cost = (Cost)p.start[n_tiles];
   } else {
-    for (int base = 0; base < p.batch; base += 32) {
+    int sum = 0;
+    for (int base = lane; base < p.batch; base += 32) {
       int r, t, k;
-      if (base + lane < p.batch) cost += cost_of(base + lane, r, t, k);
+      sum += cost_of(base, r, t, k);
     }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) cost += __shfl_xor_sync(0xFFFFFFFFu, cost, d);
-    cost *= p.heads_k;
+    cost = __reduce_add_sync(0xFFFFFFFFu, sum) * p.heads_k;
   }
-  const Shares shares(max(cost, (int64_t)1), gridDim.x, p.least_share);
+  const Shares<Cost> shares(max(cost, (Cost)1), gridDim.x, p.least_share);
   const int me = blockIdx.x;
-  const int64_t lo = me < shares.grid ? shares.begin(me) : cost, hi = me < shares.grid ? shares.begin(me + 1) : cost;
+  const Cost lo = me < shares.grid ? shares.begin(me) : cost, hi = me < shares.grid ? shares.begin(me + 1) : cost;
   int each = 0;                                    // cost of the sequence's heads
-  bool more = lo < hi && cost > 0;
+  bool more = lo < hi;
   if (more) {
     if (kListed) {
       tile = p.first_tile[me];
@@ -253,13 +250,13 @@ __device__ __forceinline__ void fetch(const AttnParams& p, const CUtensorMap* k_
       for (int base = 0;; base += 32) {            // the sequence that lo lies in
         int r = 0, t = 0, k = 0, c = 0;
         if (base + lane < p.batch) c = cost_of(base + lane, r, t, k);
-        int64_t upto = (int64_t)c * p.heads_k;
+        int upto = c * p.heads_k;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-          const int64_t o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+          const int o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
           if (lane >= d) upto += o;
         }
-        const uint32_t past = __ballot_sync(0xFFFFFFFFu, begin + upto > lo);
+        const uint32_t past = __ballot_sync(0xFFFFFFFFu, (int)begin + upto > (int)lo);
         if (past) {
           const int src = __ffs(past) - 1;
           b = base + src;
@@ -267,9 +264,9 @@ __device__ __forceinline__ void fetch(const AttnParams& p, const CUtensorMap* k_
           tokens = __shfl_sync(0xFFFFFFFFu, t, src);
           reach = __shfl_sync(0xFFFFFFFFu, k, src);
           each = __shfl_sync(0xFFFFFFFFu, c, src);
-          begin += __shfl_sync(0xFFFFFFFFu, upto, src) - (int64_t)each * p.heads_k;
-          head = (int)((uint32_t)min(lo - begin, (int64_t)0x7FFFFFFF) / (uint32_t)each);
-          begin += (int64_t)head * each;
+          begin += __shfl_sync(0xFFFFFFFFu, upto, src) - each * p.heads_k;
+          head = (int)((uint32_t)(lo - begin) / (uint32_t)each);
+          begin += head * each;
           break;
         }
         begin += __shfl_sync(0xFFFFFFFFu, upto, 31);
@@ -287,14 +284,14 @@ __device__ __forceinline__ void fetch(const AttnParams& p, const CUtensorMap* k_
       end = begin + each;
     }
     // the part of the tile that lies in this share, in units of the estimate
-    const int64_t s0 = begin + kStart;
+    const Cost s0 = begin + kStart;
     const int est = (int)(end - s0);
-    const int est_a = (int)min(max(lo - s0, (int64_t)0), (int64_t)est), est_z = (int)min(max(hi - s0, (int64_t)est_a), (int64_t)est);
+    const int est_a = (int)min(max(lo - s0, (Cost)0), (Cost)est), est_z = (int)min(max(hi - s0, (Cost)est_a), (Cost)est);
     const int blocks = ceil_div(reach, kBlockN);
     // the tile's blocks: all, or those that its tokens select, 4 words of their union per lane
     unsigned long long u[4] = {0, 0, 0, 0};
     int upto = 0, total = blocks;
-    if (selected) {
+    if (kSelected) {
       if (p.lists) {
         __syncwarp();
         for (int i = lane; i < tokens * kMaxMaskWords; i += 32) s.words[i / kMaxMaskWords][i % kMaxMaskWords] = 0;
@@ -329,8 +326,11 @@ __device__ __forceinline__ void fetch(const AttnParams& p, const CUtensorMap* k_
     }
     const int units = ceil_div(total, 2);
     // (a tile's cost is an estimate where blocks are selected: parts are in proportion)
-    const int a = est == units ? est_a : est ? (int)((int64_t)est_a * units / est) : 0;
-    const int z = est == units ? est_z : est ? (int)((int64_t)est_z * units / est) : 0;
+    int a = est_a, z = est_z;
+    if (kSelected && est != units) {
+      a = est ? (int)((int64_t)est_a * units / est) : 0;
+      z = est ? (int)((int64_t)est_z * units / est) : 0;
+    }
     const bool whole = lo <= begin && hi >= end;
     if (first && me > 0 && begin < lo && begin >= shares.begin(me - 1)) {
       int last = me;
@@ -347,7 +347,7 @@ __device__ __forceinline__ void fetch(const AttnParams& p, const CUtensorMap* k_
       ++items;
     }
     const auto nth_block = [&](int k) {            // all lanes, each with its k
-      if (!selected) return k;
+      if (!kSelected) return k;
       int at = 0;                                  // lane whose words hold it: the first with upto > k
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1)
@@ -399,9 +399,13 @@ __device__ __forceinline__ void fetch(const AttnParams& p, const CUtensorMap* k_
       r.pos = block * kBlockN;
       r.valid = k0 + lane < total ? min(kBlockN, reach - r.pos) : 0;
       r.k_scale = q8::scale_value(kb);
-      r.e_v = vb == kNanByte ? kNanByte : vb - 127;
+      r.e_v = r.valid == 0 ? kNoScale : vb == kNanByte ? kNanScale : vb - 127;
+      const bool has = r.e_v != kNanScale && r.e_v != kNoScale;
+      const int e_most = has ? r.e_v : kNoScale, e_least = has ? r.e_v : -kNoScale;
+      r.e_unit = (max(e_most, __shfl_xor_sync(0xFFFFFFFFu, e_most, 1)) & 0xFFFF) |
+                 min(e_least, __shfl_xor_sync(0xFFFFFFFFu, e_least, 1)) << 16;
       r.tokens = (1u << tokens) - 1;
-      if (selected && kT > 1) {
+      if (kSelected && kT > 1) {
         r.tokens = 0;
         const unsigned long long* m = p.mask + ((int64_t)head * p.total_q + row) * p.words + (block >> 6);
         for (int i = 0; i < tokens; ++i) {

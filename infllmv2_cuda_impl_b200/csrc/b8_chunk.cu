@@ -2,12 +2,17 @@
 // shares: b8_attn.cuh).
 //
 // Eight tokens x 16 heads are the M side:
-//     S (128 rows x 128 keys)      = [Q1 + Q2] . K^T         both K-major in shared memory, two products into one sum
-//     O (128 rows x 128 features) += [W1 + W2 + W3] . V      W in TMEM (four codes per word), V MN-major as it lies
+//     S (128 rows x 128 keys)      = [Q1 + Q2] . K^T     codes as they lie, two products into one sum (kind::f8f6f4)
+//     O (128 rows x 128 features) += W . V               fp16 weights in TMEM, values made fp16 by four warps (kind::f16)
+// Here the weights are many (128 x 128 per unit) and the values' codes are not: three 8-bit terms of every weight cost the
+// softmax 3.75 instructions for a weight of 6, conversion of V costs 0.75 per code and is shared by all rows.  (For one or two
+// tokens it is the other way round, b8_decode.cu.)  fp16 holds a weight to 2^-12 and down to 2^-24.
+//
 // Units go to two groups of four softmax warps in turn (thread = row).  Each group has a score buffer, its weights over
 // the scores, and sums of its own (M, l, O), so that neither waits for the other; the two are put together at the end
 // of the tile.  TMEM: two S and two O of 128 columns, all there is.  Warps: 0 looks blocks up and issues TMA, 1 issues
-// MMAs (in order: a group's next scores come behind the product that reads its weights), 2..5 and 6..9 are the groups.
+// MMAs (in order: a group's next scores come behind the product that reads its weights), 2..5 and 6..9 are the groups,
+// 10..13 convert values.
 #include "b8_attn.cuh"
 
 namespace ifv2 {
@@ -16,28 +21,70 @@ namespace {
 using namespace b8;
 
 constexpr int kT = 8, kRows = kT * kGroup;
-constexpr int kThreads = 320, kSoftmax = 256;
-constexpr int kStages = 5;
+constexpr int kThreads = 448, kSoftmax = 256;
+constexpr int kStages = 3;
 constexpr int kQBytes = kRows * kHeadDim;         // one of two terms
-constexpr int kRing = 2 * kQBytes, kSmem = kRing + kStages * 2 * kTileBytes + 1024;
+constexpr int kVBytes = kUnit * kHeadDim * 2;     // fp16 values of a unit: two halves of 64 features, a row per key
+constexpr int kV = 2 * kQBytes, kRing = kV + 2 * kVBytes, kSmem = kRing + kStages * 2 * kTileBytes + 1024;
+// a new reference puts the largest weight at 2^kFirst; it moves when a unit's weights add up to more than kMost
+constexpr float kFirst = 4.f, kMost = 32768.f;
 
-template <int kCode, bool kListed>
+// Instruction descriptor, kind::f16 with fp16 operands, B MN-major.
+constexpr uint32_t kIdescValues = (1u << 4) | (1u << 16) | (128u >> 3 << 17) | (128u >> 4 << 24);
+
+// A row's 128 weights as fp16 pairs, and their sums by block.
+__device__ __forceinline__ void weights(uint32_t scores, uint32_t (&w)[64], float (&sum)[2], const int (&seen)[2], const float (&c)[2],
+                                        const float (&ev)[2], float m, bool all) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const float b = ev[h] - m;
+    const uint64_t b2 = pack_f32x2(b, b), c2 = pack_f32x2(c[h], c[h]);
+    uint64_t sum2 = 0, sum2b = 0;
+#pragma unroll
+    for (int j0 = 0; j0 < kBlockN; j0 += 32) {
+      uint32_t x[32];
+      tmem_ld32_wait(scores + h * kBlockN + j0, x);
+      if (!all) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (j0 + j >= seen[h]) x[j] = 0xFF800000u;
+      }
+#pragma unroll
+      for (int j = 0; j < 32; j += 4) {
+        float y[4];
+        unpack_f32x2(fma_f32x2(pack_f32x2(x[j], x[j + 1]), c2, b2), y[0], y[1]);
+        unpack_f32x2(fma_f32x2(pack_f32x2(x[j + 2], x[j + 3]), c2, b2), y[2], y[3]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = ex2(y[e]);
+        sum2 = add_f32x2(sum2, pack_f32x2(y[0], y[1]));
+        sum2b = add_f32x2(sum2b, pack_f32x2(y[2], y[3]));
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[32 * h + (j0 + j) / 2]) : "f"(y[1]), "f"(y[0]));
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[32 * h + (j0 + j) / 2 + 1]) : "f"(y[3]), "f"(y[2]));
+      }
+    }
+    float s0, s1;
+    unpack_f32x2(add_f32x2(sum2, sum2b), s0, s1);
+    sum[h] = s0 + s1;
+  }
+}
+
+template <int kCode, bool kListed, bool kSelected>
 __global__ void __launch_bounds__(kThreads, 1)
 b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const AttnParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   __shared__ Common<kT, kStages> s;
-  __shared__ uint64_t bar_s[2], bar_p[2], bar_pv[2], bar_q, bar_drain;
+  __shared__ uint64_t bar_s[2], bar_p[2], bar_pv[2], bar_v[2], bar_q, bar_drain;
   __shared__ float s_c[kRows], s_top[2][kRows], s_lse[2][kRows];       // row's factor; a group's M and log2 of its sum
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   volatile int* gave_up = &s.gave_up;
 
   if (tid == 0) {
     s.gave_up = 0;
-    for (int i = 0; i < kStages; ++i) mbar_init(&s.full[i], 1), mbar_init(&s.empty[i], 1);
+    for (int i = 0; i < kStages; ++i) mbar_init(&s.full[i], 1), mbar_init(&s.empty[i], 9);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar_s[i], 1), mbar_init(&bar_p[i], 4), mbar_init(&bar_pv[i], 1);
-      mbar_init(&s.item_full[i], 1), mbar_init(&s.item_empty[i], 9);
+      mbar_init(&bar_s[i], 1), mbar_init(&bar_p[i], 4), mbar_init(&bar_pv[i], 1), mbar_init(&bar_v[i], 4);
+      mbar_init(&s.item_full[i], 1), mbar_init(&s.item_empty[i], 13);
     }
     mbar_init(&bar_q, 8);
     mbar_init(&bar_drain, 1);
@@ -57,28 +104,24 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
   const uint32_t tmem = s.tmem;                    // S of group g at 128 g, O at 256 + 128 g
 
   if (warp == 0) {
-    fetch<kT, kStages, kListed>(p, &k_map, &v_map, s, smem + kRing);
+    fetch<kT, kStages, kListed, kSelected>(p, &k_map, &v_map, s, smem + kRing);
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMAs
     if (elect_one()) {
       const uint32_t base = smem_u32(smem);
       constexpr uint32_t kIdescS = umma_idesc_f8(128, 128, kE4m3, kCode, false, false);
-      constexpr uint32_t kIdescO = umma_idesc_f8(128, 128, kE5m2, kCode, false, true);
       bool ok = true;
       int n = 0, queries = 0;
       const auto values = [&](int unit, bool first) {        // O += W V of a unit
-        const int stage = unit % kStages, g = unit & 1;
-        ok = ok && bounded_wait(&bar_p[g], (unit >> 1) & 1, gave_up);
+        const int g = unit & 1;
+        ok = ok && bounded_wait(&bar_p[g], (unit >> 1) & 1, gave_up) && bounded_wait(&bar_v[g], (unit >> 1) & 1, gave_up);
         if (!ok) return;
         tc_fence_after();
-        const uint32_t v = base + kRing + stage * 2 * kTileBytes + kTileBytes;
+        const uint32_t v = base + kV + g * kVBytes;
 #pragma unroll
-        for (int i = 0; i < 3; ++i)
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            umma_f8_ts(tmem + 256 + 128 * g, tmem + 128 * g + 32 * i + 8 * kk, umma_desc_sw128(v + kk * 4096, 16, 1024), kIdescO,
-                       !first || i + kk > 0);
-        umma_commit(&s.empty[stage]);
+        for (int kk = 0; kk < 8; ++kk)
+          umma_ts(tmem + 256 + 128 * g, tmem + 128 * g + 8 * kk, umma_desc_sw128(v + kk * 2048, kVBytes / 2, 1024), kIdescValues,
+                  !first || kk > 0);
         umma_commit(&bar_pv[g]);
       };
       for (int item = 0; ok; ++item) {
@@ -100,6 +143,7 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
             for (int kk = 0; kk < 4; ++kk)
               umma_f8_ss(tmem + 128 * (n & 1), umma_desc_sw128(base + j * kQBytes + kk * 32, 16, 1024), umma_desc_sw128(k + kk * 32, 16, 1024),
                          kIdescS, j + kk > 0);
+          umma_commit(&s.empty[stage]);
           umma_commit(&bar_s[n & 1]);
           if (i > 0) values(n - 1, i <= 2);
         }
@@ -111,6 +155,52 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
       }
     }
     __syncwarp();
+  } else if (warp >= 10) {
+    // ---------------------------------------------------------------- values to fp16
+    // A thread has 16 features of every 16th key.
+    const int ctid = tid - 320, c = ctid & 7;
+    int n = 0;
+    for (int item = 0;; ++item) {
+      if (!bounded_wait_warp(&s.item_full[item & 1], (item >> 1) & 1, gave_up)) break;
+      const int units = s.item[item & 1].units;
+      if (units < 0) break;
+      mbar_arrive_warp(&s.item_empty[item & 1]);
+      for (int i = 0; i < units; ++i, ++n) {
+        const int stage = n % kStages, g = n & 1;
+        bounded_wait_warp(&s.full[stage], (n / kStages) & 1, gave_up);
+        const int valid[2] = {s.block[stage][0].valid, s.block[stage][1].valid};
+        const uint8_t* from = smem + kRing + stage * 2 * kTileBytes + kTileBytes;
+        uint8_t* to = smem + kV + g * kVBytes + (c >> 2) * (kVBytes / 2);
+        if (n >= 2) bounded_wait_warp(&bar_pv[g], ((n - 2) >> 1) & 1, gave_up);      // the buffer is free again
+#pragma unroll
+        for (int j = 0; j < kUnit / 16; ++j) {
+          const int row = j * 16 + (ctid >> 3), at = row & 7;
+          uint4 x = *reinterpret_cast<const uint4*>(from + row * kHeadDim + ((c ^ at) << 4));
+          // a value row that is no key may hold anything: 0 x NaN
+          if ((row & 63) >= (row < kBlockN ? valid[0] : valid[1])) x = make_uint4(0, 0, 0, 0);
+          uint32_t h[8];
+          const uint32_t* w = reinterpret_cast<const uint32_t*>(&x);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (kCode == kE4m3) {
+              asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+                  : "=r"(h[2 * k]), "=r"(h[2 * k + 1]) : "r"(w[k]));
+            } else {                               // the upper bytes of fp16 numbers
+              h[2 * k] = __byte_perm(w[k], 0u, 0x1404);
+              h[2 * k + 1] = __byte_perm(w[k], 0u, 0x3424);
+            }
+          }
+          // (the two halves lie in the same banks: one's even pieces are written beside the other's odd ones)
+          const int first = (c & 3) * 2 + (c >> 2), second = first ^ 1;
+          const bool odd = c >> 2;
+          *reinterpret_cast<uint4*>(to + row * 128 + ((first ^ at) << 4)) = odd ? make_uint4(h[4], h[5], h[6], h[7]) : make_uint4(h[0], h[1], h[2], h[3]);
+          *reinterpret_cast<uint4*>(to + row * 128 + ((second ^ at) << 4)) = odd ? make_uint4(h[0], h[1], h[2], h[3]) : make_uint4(h[4], h[5], h[6], h[7]);
+        }
+        fence_proxy_async_smem();
+        mbar_arrive_warp(&bar_v[g]);
+        mbar_arrive_warp(&s.empty[stage]);
+      }
+    }
   } else {
     // ---------------------------------------------------------------- softmax
     // A wait that gave up only makes the results NaN: within an item every thread keeps to the same loops and barriers.
@@ -149,6 +239,22 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
       mbar_arrive_warp(&s.item_empty[item & 1]);
     };
 
+    // O times f, once the group's product before unit n has been made
+    const auto rescale = [&](float f, bool begun, int n) {
+      if (!begun) return;
+      bounded_wait_warp(&bar_pv[group], ((n - 2) >> 1) & 1, gave_up);
+      tc_fence_after();
+#pragma unroll 1
+      for (int c0 = 0; c0 < kHeadDim; c0 += 16) {
+        uint32_t o[16];
+        tmem_ld16(my_o + c0, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+        tmem_st16(my_o + c0, o);
+      }
+    };
+
     int n0 = 0;                                    // units of earlier items
     next_item(0);
     if (next.units > 0) write_query(next);
@@ -156,7 +262,10 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
     for (int item = 0; next.units >= 0; ++item) {
       const Item t = next;
       const int tok = r / kGroup;
-      const int limit = tok < t.tokens ? (p.causal ? t.reach - (t.tokens - 1 - tok) : t.reach) : 0;      // keys that the row sees
+      // keys that the row sees; rows of tokens that the tile does not have see what the last one does, for nobody
+      const int limit = tok < t.tokens && p.causal ? t.reach - (t.tokens - 1 - tok) : t.reach;
+      const uint32_t bit = 1u << min(tok, t.tokens - 1);
+      const bool idle = 2 * quad >= t.tokens;      // nor does the warp have another
       const float c_row = s_c[r];
       const bool c_nan = !(c_row == c_row);
       float m = kUnset, l = 0.f;                   // M, the sum in units of 2^(M - E)
@@ -166,14 +275,14 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
         const int n = n0 + i, stage = n % kStages;
         bounded_wait_warp(&s.full[stage], (n / kStages) & 1, gave_up);
         const Block blk[2] = {s.block[stage][0], s.block[stage][1]};
+        mbar_arrive_warp(&s.empty[stage]);
         int seen[2], e_blk[2];
         float c[2], ev[2], dv[2];
-        int e_new = e_ref;
+        int e_new = max(e_ref, (int)(int16_t)blk[0].e_unit);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          seen[h] = (blk[h].tokens >> tok) & 1 ? max(min(limit - blk[h].pos, blk[h].valid), 0) : 0;
-          e_blk[h] = blk[h].valid > 0 && blk[h].e_v != kNanByte ? blk[h].e_v : kNoScale;
-          e_new = max(e_new, e_blk[h]);
+          seen[h] = (blk[h].tokens & bit) ? max(min(limit - blk[h].pos, blk[h].valid), 0) : 0;
+          e_blk[h] = blk[h].e_v == kNanScale ? kNoScale : blk[h].e_v;
           c[h] = fmaxf(c_row * blk[h].k_scale, 1e-37f);        // (-inf of a masked key times 0 would be NaN)
         }
         if (e_new == kNoScale) e_new = 0;
@@ -195,100 +304,71 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
         }
         bounded_wait_warp(&bar_s[group], (n >> 1) & 1, gave_up);
         tc_fence_after();
-        uint32_t x[2][64];
-        tmem_ld64_wait(my_s, x[0]);
-        tmem_ld64_wait(my_s + 64, x[1]);
-        if (!__all_sync(0xFFFFFFFFu, seen[0] == kBlockN && seen[1] == kBlockN)) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int j = 0; j < 64; ++j)
-              if (j >= seen[h]) x[h][j] = 0xFF800000u;
+        if (idle) {                                // (what lies in its rows stays in its rows)
+          tc_fence_before();
+          mbar_arrive_warp(&bar_p[group]);
+          continue;
         }
-        float top = -INFINITY;
-        bool odd = false;
+        const bool all = __all_sync(0xFFFFFFFFu, seen[0] == kBlockN && seen[1] == kBlockN);
+        bool odd = c_nan;                          // a NaN among the row's numbers, or values too small beside the others'
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float a = __uint_as_float(x[h][0]), b = __uint_as_float(x[h][1]);
-#pragma unroll
-          for (int j = 2; j < 64; j += 4) {
-            a = fmaxf(fmaxf(a, __uint_as_float(x[h][j])), __uint_as_float(x[h][j + 1]));
-            if (j + 2 < 64) b = fmaxf(fmaxf(b, __uint_as_float(x[h][j + 2])), __uint_as_float(x[h][j + 3]));
-          }
-          const bool k_nan = !(blk[h].k_scale == blk[h].k_scale);
-          odd |= k_nan || c_nan || (seen[h] > 0 && (blk[h].e_v == kNanByte || e_blk[h] - e_ref < kDeepest));
-          if (!k_nan && !c_nan) top = fmaxf(top, fmaf(fmaxf(a, b), c[h], ev[h]));
-        }
-        const bool moves = top - m > kRoom;
+        for (int h = 0; h < 2; ++h)
+          odd |= !(blk[h].k_scale == blk[h].k_scale) || blk[h].e_v == kNanScale || (e_blk[h] > kNoScale && e_blk[h] - e_ref < kDeepest);
+        odd = __any_sync(0xFFFFFFFFu, odd);
         __syncwarp();
-        if (__any_sync(0xFFFFFFFFu, moves || back != 1.f)) {
-          float f = back;
-          if (moves) {
-            f = m == kUnset ? 0.f : f * ex2(m - (top - kTop));
-            l = l > 0.f ? l * (m == kUnset ? 0.f : ex2(m - (top - kTop))) : l;
-            m = top - kTop;
+        if (__any_sync(0xFFFFFFFFu, back != 1.f)) rescale(back, begun, n);
+        uint32_t w[64];                            // fp16 pairs
+        float sum[2];
+        weights(my_s, w, sum, seen, c, ev, m, all);
+        if (__any_sync(0xFFFFFFFFu, !(sum[0] + sum[1] <= kMost)) || odd) {
+          // the row's largest score: a new reference where it is far above the old one
+          float top = -INFINITY;
+#pragma unroll 1
+          for (int j0 = 0; j0 < kUnit; j0 += 16) {
+            uint32_t x[16];
+            tmem_ld16(my_s + j0, x);
+            tmem_wait_ld();
+            const int h = j0 >> 6, see = (h ? seen[1] : seen[0]) - (j0 & 63);
+            float a = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (j < see) a = fmaxf(a, __uint_as_float(x[j]));
+            const float scale = h ? blk[1].k_scale : blk[0].k_scale;
+            if (scale == scale && !c_nan) top = fmaxf(top, fmaf(a, h ? c[1] : c[0], h ? ev[1] : ev[0]));
+          }
+          float f = 1.f;
+          if (top - m > kFirst) {                  // (where the sum alone is large, it moves too)
+            f = m == kUnset ? 0.f : ex2(m - (top - kFirst));
+            l = l > 0.f ? l * f : l;
+            m = top - kFirst;
           }
           __syncwarp();
-          if (begun) {
-            bounded_wait_warp(&bar_pv[group], ((n - 2) >> 1) & 1, gave_up);
-            tc_fence_after();
+          rescale(f, begun, n);
+          weights(my_s, w, sum, seen, c, ev, m, all);
+          if (odd) {
 #pragma unroll
-            for (int c0 = 0; c0 < kHeadDim; c0 += 16) {
-              uint32_t o[16];
-              tmem_ld16(my_o + c0, o);
-              tmem_wait_ld();
+            for (int h = 0; h < 2; ++h) {
+              const bool nan_key = c_nan || !(blk[h].k_scale == blk[h].k_scale), nan_value = blk[h].e_v == kNanScale;
+              const bool none = !nan_value && e_blk[h] > kNoScale && e_blk[h] - e_ref < kDeepest;
+              if (nan_key) sum[h] = seen[h] > 0 ? NAN : 0.f;
 #pragma unroll
-              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-              tmem_st16(my_o + c0, o);
+              for (int j = 0; j < 32; ++j) {
+                const uint32_t here = (2 * j < seen[h] ? 0xFFFFu : 0u) | (2 * j + 1 < seen[h] ? 0xFFFF0000u : 0u);
+                if (nan_key || nan_value) w[32 * h + j] = here & 0x7FFF7FFFu;
+                else if (none) w[32 * h + j] = 0u;
+              }
             }
           }
         }
         begun = true;
-        odd = __any_sync(0xFFFFFFFFu, odd);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float b = ev[h] - m;
-          const uint64_t b2 = pack_f32x2(b, b), c2 = pack_f32x2(c[h], c[h]);
-          uint64_t sum2 = 0, sum2b = 0;
-          uint32_t t0[16], t1[16], t2[16];
-          const bool nan_key = c_nan || !(blk[h].k_scale == blk[h].k_scale), nan_value = blk[h].e_v == kNanByte;
-          const bool none = !nan_value && e_blk[h] - e_ref < kDeepest;      // values too small to be seen beside the others'
+        for (int j = 0; j < 64; j += 16) {
+          uint32_t part[16];
 #pragma unroll
-          for (int j = 0; j < 64; j += 4) {
-            float w[4];
-            unpack_f32x2(fma_f32x2(pack_f32x2(x[h][j], x[h][j + 1]), c2, b2), w[0], w[1]);
-            unpack_f32x2(fma_f32x2(pack_f32x2(x[h][j + 2], x[h][j + 3]), c2, b2), w[2], w[3]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = ex2(w[e]);
-            if (odd) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (nan_key) w[e] = j + e < seen[h] ? NAN : 0.f;
-            }
-            sum2 = add_f32x2(sum2, pack_f32x2(w[0], w[1]));
-            sum2b = add_f32x2(sum2b, pack_f32x2(w[2], w[3]));
-            if (odd) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                if (nan_value) w[e] = j + e < seen[h] ? NAN : 0.f;
-                if (none) w[e] = w[e] == w[e] ? 0.f : w[e];
-              }
-            }
-            split4(w[0], w[1], w[2], w[3], t0[j / 4], t1[j / 4], t2[j / 4]);
-          }
-          tmem_st16(my_s + 16 * h, t0);
-          tmem_st16(my_s + 32 + 16 * h, t1);
-          tmem_st16(my_s + 64 + 16 * h, t2);
-          float s0, s1;
-          unpack_f32x2(add_f32x2(sum2, sum2b), s0, s1);
-          l += (s0 + s1) * ex2(-dv[h]);
+          for (int k = 0; k < 16; ++k) part[k] = w[j + k];
+          tmem_st16(my_s + j, part);
         }
-        if ((r & 63) >= (r < kBlockN ? blk[0].valid : blk[1].valid)) {       // a value row that is no key may hold anything: 0 x NaN
-          uint4* row = reinterpret_cast<uint4*>(smem + kRing + stage * 2 * kTileBytes + kTileBytes + r * kHeadDim);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) row[j] = make_uint4(0, 0, 0, 0);
-        }
-        fence_proxy_async_smem();
+        l += sum[0] * ex2(-dv[0]) + sum[1] * ex2(-dv[1]);
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive_warp(&bar_p[group]);
@@ -362,19 +442,25 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
   if (warp == 1) tmem_dealloc(s.tmem, 512);
 }
 
-template <int kCode, bool kListed>
+template <int kCode, bool kListed, bool kSelected>
 int launch(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttnParams& p, cudaStream_t stream) {
-  const cudaError_t e = cudaFuncSetAttribute(b8_chunk_kernel<kCode, kListed>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  const cudaError_t e = cudaFuncSetAttribute(b8_chunk_kernel<kCode, kListed, kSelected>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return set_error((int)e, "b8_attn: %s", cudaGetErrorString(e));
-  b8_chunk_kernel<kCode, kListed><<<kB8ChunkGrid, kThreads, kSmem, stream>>>(k_map, v_map, p);
+  b8_chunk_kernel<kCode, kListed, kSelected><<<kB8ChunkGrid, kThreads, kSmem, stream>>>(k_map, v_map, p);
   return check_launch("b8_attn");
+}
+
+template <int kCode>
+int launch_with(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttnParams& p, bool listed, cudaStream_t stream) {
+  const bool selected = p.mask != nullptr || p.lists != nullptr;
+  if (listed) return selected ? launch<kCode, true, true>(k_map, v_map, p, stream) : launch<kCode, true, false>(k_map, v_map, p, stream);
+  return selected ? launch<kCode, false, true>(k_map, v_map, p, stream) : launch<kCode, false, false>(k_map, v_map, p, stream);
 }
 
 }  // namespace
 
 int b8_launch_chunk(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttnParams& p, bool listed, int code, cudaStream_t stream) {
-  if (listed) return code == kE4m3 ? launch<kE4m3, true>(k_map, v_map, p, stream) : launch<kE5m2, true>(k_map, v_map, p, stream);
-  return code == kE4m3 ? launch<kE4m3, false>(k_map, v_map, p, stream) : launch<kE5m2, false>(k_map, v_map, p, stream);
+  return code == kE4m3 ? launch_with<kE4m3>(k_map, v_map, p, listed, stream) : launch_with<kE5m2>(k_map, v_map, p, listed, stream);
 }
 
 }  // namespace ifv2

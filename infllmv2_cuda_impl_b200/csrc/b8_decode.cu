@@ -1,12 +1,13 @@
 // Attention over 8-bit blocks for one or two new tokens per sequence (formulas, operands and shares: b8_attn.cuh).
 //
 // Keys are the M side of both products, so that few query rows cost few tensor clocks:
-//     S^T (128 keys x 2 x 16 kT)        = K . [Q1 Q2]^T     the query's two terms side by side, added by the softmax
-//     O^T (128 features x 3 x 16 kT)   += V^T . [W1 W2 W3]  V is MN-major as it lies; W is written [key][column]
+//     S^T (128 keys x 16 kT)            = K . [Q1 + Q2]^T   the query's two terms one after the other
+//     O^T (128 features x 3 x 16 kT)   += V^T . [W1 W2 W3]  V is MN-major as it lies; W is written [key][column], its terms
+//                                                           side by side, so that four MMAs serve all of them: the next
+//                                                           unit's weights wait for this product, not for the scores
 // A softmax thread has a key of its own, with the tile's columns in registers: a decode step's exponentials are spread
-// over all lanes.  One A operand then serves all terms of the other side (4 MMAs for each product of a unit; term by
-// term they were 8 and 12, and A is what they cost).  Warps: 0 looks blocks up and issues TMA, 1 issues MMAs, 2..5 are
-// the softmax (thread = key = feature).  Two CTAs per SM.
+// over all lanes.  Warps: 0 looks blocks up and issues TMA, 1 issues MMAs, 2..5 are the softmax (thread = key =
+// feature).  Two CTAs per SM.
 #include "b8_attn.cuh"
 
 namespace ifv2 {
@@ -24,20 +25,14 @@ struct Shape {
   static constexpr int kPBytes = kN * kUnit;       // one of three terms
   static constexpr int kQ = 0, kP = 2 * kQBytes, kRing = (kP + 3 * kPBytes + 1023) / 1024 * 1024;
   static constexpr int kSmem = kRing + kStages * 2 * kTileBytes + 1024;
-  static constexpr int kO = 4 * kN;                // columns of O behind two S
+  static constexpr int kO = 2 * kN;                // columns of O behind two S
   static constexpr int kTmem = kT == 1 ? 128 : 256;
 };
 
-// Floats as integers of the same order, for redux.
-__device__ __forceinline__ int ordered(float x) {
-  const int i = __float_as_int(x);
-  return i ^ ((i >> 31) & 0x7FFFFFFF);
-}
-__device__ __forceinline__ float from_ordered(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7FFFFFFF)); }
-
-// Column sums over the 32 lanes: half the columns go to the other lane in each step.  Column `first` is in v[0] at the end.
-template <int kN>
-__device__ __forceinline__ int column_sums(float (&v)[kN], int lane) {
+// Column sums (or maxima) over the 32 lanes: half the columns go to the other lane in each step.  Column `first` is in v[0]
+// at the end.
+template <bool kMax, int kN>
+__device__ __forceinline__ int reduce_columns(float (&v)[kN], int lane) {
   int first = 0;
   int n = kN;
 #pragma unroll
@@ -49,17 +44,19 @@ __device__ __forceinline__ int column_sums(float (&v)[kN], int lane) {
       for (int i = 0; i < kN / 2; ++i) {
         if (i >= n) continue;
         const float mine = up ? v[i + n] : v[i], other = up ? v[i] : v[i + n];
-        v[i] = mine + __shfl_xor_sync(0xFFFFFFFFu, other, s);
+        const float got = __shfl_xor_sync(0xFFFFFFFFu, other, s);
+        v[i] = kMax ? fmaxf(mine, got) : mine + got;
       }
       if (up) first += n;
     } else {
-      v[0] += __shfl_xor_sync(0xFFFFFFFFu, v[0], s);
+      const float got = __shfl_xor_sync(0xFFFFFFFFu, v[0], s);
+      v[0] = kMax ? fmaxf(v[0], got) : v[0] + got;
     }
   }
   return first;
 }
 
-template <int kT, int kCode>
+template <int kT, int kCode, bool kSelected>
 __global__ void __launch_bounds__(kThreads, 2)
 b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const AttnParams p) {
   using S = Shape<kT>;
@@ -98,12 +95,12 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
   const uint32_t tmem_s = s.tmem, tmem_o = s.tmem + S::kO;
 
   if (warp == 0) {
-    fetch<kT, kStages, false>(p, &k_map, &v_map, s, smem + S::kRing);
+    fetch<kT, kStages, false, kSelected>(p, &k_map, &v_map, s, smem + S::kRing);
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMAs
     if (elect_one()) {
       const uint32_t base = smem_u32(smem);
-      constexpr uint32_t kIdescS = umma_idesc_f8(128, 2 * kN, kCode, kE4m3, false, false);
+      constexpr uint32_t kIdescS = umma_idesc_f8(128, kN, kCode, kE4m3, false, false);
       constexpr uint32_t kIdescO = umma_idesc_f8(128, 3 * kN, kCode, kE5m2, true, true);
       bool ok = true;
       int n = 0, queries = 0;
@@ -134,9 +131,11 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
           tc_fence_after();
           const uint32_t k = base + S::kRing + stage * 2 * kTileBytes;
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            umma_f8_ss(tmem_s + (n & 1) * 2 * kN, umma_desc_sw128(k + kk * 32, 16, 1024), umma_desc_sw128(base + S::kQ + kk * 32, 16, 1024),
-                       kIdescS, kk > 0);
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_f8_ss(tmem_s + (n & 1) * kN, umma_desc_sw128(k + kk * 32, 16, 1024),
+                         umma_desc_sw128(base + S::kQ + j * S::kQBytes + kk * 32, 16, 1024), kIdescS, j + kk > 0);
           umma_commit(&bar_s[n & 1]);
           if (i > 0) values(n - 1, i == 1);
         }
@@ -172,7 +171,6 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
       }
       fence_proxy_async_smem();
       mbar_arrive_warp(&bar_q);
-      named_sync<kSoftmax>();
     };
     Item next;
     const auto next_item = [&](int item) {
@@ -190,145 +188,153 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
     if (next.units > 0) write_query(next);
     for (int item = 0; next.units >= 0; ++item) {
       const Item t = next;
-      float l[kN];
+      // in registers: the columns' factors, references and sums
+      float c[kN], mu[kN], l[kN];
+      named_sync<kSoftmax>();                      // s_c is written, the last item's s_fl and s_red are read
 #pragma unroll
-      for (int i = 0; i < kN; ++i) l[i] = 0.f;
+      for (int i = 0; i < kN; ++i) c[i] = s_c[i], mu[i] = kUnset, l[i] = 0.f;
       if (stid < kN) s_mu[stid] = kUnset;
-      named_sync<kSoftmax>();
       int e_ref = kNoScale, deepest = 0;           // E; least eV - E of the blocks so far
+#pragma unroll 1
       for (int i = 0; i < t.units; ++i, ++n) {
         const int stage = n % kStages;
         bounded_wait_warp(&s.full[stage], (n / kStages) & 1, gave_up);
+        const Block* blk = &s.block[stage][r >> 6];
+        const float k_scale = blk->k_scale;
+        const int e_v = blk->e_v, valid = blk->valid, e_unit = blk->e_unit, e_most = max(e_ref, (int)(int16_t)e_unit);
+        const int e_new = e_most == kNoScale ? 0 : e_most;
+        // which columns' tokens see the thread's key: the last token those below `valid`, the ones before it fewer if causal
+        const int left = valid - (r & 63);         // > 0: a key
+        uint32_t sees = left > 0 ? (1u << kT) - 1 : 0u;
+        if (kT > 1 && left > 0) {
+          const int in_reach = t.reach - (blk->pos + (r & 63));
+          sees = kSelected ? blk->tokens : sees;
+#pragma unroll
+          for (int tok = 0; tok < kT; ++tok)
+            if (p.causal && in_reach <= t.tokens - 1 - tok) sees &= ~(1u << tok);
+        }
+        const bool all = __all_sync(0xFFFFFFFFu, sees == (1u << kT) - 1);
+        // eV - E; a NaN block's weights are NaN, those of a block far below the others' nothing
+        const int dv = min(e_v - e_new, 0), dv_ref = max(dv, kDeepest);
+        const float v_ref = pow2i(dv_ref), v_scale = e_v == kNanScale ? NAN : dv < kDeepest ? 0.f : v_ref;
         bounded_wait_warp(&bar_s[n & 1], (n >> 1) & 1, gave_up);
         tc_fence_after();
-        float x[kN];
-        {
-          uint32_t y[2 * kN];
-          if constexpr (kN == 16) tmem_ld32_wait(tmem_s + (n & 1) * 2 * kN + lanes, y);
-          else tmem_ld64_wait(tmem_s + (n & 1) * 2 * kN + lanes, y);
+        float w[kN];
+        bool moves = e_new != e_ref, settled = false;
+        for (;;) {
+          uint32_t x[kN];
+          if constexpr (kN == 16) {
+            tmem_ld16(tmem_s + (n & 1) * kN + lanes, x);
+            tmem_wait_ld();
+          } else {
+            tmem_ld32_wait(tmem_s + (n & 1) * kN + lanes, x);
+          }
+          const uint64_t scale2 = pack_f32x2(k_scale, k_scale);
+          if (moves && !settled) {
+            // new references: the largest x + eV of each column, and E
+            const int delta = e_ref == kNoScale ? 0 : e_new - e_ref;
+            const int bump = max(kDeepest - (deepest - delta), 0);
+            deepest = max(deepest - delta, kDeepest);
+            const float up = (float)dv_ref;
 #pragma unroll
-          for (int c = 0; c < kN; ++c) x[c] = __uint_as_float(y[c]) + __uint_as_float(y[kN + c]);
+            for (int j = 0; j < kN; ++j) {
+              w[j] = fmaf(__uint_as_float(x[j]) * k_scale, c[j], up);
+              if (!((sees >> (j / kGroup)) & 1) || !(w[j] == w[j])) w[j] = -INFINITY;
+            }
+            const int first = reduce_columns<true, kN>(w, lane);
+            s_red[quad][first] = w[0];             // (16 columns: two lanes, one value)
+            named_sync<kSoftmax>();
+            if (stid < kN) {
+              const float top = fmaxf(fmaxf(s_red[0][stid], s_red[1][stid]), fmaxf(s_red[2][stid], s_red[3][stid]));
+              const float was = s_mu[stid];
+              float now = was, fl = 0.f, fo = 0.f;
+              if (was == kUnset) {
+                if (top > -INFINITY) now = top - kTop;
+              } else {
+                now = was + (float)(bump - delta);
+                if (top - now > kRoom) now = top - kTop;
+                fl = ex2(was - now);
+                fo = ex2(was - now - (float)delta);
+              }
+              s_mu[stid] = now;
+              s_fl[stid] = fl;
+              s_fo[stid] = fo;
+            }
+            named_sync<kSoftmax>();
+#pragma unroll
+            for (int j = 0; j < kN; ++j) {
+              mu[j] = s_mu[j];
+              l[j] = l[j] > 0.f ? l[j] * s_fl[j] : l[j];
+            }
+            if (i > 0) {                           // what is in O so far
+              bounded_wait_warp(&bar_pv, (n - 1) & 1, gave_up);
+              tc_fence_after();
+#pragma unroll 1
+              for (int c0 = 0; c0 < 3 * kN; c0 += 16) {
+                uint32_t o[16];
+                tmem_ld16(tmem_o + lanes + c0, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * s_fo[(kT == 1 ? 0 : c0 & 16) + j]);
+                tmem_st16(tmem_o + lanes + c0, o);
+              }
+              tmem_wait_st();
+            }
+            settled = true;
+          }
+#pragma unroll
+          for (int j = 0; j < kN; j += 2) {
+            float a, b;
+            unpack_f32x2(fma_f32x2(mul_f32x2(pack_f32x2(x[j], x[j + 1]), scale2), pack_f32x2(c[j], c[j + 1]), pack_f32x2(-mu[j], -mu[j + 1])), a, b);
+            w[j] = ex2(a);
+            w[j + 1] = ex2(b);
+          }
+          if (!all) {
+#pragma unroll
+            for (int j = 0; j < kN; ++j)
+              if (!((sees >> (j / kGroup)) & 1)) w[j] = 0.f;
+          }
+          if (settled) break;
+          float most = w[0];
+#pragma unroll
+          for (int j = 1; j < kN; j += 2) most = fmaxf(fmaxf(most, w[j]), w[j + 1 < kN ? j + 1 : j]);
+          moves = named_any<kSoftmax>(most * v_ref > 32768.f);
+          if (!moves) break;
         }
         tc_fence_before();
         mbar_arrive_warp(&bar_sfree[n & 1]);
-        const Block mine = s.block[stage][r >> 6], other = s.block[stage][(r >> 6) ^ 1];
-        const int e_mine = mine.valid > 0 && mine.e_v != kNanByte ? mine.e_v : kNoScale;
-        const int e_other = other.valid > 0 && other.e_v != kNanByte ? other.e_v : kNoScale;
-        int e_new = max(e_ref, max(e_mine, e_other));
-        if (e_new == kNoScale) e_new = 0;
-        const int in_block = r & 63;
-        const bool here = in_block < mine.valid;
-        // keys that token i sees end at position reach - (tokens - 1 - i) if causal, reach otherwise
-        const int left = t.reach - (mine.pos + in_block);      // > 0: the last token sees this key
-        const auto sees = [&](int tok) {
-          return here && ((mine.tokens >> tok) & 1) && (p.causal ? left > t.tokens - 1 - tok : left > 0);
-        };
-        const int dv = mine.e_v - e_new;                       // (of no interest without a key or in a NaN block)
-        const float v_scale = mine.e_v == kNanByte ? NAN : pow2i(dv), v_ref = pow2i(max(min(dv, 0), kDeepest));
-        float w[kN];
-        const auto weights = [&]() {
-          float most = 0.f;
-#pragma unroll
-          for (int tok = 0; tok < kT; ++tok) {
-            const bool see = sees(tok);
-#pragma unroll
-            for (int g = 0; g < kGroup; ++g) {
-              const int c = tok * kGroup + g;
-              const float y = ex2(fmaf(x[c], s_c[c] * mine.k_scale, -s_mu[c]));
-              w[c] = see ? y : 0.f;
-              most = fmaxf(most, w[c]);
-            }
-          }
-          return most;
-        };
-        bool moves = e_new != e_ref;
-        if (!moves) moves = named_any<kSoftmax>(weights() * v_ref > 32768.f);
-        if (moves) {
-          // new references: the largest x + eV of each column, and E
-          const int delta = e_ref == kNoScale ? 0 : e_new - e_ref;
-          const int bump = max(kDeepest - (deepest - delta), 0);
-          deepest = max(deepest - delta, kDeepest);
-          const float up = (float)max(min(dv, 0), kDeepest);
-#pragma unroll
-          for (int tok = 0; tok < kT; ++tok) {
-            const bool see = sees(tok);
-#pragma unroll
-            for (int g = 0; g < kGroup; ++g) {
-              const int c = tok * kGroup + g;
-              float y = fmaf(x[c], s_c[c] * mine.k_scale, up);
-              if (!see || !(y == y)) y = -INFINITY;
-              const int top = __reduce_max_sync(0xFFFFFFFFu, ordered(y));
-              if (lane == 0) s_red[quad][c] = from_ordered(top);
-            }
-          }
-          named_sync<kSoftmax>();
-          if (stid < kN) {
-            const float top = fmaxf(fmaxf(s_red[0][stid], s_red[1][stid]), fmaxf(s_red[2][stid], s_red[3][stid]));
-            const float mu = s_mu[stid];
-            float mu_new = mu, fl = 0.f, fo = 0.f;
-            if (mu == kUnset) {
-              if (top > -INFINITY) mu_new = top - kTop;
-            } else {
-              mu_new = mu + (float)(bump - delta);
-              if (top - mu_new > kRoom) mu_new = top - kTop;
-              fl = ex2(mu - mu_new);
-              fo = ex2(mu - mu_new - (float)delta);
-            }
-            s_mu[stid] = mu_new;
-            s_fl[stid] = fl;
-            s_fo[stid] = fo;
-          }
-          named_sync<kSoftmax>();
-#pragma unroll
-          for (int c = 0; c < kN; ++c) l[c] = l[c] > 0.f ? l[c] * s_fl[c] : l[c];
-          if (i > 0) {                             // what is in O so far
-            bounded_wait_warp(&bar_pv, (n - 1) & 1, gave_up);
-            tc_fence_after();
-#pragma unroll
-            for (int c0 = 0; c0 < 3 * kN; c0 += 16) {
-              uint32_t o[16];
-              tmem_ld16(tmem_o + lanes + c0, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * s_fo[c0 % kN + c]);
-              tmem_st16(tmem_o + lanes + c0, o);
-            }
-            tmem_wait_st();
-            tc_fence_before();
-          }
-          e_ref = e_new;
-          weights();
-        }
-        if (e_mine > kNoScale) deepest = max(min(deepest, e_mine - e_ref), kDeepest);
-        if (e_other > kNoScale) deepest = max(min(deepest, e_other - e_ref), kDeepest);
+        e_ref = e_new;
+        deepest = max(min(deepest, (e_unit >> 16) - e_ref), kDeepest);
         // the one buffer of weights is free again when the product before has been made
         if (n > 0) bounded_wait_warp(&bar_pv, (n - 1) & 1, gave_up);
 #pragma unroll
+        for (int j = 0; j < kN; ++j) l[j] += w[j];
+        if (!all && !(v_scale == v_scale)) {       // (only the columns that see the key are NaN)
+#pragma unroll
+          for (int j = 0; j < kN; ++j)
+            if ((sees >> (j / kGroup)) & 1) w[j] = NAN;
+        } else {
+#pragma unroll
+          for (int j = 0; j < kN; ++j) w[j] *= v_scale;
+        }
+#pragma unroll
         for (int tok = 0; tok < kT; ++tok) {
-          const bool see = sees(tok);
           uint32_t out[3][4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float y[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int c = tok * kGroup + 4 * j + e;
-              l[c] += w[c];
-              y[e] = see ? w[c] * v_scale : 0.f;
-            }
-            split4(y[0], y[1], y[2], y[3], out[0][j], out[1][j], out[2][j]);
-          }
+          for (int j = 0; j < 4; ++j)
+            split4(w[tok * 16 + 4 * j], w[tok * 16 + 4 * j + 1], w[tok * 16 + 4 * j + 2], w[tok * 16 + 4 * j + 3], out[0][j], out[1][j], out[2][j]);
 #pragma unroll
           for (int k = 0; k < 3; ++k)
             *reinterpret_cast<uint4*>(smem + S::kP + k * S::kPBytes + tok * 16 * kUnit + r * 16) =
                 make_uint4(out[k][0], out[k][1], out[k][2], out[k][3]);
         }
-        if (!here) {                               // a value row that is no key may hold anything: 0 x NaN
+        if (left <= 0) {                           // a value row that is no key may hold anything: 0 x NaN
           uint4* row = reinterpret_cast<uint4*>(smem + S::kRing + stage * 2 * kTileBytes + kTileBytes + r * kHeadDim);
 #pragma unroll
           for (int j = 0; j < 8; ++j) row[j] = make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async_smem();
+        tc_fence_before();
         mbar_arrive_warp(&bar_p);
       }
       // the next item's query, while the last product runs (every S of this item has been read)
@@ -336,7 +342,7 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
       if (next.units > 0) write_query(next);
 
       // ---- the item's results
-      const int first = column_sums<kN>(l, lane);
+      const int first = reduce_columns<false, kN>(l, lane);
       s_red[quad][first] = l[0];                   // (16 columns: two lanes, one value)
       named_sync<kSoftmax>();
       if (t.units > 0) bounded_wait_warp(&bar_pv, (n - 1) & 1, gave_up);
@@ -376,7 +382,6 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
         }
       }
       tc_fence_before();
-      named_sync<kSoftmax>();
     }
   }
   tc_fence_before();
@@ -384,20 +389,26 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
   if (warp == 1) tmem_dealloc(s.tmem, S::kTmem);
 }
 
-template <int kT, int kCode>
+template <int kT, int kCode, bool kSelected>
 int launch(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttnParams& p, cudaStream_t stream) {
   constexpr int smem = Shape<kT>::kSmem;
-  const cudaError_t e = cudaFuncSetAttribute(b8_few_kernel<kT, kCode>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  const cudaError_t e = cudaFuncSetAttribute(b8_few_kernel<kT, kCode, kSelected>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return set_error((int)e, "b8_attn: %s", cudaGetErrorString(e));
-  b8_few_kernel<kT, kCode><<<kB8FewGrid, kThreads, smem, stream>>>(k_map, v_map, p);
+  b8_few_kernel<kT, kCode, kSelected><<<kB8FewGrid, kThreads, smem, stream>>>(k_map, v_map, p);
   return check_launch("b8_attn");
+}
+
+template <int kT, int kCode>
+int launch_with(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttnParams& p, cudaStream_t stream) {
+  return p.mask != nullptr || p.lists != nullptr ? launch<kT, kCode, true>(k_map, v_map, p, stream)
+                                                 : launch<kT, kCode, false>(k_map, v_map, p, stream);
 }
 
 }  // namespace
 
 int b8_launch_few(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttnParams& p, int tokens, int code, cudaStream_t stream) {
-  if (tokens == 1) return code == kE4m3 ? launch<1, kE4m3>(k_map, v_map, p, stream) : launch<1, kE5m2>(k_map, v_map, p, stream);
-  return code == kE4m3 ? launch<2, kE4m3>(k_map, v_map, p, stream) : launch<2, kE5m2>(k_map, v_map, p, stream);
+  if (tokens == 1) return code == kE4m3 ? launch_with<1, kE4m3>(k_map, v_map, p, stream) : launch_with<1, kE5m2>(k_map, v_map, p, stream);
+  return code == kE4m3 ? launch_with<2, kE4m3>(k_map, v_map, p, stream) : launch_with<2, kE5m2>(k_map, v_map, p, stream);
 }
 
 }  // namespace ifv2

@@ -172,8 +172,8 @@ def cache_write_b8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_ca
 
 
 @functools.lru_cache(maxsize=256)
-def _workspace_bytes(total_q, batch, heads, max_seqlen_q):
-    return int(_lib.load().ifv2_b8_attn_workspace_bytes(total_q, batch, heads, HEAD_DIM, max_seqlen_q))
+def _workspace_bytes(total_q, batch, heads, max_seqlen_q, capacity):
+    return int(_lib.load().ifv2_b8_attn_workspace_bytes(total_q, batch, heads, HEAD_DIM, max_seqlen_q, capacity))
 
 
 def infllmv2_attn_paged_b8(
@@ -227,7 +227,7 @@ def infllmv2_attn_paged_b8(
     out = torch.empty_like(q)
     lse = torch.empty(total, heads, dtype=torch.float32, device=dev) if return_softmax_lse else None
     if total and hk:
-        ws_bytes = _workspace_bytes(total, batch, heads, max_seqlen_q)
+        ws_bytes = _workspace_bytes(total, batch, heads, max_seqlen_q, cap)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         with _on(dev):
             _lib.call("ifv2_b8_attn", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
