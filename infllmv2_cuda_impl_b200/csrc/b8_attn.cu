@@ -86,7 +86,8 @@ __global__ void __launch_bounds__(kPlanThreads) b8_plan_kernel(const AttnParams 
     p.first_tile[grid_most] = tiles;
   }
   __syncthreads();
-  const Shares<int64_t> shares(max(before, (int64_t)1), grid_most, p.least_share);
+  Shares<int64_t> shares;
+  shares.deal(max(before, (int64_t)1), grid_most, p.least_share);
   for (int g = tid; g < grid_most; g += kPlanThreads) {
     const int64_t at = shares.begin(min(g, shares.grid - 1));
     int lo = 0, hi = tiles;                        // start[lo] <= at < start[hi]
@@ -98,7 +99,8 @@ __global__ void __launch_bounds__(kPlanThreads) b8_plan_kernel(const AttnParams 
   }
 }
 
-// The pieces of a tile that shares cut: CTA x has the tile that share x begins inside, if no earlier share does (join[x]).
+// The pieces of a tile that shares cut: CTA x has tile x (where tiles are few), or the tile that share x begins inside if no
+// earlier share does; join[x] says whether there is one.
 // Piece results are normal outputs with the log2 of their sums.  A warp has a head; in calls of one token per
 // sequence, where pieces are many and tiles few, the four warps of a CTA share a head's pieces.  Also: rows behind the
 // last sequence.
@@ -116,13 +118,16 @@ __global__ void __launch_bounds__(kJoinThreads) b8_join_kernel(const AttnParams 
       for (int64_t i = row0 * heads + me; i < p.total_q * heads; i += all) p.lse[i] = INFINITY;
   }
   wait_previous();
-  const int g = blockIdx.x;
-  const int4 cut = p.join[g];
+  if (p.by_tile) {                                 // (a sequence without tokens has no tile)
+    int row0;
+    if (tokens_of(p, blockIdx.x / p.heads_k, row0) == 0) return;
+  }
+  const int4 cut = p.join[blockIdx.x];
   const int column = kShared ? blockIdx.y : blockIdx.y * 4 + warp, tok = column / kGroup;
-  if (cut.w == 0 || tok >= cut.y >> 16) return;
-  // pieces: the second of CTA g - 1, the first of g, g + 1, ..., cut.z
-  const int pieces = cut.z - g + 2;
-  const auto piece = [&](int i) { return (int64_t)(i == 0 ? 2 * (g - 1) + 1 : 2 * (g - 1 + i)) * columns + column; };
+  if (cut.z >= cut.w || tok >= cut.y >> 16) return;
+  // pieces: the second of the first share, the first of those behind it
+  const int pieces = cut.w - cut.z + 1;
+  const auto piece = [&](int i) { return (int64_t)(2 * (cut.z + i) + (i == 0 ? 1 : 0)) * columns + column; };
   constexpr int kStep = kShared ? 4 : 1;
   const int i0 = kShared ? warp : 0;
   float most = -INFINITY, sum = 0.f;
@@ -292,6 +297,7 @@ extern "C" int ifv2_b8_attn(const void* q, const void* k_cache, const void* v_ca
   p.least_share = 3;
   char* ws = static_cast<char*>(workspace);
   p.join = reinterpret_cast<int4*>(ws);
+  p.by_tile = !at.listed && (int64_t)batch * heads_k <= at.grid;
   p.part_lse = reinterpret_cast<float*>(ws + at.lse_at);
   p.part_o = reinterpret_cast<float*>(ws + at.o_at);
   p.most_chunks = (int)at.chunks;
@@ -306,8 +312,9 @@ extern "C" int ifv2_b8_attn(const void* q, const void* k_cache, const void* v_ca
   }
   rc = at.tokens <= 2 ? b8_launch_few(k_map, v_map, p, at.tokens, code, s) : b8_launch_chunk(k_map, v_map, p, at.listed, code, s);
   if (rc) return rc;
-  const cudaError_t e = at.tokens == 1 ? launch_beside(b8_join_kernel<true>, dim3(at.grid, kGroup), kJoinThreads, s, p, at.tokens)
-                                       : launch_beside(b8_join_kernel<false>, dim3(at.grid, 4 * at.tokens), kJoinThreads, s, p, at.tokens);
+  const unsigned cuts = p.by_tile ? batch * heads_k : at.grid;
+  const cudaError_t e = at.tokens == 1 ? launch_beside(b8_join_kernel<true>, dim3(cuts, kGroup), kJoinThreads, s, p, at.tokens)
+                                       : launch_beside(b8_join_kernel<false>, dim3(cuts, 4 * at.tokens), kJoinThreads, s, p, at.tokens);
   if (e != cudaSuccess) return set_error((int)e, "b8_attn (join): %s", cudaGetErrorString(e));
   return check_launch("b8_attn (join)");
 }

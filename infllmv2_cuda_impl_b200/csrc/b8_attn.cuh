@@ -11,7 +11,8 @@
 //     number: a term is a byte, what it leaves over one subtraction.  Weights are 2^(x + eV - M) with M about 2^-10 of the
 //     largest so far, at most 2^15, and below 2^-16 they have the type's fixed spacing of 2^-16: 2^-27 of the largest.
 //     The values' exponents take part in M, so that contributions keep their size against one another whatever
-//     the sizes of the blocks' values are.  The sum of the softmax is held in units of 2^(M - E), E the largest eV so far.
+//     the sizes of the blocks' values are.  The sum of the softmax is held in units of 2^(M - E) with E near the blocks' eV:
+//     that of the first unit, until one is more than 2^kHighest above it.
 //
 // A tile is up to kT tokens of a sequence x the 16 query heads of a KV head.  A CTA takes an even share of the call's
 // cost, units of 128 keys plus kStart per tile, whatever the lengths are; pieces of a tile that shares cut go to a workspace
@@ -33,7 +34,7 @@ constexpr int kMaxMaskWords = 128;               // 524288 keys
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kUnset = -1e30f;                 // reference of a row that has seen no key
 constexpr float kTop = 10.f, kRoom = 15.f;       // a new reference puts the largest weight at 2^kTop; past 2^kRoom it moves
-constexpr int kDeepest = -90;                    // eV - E that the sum's range has room for
+constexpr int kDeepest = -90, kHighest = 60;     // eV - E that the sum's range has room for
 constexpr int kNoScale = -10000, kNanScale = 10000;      // eV of no block, of a NaN block
 
 struct AttnParams {
@@ -53,7 +54,8 @@ struct AttnParams {
   float scale_log2;
   int least_share;
   // workspace
-  int4* join;                                    // per CTA: the cut tile that its share begins inside (see Item)
+  int4* join;                                    // cut tiles: first token's row, tokens << 16 | head, first and last share
+  int by_tile;                                   // join has a place per tile (where tiles are few), else per share
   float *part_o, *part_lse;                      // two pieces per CTA: (2 grid, 16 kT, 128), (2 grid, 16 kT)
   int most_chunks;                               // listed tiles of a head that the workspace has room for
   int32_t* first_chunk;                          // (batch + 1) chunks of kT tokens before each sequence
@@ -67,7 +69,7 @@ template <typename Cost>
 struct Shares {
   Cost each, rest;
   int grid;
-  __device__ __forceinline__ Shares(Cost cost, int most, int least) {
+  __device__ __forceinline__ void deal(Cost cost, int most, int least) {
     grid = cost >= (Cost)most * least ? most : (int)max((uint32_t)cost / (uint32_t)least, 1u);
     each = sizeof(Cost) == 4 ? (Cost)((uint32_t)cost / (uint32_t)grid) : cost / grid;
     rest = cost - each * grid;
@@ -227,53 +229,52 @@ __device__ __forceinline__ void fetch(const AttnParams& p, const CUtensorMap* k_
     if (kSelected) n = min(n, ceil_div(p.usual * (3 + tokens), 8));
     return tokens ? kStart + n : 0;
   };
+  const int me = blockIdx.x;
+  int each = 0;                                    // cost of the sequence's heads
   if (kListed) {
     n_tiles = p.first_tile[gridDim.x];
     cost = (Cost)p.start[n_tiles];
-  } else {
-    int sum = 0;
-    for (int base = lane; base < p.batch; base += 32) {
-      int r, t, k;
-      sum += cost_of(base, r, t, k);
-    }
-    cost = __reduce_add_sync(0xFFFFFFFFu, sum) * p.heads_k;
   }
-  const Shares<Cost> shares(max(cost, (Cost)1), gridDim.x, p.least_share);
-  const int me = blockIdx.x;
-  const Cost lo = me < shares.grid ? shares.begin(me) : cost, hi = me < shares.grid ? shares.begin(me + 1) : cost;
-  int each = 0;                                    // cost of the sequence's heads
-  bool more = lo < hi;
-  if (more) {
-    if (kListed) {
-      tile = p.first_tile[me];
-    } else {
-      for (int base = 0;; base += 32) {            // the sequence that lo lies in
-        int r = 0, t = 0, k = 0, c = 0;
-        if (base + lane < p.batch) c = cost_of(base + lane, r, t, k);
-        int upto = c * p.heads_k;
+  Cost lo = 0x7FFFFFFF, hi = 0;
+  bool more = false;
+  Shares<Cost> shares;
+  for (int pass = kListed ? 1 : 0;; ++pass) {      // pass 0 adds costs up, pass 1 finds the sequence that this share begins in
+    if (pass == 1) {
+      shares.deal(max(cost, (Cost)1), gridDim.x, p.least_share);
+      lo = me < shares.grid ? shares.begin(me) : cost, hi = me < shares.grid ? shares.begin(me + 1) : cost;
+      more = lo < hi;
+      if (kListed) tile = p.first_tile[me];
+      if (kListed || !more) break;
+    }
+    int base = 0, before = 0;
+    for (; base < p.batch; base += 32) {
+      int r = 0, t = 0, k = 0, c = 0;
+      if (base + lane < p.batch) c = cost_of(base + lane, r, t, k);
+      int upto = c * p.heads_k;
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-          const int o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
-          if (lane >= d) upto += o;
-        }
-        const uint32_t past = __ballot_sync(0xFFFFFFFFu, (int)begin + upto > (int)lo);
-        if (past) {
-          const int src = __ffs(past) - 1;
-          b = base + src;
-          row = __shfl_sync(0xFFFFFFFFu, r, src);
-          tokens = __shfl_sync(0xFFFFFFFFu, t, src);
-          reach = __shfl_sync(0xFFFFFFFFu, k, src);
-          each = __shfl_sync(0xFFFFFFFFu, c, src);
-          begin += __shfl_sync(0xFFFFFFFFu, upto, src) - each * p.heads_k;
-          head = (int)((uint32_t)(lo - begin) / (uint32_t)each);
-          begin += head * each;
-          break;
-        }
-        begin += __shfl_sync(0xFFFFFFFFu, upto, 31);
+      for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+        if (lane >= d) upto += o;
       }
+      const uint32_t past = __ballot_sync(0xFFFFFFFFu, before + upto > (int)lo);
+      if (past) {
+        const int src = __ffs(past) - 1;
+        b = base + src;
+        row = __shfl_sync(0xFFFFFFFFu, r, src);
+        tokens = __shfl_sync(0xFFFFFFFFu, t, src);
+        reach = __shfl_sync(0xFFFFFFFFu, k, src);
+        each = __shfl_sync(0xFFFFFFFFu, c, src);
+        before += __shfl_sync(0xFFFFFFFFu, upto, src) - each * p.heads_k;
+        head = (int)((uint32_t)((int)lo - before) / (uint32_t)each);
+        begin = before + head * each;
+        break;
+      }
+      before += __shfl_sync(0xFFFFFFFFu, upto, 31);
     }
+    if (pass == 1) break;
+    cost = before;
   }
-  int4 cut = make_int4(0, 0, 0, 0);
+  int4 cut = make_int4(0, 0, 0, 0);                // (first and last share the same: not cut)
   int n = 0, items = 0;                            // units, items so far
   for (bool first = true; more && !*gave_up; first = false) {
     if (kListed) {
@@ -332,10 +333,12 @@ __device__ __forceinline__ void fetch(const AttnParams& p, const CUtensorMap* k_
       z = est ? (int)((int64_t)est_z * units / est) : 0;
     }
     const bool whole = lo <= begin && hi >= end;
-    if (first && me > 0 && begin < lo && begin >= shares.begin(me - 1)) {
+    const bool begins = begin >= lo;               // the tile begins in this share
+    if (p.by_tile ? begins : first && me > 0 && !begins && begin >= shares.begin(me - 1)) {
       int last = me;
       while (last + 1 < shares.grid && shares.begin(last + 1) < end) ++last;
-      cut = make_int4(row, tokens << 16 | head, last, 1);
+      cut = make_int4(row, tokens << 16 | head, p.by_tile ? me : me - 1, last);
+      if (p.by_tile && lane == 0) p.join[b * p.heads_k + head] = cut;
     }
     {
       const int slot = items & 1;
@@ -395,15 +398,11 @@ __device__ __forceinline__ void fetch(const AttnParams& p, const CUtensorMap* k_
       scales();
     }
     for (int k0 = 2 * a; k0 < 2 * z; k0 += 32) {
+      const int now = row_of, many = min(32, 2 * (z - a) - (k0 - 2 * a));
+      const bool next = k0 + 32 < 2 * z;
       Block r;
       r.pos = block * kBlockN;
       r.valid = k0 + lane < total ? min(kBlockN, reach - r.pos) : 0;
-      r.k_scale = q8::scale_value(kb);
-      r.e_v = r.valid == 0 ? kNoScale : vb == kNanByte ? kNanScale : vb - 127;
-      const bool has = r.e_v != kNanScale && r.e_v != kNoScale;
-      const int e_most = has ? r.e_v : kNoScale, e_least = has ? r.e_v : -kNoScale;
-      r.e_unit = (max(e_most, __shfl_xor_sync(0xFFFFFFFFu, e_most, 1)) & 0xFFFF) |
-                 min(e_least, __shfl_xor_sync(0xFFFFFFFFu, e_least, 1)) << 16;
       r.tokens = (1u << tokens) - 1;
       if (kSelected && kT > 1) {
         r.tokens = 0;
@@ -413,15 +412,15 @@ __device__ __forceinline__ void fetch(const AttnParams& p, const CUtensorMap* k_
           r.tokens |= (uint32_t)((w >> (block & 63)) & 1) << i;
         }
       }
-      const int now = row_of, many = min(32, 2 * (z - a) - (k0 - 2 * a));
-      const bool next = k0 + 32 < 2 * z;
       if (next) look(k0 + 32);
+      // A batch's first kStages - 1 units are asked for before their records are written, whose scales may be on their way
+      // still.  (Not more: the next one's copies wait for the products of a unit whose record is among these.)
+      const int ahead = min(2 * (kStages - 1), many);
+#pragma unroll 1
       for (int j = 0; j < many; j += 2, ++n) {
         const int stage = n % kStages;
         if (!bounded_wait_warp(&s.empty[stage], ((n / kStages) & 1) ^ 1, gave_up)) break;
-        if ((lane & ~1) == j) s.block[stage][lane & 1] = r;
         const int row0 = __shfl_sync(0xFFFFFFFFu, now, j), row1 = __shfl_sync(0xFFFFFFFFu, now, j + 1);
-        __syncwarp();
         if (lane == 0) {
           uint8_t* to = ring + stage * 2 * kTileBytes;
           mbar_expect_tx(&s.full[stage], 2 * kTileBytes);
@@ -430,7 +429,24 @@ __device__ __forceinline__ void fetch(const AttnParams& p, const CUtensorMap* k_
           tma_load_2d(to + kTileBytes, v_map, &s.full[stage], 0, row0);
           tma_load_2d(to + kTileBytes + kTileBytes / 2, v_map, &s.full[stage], 0, row1);
         }
-        if (next && j == 8) scales();
+        if (j + 2 < ahead) continue;
+        int u = j;
+        if (j + 2 == ahead) {
+          u = 0;
+          r.k_scale = q8::scale_value(kb);
+          r.e_v = r.valid == 0 ? kNoScale : vb == kNanByte ? kNanScale : vb - 127;
+          const bool has = r.e_v != kNanScale && r.e_v != kNoScale;
+          const int e_most = has ? r.e_v : kNoScale, e_least = has ? r.e_v : -kNoScale;
+          r.e_unit = (max(e_most, __shfl_xor_sync(0xFFFFFFFFu, e_most, 1)) & 0xFFFF) |
+                     min(e_least, __shfl_xor_sync(0xFFFFFFFFu, e_least, 1)) << 16;
+          if (next) scales();
+        }
+        for (; u <= j; u += 2) {
+          const int of = (n - (j - u) / 2) % kStages;
+          if ((lane & ~1) == u) s.block[of][lane & 1] = r;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s.full[of]);
+        }
       }
       if (*gave_up) break;
     }
@@ -448,7 +464,7 @@ __device__ __forceinline__ void fetch(const AttnParams& p, const CUtensorMap* k_
       }
     }
   }
-  if (lane == 0) p.join[me] = cut;
+  if (!p.by_tile && lane == 0) p.join[me] = cut;
   const int slot = items & 1;
   if (bounded_wait_warp(&s.item_empty[slot], ((items >> 1) & 1) ^ 1, gave_up) && lane == 0) {
     s.item[slot].units = -1;

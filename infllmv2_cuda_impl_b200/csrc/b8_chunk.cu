@@ -81,7 +81,7 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
 
   if (tid == 0) {
     s.gave_up = 0;
-    for (int i = 0; i < kStages; ++i) mbar_init(&s.full[i], 1), mbar_init(&s.empty[i], 9);
+    for (int i = 0; i < kStages; ++i) mbar_init(&s.full[i], 2), mbar_init(&s.empty[i], 9);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar_s[i], 1), mbar_init(&bar_p[i], 4), mbar_init(&bar_pv[i], 1), mbar_init(&bar_v[i], 4);
       mbar_init(&s.item_full[i], 1), mbar_init(&s.item_empty[i], 13);
@@ -278,14 +278,14 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
         mbar_arrive_warp(&s.empty[stage]);
         int seen[2], e_blk[2];
         float c[2], ev[2], dv[2];
-        int e_new = max(e_ref, (int)(int16_t)blk[0].e_unit);
+        const int e_most = (int16_t)blk[0].e_unit;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           seen[h] = (blk[h].tokens & bit) ? max(min(limit - blk[h].pos, blk[h].valid), 0) : 0;
           e_blk[h] = blk[h].e_v == kNanScale ? kNoScale : blk[h].e_v;
           c[h] = fmaxf(c_row * blk[h].k_scale, 1e-37f);        // (-inf of a masked key times 0 would be NaN)
         }
-        if (e_new == kNoScale) e_new = 0;
+        const int e_new = e_ref != kNoScale && e_most - e_ref <= kHighest ? e_ref : e_most == kNoScale ? 0 : e_most;
         float back = 1.f;                          // what the sums so far are multiplied with
         if (e_new != e_ref && e_ref != kNoScale) {
           const int delta = e_new - e_ref, bump = max(kDeepest - (deepest - delta), 0);

@@ -71,7 +71,7 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
 
   if (tid == 0) {
     s.gave_up = 0;
-    for (int i = 0; i < kStages; ++i) mbar_init(&s.full[i], 1), mbar_init(&s.empty[i], 1);
+    for (int i = 0; i < kStages; ++i) mbar_init(&s.full[i], 2), mbar_init(&s.empty[i], 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar_s[i], 1), mbar_init(&bar_sfree[i], 4);
       mbar_init(&s.item_full[i], 1), mbar_init(&s.item_empty[i], 5);
@@ -201,8 +201,8 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
         bounded_wait_warp(&s.full[stage], (n / kStages) & 1, gave_up);
         const Block* blk = &s.block[stage][r >> 6];
         const float k_scale = blk->k_scale;
-        const int e_v = blk->e_v, valid = blk->valid, e_unit = blk->e_unit, e_most = max(e_ref, (int)(int16_t)e_unit);
-        const int e_new = e_most == kNoScale ? 0 : e_most;
+        const int e_v = blk->e_v, valid = blk->valid, e_unit = blk->e_unit, e_most = (int16_t)e_unit;
+        const int e_new = e_ref != kNoScale && e_most - e_ref <= kHighest ? e_ref : e_most == kNoScale ? 0 : e_most;
         // which columns' tokens see the thread's key: the last token those below `valid`, the ones before it fewer if causal
         const int left = valid - (r & 63);         // > 0: a key
         uint32_t sees = left > 0 ? (1u << kT) - 1 : 0u;
@@ -215,12 +215,12 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
         }
         const bool all = __all_sync(0xFFFFFFFFu, sees == (1u << kT) - 1);
         // eV - E; a NaN block's weights are NaN, those of a block far below the others' nothing
-        const int dv = min(e_v - e_new, 0), dv_ref = max(dv, kDeepest);
+        const int dv = e_v == kNanScale ? 0 : e_v - e_new, dv_ref = max(dv, kDeepest);
         const float v_ref = pow2i(dv_ref), v_scale = e_v == kNanScale ? NAN : dv < kDeepest ? 0.f : v_ref;
         bounded_wait_warp(&bar_s[n & 1], (n >> 1) & 1, gave_up);
         tc_fence_after();
         float w[kN];
-        bool moves = e_new != e_ref, settled = false;
+        bool moves = false, settled = false;
         for (;;) {
           uint32_t x[kN];
           if constexpr (kN == 16) {
@@ -298,7 +298,8 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
           float most = w[0];
 #pragma unroll
           for (int j = 1; j < kN; j += 2) most = fmaxf(fmaxf(most, w[j]), w[j + 1 < kN ? j + 1 : j]);
-          moves = named_any<kSoftmax>(most * v_ref > 32768.f);
+          // (one vote decides for all warps, whatever each has read: a wait that gave up must not part them)
+          moves = named_any<kSoftmax>(e_new != e_ref || most * v_ref > 32768.f);
           if (!moves) break;
         }
         tc_fence_before();
