@@ -10,9 +10,11 @@
 //
 // Units go to two groups of four softmax warps in turn (thread = row).  Each group has a score buffer, its weights over
 // the scores, and sums of its own (M, l, O), so that neither waits for the other; the two are put together at the end
-// of the tile.  TMEM: two S and two O of 128 columns, all there is.  Warps: 0 looks blocks up and issues TMA, 1 issues
-// MMAs (in order: a group's next scores come behind the product that reads its weights), 2..5 and 6..9 are the groups,
-// 10..13 convert values.
+// of the tile.  TMEM: two S and two O of 128 columns, all there is, so scores are made by blocks of 64 keys: a block's
+// next scores and the product of its weights are under way while the group works on the unit's other block (by whole
+// units a group waited 1200 of 4600 clocks for its next scores).  Warps: 0 looks blocks up and issues TMA, 1 issues the MMAs
+// of the scores, 2..5 and 6..9 are the groups, 10..13 convert values, 14 issues the MMAs of the values.  (One warp that
+// issued both took 1050 clocks for a block's 12 MMAs and their waits, and paced everything.)
 #include "b8_attn.cuh"
 
 namespace ifv2 {
@@ -21,51 +23,36 @@ namespace {
 using namespace b8;
 
 constexpr int kT = 8, kRows = kT * kGroup;
-constexpr int kThreads = 448, kSoftmax = 256;
+constexpr int kThreads = 480, kSoftmax = 256;
 constexpr int kStages = 3;
 constexpr int kQBytes = kRows * kHeadDim;         // one of two terms
 constexpr int kVBytes = kUnit * kHeadDim * 2;     // fp16 values of a unit: two halves of 64 features, a row per key
 constexpr int kV = 2 * kQBytes, kRing = kV + 2 * kVBytes, kSmem = kRing + kStages * 2 * kTileBytes + 1024;
-// a new reference puts the largest weight at 2^kFirst; it moves when a unit's weights add up to more than kMost
+// a new reference puts the largest weight at 2^kFirst; it moves when a block's weights add up to more than kMost
 constexpr float kFirst = 4.f, kMost = 32768.f;
 
 // Instruction descriptor, kind::f16 with fp16 operands, B MN-major.
 constexpr uint32_t kIdescValues = (1u << 4) | (1u << 16) | (128u >> 3 << 17) | (128u >> 4 << 24);
 
-// A row's 128 weights as fp16 pairs, and their sums by block.
-__device__ __forceinline__ void weights(uint32_t scores, uint32_t (&w)[64], float (&sum)[2], const int (&seen)[2], const float (&c)[2],
-                                        const float (&ev)[2], float m, bool all) {
+// A row's 64 weights of a block as fp16 pairs, 2^(x c + b); returns their sum.
+__device__ __forceinline__ float weights(const uint32_t (&x)[64], uint32_t (&w)[32], float c, float b) {
+  const uint64_t b2 = pack_f32x2(b, b), c2 = pack_f32x2(c, c);
+  uint64_t sum2 = 0, sum2b = 0;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const float b = ev[h] - m;
-    const uint64_t b2 = pack_f32x2(b, b), c2 = pack_f32x2(c[h], c[h]);
-    uint64_t sum2 = 0, sum2b = 0;
+  for (int j = 0; j < kBlockN; j += 4) {
+    float y[4];
+    unpack_f32x2(fma_f32x2(pack_f32x2(x[j], x[j + 1]), c2, b2), y[0], y[1]);
+    unpack_f32x2(fma_f32x2(pack_f32x2(x[j + 2], x[j + 3]), c2, b2), y[2], y[3]);
 #pragma unroll
-    for (int j0 = 0; j0 < kBlockN; j0 += 32) {
-      uint32_t x[32];
-      tmem_ld32_wait(scores + h * kBlockN + j0, x);
-      if (!all) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (j0 + j >= seen[h]) x[j] = 0xFF800000u;
-      }
-#pragma unroll
-      for (int j = 0; j < 32; j += 4) {
-        float y[4];
-        unpack_f32x2(fma_f32x2(pack_f32x2(x[j], x[j + 1]), c2, b2), y[0], y[1]);
-        unpack_f32x2(fma_f32x2(pack_f32x2(x[j + 2], x[j + 3]), c2, b2), y[2], y[3]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = ex2(y[e]);
-        sum2 = add_f32x2(sum2, pack_f32x2(y[0], y[1]));
-        sum2b = add_f32x2(sum2b, pack_f32x2(y[2], y[3]));
-        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[32 * h + (j0 + j) / 2]) : "f"(y[1]), "f"(y[0]));
-        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[32 * h + (j0 + j) / 2 + 1]) : "f"(y[3]), "f"(y[2]));
-      }
-    }
-    float s0, s1;
-    unpack_f32x2(add_f32x2(sum2, sum2b), s0, s1);
-    sum[h] = s0 + s1;
+    for (int e = 0; e < 4; ++e) y[e] = ex2(y[e]);
+    sum2 = add_f32x2(sum2, pack_f32x2(y[0], y[1]));
+    sum2b = add_f32x2(sum2b, pack_f32x2(y[2], y[3]));
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[j / 2]) : "f"(y[1]), "f"(y[0]));
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[j / 2 + 1]) : "f"(y[3]), "f"(y[2]));
   }
+  float s0, s1;
+  unpack_f32x2(add_f32x2(sum2, sum2b), s0, s1);
+  return s0 + s1;
 }
 
 template <int kCode, bool kListed, bool kSelected>
@@ -74,7 +61,8 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   __shared__ Common<kT, kStages> s;
-  __shared__ uint64_t bar_s[2], bar_p[2], bar_pv[2], bar_v[2], bar_q, bar_drain;
+  // by group, and by block of a unit
+  __shared__ uint64_t bar_s[2][2], bar_p[2][2], bar_v[2][2], bar_pv[2][2], bar_q, bar_drain[2];
   __shared__ float s_c[kRows], s_top[2][kRows], s_lse[2][kRows];       // row's factor; a group's M and log2 of its sum
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   volatile int* gave_up = &s.gave_up;
@@ -83,11 +71,12 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
     s.gave_up = 0;
     for (int i = 0; i < kStages; ++i) mbar_init(&s.full[i], 2), mbar_init(&s.empty[i], 9);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar_s[i], 1), mbar_init(&bar_p[i], 4), mbar_init(&bar_pv[i], 1), mbar_init(&bar_v[i], 4);
-      mbar_init(&s.item_full[i], 1), mbar_init(&s.item_empty[i], 13);
+      for (int h = 0; h < 2; ++h)
+        mbar_init(&bar_s[i][h], 1), mbar_init(&bar_p[i][h], 4), mbar_init(&bar_v[i][h], 4), mbar_init(&bar_pv[i][h], 1);
+      mbar_init(&s.item_full[i], 1), mbar_init(&s.item_empty[i], 14);
     }
     mbar_init(&bar_q, 8);
-    mbar_init(&bar_drain, 1);
+    mbar_init(&bar_drain[0], 1), mbar_init(&bar_drain[1], 1);
     fence_barrier_init();
     prefetch_tensormap(&k_map);
     prefetch_tensormap(&v_map);
@@ -106,23 +95,27 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
   if (warp == 0) {
     fetch<kT, kStages, kListed, kSelected>(p, &k_map, &v_map, s, smem + kRing);
   } else if (warp == 1) {
-    // ---------------------------------------------------------------- MMAs
+    // ---------------------------------------------------------------- scores
     if (elect_one()) {
       const uint32_t base = smem_u32(smem);
-      constexpr uint32_t kIdescS = umma_idesc_f8(128, 128, kE4m3, kCode, false, false);
+      constexpr uint32_t kIdescS = umma_idesc_f8(128, kBlockN, kE4m3, kCode, false, false);
+      const uint32_t q_lo = umma_desc_lo(base, 16);
       bool ok = true;
-      int n = 0, queries = 0;
-      const auto values = [&](int unit, bool first) {        // O += W V of a unit
-        const int g = unit & 1;
-        ok = ok && bounded_wait(&bar_p[g], (unit >> 1) & 1, gave_up) && bounded_wait(&bar_v[g], (unit >> 1) & 1, gave_up);
+      int n0 = 0, queries = 0;
+      const auto scores = [&](int n, int h) {                // S of a unit's block
+        const int stage = n % kStages;
+        ok = ok && bounded_wait(&s.full[stage], (n / kStages) & 1, gave_up);
         if (!ok) return;
         tc_fence_after();
-        const uint32_t v = base + kV + g * kVBytes;
+        const uint32_t k_lo = umma_desc_lo(base + kRing + stage * 2 * kTileBytes + h * (kTileBytes / 2), 16);
+        const uint32_t to = tmem + 128 * (n & 1) + kBlockN * h;
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          umma_ts(tmem + 256 + 128 * g, tmem + 128 * g + 8 * kk, umma_desc_sw128(v + kk * 2048, kVBytes / 2, 1024), kIdescValues,
-                  !first || kk > 0);
-        umma_commit(&bar_pv[g]);
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            umma_f8_ss_lo(to, q_lo + ((j * kQBytes + kk * 32) >> 4), k_lo + ((kk * 32) >> 4), kUmmaDescHi, kIdescS, j + kk > 0);
+        umma_commit(&bar_s[n & 1][h]);
+        if (h == 1) umma_commit(&s.empty[stage]);
       };
       for (int item = 0; ok; ++item) {
         ok = bounded_wait(&s.item_full[item & 1], (item >> 1) & 1, gave_up);
@@ -131,27 +124,61 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
         mbar_arrive(&s.item_empty[item & 1]);
         if (units == 0) continue;
         ok = bounded_wait(&bar_q, queries++ & 1, gave_up);
-        for (int i = 0; ok && i < units; ++i, ++n) {
-          const int stage = n % kStages;
-          ok = bounded_wait(&s.full[stage], (n / kStages) & 1, gave_up);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t k = base + kRing + stage * 2 * kTileBytes;
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              umma_f8_ss(tmem + 128 * (n & 1), umma_desc_sw128(base + j * kQBytes + kk * 32, 16, 1024), umma_desc_sw128(k + kk * 32, 16, 1024),
-                         kIdescS, j + kk > 0);
-          umma_commit(&s.empty[stage]);
-          umma_commit(&bar_s[n & 1]);
-          if (i > 0) values(n - 1, i <= 2);
-        }
-        values(n - 1, units <= 2);
+        // scores are written over weights: the product that reads these is waited for
+        for (int n = max(n0 - 2, 0); n < n0; ++n) ok = ok && bounded_wait(&bar_pv[n & 1][1], (n >> 1) & 1, gave_up);
+        for (int i = 0; i < min(units, 2); ++i)
+          for (int h = 0; h < 2; ++h) scores(n0 + i, h);
+#pragma unroll 1
+        for (int i = 2; ok && i < units; i += 2)
+#pragma unroll 1
+          for (int h = 0; ok && h < 2; ++h)
+#pragma unroll 1
+            for (int u = i; ok && u < min(i + 2, units); ++u) {
+              const int n = n0 + u;
+              ok = bounded_wait(&bar_pv[n & 1][h], ((n - 2) >> 1) & 1, gave_up);
+              scores(n, h);
+            }
+        n0 += units;
       }
       if (!ok) {
-        umma_commit(&bar_drain);
-        mbar_wait_drain(&bar_drain, 0);
+        umma_commit(&bar_drain[0]);
+        mbar_wait_drain(&bar_drain[0], 0);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 14) {
+    // ---------------------------------------------------------------- values
+    if (elect_one()) {
+      const uint32_t base = smem_u32(smem);
+      bool ok = true;
+      int n0 = 0;
+      for (int item = 0; ok; ++item) {
+        ok = bounded_wait(&s.item_full[item & 1], (item >> 1) & 1, gave_up);
+        const int units = ok ? s.item[item & 1].units : -1;
+        if (units < 0) break;
+        mbar_arrive(&s.item_empty[item & 1]);
+#pragma unroll 1
+        for (int i = 0; ok && i < units; i += 2)
+#pragma unroll 1
+          for (int h = 0; ok && h < 2; ++h)
+#pragma unroll 1
+            for (int u = i; ok && u < min(i + 2, units); ++u) {
+              const int n = n0 + u, g = n & 1;
+              ok = bounded_wait(&bar_v[g][h], (n >> 1) & 1, gave_up) && bounded_wait(&bar_p[g][h], (n >> 1) & 1, gave_up);
+              if (!ok) break;
+              tc_fence_after();
+              const uint32_t v_lo = umma_desc_lo(base + kV + g * kVBytes + h * (kVBytes / 4), kVBytes / 2);
+              const uint32_t w = tmem + 128 * g + kBlockN * h;
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)
+                umma_ts_lo(tmem + 256 + 128 * g, w + 8 * kk, v_lo + ((kk * 2048) >> 4), kIdescValues, u >= 2 || h + kk > 0);
+              umma_commit(&bar_pv[g][h]);
+            }
+        n0 += units;
+      }
+      if (!ok) {
+        umma_commit(&bar_drain[1]);
+        mbar_wait_drain(&bar_drain[1], 0);
       }
     }
     __syncwarp();
@@ -171,33 +198,36 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
         const int valid[2] = {s.block[stage][0].valid, s.block[stage][1].valid};
         const uint8_t* from = smem + kRing + stage * 2 * kTileBytes + kTileBytes;
         uint8_t* to = smem + kV + g * kVBytes + (c >> 2) * (kVBytes / 2);
-        if (n >= 2) bounded_wait_warp(&bar_pv[g], ((n - 2) >> 1) & 1, gave_up);      // the buffer is free again
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          if (n >= 2) bounded_wait_warp(&bar_pv[g][h], ((n - 2) >> 1) & 1, gave_up);      // the block's place is free again
 #pragma unroll
-        for (int j = 0; j < kUnit / 16; ++j) {
-          const int row = j * 16 + (ctid >> 3), at = row & 7;
-          uint4 x = *reinterpret_cast<const uint4*>(from + row * kHeadDim + ((c ^ at) << 4));
-          // a value row that is no key may hold anything: 0 x NaN
-          if ((row & 63) >= (row < kBlockN ? valid[0] : valid[1])) x = make_uint4(0, 0, 0, 0);
-          uint32_t h[8];
-          const uint32_t* w = reinterpret_cast<const uint32_t*>(&x);
+          for (int j = 0; j < kBlockN / 16; ++j) {
+            const int row = h * kBlockN + j * 16 + (ctid >> 3), at = row & 7;
+            uint4 x = *reinterpret_cast<const uint4*>(from + row * kHeadDim + ((c ^ at) << 4));
+            // a value row that is no key may hold anything: 0 x NaN
+            if ((row & 63) >= (h ? valid[1] : valid[0])) x = make_uint4(0, 0, 0, 0);
+            uint32_t y[8];
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(&x);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if (kCode == kE4m3) {
-              asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
-                  : "=r"(h[2 * k]), "=r"(h[2 * k + 1]) : "r"(w[k]));
-            } else {                               // the upper bytes of fp16 numbers
-              h[2 * k] = __byte_perm(w[k], 0u, 0x1404);
-              h[2 * k + 1] = __byte_perm(w[k], 0u, 0x3424);
+            for (int k = 0; k < 4; ++k) {
+              if (kCode == kE4m3) {
+                asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+                    : "=r"(y[2 * k]), "=r"(y[2 * k + 1]) : "r"(w[k]));
+              } else {                               // the upper bytes of fp16 numbers
+                y[2 * k] = __byte_perm(w[k], 0u, 0x1404);
+                y[2 * k + 1] = __byte_perm(w[k], 0u, 0x3424);
+              }
             }
+            // (the two halves lie in the same banks: one's even pieces are written beside the other's odd ones)
+            const int first = (c & 3) * 2 + (c >> 2), second = first ^ 1;
+            const bool odd = c >> 2;
+            *reinterpret_cast<uint4*>(to + row * 128 + ((first ^ at) << 4)) = odd ? make_uint4(y[4], y[5], y[6], y[7]) : make_uint4(y[0], y[1], y[2], y[3]);
+            *reinterpret_cast<uint4*>(to + row * 128 + ((second ^ at) << 4)) = odd ? make_uint4(y[0], y[1], y[2], y[3]) : make_uint4(y[4], y[5], y[6], y[7]);
           }
-          // (the two halves lie in the same banks: one's even pieces are written beside the other's odd ones)
-          const int first = (c & 3) * 2 + (c >> 2), second = first ^ 1;
-          const bool odd = c >> 2;
-          *reinterpret_cast<uint4*>(to + row * 128 + ((first ^ at) << 4)) = odd ? make_uint4(h[4], h[5], h[6], h[7]) : make_uint4(h[0], h[1], h[2], h[3]);
-          *reinterpret_cast<uint4*>(to + row * 128 + ((second ^ at) << 4)) = odd ? make_uint4(h[0], h[1], h[2], h[3]) : make_uint4(h[4], h[5], h[6], h[7]);
+          fence_proxy_async_smem();
+          mbar_arrive_warp(&bar_v[g][h]);
         }
-        fence_proxy_async_smem();
-        mbar_arrive_warp(&bar_v[g]);
         mbar_arrive_warp(&s.empty[stage]);
       }
     }
@@ -239,19 +269,17 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
       mbar_arrive_warp(&s.item_empty[item & 1]);
     };
 
-    // O times f, once the group's product before unit n has been made
-    const auto rescale = [&](float f, bool begun, int n) {
-      if (!begun) return;
-      bounded_wait_warp(&bar_pv[group], ((n - 2) >> 1) & 1, gave_up);
+    // O times f, once the group's product before the one of unit n, block h, has been made
+    const auto rescale = [&](float f, int n, int h) {
+      bounded_wait_warp(&bar_pv[group][h ^ 1], ((h ? n : n - 2) >> 1) & 1, gave_up);
       tc_fence_after();
 #pragma unroll 1
-      for (int c0 = 0; c0 < kHeadDim; c0 += 16) {
-        uint32_t o[16];
-        tmem_ld16(my_o + c0, o);
-        tmem_wait_ld();
+      for (int c0 = 0; c0 < kHeadDim; c0 += 32) {
+        uint32_t o[32];
+        tmem_ld32_wait(my_o + c0, o);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-        tmem_st16(my_o + c0, o);
+        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+        tmem_st32(my_o + c0, o);
       }
     };
 
@@ -271,117 +299,109 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
       float m = kUnset, l = 0.f;                   // M, the sum in units of 2^(M - E)
       int e_ref = kNoScale, deepest = 0;           // E; least eV - E of the blocks so far
       bool begun = false;                          // O holds something
+#pragma unroll 1
       for (int i = (n0 & 1) ^ group; i < t.units; i += 2) {
         const int n = n0 + i, stage = n % kStages;
         bounded_wait_warp(&s.full[stage], (n / kStages) & 1, gave_up);
         const Block blk[2] = {s.block[stage][0], s.block[stage][1]};
         mbar_arrive_warp(&s.empty[stage]);
-        int seen[2], e_blk[2];
-        float c[2], ev[2], dv[2];
-        const int e_most = (int16_t)blk[0].e_unit;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          seen[h] = (blk[h].tokens & bit) ? max(min(limit - blk[h].pos, blk[h].valid), 0) : 0;
-          e_blk[h] = blk[h].e_v == kNanScale ? kNoScale : blk[h].e_v;
-          c[h] = fmaxf(c_row * blk[h].k_scale, 1e-37f);        // (-inf of a masked key times 0 would be NaN)
-        }
-        const int e_new = e_ref != kNoScale && e_most - e_ref <= kHighest ? e_ref : e_most == kNoScale ? 0 : e_most;
-        float back = 1.f;                          // what the sums so far are multiplied with
-        if (e_new != e_ref && e_ref != kNoScale) {
-          const int delta = e_new - e_ref, bump = max(kDeepest - (deepest - delta), 0);
-          deepest = max(deepest - delta, kDeepest);
-          l *= pow2i(min(delta - bump, 127));
-          if (m != kUnset) m += (float)bump;
-          back = pow2i(-bump);
-        }
-        e_ref = e_new;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int d = e_blk[h] > kNoScale ? max(e_blk[h] - e_ref, kDeepest) : 0;
-          deepest = min(deepest, d);
-          dv[h] = (float)d;
-          ev[h] = (float)(e_ref + d);
-        }
-        bounded_wait_warp(&bar_s[group], (n >> 1) & 1, gave_up);
-        tc_fence_after();
-        if (idle) {                                // (what lies in its rows stays in its rows)
-          tc_fence_before();
-          mbar_arrive_warp(&bar_p[group]);
-          continue;
-        }
-        const bool all = __all_sync(0xFFFFFFFFu, seen[0] == kBlockN && seen[1] == kBlockN);
-        bool odd = c_nan;                          // a NaN among the row's numbers, or values too small beside the others'
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          odd |= !(blk[h].k_scale == blk[h].k_scale) || blk[h].e_v == kNanScale || (e_blk[h] > kNoScale && e_blk[h] - e_ref < kDeepest);
-        odd = __any_sync(0xFFFFFFFFu, odd);
-        __syncwarp();
-        if (__any_sync(0xFFFFFFFFu, back != 1.f)) rescale(back, begun, n);
-        uint32_t w[64];                            // fp16 pairs
-        float sum[2];
-        weights(my_s, w, sum, seen, c, ev, m, all);
-        if (__any_sync(0xFFFFFFFFu, !(sum[0] + sum[1] <= kMost)) || odd) {
-          // the row's largest score: a new reference where it is far above the old one
-          float top = -INFINITY;
 #pragma unroll 1
-          for (int j0 = 0; j0 < kUnit; j0 += 16) {
-            uint32_t x[16];
-            tmem_ld16(my_s + j0, x);
-            tmem_wait_ld();
-            const int h = j0 >> 6, see = (h ? seen[1] : seen[0]) - (j0 & 63);
-            float a = -INFINITY;
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (j < see) a = fmaxf(a, __uint_as_float(x[j]));
-            const float scale = h ? blk[1].k_scale : blk[0].k_scale;
-            if (scale == scale && !c_nan) top = fmaxf(top, fmaf(a, h ? c[1] : c[0], h ? ev[1] : ev[0]));
+        for (int h = 0; h < 2; ++h) {
+          const float k_scale = h ? blk[1].k_scale : blk[0].k_scale;
+          const int e_v = h ? blk[1].e_v : blk[0].e_v, pos = h ? blk[1].pos : blk[0].pos, valid = h ? blk[1].valid : blk[0].valid;
+          const uint32_t selecting = h ? blk[1].tokens : blk[0].tokens;
+          bounded_wait_warp(&bar_s[group][h], (n >> 1) & 1, gave_up);
+          tc_fence_after();
+          if (idle) {                              // (what lies in its rows stays in its rows)
+            tc_fence_before();
+            mbar_arrive_warp(&bar_p[group][h]);
+            continue;
           }
-          float f = 1.f;
-          if (top - m > kFirst) {                  // (where the sum alone is large, it moves too)
-            f = m == kUnset ? 0.f : ex2(m - (top - kFirst));
-            l = l > 0.f ? l * f : l;
-            m = top - kFirst;
+          const int seen = selecting & bit ? max(min(limit - pos, valid), 0) : 0;
+          const bool all = __all_sync(0xFFFFFFFFu, seen == kBlockN);
+          uint32_t w[32];
+          // E follows a block far above it; what came before is that much smaller
+          const bool has = e_v > kNoScale && e_v < kNanScale;
+          float back = 1.f;
+          if (has && (e_ref == kNoScale || e_v - e_ref > kHighest)) {
+            if (e_ref != kNoScale) {
+              const int delta = e_v - e_ref, bump = max(kDeepest - (deepest - delta), 0);
+              deepest = max(deepest - delta, kDeepest);
+              l *= pow2i(min(delta - bump, 127));
+              if (m != kUnset) m += (float)bump;
+              back = pow2i(-bump);
+            }
+            e_ref = e_v;
           }
-          __syncwarp();
-          rescale(f, begun, n);
-          weights(my_s, w, sum, seen, c, ev, m, all);
-          if (odd) {
+          const int e_now = e_ref == kNoScale ? 0 : e_ref, d = has ? max(e_v - e_now, kDeepest) : 0;
+          deepest = min(deepest, d);
+          const float c = fmaxf(c_row * k_scale, 1e-37f);      // (-inf of a masked key times 0 would be NaN)
+          const float ev = (float)(e_now + d);
+          // a NaN among the row's numbers, or values too small beside the others'
+          const bool nan_key = c_nan || !(k_scale == k_scale), nan_value = e_v == kNanScale, none = has && e_v - e_now < kDeepest;
+          const bool odd = __any_sync(0xFFFFFFFFu, nan_key || nan_value || none);
+          float sum = 0.f;
+#pragma unroll 1
+          for (bool again = false;; again = true) {
+            if (again) {
+              // the row's largest score: a new reference where it is above the old one
+              float top = -INFINITY;
+#pragma unroll 1
+              for (int j0 = 0; j0 < kBlockN; j0 += 16) {
+                uint32_t x[16];
+                tmem_ld16(my_s + kBlockN * h + j0, x);
+                tmem_wait_ld();
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const bool nan_key = c_nan || !(blk[h].k_scale == blk[h].k_scale), nan_value = blk[h].e_v == kNanScale;
-              const bool none = !nan_value && e_blk[h] > kNoScale && e_blk[h] - e_ref < kDeepest;
-              if (nan_key) sum[h] = seen[h] > 0 ? NAN : 0.f;
-#pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                const uint32_t here = (2 * j < seen[h] ? 0xFFFFu : 0u) | (2 * j + 1 < seen[h] ? 0xFFFF0000u : 0u);
-                if (nan_key || nan_value) w[32 * h + j] = here & 0x7FFF7FFFu;
-                else if (none) w[32 * h + j] = 0u;
+                for (int j = 0; j < 16; ++j)
+                  if (j0 + j < seen) top = fmaxf(top, __uint_as_float(x[j]));
               }
+              top = nan_key ? -INFINITY : fmaf(top, c, ev);
+              float f = back;
+              if (top - m > kFirst) {
+                const float g = m == kUnset ? 0.f : ex2(m - (top - kFirst));
+                f *= g;
+                l = l > 0.f ? l * g : l;
+                m = top - kFirst;
+              }
+              __syncwarp();
+              if (begun) rescale(f, n, h);
+            }
+            uint32_t x[64];
+            tmem_ld64_wait(my_s + kBlockN * h, x);
+            if (!all) {
+#pragma unroll
+              for (int j = 0; j < 64; ++j)
+                if (j >= seen) x[j] = 0xFF800000u;
+            }
+            sum = weights(x, w, c, ev - m);
+            if (again || !(__any_sync(0xFFFFFFFFu, !(sum <= kMost) || back != 1.f) || odd)) break;
+          }
+          if (odd) {
+            if (nan_key) sum = seen > 0 ? NAN : 0.f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const uint32_t here = (2 * j < seen ? 0xFFFFu : 0u) | (2 * j + 1 < seen ? 0xFFFF0000u : 0u);
+              if (nan_key || nan_value) w[j] = here & 0x7FFF7FFFu;
+              else if (none) w[j] = 0u;
             }
           }
+          begun = true;
+          tmem_st32(my_s + kBlockN * h, w);
+          l += sum * ex2((float)-d);
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive_warp(&bar_p[group][h]);
         }
-        begun = true;
-#pragma unroll
-        for (int j = 0; j < 64; j += 16) {
-          uint32_t part[16];
-#pragma unroll
-          for (int k = 0; k < 16; ++k) part[k] = w[j + k];
-          tmem_st16(my_s + j, part);
-        }
-        l += sum[0] * ex2(-dv[0]) + sum[1] * ex2(-dv[1]);
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive_warp(&bar_p[group]);
       }
       s_top[group][r] = m;
-      s_lse[group][r] = l == 0.f ? -INFINITY : m - (float)e_ref + lg2(l);
+      s_lse[group][r] = l == 0.f ? -INFINITY : m - (float)(e_ref == kNoScale ? 0 : e_ref) + lg2(l);
       // the next item's query, while the last products run (every S of this item has been read)
       next_item(item + 1);
       if (next.units > 0) write_query(next);
 
       // ---- the item's results: each group has half of the features
       const int n1 = n0 + t.units;
-      for (int n = max(n1 - 2, n0); n < n1; ++n) bounded_wait_warp(&bar_pv[n & 1], (n >> 1) & 1, gave_up);
+      for (int n = max(n1 - 2, n0); n < n1; ++n) bounded_wait_warp(&bar_pv[n & 1][1], (n >> 1) & 1, gave_up);
       tc_fence_after();
       const float lse0 = s_lse[0][r], lse1 = s_lse[1][r];
       const float most = fmaxf(lse0, lse1), nan = lse0 != lse0 ? lse0 : lse1 != lse1 ? lse1 : 0.f;
