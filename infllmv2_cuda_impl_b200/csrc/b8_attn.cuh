@@ -100,11 +100,14 @@ __device__ __forceinline__ unsigned long long union_word(const AttnParams& p, in
 }
 
 // ------------------------------------------------------------------------ inside a CTA --
+// Bit of a unit whose two blocks are whole, seen by all tokens of the tile and not NaN.
+constexpr int kPlain = 0x100;
+
 // A block on its way through the CTA: written by the fetching warp, read by the softmax.
 struct __align__(16) Block {
   float k_scale;                                   // 2^eK, or NaN
   int e_v;                                         // eV; kNoScale without keys, kNanScale: NaN block
-  int valid;                                       // keys (0: the block only fills a unit)
+  int valid;                                       // keys (0: the block only fills a unit), and kPlain
   int e_unit;                                      // largest (low half) and least (high) eV of the unit's two blocks
   int pos;                                         // position of its first key
   uint32_t tokens;                                 // tokens that attend it
@@ -439,6 +442,11 @@ __device__ __forceinline__ void fetch(const AttnParams& p, const CUtensorMap* k_
           const int e_most = has ? r.e_v : kNoScale, e_least = has ? r.e_v : -kNoScale;
           r.e_unit = (max(e_most, __shfl_xor_sync(0xFFFFFFFFu, e_most, 1)) & 0xFFFF) |
                      min(e_least, __shfl_xor_sync(0xFFFFFFFFu, e_least, 1)) << 16;
+          // (all lanes of a pair have the same)
+          const bool plain = r.valid == kBlockN && has && r.k_scale == r.k_scale && r.tokens == (1u << tokens) - 1 &&
+                             (!p.causal || r.pos + kBlockN <= reach - (tokens - 1));
+          const bool both = __shfl_xor_sync(0xFFFFFFFFu, (int)plain, 1) && plain;
+          if (both) r.valid |= kPlain;
           if (next) scales();
         }
         for (; u <= j; u += 2) {

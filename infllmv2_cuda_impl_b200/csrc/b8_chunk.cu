@@ -34,8 +34,15 @@ constexpr float kFirst = 4.f, kMost = 32768.f;
 // Instruction descriptor, kind::f16 with fp16 operands, B MN-major.
 constexpr uint32_t kIdescValues = (1u << 4) | (1u << 16) | (128u >> 3 << 17) | (128u >> 4 << 24);
 
-// A row's 64 weights of a block as fp16 pairs, 2^(x c + b); returns their sum.
-__device__ __forceinline__ float weights(const uint32_t (&x)[64], uint32_t (&w)[32], float c, float b) {
+// A row's 64 weights of a block as fp16 pairs, 2^(x c + b), 0 from key `see` on; returns their sum.
+__device__ __forceinline__ float weights(uint32_t scores, uint32_t (&w)[32], float c, float b, bool all, int see) {
+  uint32_t x[64];
+  tmem_ld64_wait(scores, x);
+  if (!all) {
+#pragma unroll
+    for (int j = 0; j < kBlockN; ++j)
+      if (j >= see) x[j] = 0xFF800000u;
+  }
   const uint64_t b2 = pack_f32x2(b, b), c2 = pack_f32x2(c, c);
   uint64_t sum2 = 0, sum2b = 0;
 #pragma unroll
@@ -184,8 +191,11 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
     __syncwarp();
   } else if (warp >= 10) {
     // ---------------------------------------------------------------- values to fp16
-    // A thread has 16 features of every 16th key.
-    const int ctid = tid - 320, c = ctid & 7;
+    // A warp takes 8 rows x 64 features at a time, a thread 16 features.  Eight neighbouring threads have pieces of two rows whose
+    // numbers differ by 5 in the swizzle (bits 0 and 2), so that neither their reads nor their writes, of every other
+    // 16-byte piece, meet in a bank.
+    const int cwarp = warp - 10, quarter = lane >> 3, c = lane & 3, at = lane & 4 ? quarter ^ 5 : quarter;      // at: row of eight
+    const int from0 = (cwarp * 16 + at) * kHeadDim + ((c ^ at) << 4), to0 = (cwarp * 16 + at) * 128 + (((2 * c) ^ at) << 4);
     int n = 0;
     for (int item = 0;; ++item) {
       if (!bounded_wait_warp(&s.item_full[item & 1], (item >> 1) & 1, gave_up)) break;
@@ -195,18 +205,21 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
       for (int i = 0; i < units; ++i, ++n) {
         const int stage = n % kStages, g = n & 1;
         bounded_wait_warp(&s.full[stage], (n / kStages) & 1, gave_up);
-        const int valid[2] = {s.block[stage][0].valid, s.block[stage][1].valid};
-        const uint8_t* from = smem + kRing + stage * 2 * kTileBytes + kTileBytes;
-        uint8_t* to = smem + kV + g * kVBytes + (c >> 2) * (kVBytes / 2);
+        const int valid[2] = {s.block[stage][0].valid & 0xFF, s.block[stage][1].valid & 0xFF};
+        const uint8_t* tile = smem + kRing + stage * 2 * kTileBytes + kTileBytes;
+        uint8_t* place = smem + kV + g * kVBytes;
 #pragma unroll 1
         for (int h = 0; h < 2; ++h) {
           if (n >= 2) bounded_wait_warp(&bar_pv[g][h], ((n - 2) >> 1) & 1, gave_up);      // the block's place is free again
+          const int have = (h ? valid[1] : valid[0]) - cwarp * 16 - at;      // > 8 j: the thread's row in step j is a key
+          const uint8_t* from = tile + h * (kTileBytes / 2);
+          uint8_t* to = place + h * (kVBytes / 4);
 #pragma unroll
-          for (int j = 0; j < kBlockN / 16; ++j) {
-            const int row = h * kBlockN + j * 16 + (ctid >> 3), at = row & 7;
-            uint4 x = *reinterpret_cast<const uint4*>(from + row * kHeadDim + ((c ^ at) << 4));
+          for (int i = 0; i < 4; ++i) {
+            const int j = i >> 1, half = i & 1;    // eight rows, 64 features
+            uint4 x = *reinterpret_cast<const uint4*>(from + (from0 ^ (half << 6)) + j * 8 * kHeadDim);
             // a value row that is no key may hold anything: 0 x NaN
-            if ((row & 63) >= (h ? valid[1] : valid[0])) x = make_uint4(0, 0, 0, 0);
+            if (have <= 8 * j) x = make_uint4(0, 0, 0, 0);
             uint32_t y[8];
             const uint32_t* w = reinterpret_cast<const uint32_t*>(&x);
 #pragma unroll
@@ -214,16 +227,14 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
               if (kCode == kE4m3) {
                 asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
                     : "=r"(y[2 * k]), "=r"(y[2 * k + 1]) : "r"(w[k]));
-              } else {                               // the upper bytes of fp16 numbers
+              } else {                             // the upper bytes of fp16 numbers
                 y[2 * k] = __byte_perm(w[k], 0u, 0x1404);
                 y[2 * k + 1] = __byte_perm(w[k], 0u, 0x3424);
               }
             }
-            // (the two halves lie in the same banks: one's even pieces are written beside the other's odd ones)
-            const int first = (c & 3) * 2 + (c >> 2), second = first ^ 1;
-            const bool odd = c >> 2;
-            *reinterpret_cast<uint4*>(to + row * 128 + ((first ^ at) << 4)) = odd ? make_uint4(y[4], y[5], y[6], y[7]) : make_uint4(y[0], y[1], y[2], y[3]);
-            *reinterpret_cast<uint4*>(to + row * 128 + ((second ^ at) << 4)) = odd ? make_uint4(y[0], y[1], y[2], y[3]) : make_uint4(y[4], y[5], y[6], y[7]);
+            uint8_t* at_half = to + half * (kVBytes / 2) + j * 8 * 128;
+            *reinterpret_cast<uint4*>(at_half + to0) = make_uint4(y[0], y[1], y[2], y[3]);
+            *reinterpret_cast<uint4*>(at_half + (to0 ^ 16)) = make_uint4(y[4], y[5], y[6], y[7]);
           }
           fence_proxy_async_smem();
           mbar_arrive_warp(&bar_v[g][h]);
@@ -305,41 +316,58 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
         bounded_wait_warp(&s.full[stage], (n / kStages) & 1, gave_up);
         const Block blk[2] = {s.block[stage][0], s.block[stage][1]};
         mbar_arrive_warp(&s.empty[stage]);
+        if (idle) {                                // (what lies in its rows stays in its rows)
 #pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          const float k_scale = h ? blk[1].k_scale : blk[0].k_scale;
-          const int e_v = h ? blk[1].e_v : blk[0].e_v, pos = h ? blk[1].pos : blk[0].pos, valid = h ? blk[1].valid : blk[0].valid;
-          const uint32_t selecting = h ? blk[1].tokens : blk[0].tokens;
-          bounded_wait_warp(&bar_s[group][h], (n >> 1) & 1, gave_up);
-          tc_fence_after();
-          if (idle) {                              // (what lies in its rows stays in its rows)
-            tc_fence_before();
+          for (int h = 0; h < 2; ++h) {
+            bounded_wait_warp(&bar_s[group][h], (n >> 1) & 1, gave_up);
             mbar_arrive_warp(&bar_p[group][h]);
-            continue;
           }
-          const int seen = selecting & bit ? max(min(limit - pos, valid), 0) : 0;
-          const bool all = __all_sync(0xFFFFFFFFu, seen == kBlockN);
-          uint32_t w[32];
+          continue;
+        }
+        // Of both blocks: keys that the row sees, factor of the scores, eV - E.  Nearly every unit is plain (every row sees all of
+        // it, see Block) and near E: the rest of this is for the others.
+        int seen[2] = {kBlockN, kBlockN}, d[2];
+        float cs[2], back = 1.f;
+        bool all_seen[2] = {true, true}, odd = false;      // odd: a NaN among the row's numbers, or values too small beside the others'
+        const int e_most = (int16_t)blk[0].e_unit, e_least = blk[0].e_unit >> 16;
+        if ((blk[0].valid & kPlain) && e_most - e_ref <= kHighest && e_least - e_ref >= kDeepest) {
+          deepest = min(deepest, e_least - e_ref);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) d[h] = blk[h].e_v - e_ref, cs[h] = c_row * blk[h].k_scale;
+        } else {
           // E follows a block far above it; what came before is that much smaller
-          const bool has = e_v > kNoScale && e_v < kNanScale;
-          float back = 1.f;
-          if (has && (e_ref == kNoScale || e_v - e_ref > kHighest)) {
+          if (e_most > kNoScale && (e_ref == kNoScale || e_most - e_ref > kHighest)) {
             if (e_ref != kNoScale) {
-              const int delta = e_v - e_ref, bump = max(kDeepest - (deepest - delta), 0);
+              const int delta = e_most - e_ref, bump = max(kDeepest - (deepest - delta), 0);
               deepest = max(deepest - delta, kDeepest);
               l *= pow2i(min(delta - bump, 127));
               if (m != kUnset) m += (float)bump;
               back = pow2i(-bump);
             }
-            e_ref = e_v;
+            e_ref = e_most;
           }
-          const int e_now = e_ref == kNoScale ? 0 : e_ref, d = has ? max(e_v - e_now, kDeepest) : 0;
-          deepest = min(deepest, d);
-          const float c = fmaxf(c_row * k_scale, 1e-37f);      // (-inf of a masked key times 0 would be NaN)
-          const float ev = (float)(e_now + d);
-          // a NaN among the row's numbers, or values too small beside the others'
-          const bool nan_key = c_nan || !(k_scale == k_scale), nan_value = e_v == kNanScale, none = has && e_v - e_now < kDeepest;
-          const bool odd = __any_sync(0xFFFFFFFFu, nan_key || nan_value || none);
+          const int e_base = e_ref == kNoScale ? 0 : e_ref;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            seen[h] = blk[h].tokens & bit ? max(min(limit - blk[h].pos, blk[h].valid & 0xFF), 0) : 0;
+            all_seen[h] = __all_sync(0xFFFFFFFFu, seen[h] == kBlockN);
+            const bool has = blk[h].e_v > kNoScale && blk[h].e_v < kNanScale;
+            d[h] = has ? max(blk[h].e_v - e_base, kDeepest) : 0;
+            deepest = min(deepest, d[h]);
+            cs[h] = fmaxf(c_row * blk[h].k_scale, 1e-37f);     // (-inf of a masked key times 0 would be NaN)
+            odd |= !(blk[h].k_scale == blk[h].k_scale) || blk[h].e_v == kNanScale || (has && blk[h].e_v - e_base < kDeepest);
+          }
+          odd = __any_sync(0xFFFFFFFFu, odd || c_nan);
+        }
+        const int e_now = e_ref == kNoScale ? 0 : e_ref;
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h, back = 1.f) {
+          const int see = h ? seen[1] : seen[0], dv = h ? d[1] : d[0];
+          const bool all = h ? all_seen[1] : all_seen[0];
+          const float c = h ? cs[1] : cs[0], ev = (float)(e_now + dv);
+          uint32_t w[32];
+          bounded_wait_warp(&bar_s[group][h], (n >> 1) & 1, gave_up);
+          tc_fence_after();
           float sum = 0.f;
 #pragma unroll 1
           for (bool again = false;; again = true) {
@@ -353,9 +381,10 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                 tmem_wait_ld();
 #pragma unroll
                 for (int j = 0; j < 16; ++j)
-                  if (j0 + j < seen) top = fmaxf(top, __uint_as_float(x[j]));
+                  if (j0 + j < see) top = fmaxf(top, __uint_as_float(x[j]));
               }
-              top = nan_key ? -INFINITY : fmaf(top, c, ev);
+              const float k_scale = h ? blk[1].k_scale : blk[0].k_scale;
+              top = c_nan || !(k_scale == k_scale) ? -INFINITY : fmaf(top, c, ev);
               float f = back;
               if (top - m > kFirst) {
                 const float g = m == kUnset ? 0.f : ex2(m - (top - kFirst));
@@ -366,28 +395,25 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
               __syncwarp();
               if (begun) rescale(f, n, h);
             }
-            uint32_t x[64];
-            tmem_ld64_wait(my_s + kBlockN * h, x);
-            if (!all) {
-#pragma unroll
-              for (int j = 0; j < 64; ++j)
-                if (j >= seen) x[j] = 0xFF800000u;
-            }
-            sum = weights(x, w, c, ev - m);
+            sum = weights(my_s + kBlockN * h, w, c, ev - m, all, see);
             if (again || !(__any_sync(0xFFFFFFFFu, !(sum <= kMost) || back != 1.f) || odd)) break;
           }
           if (odd) {
-            if (nan_key) sum = seen > 0 ? NAN : 0.f;
+            const float k_scale = h ? blk[1].k_scale : blk[0].k_scale;
+            const int e_v = h ? blk[1].e_v : blk[0].e_v;
+            const bool nan_key = c_nan || !(k_scale == k_scale), nan_value = e_v == kNanScale;
+            const bool none = e_v > kNoScale && !nan_value && e_v - e_now < kDeepest;
+            if (nan_key) sum = see > 0 ? NAN : 0.f;
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
-              const uint32_t here = (2 * j < seen ? 0xFFFFu : 0u) | (2 * j + 1 < seen ? 0xFFFF0000u : 0u);
+              const uint32_t here = (2 * j < see ? 0xFFFFu : 0u) | (2 * j + 1 < see ? 0xFFFF0000u : 0u);
               if (nan_key || nan_value) w[j] = here & 0x7FFF7FFFu;
               else if (none) w[j] = 0u;
             }
           }
           begun = true;
           tmem_st32(my_s + kBlockN * h, w);
-          l += sum * ex2((float)-d);
+          l += sum * ex2((float)-dv);
           tmem_wait_st();
           tc_fence_before();
           mbar_arrive_warp(&bar_p[group][h]);

@@ -201,7 +201,7 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
         bounded_wait_warp(&s.full[stage], (n / kStages) & 1, gave_up);
         const Block* blk = &s.block[stage][r >> 6];
         const float k_scale = blk->k_scale;
-        const int e_v = blk->e_v, valid = blk->valid, e_unit = blk->e_unit, e_most = (int16_t)e_unit;
+        const int e_v = blk->e_v, valid = blk->valid & 0xFF, e_unit = blk->e_unit, e_most = (int16_t)e_unit;
         const int e_new = e_ref != kNoScale && e_most - e_ref <= kHighest ? e_ref : e_most == kNoScale ? 0 : e_most;
         // which columns' tokens see the thread's key: the last token those below `valid`, the ones before it fewer if causal
         const int left = valid - (r & 63);         // > 0: a key
