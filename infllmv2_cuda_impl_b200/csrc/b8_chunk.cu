@@ -252,19 +252,28 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
     const int heads = p.heads_k * kGroup;
 
     // Query rows of an item: 8 threads per row, 16 values each.
+    // (two tokens at a time, the next ones' values on their way; code that runs once per tile is kept short, since every line of
+    // it comes from far away)
     const auto write_query = [&](const Item& t) {
-#pragma unroll
-      for (int i = 0; i < kRows * 8 / kSoftmax; ++i) {
-        const int row = i * (kSoftmax / 8) + (stid >> 3), c = stid & 7;
-        uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-        if (row / kGroup < t.tokens) {
-          const uint4* src = reinterpret_cast<const uint4*>(
-              p.q + ((int64_t)(t.row + row / kGroup) * heads + t.head * kGroup + row % kGroup) * kHeadDim + c * 16);
-          x[0] = __ldg(src);
-          x[1] = __ldg(src + 1);
+      const int c = stid & 7, of_pair = stid >> 3;
+      const __nv_bfloat16* src = p.q + ((int64_t)(t.row + of_pair / kGroup) * heads + t.head * kGroup + of_pair % kGroup) * kHeadDim + c * 16;
+      const auto load = [&](int i, uint4 (&x)[2]) {
+        x[0] = x[1] = make_uint4(0, 0, 0, 0);
+        if (2 * i + of_pair / kGroup < t.tokens) {
+          const uint4* at = reinterpret_cast<const uint4*>(src + (int64_t)2 * i * heads * kHeadDim);
+          x[0] = __ldg(at), x[1] = __ldg(at + 1);
         }
+      };
+      uint4 x[2];
+      load(0, x);
+#pragma unroll 1
+      for (int i = 0; 2 * i < t.tokens; ++i) {
+        uint4 y[2];
+        load(i + 1, y);
+        const int row = 32 * i + of_pair;
         const float f = write_query16(x, smem + row * kHeadDim + ((c ^ (row & 7)) << 4), kQBytes, p.scale_log2);
         if (c == 0) s_c[row] = f;
+        x[0] = y[0], x[1] = y[1];
       }
       fence_proxy_async_smem();
       mbar_arrive_warp(&bar_q);
@@ -449,7 +458,7 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
       }
       __nv_bfloat16* out = p.out + ((int64_t)(t.row + tok) * heads + t.head * kGroup + r % kGroup) * kHeadDim + 64 * group;
       float* part = p.part_o + ((int64_t)max(t.piece, 0) * kRows + r) * kHeadDim + 64 * group;
-#pragma unroll
+#pragma unroll 1
       for (int c0 = 0; c0 < 64; c0 += 16) {
         float y[16];
 #pragma unroll
