@@ -545,7 +545,7 @@ int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void* k_scale, v
  *
  * The cache in 8 bits: codes (num_pages, heads_k, page_size, 128), code 0 e4m3, 1 e5m2, and a scale byte (e8m0, 255
  * NaN) per 64 tokens and head, (num_pages, heads_k, page_size / 64).
- * ifv2_b8_write: rows like ifv2_cache_write's (strides multiples of 4) quantised to their slots.  The rows of one
+ * ifv2_b8_write: rows like ifv2_cache_write's quantised to their slots.  The rows of one
  * block are consecutive tokens at consecutive slots; rows that begin a block set its scale, others may raise it, and
  * the block's earlier codes are then rounded to the new scale.
  * ifv2_b8_attn: q, out (total_q, heads_q, 128) bf16 of sequences cu_seqlens_q (batch + 1), none of more than

@@ -18,42 +18,47 @@ using namespace b8;
 
 constexpr int kThreads = 128, kWarps = kThreads / 32;
 constexpr int kBlock = kBlockN;                  // tokens of a block
-constexpr int kRowsPerWarp = 16;
+constexpr int kRowsPerWarp = 16, kSteps = kRowsPerWarp / 2;
 
 struct B8WriteParams {
-  const uint2 *k, *v;
-  int64_t k_token, k_head, v_token, v_head;      // strides in pieces of four values
+  const uint4 *k, *v;
+  int64_t k_token, k_head, v_token, v_head;      // strides in pieces of eight values
   uint8_t *k_cache, *v_cache, *k_scale, *v_scale;
   const int64_t* slots;
   int64_t total, limit;                          // tokens; slots of the cache
   int heads, page_size, segment;
 };
 
-__device__ __forceinline__ uint32_t amax_of(uint2 x, uint32_t amax) {
-  const uint32_t a = x.x & 0x7FFF7FFFu, b = x.y & 0x7FFF7FFFu;
-  return __vmaxu2(__vmaxu2(a, b), amax);         // bf16 magnitudes are ordered as their bits
+__device__ __forceinline__ uint32_t amax_of(const uint4& x, uint32_t amax) {
+  // bf16 magnitudes are ordered as their bits
+  amax = __vmaxu2(__vmaxu2(x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu), amax);
+  return __vmaxu2(__vmaxu2(x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu), amax);
+}
+template <int kCode>
+__device__ __forceinline__ uint32_t encode_pairs(uint32_t a, uint32_t b, float inv) {
+  const float y[4] = {__uint_as_float(a << 16), __uint_as_float(a & 0xFFFF0000u), __uint_as_float(b << 16), __uint_as_float(b & 0xFFFF0000u)};
+  return encode4<kCode>(y, inv);
 }
 
-// kAll: the CTA's warps share the run; otherwise one warp has it to itself.  `n` rows from token t0 on.
+// kAll: the CTA's warps share the run; otherwise one warp has it to itself.  `n` rows from token t0 on.  A warp takes two rows
+// at a time, 16 lanes each with 8 values.
 template <int kCode, bool kAll>
 __device__ __forceinline__ void write_run(const B8WriteParams& p, int64_t t0, int n, int64_t slot, int head, bool val, uint32_t* s_max) {
-  const int lane = threadIdx.x & 31, warp = kAll ? threadIdx.x >> 5 : 0;
-  constexpr int kStep = kAll ? kWarps : 1;
-  const uint2* src = (val ? p.v : p.k) + t0 * (val ? p.v_token : p.k_token) + (int64_t)head * (val ? p.v_head : p.k_head);
-  const int64_t step = val ? p.v_token : p.k_token;
-  uint2 x[kRowsPerWarp];
+  const int lane = threadIdx.x & 31, warp = kAll ? threadIdx.x >> 5 : 0, piece = lane & 15;
+  constexpr int kStep = 2 * (kAll ? kWarps : 1);
+  const int r0 = 2 * warp + (lane >> 4);
+  const int64_t token = val ? p.v_token : p.k_token;
+  const uint4* src = (val ? p.v : p.k) + (t0 + r0) * token + (int64_t)head * (val ? p.v_head : p.k_head) + piece;
+  uint4 x[kSteps];
 #pragma unroll
-  for (int i = 0; i < kRowsPerWarp; ++i) {
-    const int r = warp + i * kStep;
-    x[i] = r < n ? __ldcs(src + r * step + lane) : make_uint2(0u, 0u);
-  }
+  for (int i = 0; i < kSteps; ++i, src += kStep * token) x[i] = r0 + i * kStep < n ? __ldcs(src) : make_uint4(0u, 0u, 0u, 0u);
   const int64_t page = slot / p.page_size;
   const int place = (int)(slot - page * p.page_size), off = place & (kBlock - 1);
   uint8_t* scale = (val ? p.v_scale : p.k_scale) + (page * p.heads + head) * (p.page_size / kBlock) + place / kBlock;
   const int before = off > 0 ? *scale : 0;
   uint32_t m2 = 0;
 #pragma unroll
-  for (int i = 0; i < kRowsPerWarp; ++i) m2 = amax_of(x[i], m2);
+  for (int i = 0; i < kSteps; ++i) m2 = amax_of(x[i], m2);
   uint32_t amax = __reduce_max_sync(0xFFFFFFFFu, max(m2 & 0xFFFFu, m2 >> 16));
   if (kAll) {
     if (lane == 0) s_max[warp] = amax;
@@ -62,26 +67,28 @@ __device__ __forceinline__ void write_run(const B8WriteParams& p, int64_t t0, in
     for (int w = 0; w < kWarps; ++w) amax = max(amax, s_max[w]);
   }
   const int byte = max(scale_byte<kCode>(amax << 16), before);
-  const float inv = byte == kNanByte ? 0.f : q8::inverse_scale(byte);
-  uint8_t* rows = (val ? p.v_cache : p.k_cache) + ((page * p.heads + head) * (int64_t)p.page_size + place) * kHeadDim;
+  uint8_t* rows = (val ? p.v_cache : p.k_cache) + ((page * p.heads + head) * (int64_t)p.page_size + place) * kHeadDim + piece * 8;
   if (byte > before && off > 0 && byte != kNanByte) {            // earlier rows of the block: to the new scale
     const float down = __uint_as_float((uint32_t)(127 - min(byte - before, 64)) << 23);
-    for (int r = warp - off; r < 0; r += kStep) {
-      uint32_t* at = reinterpret_cast<uint32_t*>(rows + (int64_t)r * kHeadDim) + lane;
-      float y[4];
-      decode4<kCode>(y, *at);
-      *at = encode4<kCode>(y, down);
+    for (int r = r0 - off; r < 0; r += kStep) {
+      uint2* at = reinterpret_cast<uint2*>(rows + (int64_t)r * kHeadDim);
+      const uint2 c = *at;
+      float a[4], b[4];
+      decode4<kCode>(a, c.x);
+      decode4<kCode>(b, c.y);
+      *at = make_uint2(encode4<kCode>(a, down), encode4<kCode>(b, down));
     }
   }
+  uint8_t* to = rows + r0 * kHeadDim;
+  if (byte == kNanByte) {
 #pragma unroll
-  for (int i = 0; i < kRowsPerWarp; ++i) {
-    const int r = warp + i * kStep;
-    if (r < n) {
-      const float y[4] = {__uint_as_float(x[i].x << 16), __uint_as_float(x[i].x & 0xFFFF0000u), __uint_as_float(x[i].y << 16),
-                          __uint_as_float(x[i].y & 0xFFFF0000u)};
-      reinterpret_cast<uint32_t*>(rows + (int64_t)r * kHeadDim)[lane] = byte == kNanByte ? 0u : encode4<kCode>(y, inv);
-    }
+    for (int i = 0; i < kSteps; ++i) x[i] = make_uint4(0u, 0u, 0u, 0u);
   }
+  const float inv = q8::inverse_scale(byte);
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i)
+    if (r0 + i * kStep < n)
+      *reinterpret_cast<uint2*>(to + i * kStep * kHeadDim) = make_uint2(encode_pairs<kCode>(x[i].x, x[i].y, inv), encode_pairs<kCode>(x[i].z, x[i].w, inv));
   if (kAll) __syncthreads();                     // s_max is free again; `before` has been read by every warp
   else __syncwarp();
   if (warp == 0 && lane == 0) *scale = (uint8_t)byte;
@@ -147,15 +154,15 @@ extern "C" int ifv2_b8_write(const void* k, const void* v, int64_t k_token, int6
   IFV2_REQUIRE(heads_k <= 32767 && total < (1ll << 31), IFV2_ERR_TOO_LARGE, "b8_write: at most 32767 heads and 2^31 - 1 tokens");
   if (total == 0 || num_pages == 0) return IFV2_OK;
   IFV2_REQUIRE(k && v && k_cache && v_cache && k_scale && v_scale && slots, IFV2_ERR_INVALID_ARG, "b8_write: null pointer");
-  IFV2_REQUIRE(((k_token | k_head | v_token | v_head) & 3) == 0 &&
-               ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 7) == 0 &&
-               ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 3) == 0,
-               IFV2_ERR_INVALID_ARG, "b8_write: rows of k and v must begin at multiples of 8 bytes, caches at multiples of 4");
+  IFV2_REQUIRE(((k_token | k_head | v_token | v_head) & 7) == 0 &&
+               ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0 &&
+               ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 7) == 0,
+               IFV2_ERR_INVALID_ARG, "b8_write: rows of k and v must begin at multiples of 16 bytes, caches at multiples of 8");
   // The longest segment that still gives every SM a few CTAs: with short ones many CTAs find that no run begins in
   // theirs, with long ones the runs of a decode step queue up in few.
   int segment = kBlockN;
   while (segment > 1 && ceil_div64(total, segment) * heads_k * 2 < 4 * kNumSMs) segment /= 4;
-  B8WriteParams p{static_cast<const uint2*>(k), static_cast<const uint2*>(v), k_token / 4, k_head / 4, v_token / 4, v_head / 4,
+  B8WriteParams p{static_cast<const uint4*>(k), static_cast<const uint4*>(v), k_token / 8, k_head / 8, v_token / 8, v_head / 8,
                   static_cast<uint8_t*>(k_cache), static_cast<uint8_t*>(v_cache), static_cast<uint8_t*>(k_scale),
                   static_cast<uint8_t*>(v_scale), slots, total, num_pages * page_size, heads_k, page_size, segment};
   const dim3 grid((unsigned)ceil_div64(total, segment), 2 * heads_k);
