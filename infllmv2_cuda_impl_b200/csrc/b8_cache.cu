@@ -95,7 +95,7 @@ __device__ __forceinline__ void write_run(const B8WriteParams& p, int64_t t0, in
 }
 
 template <int kCode>
-__global__ void __launch_bounds__(kThreads) b8_write_kernel(const B8WriteParams p) {
+__global__ void __launch_bounds__(kThreads, 8) b8_write_kernel(const B8WriteParams p) {
   __shared__ int64_t s_slot[2 * kBlock + 1];     // of the token before the segment, the segment's, and 63 behind it
   __shared__ uint64_t s_start;                   // tokens of the segment that begin a run
   __shared__ uint64_t s_end[2];                  // tokens (from the segment's first on) that do not continue one
