@@ -40,6 +40,7 @@ __global__ void __launch_bounds__(kPlanThreads) b8_plan_kernel(const AttnParams 
   __shared__ int64_t scratch[32], s_total;
   const int tid = threadIdx.x;
   allow_next();
+  wait_previous();
   int64_t before = 0;
   for (int base = 0; base < p.batch; base += kPlanThreads) {
     const int b = base + tid;
@@ -109,6 +110,7 @@ __global__ void __launch_bounds__(kJoinThreads) b8_join_kernel(const AttnParams 
   __shared__ float4 s_acc[4][32];
   __shared__ float s_most[4], s_sum[4];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, heads = p.heads_k * kGroup, columns = kGroup * tokens_per_tile;
+  wait_previous();
   {
     const int64_t row0 = min(max((int64_t)p.cu_q[p.batch], (int64_t)0), p.total_q);
     const int64_t me = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kJoinThreads + tid, all = (int64_t)gridDim.x * gridDim.y * kJoinThreads;
@@ -117,7 +119,6 @@ __global__ void __launch_bounds__(kJoinThreads) b8_join_kernel(const AttnParams 
     if (p.lse)
       for (int64_t i = row0 * heads + me; i < p.total_q * heads; i += all) p.lse[i] = INFINITY;
   }
-  wait_previous();
   if (p.by_tile) {                                 // (a sequence without tokens has no tile)
     int row0;
     if (tokens_of(p, blockIdx.x / p.heads_k, row0) == 0) return;
@@ -184,21 +185,6 @@ __global__ void __launch_bounds__(kJoinThreads) b8_join_kernel(const AttnParams 
 }
 
 // ------------------------------------------------------------------------------- host --
-// Launch that may start beside the kernel in front of it.
-template <typename... Params, typename... Args>
-cudaError_t launch_beside(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_t stream, const Args&... args) {
-  cudaLaunchAttribute attribute{};
-  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t config{};
-  config.gridDim = grid;
-  config.blockDim = dim3(threads);
-  config.stream = stream;
-  config.attrs = &attribute;
-  config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, kernel, args...);
-}
-
 struct Layout {
   int tokens, grid;                                // of a tile; CTAs
   bool listed;
@@ -307,14 +293,15 @@ extern "C" int ifv2_b8_attn(const void* q, const void* k_cache, const void* v_ca
   p.first_tile = reinterpret_cast<int32_t*>(ws + at.first_at);
   cudaStream_t s = (cudaStream_t)stream;
   if (at.listed) {
-    b8_plan_kernel<<<1, kPlanThreads, 0, s>>>(p, at.grid);
+    const cudaError_t e = launch_beside(b8_plan_kernel, dim3(1), kPlanThreads, 0, s, p, at.grid);
+    if (e != cudaSuccess) return set_error((int)e, "b8_attn (plan): %s", cudaGetErrorString(e));
     if ((rc = check_launch("b8_attn (plan)"))) return rc;
   }
   rc = at.tokens <= 2 ? b8_launch_few(k_map, v_map, p, at.tokens, code, s) : b8_launch_chunk(k_map, v_map, p, at.listed, code, s);
   if (rc) return rc;
   const unsigned cuts = p.by_tile ? batch * heads_k : at.grid;
-  const cudaError_t e = at.tokens == 1 ? launch_beside(b8_join_kernel<true>, dim3(cuts, kGroup), kJoinThreads, s, p, at.tokens)
-                                       : launch_beside(b8_join_kernel<false>, dim3(cuts, 4 * at.tokens), kJoinThreads, s, p, at.tokens);
+  const cudaError_t e = at.tokens == 1 ? launch_beside(b8_join_kernel<true>, dim3(cuts, kGroup), kJoinThreads, 0, s, p, at.tokens)
+                                       : launch_beside(b8_join_kernel<false>, dim3(cuts, 4 * at.tokens), kJoinThreads, 0, s, p, at.tokens);
   if (e != cudaSuccess) return set_error((int)e, "b8_attn (join): %s", cudaGetErrorString(e));
   return check_launch("b8_attn (join)");
 }

@@ -19,6 +19,7 @@
 // and are joined by a second kernel.  Where a sequence has one tile per head (a decode step, drafts) every CTA finds
 // its share by itself, from the lengths; otherwise a kernel in front lists the tiles.
 #pragma once
+#include <atomic>
 #include <type_traits>
 #include "b8.cuh"
 
@@ -95,7 +96,7 @@ __device__ __forceinline__ unsigned long long union_word(const AttnParams& p, in
   if (w * 64 >= blocks) return 0;
   const unsigned long long* m = p.mask + ((int64_t)head * p.total_q + row) * p.words + w;
   unsigned long long u = 0;
-  for (int t = 0; t < tokens; ++t) u |= __ldg(m + (int64_t)t * p.words);
+  for (int t = 0; t < tokens; ++t) u |= *(m + (int64_t)t * p.words);
   return below(u, w, blocks);
 }
 
@@ -215,68 +216,84 @@ struct Common {
 };
 
 // ---------------------------------------------------------------------- fetching warp --
-// All lanes run it.  kListed: tiles come from the kernel in front.
-template <int kT, int kStages, bool kListed, bool kSelected>
-__device__ __forceinline__ void fetch(const AttnParams& p, const CUtensorMap* k_map, const CUtensorMap* v_map, Common<kT, kStages>& s,
-                                      uint8_t* ring) {
+// Where a CTA's share begins.  All lanes of a warp work it out, before the CTA's barriers and tensor memory are there.
+// kListed: tiles come from the kernel in front.
+template <int kT, bool kListed, bool kSelected>
+struct Deal {
   using Cost = typename std::conditional<kListed, int64_t, int>::type;
-  const int lane = threadIdx.x & 31;
-  volatile int* gave_up = &s.gave_up;
+  Shares<Cost> shares;
+  Cost lo = 0x7FFFFFFF, hi = 0, begin = 0;         // of the share; of the tile it begins in
   int b = 0, head = 0, row = 0, tokens = 0, reach = 0, tile = 0, n_tiles = 0;
-  Cost cost = 0, begin = 0, end = 0;               // of the call; of the tile
-  // cost of a head of sequence b, not listed
-  const auto cost_of = [&](int b, int& row, int& tokens, int& reach) {
+  int each = 0;                                    // cost of the sequence's heads
+  bool more = false;
+  // cost of a head of sequence b
+  static __device__ __forceinline__ int cost_of(const AttnParams& p, int b, int& row, int& tokens, int& reach) {
     tokens = min(tokens_of(p, b, row), kT);
     reach = keys_of(p, b);
     int n = ceil_div(reach, kUnit);
     if (kSelected) n = min(n, ceil_div(p.usual * (3 + tokens), 8));
     return tokens ? kStart + n : 0;
-  };
-  const int me = blockIdx.x;
-  int each = 0;                                    // cost of the sequence's heads
-  if (kListed) {
-    n_tiles = p.first_tile[gridDim.x];
-    cost = (Cost)p.start[n_tiles];
   }
-  Cost lo = 0x7FFFFFFF, hi = 0;
-  bool more = false;
-  Shares<Cost> shares;
-  for (int pass = kListed ? 1 : 0;; ++pass) {      // pass 0 adds costs up, pass 1 finds the sequence that this share begins in
-    if (pass == 1) {
-      shares.deal(max(cost, (Cost)1), gridDim.x, p.least_share);
-      lo = me < shares.grid ? shares.begin(me) : cost, hi = me < shares.grid ? shares.begin(me + 1) : cost;
-      more = lo < hi;
-      if (kListed) tile = p.first_tile[me];
-      if (kListed || !more) break;
+  __device__ __forceinline__ void begins(Cost cost, const AttnParams& p) {
+    const int me = blockIdx.x;
+    shares.deal(max(cost, (Cost)1), gridDim.x, p.least_share);
+    lo = me < shares.grid ? shares.begin(me) : cost, hi = me < shares.grid ? shares.begin(me + 1) : cost;
+    more = lo < hi;
+  }
+  __device__ __forceinline__ void work_out(const AttnParams& p) {
+    const int lane = threadIdx.x & 31;
+    if (kListed) {
+      n_tiles = p.first_tile[gridDim.x];
+      begins((Cost)p.start[n_tiles], p);
+      tile = p.first_tile[blockIdx.x];
+      return;
     }
-    int base = 0, before = 0;
-    for (; base < p.batch; base += 32) {
-      int r = 0, t = 0, k = 0, c = 0;
-      if (base + lane < p.batch) c = cost_of(base + lane, r, t, k);
-      int upto = c * p.heads_k;
+    for (int pass = 0;; ++pass) {                  // pass 0 adds costs up, pass 1 finds the sequence that the share begins in
+      int before = 0;
+      for (int base = 0; base < p.batch; base += 32) {
+        int r = 0, t = 0, k = 0, c = 0;
+        if (base + lane < p.batch) c = cost_of(p, base + lane, r, t, k);
+        int upto = c * p.heads_k;
 #pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
-        if (lane >= d) upto += o;
+        for (int d = 1; d < 32; d <<= 1) {
+          const int o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+          if (lane >= d) upto += o;
+        }
+        const uint32_t past = __ballot_sync(0xFFFFFFFFu, before + upto > (int)lo);
+        if (past) {
+          const int src = __ffs(past) - 1;
+          b = base + src;
+          row = __shfl_sync(0xFFFFFFFFu, r, src);
+          tokens = __shfl_sync(0xFFFFFFFFu, t, src);
+          reach = __shfl_sync(0xFFFFFFFFu, k, src);
+          each = __shfl_sync(0xFFFFFFFFu, c, src);
+          before += __shfl_sync(0xFFFFFFFFu, upto, src) - each * p.heads_k;
+          head = (int)((uint32_t)((int)lo - before) / (uint32_t)each);
+          begin = before + head * each;
+          return;
+        }
+        before += __shfl_sync(0xFFFFFFFFu, upto, 31);
       }
-      const uint32_t past = __ballot_sync(0xFFFFFFFFu, before + upto > (int)lo);
-      if (past) {
-        const int src = __ffs(past) - 1;
-        b = base + src;
-        row = __shfl_sync(0xFFFFFFFFu, r, src);
-        tokens = __shfl_sync(0xFFFFFFFFu, t, src);
-        reach = __shfl_sync(0xFFFFFFFFu, k, src);
-        each = __shfl_sync(0xFFFFFFFFu, c, src);
-        before += __shfl_sync(0xFFFFFFFFu, upto, src) - each * p.heads_k;
-        head = (int)((uint32_t)((int)lo - before) / (uint32_t)each);
-        begin = before + head * each;
-        break;
-      }
-      before += __shfl_sync(0xFFFFFFFFu, upto, 31);
+      if (pass == 1) return;
+      begins(before, p);
+      if (!more) return;
     }
-    if (pass == 1) break;
-    cost = before;
   }
+};
+
+// All lanes of a warp run it.
+template <int kT, int kStages, bool kListed, bool kSelected>
+__device__ __forceinline__ void fetch(const AttnParams& p, const CUtensorMap* k_map, const CUtensorMap* v_map, Common<kT, kStages>& s,
+                                      uint8_t* ring, const Deal<kT, kListed, kSelected>& deal) {
+  using D = Deal<kT, kListed, kSelected>;
+  using Cost = typename D::Cost;
+  const int lane = threadIdx.x & 31, me = blockIdx.x;
+  volatile int* gave_up = &s.gave_up;
+  const Shares<Cost>& shares = deal.shares;
+  const Cost lo = deal.lo, hi = deal.hi;
+  int b = deal.b, head = deal.head, row = deal.row, tokens = deal.tokens, reach = deal.reach, tile = deal.tile, each = deal.each;
+  Cost begin = deal.begin, end = 0;                // of the tile
+  bool more = deal.more;
   int4 cut = make_int4(0, 0, 0, 0);                // (first and last share the same: not cut)
   int n = 0, items = 0;                            // units, items so far
   for (bool first = true; more && !*gave_up; first = false) {
@@ -295,38 +312,54 @@ __device__ __forceinline__ void fetch(const AttnParams& p, const CUtensorMap* k_
     // the tile's blocks: all, or those that its tokens select, 4 words of their union per lane
     unsigned long long u[4] = {0, 0, 0, 0};
     int upto = 0, total = blocks;
+    const int32_t* list = nullptr;                 // one token's ascending list, walked as it is
     if (kSelected) {
-      if (p.lists) {
-        __syncwarp();
-        for (int i = lane; i < tokens * kMaxMaskWords; i += 32) s.words[i / kMaxMaskWords][i % kMaxMaskWords] = 0;
-        __syncwarp();
-        for (int t = 0; t < tokens; ++t) {
-          const int32_t* list = p.lists + ((int64_t)head * p.total_q + row + t) * p.topk;
-          for (int i = lane; i < p.topk; i += 32) {
-            const int block = __ldg(list + i);
-            if (block >= 0 && block < blocks)
-              atomicOr(reinterpret_cast<uint32_t*>(s.words[t]) + (block >> 5), 1u << (block & 31));
-          }
+      if (p.lists && tokens == 1) {
+        list = p.lists + ((int64_t)head * p.total_q + row) * p.topk;
+        bool ascending = true;                     // blocks of the sequence in front, nothing of it behind
+        total = 0;
+        for (int base = 0; base < p.topk; base += 32) {
+          const int i = base + lane;
+          const int x = i < p.topk ? *(list + i) : -1, y = i + 1 < p.topk ? *(list + i + 1) : -1;
+          const bool valid = x >= 0 && x < blocks, then = y >= 0 && y < blocks;
+          ascending &= valid ? !then || y > x : !then;
+          total += __popc(__ballot_sync(0xFFFFFFFFu, valid));
         }
-        __syncwarp();
+        if (!__all_sync(0xFFFFFFFFu, ascending)) list = nullptr;
       }
-      int count = 0;
+      if (list == nullptr) {
+        if (p.lists) {
+          __syncwarp();
+          for (int i = lane; i < tokens * kMaxMaskWords; i += 32) s.words[i / kMaxMaskWords][i % kMaxMaskWords] = 0;
+          __syncwarp();
+          for (int t = 0; t < tokens; ++t) {
+            const int32_t* from = p.lists + ((int64_t)head * p.total_q + row + t) * p.topk;
+            for (int i = lane; i < p.topk; i += 32) {
+              const int block = *(from + i);
+              if (block >= 0 && block < blocks)
+                atomicOr(reinterpret_cast<uint32_t*>(s.words[t]) + (block >> 5), 1u << (block & 31));
+            }
+          }
+          __syncwarp();
+        }
+        int count = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int w = 4 * lane + i;
-        if (p.lists)
-          for (int t = 0; t < tokens; ++t) u[i] |= s.words[t][w];
-        else if (w < p.words)
-          u[i] = union_word(p, head, row, tokens, w, blocks);
-        count += __popcll(u[i]);
-      }
-      upto = count;
+        for (int i = 0; i < 4; ++i) {
+          const int w = 4 * lane + i;
+          if (p.lists)
+            for (int t = 0; t < tokens; ++t) u[i] |= s.words[t][w];
+          else if (w < p.words)
+            u[i] = union_word(p, head, row, tokens, w, blocks);
+          count += __popcll(u[i]);
+        }
+        upto = count;
 #pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
-        if (lane >= d) upto += o;
+        for (int d = 1; d < 32; d <<= 1) {
+          const int o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+          if (lane >= d) upto += o;
+        }
+        total = __shfl_sync(0xFFFFFFFFu, upto, 31);
       }
-      total = __shfl_sync(0xFFFFFFFFu, upto, 31);
     }
     const int units = ceil_div(total, 2);
     // (a tile's cost is an estimate where blocks are selected: parts are in proportion)
@@ -354,6 +387,7 @@ __device__ __forceinline__ void fetch(const AttnParams& p, const CUtensorMap* k_
     }
     const auto nth_block = [&](int k) {            // all lanes, each with its k
       if (!kSelected) return k;
+      if (list) return *(list + k);
       int at = 0;                                  // lane whose words hold it: the first with upto > k
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1)
@@ -384,7 +418,7 @@ __device__ __forceinline__ void fetch(const AttnParams& p, const CUtensorMap* k_
     const auto look = [&](int k0) {
       block = nth_block(min(k0 + lane, total - 1));
       const int in_table = (int)(__umulhi(2u * (uint32_t)block, p.page_mul) >> p.page_shift);
-      page = p.block_table ? __ldg(p.block_table + (int64_t)b * p.bt_stride + in_table) : b;
+      page = p.block_table ? *(p.block_table + (int64_t)b * p.bt_stride + in_table) : b;
     };
     int row_of, kb, vb;
     const auto scales = [&]() {
@@ -393,8 +427,8 @@ __device__ __forceinline__ void fetch(const AttnParams& p, const CUtensorMap* k_
       const int place = block * kBlockN - in_table * p.length;
       const int r = (int)(((int64_t)(bad ? 0 : page) * p.heads_k + head) * p.length) + place;
       row_of = r;
-      kb = bad ? kNanByte : __ldg(p.k_scale + r / kBlockN);
-      vb = bad ? kNanByte : __ldg(p.v_scale + r / kBlockN);
+      kb = bad ? kNanByte : *(p.k_scale + r / kBlockN);
+      vb = bad ? kNanByte : *(p.v_scale + r / kBlockN);
     };
     if (z > a) {
       look(2 * a);
@@ -407,11 +441,11 @@ __device__ __forceinline__ void fetch(const AttnParams& p, const CUtensorMap* k_
       r.pos = block * kBlockN;
       r.valid = k0 + lane < total ? min(kBlockN, reach - r.pos) : 0;
       r.tokens = (1u << tokens) - 1;
-      if (kSelected && kT > 1) {
+      if (kSelected && kT > 1 && !list) {
         r.tokens = 0;
         const unsigned long long* m = p.mask + ((int64_t)head * p.total_q + row) * p.words + (block >> 6);
         for (int i = 0; i < tokens; ++i) {
-          const unsigned long long w = p.lists ? s.words[i][block >> 6] : __ldg(m + (int64_t)i * p.words);
+          const unsigned long long w = p.lists ? s.words[i][block >> 6] : *(m + (int64_t)i * p.words);
           r.tokens |= (uint32_t)((w >> (block & 63)) & 1) << i;
         }
       }
@@ -462,12 +496,12 @@ __device__ __forceinline__ void fetch(const AttnParams& p, const CUtensorMap* k_
     if (end >= hi) break;
     if (kListed) {
       ++tile;
-      more = tile < n_tiles;
+      more = tile < deal.n_tiles;
     } else {
       begin = end;
       if (++head == p.heads_k) {
         head = 0;
-        do ++b; while (b < p.batch && (each = cost_of(b, row, tokens, reach)) == 0);
+        do ++b; while (b < p.batch && (each = D::cost_of(p, b, row, tokens, reach)) == 0);
         more = b < p.batch;
       }
     }
@@ -483,9 +517,42 @@ __device__ __forceinline__ void fetch(const AttnParams& p, const CUtensorMap* k_
     for (int i = max(n - kStages, 0); i < n; ++i) mbar_wait_drain(&s.full[i % kStages], (i / kStages) & 1);
 }
 
-// The kernels that the parts of the call are: each may start beside the one before it.
+// Each kernel of a call may start beside the one in front of it, the first beside whatever is in front of the call: it
+// touches no memory before that one's end, which every thread waits for, so that what comes behind the call comes
+// behind all of it.  So the inputs may be written while a kernel lives already, and are read by ordinary loads (a read-only
+// one might find a line that was fetched before).
 __device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void wait_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  fence_proxy_async_global();                      // what that one wrote is read by TMA too
+}
+
+template <typename... Params, typename... Args>
+cudaError_t launch_beside(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream, const Args&... args) {
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, args...);
+}
+
+// The dynamic shared memory of a kernel is allowed once per device.
+inline cudaError_t allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (device & 63);
+  if (device < 64 && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && device < 64) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
 
 }  // namespace b8
 

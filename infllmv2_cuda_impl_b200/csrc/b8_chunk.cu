@@ -74,7 +74,7 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   volatile int* gave_up = &s.gave_up;
 
-  if (tid == 0) {
+  if (tid == 64) {
     s.gave_up = 0;
     for (int i = 0; i < kStages; ++i) mbar_init(&s.full[i], 2), mbar_init(&s.empty[i], 9);
     for (int i = 0; i < 2; ++i) {
@@ -92,15 +92,17 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
     tmem_alloc(&s.tmem, 512);
     tmem_relinquish();
   }
+  wait_previous();
+  Deal<kT, kListed, kSelected> deal;
+  if (warp == 0) deal.work_out(p);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   allow_next();
-  if (kListed) wait_previous();
   const uint32_t tmem = s.tmem;                    // S of group g at 128 g, O at 256 + 128 g
 
   if (warp == 0) {
-    fetch<kT, kStages, kListed, kSelected>(p, &k_map, &v_map, s, smem + kRing);
+    fetch<kT, kStages, kListed, kSelected>(p, &k_map, &v_map, s, smem + kRing, deal);
   } else if (warp == 1) {
     // ---------------------------------------------------------------- scores
     if (elect_one()) {
@@ -261,7 +263,7 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
         x[0] = x[1] = make_uint4(0, 0, 0, 0);
         if (2 * i + of_pair / kGroup < t.tokens) {
           const uint4* at = reinterpret_cast<const uint4*>(src + (int64_t)2 * i * heads * kHeadDim);
-          x[0] = __ldg(at), x[1] = __ldg(at + 1);
+          x[0] = *at, x[1] = *(at + 1);
         }
       };
       uint4 x[2];
@@ -499,9 +501,11 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
 
 template <int kCode, bool kListed, bool kSelected>
 int launch(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttnParams& p, cudaStream_t stream) {
-  const cudaError_t e = cudaFuncSetAttribute(b8_chunk_kernel<kCode, kListed, kSelected>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  static std::atomic<uint64_t> allowed{0};
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(b8_chunk_kernel<kCode, kListed, kSelected>), kSmem, allowed);
+  if (e == cudaSuccess)
+    e = launch_beside(b8_chunk_kernel<kCode, kListed, kSelected>, dim3(kB8ChunkGrid), kThreads, kSmem, stream, k_map, v_map, p);
   if (e != cudaSuccess) return set_error((int)e, "b8_attn: %s", cudaGetErrorString(e));
-  b8_chunk_kernel<kCode, kListed, kSelected><<<kB8ChunkGrid, kThreads, kSmem, stream>>>(k_map, v_map, p);
   return check_launch("b8_attn");
 }
 

@@ -69,7 +69,7 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   volatile int* gave_up = &s.gave_up;
 
-  if (tid == 0) {
+  if (tid == 64) {
     s.gave_up = 0;
     for (int i = 0; i < kStages; ++i) mbar_init(&s.full[i], 2), mbar_init(&s.empty[i], 1);
     for (int i = 0; i < 2; ++i) {
@@ -88,6 +88,9 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
     tmem_alloc(&s.tmem, S::kTmem);
     tmem_relinquish();
   }
+  wait_previous();
+  Deal<kT, false, kSelected> deal;
+  if (warp == 0) deal.work_out(p);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -95,7 +98,7 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
   const uint32_t tmem_s = s.tmem, tmem_o = s.tmem + S::kO;
 
   if (warp == 0) {
-    fetch<kT, kStages, false, kSelected>(p, &k_map, &v_map, s, smem + S::kRing);
+    fetch<kT, kStages, false, kSelected>(p, &k_map, &v_map, s, smem + S::kRing, deal);
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMAs
     if (elect_one()) {
@@ -163,8 +166,8 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
         uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
         if (i < t.tokens) {
           const uint4* src = reinterpret_cast<const uint4*>(p.q + ((int64_t)(t.row + i) * heads + t.head * kGroup + (stid >> 3)) * kHeadDim + c * 16);
-          x[0] = __ldg(src);
-          x[1] = __ldg(src + 1);
+          x[0] = *src;
+          x[1] = *(src + 1);
         }
         const float f = write_query16(x, smem + S::kQ + col * kHeadDim + ((c ^ (col & 7)) << 4), S::kQBytes, p.scale_log2);
         if (c == 0) s_c[col] = f;
@@ -393,9 +396,10 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
 template <int kT, int kCode, bool kSelected>
 int launch(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttnParams& p, cudaStream_t stream) {
   constexpr int smem = Shape<kT>::kSmem;
-  const cudaError_t e = cudaFuncSetAttribute(b8_few_kernel<kT, kCode, kSelected>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<uint64_t> allowed{0};
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(b8_few_kernel<kT, kCode, kSelected>), smem, allowed);
+  if (e == cudaSuccess) e = launch_beside(b8_few_kernel<kT, kCode, kSelected>, dim3(kB8FewGrid), kThreads, smem, stream, k_map, v_map, p);
   if (e != cudaSuccess) return set_error((int)e, "b8_attn: %s", cudaGetErrorString(e));
-  b8_few_kernel<kT, kCode, kSelected><<<kB8FewGrid, kThreads, smem, stream>>>(k_map, v_map, p);
   return check_launch("b8_attn");
 }
 
