@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(kPlanThreads) b8_plan_kernel(const AttnParams 
   __shared__ int64_t scratch[32], s_total;
   const int tid = threadIdx.x;
   allow_next();
-  wait_previous();
+  wait_inputs();
   int64_t before = 0;
   for (int base = 0; base < p.batch; base += kPlanThreads) {
     const int b = base + tid;
@@ -102,15 +102,16 @@ __global__ void __launch_bounds__(kPlanThreads) b8_plan_kernel(const AttnParams 
 
 // The pieces of a tile that shares cut: CTA x has tile x (where tiles are few), or the tile that share x begins inside if no
 // earlier share does; join[x] says whether there is one.
-// Piece results are normal outputs with the log2 of their sums.  A warp has a head; in calls of one token per
-// sequence, where pieces are many and tiles few, the four warps of a CTA share a head's pieces.  Also: rows behind the
-// last sequence.
+// Piece results are normal outputs with the log2 of their sums.  A warp has a head; where tiles are few and pieces many (one
+// sequence of 12001 tokens, two heads: 32 pieces a tile), the four warps of a CTA share a head's pieces.  Also: rows behind
+// the last sequence.
 template <bool kShared>
 __global__ void __launch_bounds__(kJoinThreads) b8_join_kernel(const AttnParams p, int tokens_per_tile) {
   __shared__ float4 s_acc[4][32];
   __shared__ float s_most[4], s_sum[4];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, heads = p.heads_k * kGroup, columns = kGroup * tokens_per_tile;
-  wait_previous();
+  allow_next();
+  wait_inputs();
   {
     const int64_t row0 = min(max((int64_t)p.cu_q[p.batch], (int64_t)0), p.total_q);
     const int64_t me = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kJoinThreads + tid, all = (int64_t)gridDim.x * gridDim.y * kJoinThreads;
@@ -300,7 +301,8 @@ extern "C" int ifv2_b8_attn(const void* q, const void* k_cache, const void* v_ca
   rc = at.tokens <= 2 ? b8_launch_few(k_map, v_map, p, at.tokens, code, s) : b8_launch_chunk(k_map, v_map, p, at.listed, code, s);
   if (rc) return rc;
   const unsigned cuts = p.by_tile ? batch * heads_k : at.grid;
-  const cudaError_t e = at.tokens == 1 ? launch_beside(b8_join_kernel<true>, dim3(cuts, kGroup), kJoinThreads, 0, s, p, at.tokens)
+  const bool shared = at.tokens == 1 && cuts < 64;
+  const cudaError_t e = shared ? launch_beside(b8_join_kernel<true>, dim3(cuts, kGroup), kJoinThreads, 0, s, p, at.tokens)
                                        : launch_beside(b8_join_kernel<false>, dim3(cuts, 4 * at.tokens), kJoinThreads, 0, s, p, at.tokens);
   if (e != cudaSuccess) return set_error((int)e, "b8_attn (join): %s", cudaGetErrorString(e));
   return check_launch("b8_attn (join)");

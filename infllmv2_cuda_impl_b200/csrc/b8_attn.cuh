@@ -22,6 +22,7 @@
 #include <atomic>
 #include <type_traits>
 #include "b8.cuh"
+#include "beside.cuh"
 
 namespace ifv2 {
 namespace b8 {
@@ -517,29 +518,10 @@ __device__ __forceinline__ void fetch(const AttnParams& p, const CUtensorMap* k_
     for (int i = max(n - kStages, 0); i < n; ++i) mbar_wait_drain(&s.full[i % kStages], (i / kStages) & 1);
 }
 
-// Each kernel of a call may start beside the one in front of it, the first beside whatever is in front of the call: it
-// touches no memory before that one's end, which every thread waits for, so that what comes behind the call comes
-// behind all of it.  So the inputs may be written while a kernel lives already, and are read by ordinary loads (a read-only
-// one might find a line that was fetched before).
-__device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_previous() {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+// Each kernel of a call may start beside the one in front of it, the first beside whatever is in front of the call.
+__device__ __forceinline__ void wait_inputs() {
+  wait_previous();
   fence_proxy_async_global();                      // what that one wrote is read by TMA too
-}
-
-template <typename... Params, typename... Args>
-cudaError_t launch_beside(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream, const Args&... args) {
-  cudaLaunchAttribute attribute{};
-  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t config{};
-  config.gridDim = grid;
-  config.blockDim = dim3(threads);
-  config.dynamicSmemBytes = smem;
-  config.stream = stream;
-  config.attrs = &attribute;
-  config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, kernel, args...);
 }
 
 // The dynamic shared memory of a kernel is allowed once per device.

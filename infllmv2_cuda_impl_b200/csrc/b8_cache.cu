@@ -10,6 +10,7 @@
 // between the maximum and the codes, so that they are read once.  What bounds it is memory where tokens are many, and
 // the way from slot to row to scale to code where they are few.
 #include "b8.cuh"
+#include "beside.cuh"
 
 namespace ifv2 {
 namespace {
@@ -100,6 +101,8 @@ __global__ void __launch_bounds__(kThreads, 8) b8_write_kernel(const B8WritePara
   __shared__ uint64_t s_start;                   // tokens of the segment that begin a run
   __shared__ uint64_t s_end[2];                  // tokens (from the segment's first on) that do not continue one
   __shared__ uint32_t s_max[kWarps];
+  allow_next();
+  wait_previous();
   const int64_t t0 = (int64_t)blockIdx.x * p.segment;
   const int head = blockIdx.y >> 1;
   const bool val = blockIdx.y & 1;
@@ -166,7 +169,8 @@ extern "C" int ifv2_b8_write(const void* k, const void* v, int64_t k_token, int6
                   static_cast<uint8_t*>(k_cache), static_cast<uint8_t*>(v_cache), static_cast<uint8_t*>(k_scale),
                   static_cast<uint8_t*>(v_scale), slots, total, num_pages * page_size, heads_k, page_size, segment};
   const dim3 grid((unsigned)ceil_div64(total, segment), 2 * heads_k);
-  if (code == kE4m3) b8_write_kernel<kE4m3><<<grid, kThreads, 0, (cudaStream_t)stream>>>(p);
-  else b8_write_kernel<kE5m2><<<grid, kThreads, 0, (cudaStream_t)stream>>>(p);
+  const cudaError_t e = launch_beside(code == kE4m3 ? b8_write_kernel<kE4m3> : b8_write_kernel<kE5m2>, grid, kThreads, 0,
+                                      (cudaStream_t)stream, p);
+  if (e != cudaSuccess) return set_error((int)e, "b8_write: %s", cudaGetErrorString(e));
   return check_launch("b8_write");
 }

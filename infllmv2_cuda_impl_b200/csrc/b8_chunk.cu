@@ -92,7 +92,7 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
     tmem_alloc(&s.tmem, 512);
     tmem_relinquish();
   }
-  wait_previous();
+  wait_inputs();
   Deal<kT, kListed, kSelected> deal;
   if (warp == 0) deal.work_out(p);
   tc_fence_before();

@@ -88,7 +88,7 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
     tmem_alloc(&s.tmem, S::kTmem);
     tmem_relinquish();
   }
-  wait_previous();
+  wait_inputs();
   Deal<kT, false, kSelected> deal;
   if (warp == 0) deal.work_out(p);
   tc_fence_before();

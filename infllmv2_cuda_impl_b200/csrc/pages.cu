@@ -8,7 +8,7 @@
 //
 // What bounds it is latency: lengths, their sums, a page's number, its slot follow one another.  Every CTA adds up all
 // requests by itself (a second launch or a wait for another CTA would cost more than the 1-2 us of a few thousand).
-#include "common.cuh"
+#include "beside.cuh"
 
 namespace ifv2 {
 namespace {
@@ -57,6 +57,8 @@ __global__ void __launch_bounds__(kThreads) pages_resize_kernel(const ResizePara
   __shared__ int64_t scratch[24];
   __shared__ int64_t s_prefix[3][kThreads];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  allow_next();
+  wait_previous();
   const int ring = p.num_pages;
   const int first = (int)(((int64_t)p.range[0] % ring + ring) % ring);
   const int count = min(max(p.range[1], 0), ring);
@@ -166,6 +168,8 @@ struct WriteParams {
 
 __global__ void __launch_bounds__(kThreads) cache_write_kernel(const WriteParams p) {
   __shared__ int64_t s_slot[kTokens];
+  allow_next();
+  wait_previous();
   const int64_t t0 = (int64_t)blockIdx.x * kTokens;
   const int tokens = (int)min((int64_t)kTokens, p.total - t0);
   if (threadIdx.x < tokens) {
@@ -226,7 +230,8 @@ extern "C" int ifv2_pages_resize(const int32_t* seqlens, const int32_t* targets,
   // one CTA for a decode step; otherwise a CTA per 1024 tokens or 16 requests, up to one per SM
   const int64_t want = max(ceil_div64(total, 1024), (int64_t)ceil_div(batch, 16));
   const int grid = (int)min(max(want, (int64_t)1), (int64_t)kNumSMs);
-  pages_resize_kernel<<<grid, kThreads, smem, (cudaStream_t)stream>>>(p);
+  const cudaError_t e = launch_beside(pages_resize_kernel, dim3(grid), kThreads, smem, (cudaStream_t)stream, p);
+  if (e != cudaSuccess) return set_error((int)e, "pages_resize: %s", cudaGetErrorString(e));
   return check_launch("pages_resize");
 }
 
@@ -245,6 +250,7 @@ extern "C" int ifv2_cache_write(const void* k, const void* v, int64_t k_token, i
                IFV2_ERR_INVALID_ARG, "cache_write: rows must begin at multiples of 16 bytes");
   WriteParams p{static_cast<const uint4*>(k), static_cast<const uint4*>(v), k_token / 8, k_head / 8, v_token / 8, v_head / 8,
                 static_cast<uint4*>(k_cache), static_cast<uint4*>(v_cache), slots, total, num_pages * page_size, heads_k};
-  cache_write_kernel<<<(unsigned)ceil_div64(total, kTokens), kThreads, 0, (cudaStream_t)stream>>>(p);
+  const cudaError_t e = launch_beside(cache_write_kernel, dim3((unsigned)ceil_div64(total, kTokens)), kThreads, 0, (cudaStream_t)stream, p);
+  if (e != cudaSuccess) return set_error((int)e, "cache_write: %s", cudaGetErrorString(e));
   return check_launch("cache_write");
 }
