@@ -226,6 +226,8 @@ def infllmv2_attn_paged_b8(
         if topk_idx.shape[2] == 0:                     # (a list of no entries has no address)
             topk_idx = torch.full((hk, total, 1), -1, dtype=torch.int32, device=dev)
     q = q.contiguous()
+    if q.data_ptr() & 15:
+        q = q.clone()
     out = torch.empty_like(q)
     lse = torch.empty(total, heads, dtype=torch.float32, device=dev) if return_softmax_lse else None
     if total and hk:
