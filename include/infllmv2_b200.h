@@ -553,8 +553,10 @@ int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void* k_scale, v
  * block_table_stride) or null (sequence b is page b).  64-key blocks that a token attends: topk_idx (heads_k, total_q,
  * topk), entries below 0 unused, or mask (heads_k, total_q, mask_words), a word per 64 blocks of a sequence's capacity, at
  * most 524288 keys; both null: all.  lse (total_q, heads_q) fp32 or null.  Tokens without keys and rows behind the last sequence get 0, lse
- * +inf; tokens that see a NaN block or a page that the cache does not have get NaN.  Caches begin at a multiple of 16
- * bytes. */
+ * +inf; tokens that see a NaN block or a page that the cache does not have get NaN.  Codes are finite numbers (ifv2_b8_write
+ * writes no others); of a sequence with more than max_seqlen_q tokens some rows are not written.  Caches begin at a
+ * multiple of 16 bytes.  status: the status block; its word 1 gets site 101 or 102 where a wait was given up (no word 0
+ * is kept: the call's other thread blocks go on). */
 int ifv2_pages_resize(const int32_t* seqlens, const int32_t* targets, int32_t* block_table, int64_t table_stride,
                       int width, int32_t* free_pages, int num_pages, const int32_t* free_range,
                       int32_t* seqlens_out, int32_t* free_range_out, int32_t* cu_seqlens, int32_t* positions,
@@ -575,7 +577,7 @@ int ifv2_b8_attn(const void* q, const void* k_cache, const void* v_cache, const 
                  const int32_t* block_table, int block_table_stride, const int32_t* topk_idx, int topk,
                  const int64_t* mask, int mask_words, int batch, int64_t total_q, int max_seqlen_q,
                  int64_t num_pages, int64_t length, int code, int heads_q, int heads_k, int head_dim,
-                 float softmax_scale, int causal, void* workspace, int64_t workspace_bytes, void* stream);
+                 float softmax_scale, int causal, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
 
 /* ---------------------------------------------------------------- self-tests -------------- */
 /* Test infrastructure shipped in the library so that a deployment can check the tensor-core

@@ -99,7 +99,7 @@ SIGNATURES = {
     "ifv2_cache_write": [c_void_p] * 2 + [c_int64] * 4 + [c_void_p] * 3 + [c_int64, c_int, c_int64, c_int, c_int, c_void_p],
     "ifv2_b8_write": [c_void_p] * 2 + [c_int64] * 4 + [c_void_p] * 5 + [c_int64, c_int, c_int, c_int64, c_int, c_int, c_void_p],
     "ifv2_b8_attn": [c_void_p] * 10 + [c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int64, c_int, c_int64, c_int64] + [c_int] * 4 +
-                    [c_float, c_int, c_void_p, c_int64, c_void_p],
+                    [c_float, c_int, c_void_p, c_int64, c_void_p, c_void_p],
 }
 _INT64_RETURNS = {
     "ifv2_sparse_attn_bwd_workspace_bytes": [c_int64, c_int, c_int],

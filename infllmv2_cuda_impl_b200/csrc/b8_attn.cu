@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(kPlanThreads) b8_plan_kernel(const AttnParams 
 // sequence of 12001 tokens, two heads: 32 pieces a tile), the four warps of a CTA share a head's pieces.  Also: rows behind
 // the last sequence.
 template <bool kShared>
-__global__ void __launch_bounds__(kJoinThreads) b8_join_kernel(const AttnParams p, int tokens_per_tile) {
+__global__ void __launch_bounds__(kJoinThreads) b8_join_kernel(const AttnParams p, int tokens_per_tile, int shares) {
   __shared__ float4 s_acc[4][32];
   __shared__ float s_most[4], s_sum[4];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, heads = p.heads_k * kGroup, columns = kGroup * tokens_per_tile;
@@ -127,6 +127,8 @@ __global__ void __launch_bounds__(kJoinThreads) b8_join_kernel(const AttnParams 
   const int4 cut = p.join[blockIdx.x];
   const int column = kShared ? blockIdx.y : blockIdx.y * 4 + warp, tok = column / kGroup;
   if (cut.z >= cut.w || tok >= cut.y >> 16) return;
+  // (what stands here after a CTA gave up may be anything)
+  if (cut.z < 0 || cut.w >= shares || cut.x < 0 || cut.x + (int64_t)tok >= p.total_q || (cut.y & 0xFFFF) >= p.heads_k) return;
   // pieces: the second of the first share, the first of those behind it
   const int pieces = cut.w - cut.z + 1;
   const auto piece = [&](int i) { return (int64_t)(2 * (cut.z + i) + (i == 0 ? 1 : 0)) * columns + column; };
@@ -224,16 +226,16 @@ extern "C" int ifv2_b8_attn(const void* q, const void* k_cache, const void* v_ca
                             const int32_t* block_table, int block_table_stride, const int32_t* topk_idx, int topk, const int64_t* mask,
                             int mask_words, int batch, int64_t total_q, int max_seqlen_q, int64_t num_pages, int64_t length, int code,
                             int heads_q, int heads_k, int head_dim, float softmax_scale, int causal, void* workspace,
-                            int64_t workspace_bytes, void* stream) {
+                            int64_t workspace_bytes, int32_t* status, void* stream) {
   IFV2_REQUIRE(head_dim == kHeadDim && heads_k >= 1 && heads_q == heads_k * kGroup, IFV2_ERR_UNSUPPORTED,
                "b8_attn: head_dim must be %d, with %d query heads per KV head", kHeadDim, kGroup);
   IFV2_REQUIRE(code == kE4m3 || code == kE5m2, IFV2_ERR_INVALID_ARG, "b8_attn: code must be 0 (e4m3) or 1 (e5m2)");
   IFV2_REQUIRE(batch >= 0 && total_q >= 0 && max_seqlen_q >= 0 && num_pages >= 0 && length >= kBlockN && length % kBlockN == 0 &&
-               mask_words >= 0 && topk >= 0 && (block_table == nullptr || block_table_stride >= 1), IFV2_ERR_INVALID_ARG,
+               mask_words >= 0 && topk >= 0 && topk < (1 << 30) && (block_table == nullptr || block_table_stride >= 1), IFV2_ERR_INVALID_ARG,
                "b8_attn: bad sizes");
   IFV2_REQUIRE(mask == nullptr || topk_idx == nullptr, IFV2_ERR_INVALID_ARG, "b8_attn: block lists and a mask exclude one another");
   if (total_q == 0) return IFV2_OK;
-  IFV2_REQUIRE(batch >= 1 && q && out && cu_seqlens_q && cache_seqlens && workspace, IFV2_ERR_INVALID_ARG, "b8_attn: null pointer");
+  IFV2_REQUIRE(batch >= 1 && q && out && cu_seqlens_q && cache_seqlens && workspace && status, IFV2_ERR_INVALID_ARG, "b8_attn: null pointer");
   IFV2_REQUIRE(num_pages >= 1 && (block_table || num_pages >= batch) && k_cache && v_cache && k_scale && v_scale, IFV2_ERR_INVALID_ARG,
                "b8_attn: the cache has too few pages");
   const int64_t cap = block_table ? (int64_t)block_table_stride * length : length;
@@ -271,7 +273,7 @@ extern "C" int ifv2_b8_attn(const void* q, const void* k_cache, const void* v_ca
   p.heads_k = heads_k;
   p.length = (int)length;
   p.causal = causal;
-  p.usual = topk_idx ? (topk > 0 ? topk : 1) : kUsualBlocks;
+  p.usual = topk_idx ? min(max(topk, 1), kMaxMaskWords * 64) : kUsualBlocks;
   p.total_q = total_q;
   p.capacity = cap;
   p.pages = (int)num_pages;                        // (below 2^31 / 64, as the cache's rows are)
@@ -282,6 +284,7 @@ extern "C" int ifv2_b8_attn(const void* q, const void* k_cache, const void* v_ca
   while ((2u << p.page_shift) < n) ++p.page_shift;
   p.page_mul = (uint32_t)(((1ull << (31 + p.page_shift)) + n - 1) / n);
   p.least_share = 3;
+  p.status = status;
   char* ws = static_cast<char*>(workspace);
   p.join = reinterpret_cast<int4*>(ws);
   p.by_tile = !at.listed && (int64_t)batch * heads_k <= at.grid;
@@ -302,8 +305,8 @@ extern "C" int ifv2_b8_attn(const void* q, const void* k_cache, const void* v_ca
   if (rc) return rc;
   const unsigned cuts = p.by_tile ? batch * heads_k : at.grid;
   const bool shared = at.tokens == 1 && cuts < 64;
-  const cudaError_t e = shared ? launch_beside(b8_join_kernel<true>, dim3(cuts, kGroup), kJoinThreads, 0, s, p, at.tokens)
-                                       : launch_beside(b8_join_kernel<false>, dim3(cuts, 4 * at.tokens), kJoinThreads, 0, s, p, at.tokens);
+  const cudaError_t e = shared ? launch_beside(b8_join_kernel<true>, dim3(cuts, kGroup), kJoinThreads, 0, s, p, at.tokens, at.grid)
+                                       : launch_beside(b8_join_kernel<false>, dim3(cuts, 4 * at.tokens), kJoinThreads, 0, s, p, at.tokens, at.grid);
   if (e != cudaSuccess) return set_error((int)e, "b8_attn (join): %s", cudaGetErrorString(e));
   return check_launch("b8_attn (join)");
 }

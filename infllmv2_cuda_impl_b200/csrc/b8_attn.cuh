@@ -55,6 +55,7 @@ struct AttnParams {
   int pages;
   float scale_log2;
   int least_share;
+  int32_t* status;                               // [1]: the first kernel that gave a wait up
   // workspace
   int4* join;                                    // cut tiles: first token's row, tokens << 16 | head, first and last share
   int by_tile;                                   // join has a place per tile (where tiles are few), else per share
@@ -239,7 +240,7 @@ struct Deal {
     const int me = blockIdx.x;
     shares.deal(max(cost, (Cost)1), gridDim.x, p.least_share);
     lo = me < shares.grid ? shares.begin(me) : cost, hi = me < shares.grid ? shares.begin(me + 1) : cost;
-    more = lo < hi;
+    more = lo < hi && cost > 0;                    // (no tile, no item: the list has none to read)
   }
   __device__ __forceinline__ void work_out(const AttnParams& p) {
     const int lane = threadIdx.x & 31;

@@ -496,6 +496,7 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
   }
   tc_fence_before();
   __syncthreads();
+  if (tid == 0 && s.gave_up) atomicCAS(p.status + 1, 0, 102);
   if (warp == 1) tmem_dealloc(s.tmem, 512);
 }
 

@@ -390,6 +390,7 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
   }
   tc_fence_before();
   __syncthreads();
+  if (tid == 0 && s.gave_up) atomicCAS(p.status + 1, 0, 101);
   if (warp == 1) tmem_dealloc(s.tmem, S::kTmem);
 }
 

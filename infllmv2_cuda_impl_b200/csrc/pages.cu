@@ -223,8 +223,8 @@ extern "C" int ifv2_pages_resize(const int32_t* seqlens, const int32_t* targets,
   ResizeParams p{seqlens, targets, block_table, table_stride, free_pages, free_range, seqlens_out, free_range_out,
                  cu_seqlens, positions, slots, batch, width, num_pages, page_size, total};
   const int smem = 4 * (3 * batch + 1);
-  if (smem > 40 * 1024) {                          // (beside the static part)
-    const cudaError_t e = cudaFuncSetAttribute(pages_resize_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (smem > 40 * 1024) {                          // (beside the static part; for all sizes at once, as calls may be made by several threads)
+    const cudaError_t e = cudaFuncSetAttribute(pages_resize_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * (3 * kMaxBatch + 1));
     if (e != cudaSuccess) return set_error((int)e, "pages_resize: %s", cudaGetErrorString(e));
   }
   // one CTA for a decode step; otherwise a CTA per 1024 tokens or 16 requests, up to one per SM

@@ -22,7 +22,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .attention import BLOCK_N, GROUP, HEAD_DIM
+from .attention import BLOCK_N, GROUP, HEAD_DIM, _status_words
 from .ops import _on, _require_cuda, _stream
 from .quant_cache import _cu, _ints, _no_gradient, _ptr, _table
 from .rotary import _rows
@@ -194,7 +194,9 @@ def infllmv2_attn_paged_b8(
     topk) 64-token blocks that a token attends, -1 unused, or block_mask: the same packed, int64 (nheads_k, total_q,
     words) with a word per 64 blocks of a sequence's capacity; None = all.
     Tokens that see no key get 0 (softmax_lse +inf), and so do rows behind the last sequence.  A token that sees a key of a
-    NaN block, or of a page that the cache does not have, gets NaN.
+    NaN block, or of a page that the cache does not have, gets NaN.  Codes are finite (cache_write_b8 writes no others).
+    A sequence with more than max_seqlen_q tokens has rows that are not written.  Blocks are selected among at most
+    524288 keys of capacity.
     Returns out (total_q, nheads, 128) [, softmax_lse (total_q, nheads) fp32].  Forward only."""
     what = "infllmv2_attn_paged_b8"
     pages, hk, length, code, dev = _check_b8(what, k_cache, v_cache, k_scale, v_scale)
@@ -206,8 +208,8 @@ def infllmv2_attn_paged_b8(
     total = shape[0]
     cu_seqlens_q, batch = _cu(what, cu_seqlens_q, dev)
     cache_seqlens = _ints(what, "cache_seqlens", cache_seqlens, (batch,), dev)
-    if max_seqlen_q < 1:
-        raise ValueError(f"{what}: max_seqlen_q must be positive")
+    if not 1 <= max_seqlen_q < 2 ** 31:
+        raise ValueError(f"{what}: max_seqlen_q must be positive and below 2^31")
     width, cap = 0, length
     if block_table is not None:
         block_table, width = _table(what, block_table, batch, dev)
@@ -239,5 +241,5 @@ def infllmv2_attn_paged_b8(
                       _ptr(topk_idx), topk_idx.shape[2] if topk_idx is not None else 0, _ptr(block_mask),
                       words if block_mask is not None else 0, batch, total, max_seqlen_q, pages, length, code, heads,
                       hk, HEAD_DIM, HEAD_DIM ** -0.5 if softmax_scale is None else float(softmax_scale), 1 if causal else 0,
-                      ws.data_ptr(), ws_bytes, _stream(dev))
+                      ws.data_ptr(), ws_bytes, _status_words(dev).data_ptr(), _stream(dev))
     return (out, lse) if return_softmax_lse else out

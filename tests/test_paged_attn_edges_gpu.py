@@ -207,3 +207,27 @@ def test_keys_past_32_bits():
         q, cu_q = queries(new, hk, 66), cu(new)
         got = attend(q, cache, cu_q, max(new), [n], torch.tensor([own], dtype=torch.int32))
         check(got, q, kk, vv, cu_q, [n], torch.tensor([[0, 1]]))
+
+
+@pytest.mark.parametrize("most", [1, 2, 8, 20])
+@pytest.mark.parametrize("batch", [3, 400])
+def test_no_sequence_has_a_token(most, batch):
+    """Rows, but none of a sequence: no tile for anyone, whichever way tiles are dealt."""
+    lens = [100] * batch
+    cache, table, _, _ = make([100], 2, 64, E4M3, 67)
+    table = table.expand(batch, -1).contiguous()
+    q = queries([5], 2, 68)
+    for more in (dict(), dict(topk_idx=ints([[[0, 1]] * 5] * 2))):
+        out, lse = attend(q, cache, torch.zeros(batch + 1, dtype=torch.int32), most, lens, table, **more)
+        assert bool((out == 0).all()) and bool((lse == math.inf).all())
+    infllm_v2.check_device_status()
+
+
+@pytest.mark.parametrize("new", [[1, 1], [4, 3], [12, 9]])
+def test_lists_longer_than_the_blocks_there_are(new):
+    lens, hk = [700, 300], 2
+    cache, table, k, v = make(lens, hk, 64, E4M3, 69)
+    q, cu_q = queries(new, hk, 70), cu(new)
+    lists = (torch.arange(20001, dtype=torch.int32) * 7 % 30000).expand(hk, sum(new), -1).contiguous()
+    lists[1] = lists[1] % 5
+    check(attend(q, cache, cu_q, max(new), lens, table, topk_idx=lists.to(DEV)), q, k, v, cu_q, lens, table, True, lists)
