@@ -47,6 +47,16 @@ __device__ __forceinline__ void block_scan3(int64_t (&v)[3], int64_t* scratch) {
   __syncthreads();
 }
 
+// Place `off` behind `first` in a ring; neither is above its size.  (A 64-bit remainder takes some 100 instructions.)
+__device__ __forceinline__ int ring_at(int first, int off, int ring) {
+  const uint32_t x = (uint32_t)first + (uint32_t)off;
+  return (int)(x >= (uint32_t)ring ? x - (uint32_t)ring : x);
+}
+
+__device__ __forceinline__ int pages_of(int tokens, int page_size) {
+  return (int)(((uint32_t)tokens + (uint32_t)page_size - 1) / (uint32_t)page_size);
+}
+
 __device__ __forceinline__ int sat32(int64_t x) { return (int)min(x, (int64_t)0x7FFFFFFF); }
 
 __global__ void __launch_bounds__(kThreads) pages_resize_kernel(const ResizeParams p) {
@@ -55,12 +65,14 @@ __global__ void __launch_bounds__(kThreads) pages_resize_kernel(const ResizePara
   int32_t* s_old = smem + p.batch + 1;           // (batch)
   int32_t* s_take = s_old + p.batch;             // (batch) pages that requests before it take; -1: refused
   __shared__ int64_t scratch[24];
-  __shared__ int64_t s_prefix[3][kThreads];
+  __shared__ int64_t s_back[kThreads];           // of the chunk's requests: pages given back up to it, pages before and after
+  __shared__ int s_had[kThreads], s_want[kThreads];
+  __shared__ int64_t s_sum[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   allow_next();
   wait_previous();
   const int ring = p.num_pages;
-  const int first = (int)(((int64_t)p.range[0] % ring + ring) % ring);
+  const int place = p.range[0] % ring, first = place < 0 ? place + ring : place;
   const int count = min(max(p.range[1], 0), ring);
   const int64_t reach = (int64_t)p.width * p.page_size;
 
@@ -73,16 +85,17 @@ __global__ void __launch_bounds__(kThreads) pages_resize_kernel(const ResizePara
     if (b < p.batch) {
       old = (int)min((int64_t)max(p.seqlens[b], 0), reach);
       target = max(p.targets[b], 0);
-      had = (int)ceil_div64(old, p.page_size);
-      want = (int)ceil_div64(target, p.page_size);
+      had = pages_of(old, p.page_size);
+      want = pages_of(target, p.page_size);
       v[0] = max(target - old, 0);
       if (want <= p.width) v[1] = max(want - had, 0);
       v[2] = max(had - want, 0);
     }
     const int64_t mine[3] = {v[0], v[1], v[2]};
     block_scan3(v, scratch);
-    for (int k = 0; k < 3; ++k) s_prefix[k][tid] = before[k] + v[k];
-    __syncthreads();
+    s_back[tid] = before[2] + v[2];
+    s_had[tid] = had, s_want[tid] = want;
+    if (tid == kThreads - 1) s_sum[0] = before[0] + v[0], s_sum[1] = before[1] + v[1];
     const bool granted = want <= p.width && (mine[1] == 0 || before[1] + v[1] <= count);
     if (b < p.batch) {
       s_cu[b] = sat32(before[0] + v[0] - mine[0]);
@@ -110,16 +123,15 @@ __global__ void __launch_bounds__(kThreads) pages_resize_kernel(const ResizePara
       if (req % gridDim.x != blockIdx.x) continue;
       const int take = s_take[req];
       if (take < 0) continue;
-      const int old_r = s_old[req], target_r = max(p.targets[req], 0);
-      const int had_r = (int)ceil_div64(old_r, p.page_size), want_r = (int)ceil_div64(target_r, p.page_size);
+      const int had_r = s_had[r], want_r = s_want[r];
       int32_t* row = p.table + (int64_t)req * p.table_stride;
       for (int i = had_r + lane; i < want_r; i += 32)
-        row[i] = p.ring[(int)(((int64_t)first + take + i - had_r) % ring)];
-      const int64_t behind = s_prefix[2][r] - max(had_r - want_r, 0);        // pages given back by earlier requests
+        row[i] = p.ring[ring_at(first, take + i - had_r, ring)];
+      const int64_t behind = s_back[r] - max(had_r - want_r, 0);             // pages given back by earlier requests
       for (int i = want_r + lane; i < had_r; i += 32)
         p.ring[(int)(((int64_t)first + count + behind + i - want_r) % ring)] = row[i];
     }
-    for (int k = 0; k < 3; ++k) before[k] = s_prefix[k][kThreads - 1];
+    before[0] = s_sum[0], before[1] = s_sum[1], before[2] = s_back[kThreads - 1];
     __syncthreads();
   }
   if (tid == 0) {
@@ -141,10 +153,10 @@ __global__ void __launch_bounds__(kThreads) pages_resize_kernel(const ResizePara
       pos = s_old[b] + (int)(t - s_cu[b]);
       const int take = s_take[b];
       if (take >= 0) {
-        const int i = pos / p.page_size, had = (int)ceil_div64(s_old[b], p.page_size);
+        const int i = pos / p.page_size, had = pages_of(s_old[b], p.page_size);
         // (a page of this step may not stand in the table yet: it is looked up where the table's row gets it from)
         const int page = i < had ? p.table[(int64_t)b * p.table_stride + i]
-                                 : p.ring[(int)(((int64_t)first + take + i - had) % ring)];
+                                 : p.ring[ring_at(first, take + i - had, ring)];
         if (page >= 0) slot = (int64_t)page * p.page_size + (pos - i * p.page_size);
       }
     }
@@ -227,8 +239,8 @@ extern "C" int ifv2_pages_resize(const int32_t* seqlens, const int32_t* targets,
     const cudaError_t e = cudaFuncSetAttribute(pages_resize_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * (3 * kMaxBatch + 1));
     if (e != cudaSuccess) return set_error((int)e, "pages_resize: %s", cudaGetErrorString(e));
   }
-  // one CTA for a decode step; otherwise a CTA per 1024 tokens or 16 requests, up to one per SM
-  const int64_t want = max(ceil_div64(total, 1024), (int64_t)ceil_div(batch, 16));
+  // a CTA per 256 tokens or 8 requests, up to one per SM
+  const int64_t want = max(ceil_div64(total, 256), (int64_t)ceil_div(batch, 8));
   const int grid = (int)min(max(want, (int64_t)1), (int64_t)kNumSMs);
   const cudaError_t e = launch_beside(pages_resize_kernel, dim3(grid), kThreads, smem, (cudaStream_t)stream, p);
   if (e != cudaSuccess) return set_error((int)e, "pages_resize: %s", cudaGetErrorString(e));
