@@ -105,83 +105,74 @@ __global__ void __launch_bounds__(kPlanThreads) b8_plan_kernel(const AttnParams 
 // Piece results are normal outputs with the log2 of their sums.  A warp has a head; where tiles are few and pieces many (one
 // sequence of 12001 tokens, two heads: 32 pieces a tile), the four warps of a CTA share a head's pieces.  Also: rows behind
 // the last sequence.
+// What bounds it is latency: trips to memory of 0.7 us, here two.  (A warp stops at the first instruction that wants a number
+// that is not there yet, so what does not depend on it is asked for before.)
 template <bool kShared>
 __global__ void __launch_bounds__(kJoinThreads) b8_join_kernel(const AttnParams p, int tokens_per_tile, int shares) {
   __shared__ float4 s_acc[4][32];
-  __shared__ float s_most[4], s_sum[4];
+  __shared__ float s_sum[4];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, heads = p.heads_k * kGroup, columns = kGroup * tokens_per_tile;
   allow_next();
   wait_inputs();
-  {
-    const int64_t row0 = min(max((int64_t)p.cu_q[p.batch], (int64_t)0), p.total_q);
+  const int4 cut = p.join[blockIdx.x];
+  const int rows = p.cu_q[p.batch];
+  int row0 = 0, some = 1;
+  if (p.by_tile) some = tokens_of(p, blockIdx.x / p.heads_k, row0);        // (a sequence without tokens has no tile)
+  if (rows < p.total_q) {
     const int64_t me = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kJoinThreads + tid, all = (int64_t)gridDim.x * gridDim.y * kJoinThreads;
     uint4* out = reinterpret_cast<uint4*>(p.out);
-    for (int64_t i = row0 * heads * 16 + me; i < p.total_q * heads * 16; i += all) out[i] = make_uint4(0, 0, 0, 0);
+    for (int64_t i = (int64_t)max(rows, 0) * heads * 16 + me; i < p.total_q * heads * 16; i += all) out[i] = make_uint4(0, 0, 0, 0);
     if (p.lse)
-      for (int64_t i = row0 * heads + me; i < p.total_q * heads; i += all) p.lse[i] = INFINITY;
+      for (int64_t i = (int64_t)max(rows, 0) * heads + me; i < p.total_q * heads; i += all) p.lse[i] = INFINITY;
   }
-  if (p.by_tile) {                                 // (a sequence without tokens has no tile)
-    int row0;
-    if (tokens_of(p, blockIdx.x / p.heads_k, row0) == 0) return;
-  }
-  const int4 cut = p.join[blockIdx.x];
   const int column = kShared ? blockIdx.y : blockIdx.y * 4 + warp, tok = column / kGroup;
-  if (cut.z >= cut.w || tok >= cut.y >> 16) return;
+  if (some == 0 || cut.z >= cut.w || tok >= cut.y >> 16) return;
   // (what stands here after a CTA gave up may be anything)
   if (cut.z < 0 || cut.w >= shares || cut.x < 0 || cut.x + (int64_t)tok >= p.total_q || (cut.y & 0xFFFF) >= p.heads_k) return;
   // pieces: the second of the first share, the first of those behind it
   const int pieces = cut.w - cut.z + 1;
-  const auto piece = [&](int i) { return (int64_t)(2 * (cut.z + i) + (i == 0 ? 1 : 0)) * columns + column; };
-  constexpr int kStep = kShared ? 4 : 1;
-  const int i0 = kShared ? warp : 0;
-  float most = -INFINITY, sum = 0.f;
-  bool nan = false;
+  const auto piece = [&](int i) { return (2 * (cut.z + i) + (i == 0)) * columns + column; };
+  constexpr int kStep = kShared ? 4 : 1, kAtOnce = kShared ? 8 : 4;
+  float4 o[kAtOnce];
+  const auto load = [&](int i) {                   // (a piece that is not there: the last one, which gets no weight)
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u)
+      o[u] = reinterpret_cast<const float4*>(p.part_o + (int64_t)piece(min(i + u * kStep, pieces - 1)) * kHeadDim)[lane];
+  };
+  int i = kShared ? warp : 0;
+  load(i);
+  float most = -INFINITY;
+  for (int j = lane; j < pieces; j += 32) most = fmaxf(most, p.part_lse[piece(j)]);
+  asm("redux.sync.max.f32 %0, %0, 0xFFFFFFFF;" : "+f"(most));
+  const float ref = most == -INFINITY ? 0.f : most;
+  float sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int base = i0; base < pieces; base += 32 * kStep) {
-    const int mine = base + lane * kStep, n = min(32, (pieces - base + kStep - 1) / kStep);
-    const float x = mine < pieces ? p.part_lse[piece(mine)] : -INFINITY;
-    nan |= __any_sync(0xFFFFFFFFu, x != x);
-    float top = x;
+#pragma unroll 1
+  for (; i < pieces; i += kAtOnce * kStep) {
+    float w[kAtOnce];
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-    top = fmaxf(top, most);
-    const float ref = top == -INFINITY ? 0.f : top, back = ex2(most - ref), f = x == x ? ex2(x - ref) : 0.f;
-    sum *= back, acc.x *= back, acc.y *= back, acc.z *= back, acc.w *= back;
-    most = top;
-    for (int i = 0; i < n; i += 8) {
-      float4 o[8];
-      float w[8];
+    for (int u = 0; u < kAtOnce; ++u) w[u] = p.part_lse[piece(min(i + u * kStep, pieces - 1))];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        w[u] = __shfl_sync(0xFFFFFFFFu, f, (i + u) & 31);
-        if (i + u >= n) w[u] = 0.f;
-        o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (w[u] > 0.f) o[u] = reinterpret_cast<const float4*>(p.part_o + piece(base + (i + u) * kStep) * kHeadDim)[lane];
-      }
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        sum += w[u];
-        acc.x += w[u] * o[u].x, acc.y += w[u] * o[u].y, acc.z += w[u] * o[u].z, acc.w += w[u] * o[u].w;
-      }
+    for (int u = 0; u < kAtOnce; ++u) {
+      w[u] = i + u * kStep < pieces ? ex2(w[u] - ref) : 0.f;           // (NaN: the sum is, and all that it divides)
+      sum += w[u];
+      acc.x += w[u] * o[u].x, acc.y += w[u] * o[u].y, acc.z += w[u] * o[u].z, acc.w += w[u] * o[u].w;
     }
+    if (i + kAtOnce * kStep < pieces) load(i + kAtOnce * kStep);
   }
-  if (nan) sum = NAN;
   if (kShared) {
     s_acc[warp][lane] = acc;
-    if (lane == 0) s_most[warp] = most, s_sum[warp] = sum;
+    if (lane == 0) s_sum[warp] = sum;
     __syncthreads();
     if (warp != 0) return;
-    most = fmaxf(fmaxf(s_most[0], s_most[1]), fmaxf(s_most[2], s_most[3]));
-    sum = 0.f, acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float f = s_most[w] == -INFINITY ? 0.f : ex2(s_most[w] - most), z = s_sum[w];
+    for (int w = 1; w < 4; ++w) {
       const float4 a = s_acc[w][lane];
-      sum += z != z ? z : f * z;
-      acc.x += f * a.x, acc.y += f * a.y, acc.z += f * a.z, acc.w += f * a.w;
+      sum += s_sum[w];
+      acc.x += a.x, acc.y += a.y, acc.z += a.z, acc.w += a.w;
     }
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const float inv = sum == 0.f ? 0.f : rcp(sum);   // (to 1 ulp; a sum is 0 or between 1 and the number of pieces)
   const int64_t row = (int64_t)(cut.x + tok) * heads + (cut.y & 0xFFFF) * kGroup + column % kGroup;
   reinterpret_cast<uint2*>(p.out + row * kHeadDim)[lane] = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
   if (p.lse && lane == 0) p.lse[row] = sum == 0.f ? INFINITY : (most + lg2(sum)) * kLn2;
