@@ -7,7 +7,8 @@
 // other operand of each product is split into 8-bit numbers instead.
 //   * A query row, scaled by a power of two to a largest magnitude of 224..448, is the sum of two e4m3 numbers, to
 //     2^-10, that is 2^-18 of its largest element: for bf16 rows exact down to elements 2^-10 of the largest.
-//   * A weight is the sum of three e5m2 numbers, to 2^-9 of it (half a bf16 step).  e5m2 is the upper byte of an fp16
+//   * For few tokens a weight is the sum of three e5m2 numbers, to 2^-9 of it (half a bf16 step); for several it is an fp16
+//     number and the values' codes become fp16 too (b8_chunk.cu).  e5m2 is the upper byte of an fp16
 //     number: a term is a byte, what it leaves over one subtraction.  Weights are 2^(x + eV - M) with M about 2^-10 of the
 //     largest so far, at most 2^15, and below 2^-16 they have the type's fixed spacing of 2^-16: 2^-27 of the largest.
 //     The values' exponents take part in M, so that contributions keep their size against one another whatever

