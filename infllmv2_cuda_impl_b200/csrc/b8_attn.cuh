@@ -224,7 +224,7 @@ struct Common {
 };
 
 // ---------------------------------------------------------------------- fetching warp --
-// Where a CTA's share begins.  All lanes of a warp work it out, before the CTA's barriers and tensor memory are there.
+// Where a CTA's share begins.  It is worked out before the CTA's barriers and tensor memory are there.
 // kListed: tiles come from the kernel in front.
 template <int kT, bool kListed, bool kSelected>
 struct Deal {
@@ -248,7 +248,23 @@ struct Deal {
     lo = me < shares.grid ? shares.begin(me) : cost, hi = me < shares.grid ? shares.begin(me + 1) : cost;
     more = lo < hi && cost > 0;                    // (no tile, no item: the list has none to read)
   }
-  __device__ __forceinline__ void work_out(const AttnParams& p) {
+  // A warp's part of the sequences, and the sum of their costs: all warps of the CTA.  (By one warp 256 sequences took eight
+  // trips to memory one after the other.)
+  static __device__ __forceinline__ int part(const AttnParams& p) { return ceil_div(p.batch, (int)blockDim.x) * 32; }
+  static __device__ __forceinline__ void add_up(const AttnParams& p, int* sums) {
+    if (kListed) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = part(p), end = min((warp + 1) * n, p.batch);
+    int sum = 0;
+#pragma unroll 4
+    for (int b = warp * n + lane; b < end; b += 32) {
+      int r, t, k;
+      sum += cost_of(p, b, r, t, k);
+    }
+    sum = __reduce_add_sync(0xFFFFFFFFu, sum);
+    if (lane == 0) sums[warp] = sum * p.heads_k;
+  }
+  // From these sums the share, and the sequence that it begins in: one warp.
+  __device__ __forceinline__ void work_out(const AttnParams& p, const int* sums) {
     const int lane = threadIdx.x & 31;
     if (kListed) {
       n_tiles = p.first_tile[gridDim.x];
@@ -256,35 +272,37 @@ struct Deal {
       tile = p.first_tile[blockIdx.x];
       return;
     }
-    for (int pass = 0;; ++pass) {                  // pass 0 adds costs up, pass 1 finds the sequence that the share begins in
-      int before = 0;
-      for (int base = 0; base < p.batch; base += 32) {
-        int r = 0, t = 0, k = 0, c = 0;
-        if (base + lane < p.batch) c = cost_of(p, base + lane, r, t, k);
-        int upto = c * p.heads_k;
+    const auto sum_up_to = [&](int x) {
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-          const int o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
-          if (lane >= d) upto += o;
-        }
-        const uint32_t past = __ballot_sync(0xFFFFFFFFu, before + upto > (int)lo);
-        if (past) {
-          const int src = __ffs(past) - 1;
-          b = base + src;
-          row = __shfl_sync(0xFFFFFFFFu, r, src);
-          tokens = __shfl_sync(0xFFFFFFFFu, t, src);
-          reach = __shfl_sync(0xFFFFFFFFu, k, src);
-          each = __shfl_sync(0xFFFFFFFFu, c, src);
-          before += __shfl_sync(0xFFFFFFFFu, upto, src) - each * p.heads_k;
-          head = (int)((uint32_t)((int)lo - before) / (uint32_t)each);
-          begin = before + head * each;
-          return;
-        }
-        before += __shfl_sync(0xFFFFFFFFu, upto, 31);
+      for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xFFFFFFFFu, x, d);
+        if (lane >= d) x += o;
       }
-      if (pass == 1) return;
-      begins(before, p);
-      if (!more) return;
+      return x;
+    };
+    const int mine = lane < (int)(blockDim.x >> 5) ? sums[lane] : 0, upto_part = sum_up_to(mine);
+    begins(__shfl_sync(0xFFFFFFFFu, upto_part, 31), p);
+    if (!more) return;
+    const int in = __ffs(__ballot_sync(0xFFFFFFFFu, upto_part > (int)lo)) - 1;
+    int before = __shfl_sync(0xFFFFFFFFu, upto_part - mine, in);
+    for (int base = in * part(p); base < p.batch; base += 32) {
+      int r = 0, t = 0, k = 0, c = 0;
+      if (base + lane < p.batch) c = cost_of(p, base + lane, r, t, k);
+      const int upto = sum_up_to(c * p.heads_k);
+      const uint32_t past = __ballot_sync(0xFFFFFFFFu, before + upto > (int)lo);
+      if (past) {
+        const int src = __ffs(past) - 1;
+        b = base + src;
+        row = __shfl_sync(0xFFFFFFFFu, r, src);
+        tokens = __shfl_sync(0xFFFFFFFFu, t, src);
+        reach = __shfl_sync(0xFFFFFFFFu, k, src);
+        each = __shfl_sync(0xFFFFFFFFu, c, src);
+        before += __shfl_sync(0xFFFFFFFFu, upto, src) - each * p.heads_k;
+        head = (int)((uint32_t)((int)lo - before) / (uint32_t)each);
+        begin = before + head * each;
+        return;
+      }
+      before += __shfl_sync(0xFFFFFFFFu, upto, 31);
     }
   }
 };

@@ -79,6 +79,7 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
   __shared__ uint64_t bar_s[2][2], bar_p[2][2], bar_v[2][2], bar_pv[2][2], bar_q, bar_drain[2];
   __shared__ float s_c[kRows], s_top[2][kRows], s_lse[2][kRows];       // row's factor; a group's M and log2 of its sum
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  __shared__ int s_cost[kThreads / 32];
   volatile int* gave_up = &s.gave_up;
 
   if (tid == 64) {
@@ -101,7 +102,9 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
   }
   wait_inputs();
   Deal<kT, kListed, kSelected> deal;
-  if (warp == 0) deal.work_out(p);
+  deal.add_up(p, s_cost);
+  __syncthreads();
+  if (warp == 0) deal.work_out(p, s_cost);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();

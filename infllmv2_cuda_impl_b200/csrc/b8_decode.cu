@@ -74,6 +74,7 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
   __shared__ uint64_t bar_s[2], bar_sfree[2], bar_p, bar_pv, bar_q, bar_drain;
   __shared__ float s_c[kN], s_mu[kN], s_fl[kN], s_fo[kN], s_red[4][kN];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  __shared__ int s_cost[kThreads / 32];
   volatile int* gave_up = &s.gave_up;
 
   if (tid == 64) {
@@ -97,7 +98,9 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
   }
   wait_inputs();
   Deal<kT, false, kSelected> deal;
-  if (warp == 0) deal.work_out(p);
+  deal.add_up(p, s_cost);
+  __syncthreads();
+  if (warp == 0) deal.work_out(p, s_cost);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
