@@ -409,6 +409,10 @@ __device__ __forceinline__ void fetch(const AttnParams& p, const CUtensorMap* k_
         s.item[slot] = Item{row, head, tokens, reach, z - a, whole ? -1 : 2 * me + (lo <= begin ? 1 : 0)};
         mbar_arrive(&s.item_full[slot]);
       }
+      // its query rows, 4096 bytes a token, are on their way when the softmax comes to them
+      const __nv_bfloat16* q = p.q + ((int64_t)row * p.heads_k + head) * (kGroup * kHeadDim) + lane * 64;
+      for (int i = 0; i < tokens; ++i)
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(q + (int64_t)i * p.heads_k * (kGroup * kHeadDim)));
       ++items;
     }
     const auto nth_block = [&](int k) {            // all lanes, each with its k
