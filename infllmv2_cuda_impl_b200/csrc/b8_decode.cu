@@ -72,7 +72,7 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   __shared__ Common<kT, kStages> s;
   __shared__ uint64_t bar_s[2], bar_sfree[2], bar_p, bar_pv, bar_q, bar_drain;
-  __shared__ float s_c[kN], s_mu[kN], s_fl[kN], s_fo[kN], s_red[4][kN];
+  __shared__ __align__(16) float s_c[kN], s_mu[kN], s_fl[kN], s_fo[kN], s_red[4][kN];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   __shared__ int s_cost[kThreads / 32];
   volatile int* gave_up = &s.gave_up;
@@ -201,11 +201,12 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
     if (next.units > 0) write_query(next);
     for (int item = 0; next.units >= 0; ++item) {
       const Item t = next;
-      // in registers: the columns' factors, references and sums
-      float c[kN], mu[kN], l[kN];
+      // sums in registers; the columns' factors and references are read four at a time where they are used (in registers they
+      // took two for every column, and what did not fit was spilled)
+      float l[kN];
       named_sync<kSoftmax>();                      // s_c is written, the last item's s_fl and s_red are read
 #pragma unroll
-      for (int i = 0; i < kN; ++i) c[i] = s_c[i], mu[i] = kUnset, l[i] = 0.f;
+      for (int i = 0; i < kN; ++i) l[i] = 0.f;
       if (stid < kN) s_mu[stid] = kUnset;
       int e_ref = kNoScale, deepest = 0;           // E; least eV - E of the blocks so far
 #pragma unroll 1
@@ -251,7 +252,7 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
             const float up = (float)dv_ref;
 #pragma unroll
             for (int j = 0; j < kN; ++j) {
-              w[j] = fmaf(__uint_as_float(x[j]) * k_scale, c[j], up);
+              w[j] = fmaf(__uint_as_float(x[j]) * k_scale, s_c[j], up);
               if (!((sees >> (j / kGroup)) & 1) || !(w[j] == w[j])) w[j] = -INFINITY;
             }
             const int first = reduce_columns<true, kN>(w, lane);
@@ -275,10 +276,7 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
             }
             named_sync<kSoftmax>();
 #pragma unroll
-            for (int j = 0; j < kN; ++j) {
-              mu[j] = s_mu[j];
-              l[j] = l[j] > 0.f ? l[j] * s_fl[j] : l[j];
-            }
+            for (int j = 0; j < kN; ++j) l[j] = l[j] > 0.f ? l[j] * s_fl[j] : l[j];
             if (i > 0) {                           // what is in O so far
               bounded_wait_warp(&bar_pv, (n - 1) & 1, gave_up);
               tc_fence_after();
@@ -296,11 +294,13 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
             settled = true;
           }
 #pragma unroll
-          for (int j = 0; j < kN; j += 2) {
-            float a, b;
-            unpack_f32x2(fma_f32x2(mul_f32x2(pack_f32x2(x[j], x[j + 1]), scale2), pack_f32x2(c[j], c[j + 1]), pack_f32x2(-mu[j], -mu[j + 1])), a, b);
-            w[j] = ex2(a);
-            w[j + 1] = ex2(b);
+          for (int j = 0; j < kN; j += 4) {
+            const float4 c = *reinterpret_cast<const float4*>(s_c + j), mu = *reinterpret_cast<const float4*>(s_mu + j);
+            float y[4];
+            unpack_f32x2(fma_f32x2(mul_f32x2(pack_f32x2(x[j], x[j + 1]), scale2), pack_f32x2(c.x, c.y), pack_f32x2(-mu.x, -mu.y)), y[0], y[1]);
+            unpack_f32x2(fma_f32x2(mul_f32x2(pack_f32x2(x[j + 2], x[j + 3]), scale2), pack_f32x2(c.z, c.w), pack_f32x2(-mu.z, -mu.w)), y[2], y[3]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[j + e] = ex2(y[e]);
           }
           if (!all) {
 #pragma unroll
