@@ -292,6 +292,7 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
               tmem_wait_st();
             }
             settled = true;
+            continue;                              // (the scores are fetched again: 16 kT registers less until here)
           }
 #pragma unroll
           for (int j = 0; j < kN; j += 4) {
@@ -359,21 +360,22 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
       const int first = reduce_columns<false, kN>(l, lane);
       s_red[quad][first] = l[0];                   // (16 columns: two lanes, one value)
       named_sync<kSoftmax>();
-      if (t.units > 0) bounded_wait_warp(&bar_pv, (n - 1) & 1, gave_up);
-      tc_fence_after();
       if (stid < kN) {
         const float sum = s_red[0][stid] + s_red[1][stid] + s_red[2][stid] + s_red[3][stid];
         const bool none = sum == 0.f;
         const float lse2 = none ? -INFINITY : s_mu[stid] + lg2(sum);
-        s_fl[stid] = none ? 0.f : 1.f / sum;
+        s_fl[stid] = none ? 0.f : rcp(sum);
         const int tok = stid / kGroup;
         if (t.piece >= 0) p.part_lse[(int64_t)t.piece * kN + stid] = lse2;
         else if (p.lse && tok < t.tokens)
           p.lse[(int64_t)(t.row + tok) * heads + t.head * kGroup + stid % kGroup] = none ? INFINITY : lse2 * kLn2;
       }
+      if (t.units > 0) bounded_wait_warp(&bar_pv, (n - 1) & 1, gave_up);
+      tc_fence_after();
       named_sync<kSoftmax>();
-      const float e_half = pow2i(e_ref > kNoScale ? e_ref / 2 : 0), e_rest = pow2i(e_ref > kNoScale ? e_ref - e_ref / 2 : 0);
       const bool lost = *gave_up;
+      // 2^E; a block's smallest exponent is -127
+      const float e_scale = lost ? NAN : e_ref == -127 ? __uint_as_float(1u << 22) : pow2i(e_ref > kNoScale ? e_ref : 0);
 #pragma unroll
       for (int tok = 0; tok < kT; ++tok) {
         if (tok >= t.tokens) continue;
@@ -383,16 +385,26 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
           for (int k = 0; k < 3; ++k) tmem_ld16(tmem_o + lanes + k * kN + tok * kGroup, o[k]);
           tmem_wait_ld();
         }
+        float y[16];
 #pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          const int col = tok * kGroup + c;
-          const float f = s_fl[col];
-          float y = 0.f;
-          if (t.units > 0 && f != 0.f)
-            y = q8::mul_exact(q8::mul_exact((__uint_as_float(o[0][c]) + __uint_as_float(o[1][c]) + __uint_as_float(o[2][c])) * f, e_half), e_rest);
-          if (lost) y = NAN;
-          if (t.piece < 0) p.out[((int64_t)(t.row + tok) * heads + t.head * kGroup + c) * kHeadDim + r] = __float2bfloat16(y);
-          else p.part_o[((int64_t)t.piece * kN + col) * kHeadDim + r] = y;
+        for (int c0 = 0; c0 < 16; c0 += 4) {
+          const float4 f4 = *reinterpret_cast<const float4*>(s_fl + tok * kGroup + c0);
+          const float f[4] = {f4.x, f4.y, f4.z, f4.w};
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int i = c0 + c;
+            y[i] = q8::mul_exact((__uint_as_float(o[0][i]) + __uint_as_float(o[1][i]) + __uint_as_float(o[2][i])) * f[c], e_scale);
+            if (f[c] == 0.f && !lost) y[i] = 0.f;  // (no key: O may be anything)
+          }
+        }
+        if (t.piece < 0) {
+          __nv_bfloat16* out = p.out + ((int64_t)(t.row + tok) * heads + t.head * kGroup) * kHeadDim + r;
+#pragma unroll
+          for (int c = 0; c < 16; ++c) out[c * kHeadDim] = __float2bfloat16(y[c]);
+        } else {
+          float* part = p.part_o + ((int64_t)t.piece * kN + tok * kGroup) * kHeadDim + r;
+#pragma unroll
+          for (int c = 0; c < 16; ++c) part[c * kHeadDim] = y[c];
         }
       }
       tc_fence_before();
