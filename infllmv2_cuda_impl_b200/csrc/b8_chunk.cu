@@ -18,7 +18,7 @@
 //
 // What bounds it: a unit takes 2150 clocks.  Its exponentials need 1024 of them in the special-function units, its products 1024
 // in the tensor cores, and shared memory 1660 (scores of 64 keys read the query again; values are read, written as fp16 and
-// read by the product).  A chunk of 4096 tokens over 32768: 1.88 ms, 1.10 PFLOP/s of the attention's own FLOPs (a third of the
+// read by the product).  A chunk of 4096 tokens over 32768: 1.88 ms, 1.1 PFLOP/s of the attention's own FLOPs (a third of the
 // products serves the query's second term).  Tried and slower: scores of whole units; 16 softmax warps, two to a row's 32 keys
 // each (1880 -> 2167 us: the vote that holds them together); scores fetched from TMEM in halves; masked and unmasked
 // forms of the weights' code.
@@ -80,6 +80,7 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
   __shared__ float s_c[kRows], s_top[2][kRows], s_lse[2][kRows];       // row's factor; a group's M and log2 of its sum
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   __shared__ int s_cost[kThreads / 32];
+  __shared__ Item s_now;                           // the softmax's item, for its end (in registers it was spilled)
   volatile int* gave_up = &s.gave_up;
 
   if (tid == 64) {
@@ -320,7 +321,8 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
     if (next.units > 0) write_query(next);
     named_sync<kSoftmax>();
     for (int item = 0; next.units >= 0; ++item) {
-      const Item t = next;
+      if (stid == 0) s_now = next;
+      const struct { int tokens, reach, units; } t{next.tokens, next.reach, next.units};
       const int tok = r / kGroup;
       // keys that the row sees; rows of tokens that the tile does not have see what the last one does, for nobody
       const int limit = tok < t.tokens && p.causal ? t.reach - (t.tokens - 1 - tok) : t.reach;
@@ -447,7 +449,8 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
       if (next.units > 0) write_query(next);
 
       // ---- the item's results: each group has half of the features
-      const int n1 = n0 + t.units;
+      const Item of = s_now;
+      const int n1 = n0 + of.units;
       for (int n = max(n1 - 2, n0); n < n1; ++n) bounded_wait_warp(&bar_pv[n & 1][1], (n >> 1) & 1, gave_up);
       tc_fence_after();
       const float lse0 = s_lse[0][r], lse1 = s_lse[1][r];
@@ -455,21 +458,21 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
       const bool none = most == -INFINITY;
       const float lse2 = none ? -INFINITY + nan : most + lg2(ex2(lse0 - most) + ex2(lse1 - most)) + nan;
       const bool lost = *gave_up;
-      if (group == 0 && tok < t.tokens) {
-        if (t.piece >= 0) p.part_lse[(int64_t)t.piece * kRows + r] = lse2;
-        else if (p.lse) p.lse[(int64_t)(t.row + tok) * heads + t.head * kGroup + r % kGroup] = none && nan == 0.f ? INFINITY : lse2 * kLn2;
+      if (group == 0 && tok < of.tokens) {
+        if (of.piece >= 0) p.part_lse[(int64_t)of.piece * kRows + r] = lse2;
+        else if (p.lse) p.lse[(int64_t)(of.row + tok) * heads + of.head * kGroup + r % kGroup] = none && nan == 0.f ? INFINITY : lse2 * kLn2;
       }
       // 2^(M - lse) in two steps, so that neither leaves fp32's range
       float f[2];
       bool with[2];
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
-        with[g] = t.units > (g ^ (n0 & 1));        // this group had a unit
+        with[g] = of.units > (g ^ (n0 & 1));        // this group had a unit
         f[g] = none ? nan : ex2(0.5f * (s_top[g][r] - lse2));
         if (s_lse[g][r] == -INFINITY) f[g] = nan;
       }
-      __nv_bfloat16* out = p.out + ((int64_t)(t.row + tok) * heads + t.head * kGroup + r % kGroup) * kHeadDim + 64 * group;
-      float* part = p.part_o + ((int64_t)max(t.piece, 0) * kRows + r) * kHeadDim + 64 * group;
+      __nv_bfloat16* out = p.out + ((int64_t)(of.row + tok) * heads + of.head * kGroup + r % kGroup) * kHeadDim + 64 * group;
+      float* part = p.part_o + ((int64_t)max(of.piece, 0) * kRows + r) * kHeadDim + 64 * group;
 #pragma unroll 1
       for (int c0 = 0; c0 < 64; c0 += 16) {
         float y[16];
@@ -488,13 +491,13 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
           }
         }
         if (lost) y[0] = y[4] = y[8] = y[12] = NAN;
-        if (tok < t.tokens && t.piece < 0) {
+        if (tok < of.tokens && of.piece < 0) {
           uint4 a, b;
           a.x = pack_bf16(y[0], y[1]), a.y = pack_bf16(y[2], y[3]), a.z = pack_bf16(y[4], y[5]), a.w = pack_bf16(y[6], y[7]);
           b.x = pack_bf16(y[8], y[9]), b.y = pack_bf16(y[10], y[11]), b.z = pack_bf16(y[12], y[13]), b.w = pack_bf16(y[14], y[15]);
           reinterpret_cast<uint4*>(out + c0)[0] = a;
           reinterpret_cast<uint4*>(out + c0)[1] = b;
-        } else if (tok < t.tokens) {
+        } else if (tok < of.tokens) {
 #pragma unroll
           for (int j = 0; j < 16; j += 4) *reinterpret_cast<float4*>(part + c0 + j) = make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]);
         }

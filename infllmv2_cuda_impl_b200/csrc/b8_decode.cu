@@ -9,12 +9,13 @@
 // over all lanes.  Warps: 0 looks blocks up and issues TMA, 1 issues MMAs, 2..5 are the softmax (thread = key =
 // feature).  Two CTAs per SM.
 //
-// What bounds it is memory, and at both ends latency.  64 sequences of 16000 tokens, 2 KV heads: 94 us with the join, 5.6 TB/s,
-// 86 % of the copy bandwidth.  A CTA makes a unit of 32 KB in 1.1 us, so that the SMs could take 8.6 TB/s; what 135 MB (21
-// us) cost above that is 5 us until the first unit is there (lengths, list, page, tile: each a trip to memory of 0.7 us), CTAs that
-// end 5 us apart, and the join, 4 us with its release.  Tried and slower or equal: four sequences per lane in the deal
-// (one sequence 11.0 -> 11.7 us, 256 sequences 62.9 -> 61.5), joins that work the cuts out instead of reading them (+1 to
-// +4 us), going through the join's code once over zeros while it waits (+0.3 us).
+// What bounds it is memory, and at both ends latency.  64 sequences of 16000 tokens, 2 KV heads: 87 us with the join, 6.1 TB/s,
+// 93 % of the copy bandwidth.  64 selected blocks of 64 sequences, 135 MB: 34-36 us where the bytes take 21: 5 us until the first
+// unit is there (lengths, list, page, tile: each a trip to memory of 0.7 us), CTAs that end some us apart, and the join.  Short
+// sequences pay for the start and end of tiles: 4096 of 200 tokens 164 us where the bytes take 65.
+// Registers decide: with the columns' factors and references in them 30 words were spilled, and every call took 5 us more.
+// Tried and slower or equal: four sequences per lane in the deal (one sequence +0.6 us, 256 sequences -1.2), joins that
+// work the cuts out instead of reading them (+1 to +4 us), going through the join's code once over zeros while it waits (+0.3).
 #include "b8_attn.cuh"
 
 namespace ifv2 {
