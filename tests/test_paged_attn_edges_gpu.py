@@ -231,3 +231,32 @@ def test_lists_longer_than_the_blocks_there_are(new):
     lists = (torch.arange(20001, dtype=torch.int32) * 7 % 30000).expand(hk, sum(new), -1).contiguous()
     lists[1] = lists[1] % 5
     check(attend(q, cache, cu_q, max(new), lens, table, topk_idx=lists.to(DEV)), q, k, v, cu_q, lens, table, True, lists)
+
+
+@pytest.mark.parametrize("dtype", [E4M3, E5M2])
+@pytest.mark.parametrize("new", [[1], [2], [10]])
+def test_blocks_of_the_smallest_scale(new, dtype):
+    """Values whose block has the exponent -127, alone and before a block of the usual size.  Results stay above 2^-126 where it is
+    alone: below, 32-bit arithmetic may give 0, so that is what they may be off by."""
+    for lens, v_size in (([3], 2.0 ** -122), ([130], lambda pos: torch.where(pos < 64, 2.0 ** -122, 1.0).double())):
+        cache, table, k, v = make(lens, 1, 64, dtype, 71, v_size=v_size)
+        assert int(cache[3].view(torch.uint8)[int(table[0, 0])]) == 0
+        q, cu_q = queries(new, 1, 72), cu(new)
+        out, lse = (x.cpu() for x in attend(q, cache, cu_q, max(new), lens, table))
+        ref, ref_lse, size, _ = paged.attend(q, k, v, cu_q.tolist(), lens, table, True, None, None)
+        none = ref_lse == math.inf
+        assert torch.equal(none, lse == math.inf)
+        assert bool(((out.double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 2.0 ** -7 * size + 2.0 ** -126).all())
+        assert not bool((out.double()[~none] == 0).all())
+
+
+@pytest.mark.parametrize("most", [1, 2, 5])
+def test_thousands_of_sequences(most):
+    """More sequences than a CTA has threads, over pages that they share."""
+    batch = 2500
+    cache, table, k, v = make([128] * 5, 1, 64, E4M3, 73)
+    lens = [(i * 29) % 129 for i in range(batch)]
+    new = [1 + (i * 7) % most if i % 13 else 0 for i in range(batch)]
+    table = table[torch.arange(batch) % 5].contiguous()
+    q, cu_q = queries(new, 1, 74), cu(new)
+    check(attend(q, cache, cu_q, most, lens, table), q, k, v, cu_q, lens, table)
