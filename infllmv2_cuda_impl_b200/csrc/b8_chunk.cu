@@ -366,6 +366,9 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
               l *= pow2i(min(delta - bump, 127));
               if (m != kUnset) m += (float)bump;
               back = pow2i(-bump);
+            } else if (m != kUnset) {
+              // only NaN blocks so far, whose eV was taken to be 0: it may be anything, E from here on, and then l stays as it is
+              m += (float)e_most;
             }
             e_ref = e_most;
           }

@@ -1,0 +1,56 @@
+"""GPU: blocks that are NaN and pages that are not there, beside blocks that are neither.  Tolerances: tests/test_paged_attn_gpu.py.
+
+Many sequences read the same pages, so that a thread block has whole tiles and its units follow one another in one share."""
+import math
+
+import pytest
+import torch
+
+import infllm_v2
+from oracle import paged
+from helpers import cu
+from test_paged_attn_gpu import E4M3, E5M2, check, make, queries
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def attend(q, cache, cu_q, most, lens, table, **more):
+    return infllm_v2.infllmv2_attn_paged_b8(q.to(DEV), *cache, cu_q.to(DEV), most, torch.tensor(lens, dtype=torch.int32, device=DEV),
+                                            block_table=table.to(DEV), return_softmax_lse=True, **more)
+
+
+def many(length, new, hk, dtype, seed, k_size=1.0, v_size=1.0, sequences=None):
+    """`sequences` sequences of one table's pages: (cache, table, k, v, lens, q, cu_q)."""
+    cache, table, k, v = make([length], hk, 64, dtype, seed, k_size, v_size)
+    n = sequences or (150 if new <= 2 else 80)
+    q = queries([new] * n, hk, seed + 1)
+    return cache, table.expand(n, -1).contiguous(), k, v, [length] * n, q, cu([new] * n)
+
+
+def check_some(got, q, k, v, cu_q, lens, table, causal=True, lists=None):
+    """`check` of the first, a middle and the last sequence."""
+    some = [0, len(lens) // 2, len(lens) - 1]
+    rows = torch.cat([torch.arange(int(cu_q[b]), int(cu_q[b + 1])) for b in some])
+    check([x.cpu()[rows] for x in got], q[rows], k, v, cu([int(cu_q[b + 1] - cu_q[b]) for b in some]), [lens[b] for b in some],
+          table[some], causal, None if lists is None else lists[:, rows])
+
+
+def spoil(cache, numbers, which, table, blocks):
+    """Blocks of sequence 0 become NaN: their scale bytes, and what the formula reads."""
+    for block in blocks:
+        page = int(table[0, block])
+        cache[2 + which].view(torch.uint8)[page] = 255
+        numbers[page] = math.nan
+
+
+@pytest.mark.parametrize("dtype", [E4M3, E5M2])
+@pytest.mark.parametrize("new", [1, 2, 3, 20])
+@pytest.mark.parametrize("size", [1.0, 2.0 ** -60, 2.0 ** 60])
+def test_lse_behind_nan_values(dtype, new, size):
+    """The values of a tile's first two units are NaN, the keys are not: the sums go on as if nothing were wrong with the values."""
+    cache, table, k, v, lens, q, cu_q = many(64 * 11 + 7, new, 1, dtype, 81, v_size=size, sequences=60 if new == 20 else None)
+    spoil(cache, v, 1, table, range(4))
+    got = attend(q, cache, cu_q, new, lens, table)
+    check_some(got, q, k, v, cu_q, lens, table)
+    assert bool(got[0].isnan().all()) and not bool(got[1].isnan().any())
