@@ -217,7 +217,8 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
         const Block* blk = &s.block[stage][r >> 6];
         const float k_scale = blk->k_scale;
         const int e_v = blk->e_v, valid = blk->valid & 0xFF, e_unit = blk->e_unit, e_most = (int16_t)e_unit;
-        const int e_new = e_ref != kNoScale && e_most - e_ref <= kHighest ? e_ref : e_most == kNoScale ? 0 : e_most;
+        // E of this unit: none is chosen before a block has one (NaN values are taken to be at E, whatever it becomes)
+        const int e_new = e_ref != kNoScale && e_most - e_ref <= kHighest ? e_ref : e_most;
         // which columns' tokens see the thread's key: the last token those below `valid`, the ones before it fewer if causal
         const int left = valid - (r & 63);         // > 0: a key
         uint32_t sees = left > 0 ? (1u << kT) - 1 : 0u;

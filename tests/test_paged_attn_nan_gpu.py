@@ -54,3 +54,18 @@ def test_lse_behind_nan_values(dtype, new, size):
     got = attend(q, cache, cu_q, new, lens, table)
     check_some(got, q, k, v, cu_q, lens, table)
     assert bool(got[0].isnan().all()) and not bool(got[1].isnan().any())
+
+
+@pytest.mark.parametrize("dtype", [E4M3, E5M2])
+@pytest.mark.parametrize("new", [2, 5, 12])
+@pytest.mark.parametrize("size", [2.0 ** -100, 2.0 ** 70])
+def test_a_neighbour_of_nan_values_keeps_its_own(dtype, new, size):
+    """The first token of each sequence selects blocks of NaN values in front of the others' blocks of very small or large ones."""
+    cache, table, k, v, lens, q, cu_q = many(64 * 10, new, 1, dtype, 83, v_size=size, sequences=150 if new == 2 else 40)
+    spoil(cache, v, 1, table, range(4))
+    lists = torch.tensor([4, 5, 6, 8], dtype=torch.int32).repeat(1, q.shape[0], 1)
+    lists[0, ::new] = torch.tensor([0, 1, 2, 3], dtype=torch.int32)
+    got = attend(q, cache, cu_q, new, lens, table, topk_idx=lists.to(DEV), causal=False)
+    check_some(got, q, k, v, cu_q, lens, table, False, lists)
+    nan = got[0].isnan().all(-1).all(-1)
+    assert bool(nan[::new].all()) and int(nan.sum()) == len(lens)
