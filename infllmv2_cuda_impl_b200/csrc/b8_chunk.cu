@@ -465,14 +465,15 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
         if (of.piece >= 0) p.part_lse[(int64_t)of.piece * kRows + r] = lse2;
         else if (p.lse) p.lse[(int64_t)(of.row + tok) * heads + of.head * kGroup + r % kGroup] = none && nan == 0.f ? INFINITY : lse2 * kLn2;
       }
-      // 2^(M - lse) in two steps, so that neither leaves fp32's range
+      // 2^(M - lse) in two steps, so that neither leaves fp32's range; below 0: the group has no key of this row's.  (A product
+      // that 2^(M - lse) makes 0 is added all the same: it is NaN where the row sees a NaN block.)
       float f[2];
       bool with[2];
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         with[g] = of.units > (g ^ (n0 & 1));        // this group had a unit
         f[g] = none ? nan : ex2(0.5f * (s_top[g][r] - lse2));
-        if (s_lse[g][r] == -INFINITY) f[g] = nan;
+        if (s_lse[g][r] == -INFINITY) f[g] = -1.f;
       }
       __nv_bfloat16* out = p.out + ((int64_t)(of.row + tok) * heads + of.head * kGroup + r % kGroup) * kHeadDim + 64 * group;
       float* part = p.part_o + ((int64_t)max(of.piece, 0) * kRows + r) * kHeadDim + 64 * group;
@@ -488,7 +489,7 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
           __syncwarp();
           tmem_ld16(tmem + 256 + 128 * g + lanes + 64 * group + c0, o);
           tmem_wait_ld();
-          if (f[g] != 0.f) {
+          if (!(f[g] < 0.f)) {
 #pragma unroll
             for (int j = 0; j < 16; ++j) y[j] += q8::mul_exact(q8::mul_exact(__uint_as_float(o[j]), f[g]), f[g]);
           }

@@ -69,3 +69,16 @@ def test_a_neighbour_of_nan_values_keeps_its_own(dtype, new, size):
     check_some(got, q, k, v, cu_q, lens, table, False, lists)
     nan = got[0].isnan().all(-1).all(-1)
     assert bool(nan[::new].all()) and int(nan.sum()) == len(lens)
+
+
+@pytest.mark.parametrize("new", [1, 2, 3, 20])
+@pytest.mark.parametrize("nan_unit,high_unit", [(0, 1), (1, 0), (0, 2), (2, 1), (1, 4)])
+def test_nan_values_of_the_lowest_weight(new, nan_unit, high_unit):
+    """A NaN block reaches every token that sees it, however far its keys' scores are below those of another unit."""
+    cache, table, k, v, lens, q, cu_q = many(64 * 10, new, 1, E4M3, 85, lambda p: torch.where(p // 128 == high_unit, 300.0, 0.01).double(),
+                                             sequences=60 if new == 20 else None)
+    spoil(cache, v, 1, table, [2 * nan_unit])
+    out, lse = attend(q, cache, cu_q, new, lens, table)
+    assert bool(out.isnan().all()) and not bool(lse.isnan().any())
+    # (far enough apart that even the square root of a weight of the one is nothing beside the other's: 252 log(2))
+    assert float(lse.min()) > 200
