@@ -218,7 +218,10 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
       for (int i = 0; i < units; ++i, ++n) {
         const int stage = n % kStages, g = n & 1;
         bounded_wait_warp(&s.full[stage], (n / kStages) & 1, gave_up);
-        const int valid[2] = {s.block[stage][0].valid & 0xFF, s.block[stage][1].valid & 0xFF};
+        // (of a page that is not there another one is read in its place: its values may be anything, and count as rows that are no keys)
+        int valid[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) valid[h] = s.block[stage][h].e_v == kNanScale ? 0 : s.block[stage][h].valid & 0xFF;
         const uint8_t* tile = smem + kRing + stage * 2 * kTileBytes + kTileBytes;
         uint8_t* place = smem + kV + g * kVBytes;
 #pragma unroll 1

@@ -82,3 +82,27 @@ def test_nan_values_of_the_lowest_weight(new, nan_unit, high_unit):
     assert bool(out.isnan().all()) and not bool(lse.isnan().any())
     # (far enough apart that even the square root of a weight of the one is nothing beside the other's: 252 log(2))
     assert float(lse.min()) > 200
+
+
+@pytest.mark.parametrize("dtype", [E4M3, E5M2])
+@pytest.mark.parametrize("new", [2, 8, 13])
+@pytest.mark.parametrize("missing", [-1, 10 ** 6])
+def test_missing_pages_of_a_neighbour(dtype, new, missing):
+    """Tokens that see nothing of a page which the cache does not have keep their result, whatever lies in page 0."""
+    lens = [64 * 5 + 1, 64 * 7 + 30]
+    cache, table, k, v = make(lens, 2, 64, dtype, 87)
+    cache = [torch.cat([torch.full_like(c.view(torch.uint8)[:1], 0x7F if i < 2 else 130), c.view(torch.uint8)]).view(c.dtype)
+             for i, c in enumerate(cache)]                         # (a page of NaN codes in front)
+    k, v = (torch.cat([torch.zeros_like(x[:1]), x]) for x in (k, v))
+    table = table + 1
+    table[0, 5] = missing                                          # of one key: only the last token sees it
+    q, cu_q = queries([new, new], 2, 88), cu([new, new])
+    out, lse = attend(q, cache, cu_q, new, lens, table)
+    check((out, lse), q, k, v, cu_q, lens, table)
+    assert not bool(out[:new - 1].isnan().any()) and bool(out[new - 1].isnan().all()) and not bool(out[new:].isnan().any())
+    table[1, 3] = missing                                          # a whole block that one token selects
+    lists = torch.tensor([0, 1, 6], dtype=torch.int32).repeat(2, 2 * new, 1)
+    lists[:, new + 1, 1] = 3
+    out, lse = attend(q, cache, cu_q, new, lens, table, topk_idx=lists.to(DEV))
+    check((out, lse), q, k, v, cu_q, lens, table, True, lists)
+    assert bool(out[new + 1].isnan().all()) and int(out.isnan().all(-1).all(-1).sum()) == 1
