@@ -208,7 +208,7 @@ __device__ __forceinline__ float write_query16(const uint4 (&x)[2], uint8_t* at,
   }
   *reinterpret_cast<uint4*>(at) = make_uint4(first[0], first[1], first[2], first[3]);
   *reinterpret_cast<uint4*>(at + second_at) = make_uint4(second[0], second[1], second[2], second[3]);
-  return fabsf(scale_log2) * q8::scale_value(byte);
+  return q8::mul_exact(fabsf(scale_log2), q8::scale_value(byte));      // (may be subnormal, beside a key's 2^120)
 }
 
 // Barriers and records that the roles share.

@@ -359,7 +359,7 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
         if ((blk[0].valid & kPlain) && e_most - e_ref <= kHighest && e_least - e_ref >= kDeepest) {
           deepest = min(deepest, e_least - e_ref);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) d[h] = blk[h].e_v - e_ref, cs[h] = c_row * blk[h].k_scale;
+          for (int h = 0; h < 2; ++h) d[h] = blk[h].e_v - e_ref, cs[h] = q8::mul_exact(c_row, blk[h].k_scale);
         } else {
           // E follows a block far above it; what came before is that much smaller
           if (e_most > kNoScale && (e_ref == kNoScale || e_most - e_ref > kHighest)) {
@@ -383,7 +383,7 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
             const bool has = blk[h].e_v > kNoScale && blk[h].e_v < kNanScale;
             d[h] = has ? max(blk[h].e_v - e_base, kDeepest) : 0;
             deepest = min(deepest, d[h]);
-            cs[h] = fmaxf(c_row * blk[h].k_scale, 1e-37f);     // (-inf of a masked key times 0 would be NaN)
+            cs[h] = fmaxf(q8::mul_exact(c_row, blk[h].k_scale), 1e-37f);     // (-inf of a masked key times 0 would be NaN)
             odd |= !(blk[h].k_scale == blk[h].k_scale) || blk[h].e_v == kNanScale || (has && blk[h].e_v - e_base < kDeepest);
           }
           odd = __any_sync(0xFFFFFFFFu, odd || c_nan);

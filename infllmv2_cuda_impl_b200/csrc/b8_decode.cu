@@ -245,6 +245,7 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
           } else {
             tmem_ld32_wait(tmem_s + (n & 1) * kN + lanes, x);
           }
+          // (the two factors first: one may be 2^120 where the other is 2^-120)
           const uint64_t scale2 = pack_f32x2(k_scale, k_scale);
           if (moves && !settled) {
             // new references: the largest x + eV of each column, and E
@@ -254,7 +255,7 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
             const float up = (float)dv_ref;
 #pragma unroll
             for (int j = 0; j < kN; ++j) {
-              w[j] = fmaf(__uint_as_float(x[j]) * k_scale, s_c[j], up);
+              w[j] = fmaf(__uint_as_float(x[j]), q8::mul_exact(k_scale, s_c[j]), up);
               if (!((sees >> (j / kGroup)) & 1) || !(w[j] == w[j])) w[j] = -INFINITY;
             }
             const int first = reduce_columns<true, kN>(w, lane);
@@ -300,8 +301,8 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
           for (int j = 0; j < kN; j += 4) {
             const float4 c = *reinterpret_cast<const float4*>(s_c + j), mu = *reinterpret_cast<const float4*>(s_mu + j);
             float y[4];
-            unpack_f32x2(fma_f32x2(mul_f32x2(pack_f32x2(x[j], x[j + 1]), scale2), pack_f32x2(c.x, c.y), pack_f32x2(-mu.x, -mu.y)), y[0], y[1]);
-            unpack_f32x2(fma_f32x2(mul_f32x2(pack_f32x2(x[j + 2], x[j + 3]), scale2), pack_f32x2(c.z, c.w), pack_f32x2(-mu.z, -mu.w)), y[2], y[3]);
+            unpack_f32x2(fma_f32x2(pack_f32x2(x[j], x[j + 1]), q8::mul_exact2(pack_f32x2(c.x, c.y), scale2), pack_f32x2(-mu.x, -mu.y)), y[0], y[1]);
+            unpack_f32x2(fma_f32x2(pack_f32x2(x[j + 2], x[j + 3]), q8::mul_exact2(pack_f32x2(c.z, c.w), scale2), pack_f32x2(-mu.z, -mu.w)), y[2], y[3]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) w[j + e] = ex2(y[e]);
           }
