@@ -347,7 +347,7 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
                 make_uint4(out[k][0], out[k][1], out[k][2], out[k][3]);
         }
         // a value row that is no key, or of a page that is not there (another one is read in its place), may hold anything: 0 x NaN
-        if (left <= 0 || !(v_scale == v_scale)) {
+        if (left <= 0 || s.block[stage][r >> 6].e_v == kNanScale) {
           uint4* row = reinterpret_cast<uint4*>(smem + S::kRing + stage * 2 * kTileBytes + kTileBytes + r * kHeadDim);
 #pragma unroll
           for (int j = 0; j < 8; ++j) row[j] = make_uint4(0, 0, 0, 0);
