@@ -556,7 +556,7 @@ int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void* k_scale, v
  * +inf; tokens that see a NaN block or a page that the cache does not have get NaN.  Codes are finite numbers (ifv2_b8_write
  * writes no others); of a sequence with more than max_seqlen_q tokens some rows are not written.  Caches begin at a
  * multiple of 16 bytes.  status: the status block; its word 1 gets site 101 or 102 where a wait was given up (no word 0
- * is kept: the call's other thread blocks go on). */
+ * is kept: the call's other thread blocks go on; rows of the tile are NaN, those of tiles behind it undefined). */
 int ifv2_pages_resize(const int32_t* seqlens, const int32_t* targets, int32_t* block_table, int64_t table_stride,
                       int width, int32_t* free_pages, int num_pages, const int32_t* free_range,
                       int32_t* seqlens_out, int32_t* free_range_out, int32_t* cu_seqlens, int32_t* positions,

@@ -260,7 +260,8 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
     }
   } else {
     // ---------------------------------------------------------------- softmax
-    // A wait that gave up only makes the results NaN: within an item every thread keeps to the same loops and barriers.
+    // A wait that gave up makes the tile's results NaN, the CTA's tiles behind it are not written, and the status block says so.
+    // Within an item every thread keeps to the same loops and barriers.
     const int group = (warp - 2) >> 2, quad = warp & 3, r = quad * 32 + lane;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     const uint32_t my_s = tmem + 128 * group + lanes, my_o = tmem + 256 + 128 * group + lanes;
@@ -460,10 +461,10 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
       for (int n = max(n1 - 2, n0); n < n1; ++n) bounded_wait_warp(&bar_pv[n & 1][1], (n >> 1) & 1, gave_up);
       tc_fence_after();
       const float lse0 = s_lse[0][r], lse1 = s_lse[1][r];
-      const float most = fmaxf(lse0, lse1), nan = lse0 != lse0 ? lse0 : lse1 != lse1 ? lse1 : 0.f;
+      const bool lost = *gave_up;                  // a wait ran out: nothing here can be trusted
+      const float most = fmaxf(lse0, lse1), nan = lost ? NAN : lse0 != lse0 ? lse0 : lse1 != lse1 ? lse1 : 0.f;
       const bool none = most == -INFINITY;
       const float lse2 = none ? -INFINITY + nan : most + lg2(ex2(lse0 - most) + ex2(lse1 - most)) + nan;
-      const bool lost = *gave_up;
       if (group == 0 && tok < of.tokens) {
         if (of.piece >= 0) p.part_lse[(int64_t)of.piece * kRows + r] = lse2;
         else if (p.lse) p.lse[(int64_t)(of.row + tok) * heads + of.head * kGroup + r % kGroup] = none && nan == 0.f ? INFINITY : lse2 * kLn2;
@@ -497,7 +498,6 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
             for (int j = 0; j < 16; ++j) y[j] += q8::mul_exact(q8::mul_exact(__uint_as_float(o[j]), f[g]), f[g]);
           }
         }
-        if (lost) y[0] = y[4] = y[8] = y[12] = NAN;
         if (tok < of.tokens && of.piece < 0) {
           uint4 a, b;
           a.x = pack_bf16(y[0], y[1]), a.y = pack_bf16(y[2], y[3]), a.z = pack_bf16(y[4], y[5]), a.w = pack_bf16(y[6], y[7]);

@@ -163,7 +163,8 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
     __syncwarp();
   } else {
     // ---------------------------------------------------------------- softmax
-    // A wait that gave up only makes the results NaN: within an item every thread keeps to the same loops and barriers.
+    // A wait that gave up makes the tile's results NaN, the CTA's tiles behind it are not written, and the status block says so.
+    // Within an item every thread keeps to the same loops and barriers.
     const int quad = warp & 3, r = quad * 32 + lane;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     const int stid = tid - 64;
@@ -367,12 +368,12 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
       if (stid < kN) {
         const float sum = s_red[0][stid] + s_red[1][stid] + s_red[2][stid] + s_red[3][stid];
         const bool none = sum == 0.f;
-        const float lse2 = none ? -INFINITY : s_mu[stid] + lg2(sum);
+        const float lse2 = *gave_up ? NAN : none ? -INFINITY : s_mu[stid] + lg2(sum);
         s_fl[stid] = none ? 0.f : rcp(sum);
         const int tok = stid / kGroup;
         if (t.piece >= 0) p.part_lse[(int64_t)t.piece * kN + stid] = lse2;
         else if (p.lse && tok < t.tokens)
-          p.lse[(int64_t)(t.row + tok) * heads + t.head * kGroup + stid % kGroup] = none ? INFINITY : lse2 * kLn2;
+          p.lse[(int64_t)(t.row + tok) * heads + t.head * kGroup + stid % kGroup] = lse2 == -INFINITY ? INFINITY : lse2 * kLn2;
       }
       if (t.units > 0) bounded_wait_warp(&bar_pv, (n - 1) & 1, gave_up);
       tc_fence_after();
