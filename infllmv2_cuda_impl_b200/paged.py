@@ -24,7 +24,7 @@ import torch
 from . import _lib
 from .attention import BLOCK_N, GROUP, HEAD_DIM, _status_words
 from .ops import _on, _require_cuda, _stream
-from .quant_cache import _cu, _ints, _no_gradient, _ptr, _table
+from .quant_cache import _cu, _ints, _no_gradient, _no_tangent, _ptr, _table
 from .rotary import _rows
 
 _CODES = {torch.float8_e4m3fn: 0, torch.float8_e5m2: 1}
@@ -205,6 +205,7 @@ def infllmv2_attn_paged_b8(
         raise ValueError(f"{what}: q must be (total_q, {heads}, {HEAD_DIM}) bf16 ({GROUP} heads per KV head) on the cache's device")
     if q.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError(f"{what}: forward only, as infllmv2_attn_with_kvcache")
+    _no_tangent(what, q)
     total = shape[0]
     cu_seqlens_q, batch = _cu(what, cu_seqlens_q, dev)
     cache_seqlens = _ints(what, "cache_seqlens", cache_seqlens, (batch,), dev)

@@ -22,6 +22,7 @@ from .attention import BLOCK_N, GROUP, HEAD_DIM
 from .ops import _on, _require_cuda, _stream
 from .rotary import _no_gradient as _no_table_gradient, _rows, _tables
 
+_forward_ad = torch.autograd.forward_ad
 _LIST = 256      # longest block list that the attention takes without a mask
 _CODES = {torch.float8_e4m3fn: 0, torch.int8: 1}
 
@@ -89,6 +90,13 @@ def _cu(what, cu_seqlens, dev):
 def _no_gradient(what, k, v):
     if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         raise NotImplementedError(f"{what}: nothing flows back from a cache (pass k.detach() and v.detach())")
+    _no_tangent(what, k, v)
+
+
+def _no_tangent(what, *rows):
+    """(A forward-mode tangent is there in every gradient mode, and would be dropped without a word.)"""
+    if _forward_ad._current_level >= 0 and any(_forward_ad.unpack_dual(t).tangent is not None for t in rows):
+        raise NotImplementedError(f"{what}: no forward-mode derivative (pass the primal tensors)")
 
 
 def cache_fill_q8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -208,6 +216,7 @@ def infllmv2_attn_with_kvcache_q8(
                          "cache's device")
     if q.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError(f"{what}: forward only, as infllmv2_attn_with_kvcache")
+    _no_tangent(what, q)
     k_ptr = v_ptr = None
     if k is not None and v is not None:
         new = (batch, 1, hk, HEAD_DIM)
