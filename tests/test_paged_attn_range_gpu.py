@@ -1,13 +1,11 @@
 """GPU: attention over 8-bit blocks at the edges of its arithmetic: queries and keys of the largest and smallest sizes, scores that
 move the references, walks of many selected blocks.  Tolerances: tests/test_paged_attn_gpu.py, and `check_exact`."""
-import math
-
 import pytest
 import torch
 
 import infllm_v2
 from oracle import paged
-from helpers import cu, det_tensor
+from helpers import cu
 from test_paged_attn_gpu import E4M3, E5M2, _floor, check, make, queries
 
 pytestmark = pytest.mark.gpu
@@ -32,3 +30,58 @@ def test_large_keys_and_small_queries(dtype, new, q_log, k_log):
     q = (queries([new, new], 1, 92).double() * 2.0 ** q_log).to(torch.bfloat16)
     cu_q = cu([new, new])
     check(attend(q, cache, cu_q, new, lens, table), q, k, v, cu_q, lens, table)
+
+
+def check_exact(got, q, k, v, cu_q, lens, table, **more):
+    """`check` for queries that two e4m3 terms hold exactly: scores are off by the fp32 rounding of their 128 products alone, 2^-20 of
+    the sum of their magnitudes, and so are results and log-sum-exps."""
+    x = q.double().abs().amax(-1, keepdim=True)
+    step = torch.pow(torch.tensor(2.0, dtype=torch.float64), 8.0 - torch.floor(torch.log2(x)))
+    step = torch.where(x * step > 448, step / 2, step)
+    y = q.double() * step * 4                                      # the second term's least step is 2^-9, a first one's rest of 2^-2 x 8 bits
+    assert bool((y == y.round()).all()) and float((x * step).max()) <= 448
+    out, lse = (t.cpu()[:q.shape[0]] for t in got)
+    ref, ref_lse, size, reach = paged.attend(q, k, v, cu_q.tolist(), lens, table, **more)
+    slack = (reach + 1) * 2.0 ** -20
+    assert float(slack.max()) < 2.0 ** -8
+    err = (lse.double() - ref_lse).abs()
+    assert bool((err <= slack + 2.0 ** -21 * ref_lse.abs()).all()), float((err - slack).max())
+    tol = 2.0 ** -8 * ref.abs() + size * (2.0 ** -9 + 2.0 ** -11) * 1.125 + size * (2 * slack)[..., None] + _floor(v, size) + 2.0 ** -133
+    err = (out.double() - ref).abs()
+    assert bool((err <= tol).all()), (float((err / tol).max()), (err > tol).nonzero()[:4].tolist())
+
+
+@pytest.mark.parametrize("dtype", [E4M3, E5M2])
+@pytest.mark.parametrize("new", [1, 2, 4, 9, 40])
+@pytest.mark.parametrize("up", [True, False])
+def test_references_that_move(dtype, new, up):
+    """Every block's scores above those before it, or below, and values whose blocks differ: what is rescaled on the way is off by no
+    more than what is not."""
+    length = 64 * 13 + 30
+    grow = lambda p: 2.0 * (1.0 + (p if up else length - p) // 64).double()        # noqa: E731
+    cache, table, k, v = make([length], 1, 64, dtype, 95, grow, lambda p: torch.pow(2.0, (p // 64 % 5 - 2).double()))
+    n = 1 if new > 9 else 60
+    q = queries([new] * n, 1, 96, 2.0)
+    table = table.expand(n, -1).contiguous()
+    got = attend(q, cache, cu([new] * n), new, [length] * n, table)
+    few = min(n, 3)
+    check_exact(got, q[:few * new], k, v, cu([new] * few), [length] * few, table)
+
+
+@pytest.mark.parametrize("new", [[1, 1], [2, 1], [3, 2], [9, 4]])
+@pytest.mark.parametrize("causal", [True, False])
+def test_masks_of_many_blocks(new, causal):
+    """Hundreds of selected blocks a token, other ones for every token, as lists and as masks, with an order and without."""
+    lens, hk = [10000, 3000], 2
+    cache, table, k, v = make(lens, hk, 256, E4M3, 97)
+    cap = table.shape[1] * 256
+    g = torch.Generator().manual_seed(98)
+    lists = torch.stack([torch.stack([torch.randperm(cap // 64, generator=g)[:120].sort().values for _ in range(sum(new))]) for _ in range(hk)])
+    lists = lists.to(torch.int32)
+    q, cu_q = queries(new, hk, 99), cu(new)
+    mask, _ = infllm_v2.topk_to_uint64(lists.to(DEV), cap, 64)
+    for more in (dict(topk_idx=lists.to(DEV)), dict(block_mask=mask)):
+        got = attend(q, cache, cu_q, max(new), lens, table, causal=causal, **more)
+        check(got, q, k, v, cu_q, lens, table, causal, lists)
+    everything = torch.full_like(mask, -1)
+    check(attend(q, cache, cu_q, max(new), lens, table, causal=causal, block_mask=everything), q, k, v, cu_q, lens, table, causal)
