@@ -536,7 +536,8 @@ int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void* k_scale, v
  * (num_pages) is a ring of page numbers, free_range = (place of the first free one, their number).  New pages are taken
  * from its front in the order of the requests and written into block_table (batch rows of table_stride, `width` used);
  * pages of shortened requests go behind its end.  Requests that need more than `width` pages, or more than are left
- * for them and those before them, are refused: length kept, slots -1.  Written: seqlens_out (batch), free_range_out
+ * for them and those before them, are refused: length kept, slots -1 (their tokens are counted in
+ * cu_seqlens; what an attention gives for these rows means nothing).  Written: seqlens_out (batch), free_range_out
  * (2), cu_seqlens (batch + 1), positions (total) and slots (total, page * page_size + place, -1 in rows behind the last
  * new token); none overlaps an input.  batch <= 16384, width * page_size and total below 2^31.
  *

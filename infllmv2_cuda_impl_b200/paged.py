@@ -49,7 +49,9 @@ def pages_resize(seqlens: torch.Tensor, targets: torch.Tensor, block_table: torc
     (target 0: all of them); its row keeps what stood there.  Pages given back can be taken by the next call.
     total: the number of new tokens, sum(max(targets - seqlens, 0)); positions and slots get this many rows.
     A request that would need more pages than its row has is refused, and where the ring runs out, that request and all
-    behind it that need a page: they keep their length, and the slots of their tokens are -1.
+    behind it that need a page: they keep their length, and the slots of their tokens are -1.  Their tokens are counted in
+    cu_seqlens all the same, and rows that an attention over this step gives for them mean nothing (their keys are not
+    there, and the edge is set as if they were): drop the rows whose slot is -1.
 
     Returns (seqlens, free_range, cu_seqlens, positions, slots): lengths after the step, the ring's new range, (batch + 1,)
     int32 first rows of the requests' new tokens, and per new token its position (int32) and slot (int64); rows behind
@@ -195,8 +197,10 @@ def infllmv2_attn_paged_b8(
     words) with a word per 64 blocks of a sequence's capacity; None = all.
     Tokens that see no key get 0 (softmax_lse +inf), and so do rows behind the last sequence.  A token that sees a key of a
     NaN block, or of a page that the cache does not have, gets NaN.  Codes are finite (cache_write_b8 writes no others).
-    A sequence with more than max_seqlen_q tokens has rows that are not written.  Blocks are selected among at most
-    524288 keys of capacity.
+    A sequence with more than max_seqlen_q tokens has rows that are not written, and rows of a request that `pages_resize`
+    refused (slots -1) mean nothing.  Blocks are selected among at most 524288 keys of capacity.  Weights are rounded to 9 bits
+    (2^-9 + 2^-11 of each) where max_seqlen_q is 1 or 2, to fp16 (2^-11) elsewhere, queries to 2^-17.8 of the row's largest
+    element; scores must stay in fp32's range.
     Returns out (total_q, nheads, 128) [, softmax_lse (total_q, nheads) fp32].  Forward only."""
     what = "infllmv2_attn_paged_b8"
     pages, hk, length, code, dev = _check_b8(what, k_cache, v_cache, k_scale, v_scale)
