@@ -10,8 +10,9 @@ namespace ifv2 {
 __device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// beside: the kernel may start while the one in front of it still runs.
 template <typename... Params, typename... Args>
-cudaError_t launch_beside(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream, const Args&... args) {
+cudaError_t launch_kernel(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream, bool beside, const Args&... args) {
   cudaLaunchAttribute attribute{};
   attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attribute.val.programmaticStreamSerializationAllowed = 1;
@@ -21,8 +22,12 @@ cudaError_t launch_beside(void (*kernel)(Params...), dim3 grid, int threads, siz
   config.dynamicSmemBytes = smem;
   config.stream = stream;
   config.attrs = &attribute;
-  config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, kernel, args...);
+  config.numAttrs = beside ? 1 : 0;
+  return cudaLaunchKernelEx(&config, kernel, Params(args)...);
+}
+template <typename... Params, typename... Args>
+cudaError_t launch_beside(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream, const Args&... args) {
+  return launch_kernel(kernel, grid, threads, smem, stream, true, args...);
 }
 
 }  // namespace ifv2

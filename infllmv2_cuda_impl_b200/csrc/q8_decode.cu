@@ -11,6 +11,7 @@
 //
 // Launches: [prepare: long block lists, append where sequences may share rows] -> split -> combine.
 #include <type_traits>
+#include "beside.cuh"
 #include "block_list.cuh"
 #include "mma_sync.cuh"
 #include "q8.cuh"
@@ -139,12 +140,8 @@ struct RowPart {
   }
 };
 
-// A kernel that the next one of the call may start beside: that one reads what this one writes only after its wait,
-// which every thread of it makes before it ends, so that whatever comes after the call comes after both.
-__device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
-// One CTA per (sequence, KV head): block lists -> mask row; the new key (rotated) and value -> their row.
+// One CTA per (sequence, KV head): block lists -> mask row; the new key (rotated) and value -> their row.  (The next kernel of the call
+// may start beside this one: what it reads of this one's it reads after its wait, which every thread of it makes before it ends.)
 template <int kCode>
 __global__ void __launch_bounds__(kThreads) q8_prepare_kernel(const Q8PrepareParams a, const Q8DecodeParams p) {
   extern __shared__ unsigned long long row_words[];
@@ -948,23 +945,6 @@ static auto split_kernel(int page, bool copied) {
        : copied     ? q8_split_kernel<kCode, 0, kRotate, true> : q8_split_kernel<kCode, 0, kRotate, false>;
 }
 
-// beside: the kernel may start while the one before it in the stream still runs (see wait_previous).
-template <typename... Params, typename... Args>
-static cudaError_t launch(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream, bool beside,
-                          const Args&... args) {
-  cudaLaunchAttribute attribute{};
-  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t config{};
-  config.gridDim = grid;
-  config.blockDim = dim3(threads);
-  config.dynamicSmemBytes = smem;
-  config.stream = stream;
-  config.attrs = &attribute;
-  config.numAttrs = beside ? 1 : 0;
-  return cudaLaunchKernelEx(&config, kernel, Params(args)...);
-}
-
 extern "C" int64_t ifv2_q8_decode_workspace_bytes(int batch, int heads_q, int head_dim) {
   if (batch < 0 || heads_q < 0 || head_dim != kHeadDim) return 0;
   // masks: every split of every (sequence, KV head), at most kMaxCtas of them or one each; no mask: two per CTA
@@ -1092,13 +1072,13 @@ extern "C" int ifv2_q8_decode(const void* q, void* k_cache, void* v_cache, void*
     grid = pairs * (kStart + (n_blocks < p.most_blocks ? n_blocks : p.most_blocks));
     if (grid > kMaxCtas) grid = kMaxCtas;
   }
-  e = launch(kernel, dim3((unsigned)grid), kThreads, kSmemBytes, st, prepared, map_k, map_v, p);
+  e = launch_kernel(kernel, dim3((unsigned)grid), kThreads, kSmemBytes, st, prepared, map_k, map_v, p);
   if (e != cudaSuccess) return set_error((int)e, "q8_split: launch failed: %s", cudaGetErrorString(e));
   if (p.splits == 1) return IFV2_OK;               // the split kernel wrote the results
   const int64_t per_pair = p.splits ? p.splits : ceil_div64(grid, pairs);
   const int warps = per_pair > 16 ? 8 : per_pair > 6 ? 4 : 1;      // that share a row's partials
   auto join = warps == 8 ? q8_combine_kernel<8> : warps == 4 ? q8_combine_kernel<4> : q8_combine_kernel<1>;
-  e = launch(join, dim3(2 * warps, (unsigned)pairs), 256, 0, st, true, p, (int)grid);
+  e = launch_kernel(join, dim3(2 * warps, (unsigned)pairs), 256, 0, st, true, p, (int)grid);
   if (e != cudaSuccess) return set_error((int)e, "q8_combine: launch failed: %s", cudaGetErrorString(e));
   return IFV2_OK;
 }
