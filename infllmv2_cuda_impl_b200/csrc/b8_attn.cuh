@@ -6,14 +6,14 @@
 // over the keys that token t sees.  The codes go to the tensor cores as they lie in memory (kind::f8f6f4): the
 // other operand of each product is split into 8-bit numbers instead.
 //   * A query row, scaled by a power of two to a largest magnitude of 224..448, is the sum of two e4m3 numbers, to
-//     2^-10, that is 2^-18 of its largest element: for bf16 rows exact down to elements 2^-10 of the largest.
+//     2^-10, that is 2^-17.8 of its largest element or less: for bf16 rows exact down to elements 2^-9.8 of the largest.
 //   * For few tokens a weight is the sum of three e5m2 numbers, to 2^-9 of it (half a bf16 step); for several it is an fp16
 //     number and the values' codes become fp16 too (b8_chunk.cu).  e5m2 is the upper byte of an fp16
 //     number: a term is a byte, what it leaves over one subtraction.  Weights are 2^(x + eV - M) with M about 2^-10 of the
 //     largest so far, at most 2^15, and below 2^-16 they have the type's fixed spacing of 2^-16: 2^-27 of the largest.
 //     The values' exponents take part in M, so that contributions keep their size against one another whatever
-//     the sizes of the blocks' values are.  The sum of the softmax is held in units of 2^(M - E) with E near the blocks' eV:
-//     that of the first unit, until one is more than 2^kHighest above it.
+//     the sizes of the blocks' values are.  The sum of the softmax has a reference of its own for several tokens, and for few is
+//     held in units of 2^(M - E) with E near the blocks' eV: that of the first unit, until one is more than 2^kHighest above it.
 //
 // A tile is up to kT tokens of a sequence x the 16 query heads of a KV head.  A CTA takes an even share of the call's
 // cost, units of 128 keys plus kStart per tile, whatever the lengths are; pieces of a tile that shares cut go to a workspace

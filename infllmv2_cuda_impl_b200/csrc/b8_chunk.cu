@@ -35,8 +35,12 @@ constexpr int kStages = 3;
 constexpr int kQBytes = kRows * kHeadDim;         // one of two terms
 constexpr int kVBytes = kUnit * kHeadDim * 2;     // fp16 values of a unit: two halves of 64 features, a row per key
 constexpr int kV = 2 * kQBytes, kRing = kV + 2 * kVBytes, kSmem = kRing + kStages * 2 * kTileBytes + 1024;
-// a new reference puts the largest weight at 2^kFirst; it moves when a block's weights add up to more than kMost
-constexpr float kFirst = 4.f, kMost = 32768.f;
+// Every row has two references.  M is for what goes to the tensor cores: weights are 2^(x + eV - M).  A new one puts the largest
+// weight at 2^kFirst; it moves when a block's weights add up to more than kMost.  R is for the sum l = sum 2^(x - R), in which the
+// values' sizes have no part: it moves when a score is more than kApart above it.  A block adds 2^(M - R - eV) of its weights' sum;
+// that is at most 2^kDeep: where eV is less, the weights are taken with M - R - kDeep in its place, below 2^(kApart - kDeep)
+// (nothing in fp16) unless they add up to kLeast, which shows that R is too low.
+constexpr float kFirst = 4.f, kMost = 32768.f, kApart = 20.f, kDeep = 86.f, kLeast = 0x1p-30f;
 
 // Instruction descriptor, kind::f16 with fp16 operands, B MN-major.
 constexpr uint32_t kIdescValues = (1u << 4) | (1u << 16) | (128u >> 3 << 17) | (128u >> 4 << 24);
@@ -334,8 +338,7 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
       const bool idle = 2 * quad >= t.tokens;      // nor does the warp have another
       const float c_row = s_c[r];
       const bool c_nan = !(c_row == c_row);
-      float m = kUnset, l = 0.f;                   // M, the sum in units of 2^(M - E)
-      int e_ref = kNoScale, deepest = 0;           // E; least eV - E of the blocks so far
+      float m = kUnset, ref = 0.f, l = 0.f;        // M; R; the sum in units of 2^R
       bool begun = false;                          // O holds something
 #pragma unroll 1
       for (int i = (n0 & 1) ^ group; i < t.units; i += 2) {
@@ -351,58 +354,39 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
           }
           continue;
         }
-        // Of both blocks: keys that the row sees, factor of the scores, eV - E.  Nearly every unit is plain (every row sees all of
-        // it, see Block) and near E: the rest of this is for the others.
-        int seen[2] = {kBlockN, kBlockN}, d[2];
-        float cs[2], back = 1.f;
-        bool all_seen[2] = {true, true}, odd = false;      // odd: a NaN among the row's numbers, or values too small beside the others'
-        const int e_most = (int16_t)blk[0].e_unit, e_least = blk[0].e_unit >> 16;
-        if ((blk[0].valid & kPlain) && e_most - e_ref <= kHighest && e_least - e_ref >= kDeepest) {
-          deepest = min(deepest, e_least - e_ref);
+        // Of both blocks: keys that the row sees, factor of the scores.  Nearly every unit is plain (every row sees all of it, see
+        // Block): the rest of this is for the others.
+        int seen[2] = {kBlockN, kBlockN};
+        float cs[2];
+        bool all_seen[2] = {true, true}, odd = false;      // odd: a NaN among the warp's numbers
+        if (blk[0].valid & kPlain) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) d[h] = blk[h].e_v - e_ref, cs[h] = q8::mul_exact(c_row, blk[h].k_scale);
+          for (int h = 0; h < 2; ++h) cs[h] = q8::mul_exact(c_row, blk[h].k_scale);
         } else {
-          // E follows a block far above it; what came before is that much smaller
-          if (e_most > kNoScale && (e_ref == kNoScale || e_most - e_ref > kHighest)) {
-            if (e_ref != kNoScale) {
-              const int delta = e_most - e_ref, bump = max(kDeepest - (deepest - delta), 0);
-              deepest = max(deepest - delta, kDeepest);
-              l *= pow2i(min(delta - bump, 127));
-              if (m != kUnset) m += (float)bump;
-              back = pow2i(-bump);
-            } else if (m != kUnset) {
-              // only NaN blocks so far, whose eV was taken to be 0: it may be anything, E from here on, and then l stays as it is
-              m += (float)e_most;
-            }
-            e_ref = e_most;
-          }
-          const int e_base = e_ref == kNoScale ? 0 : e_ref;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             seen[h] = blk[h].tokens & bit ? max(min(limit - blk[h].pos, blk[h].valid & 0xFF), 0) : 0;
             all_seen[h] = __all_sync(0xFFFFFFFFu, seen[h] == kBlockN);
-            const bool has = blk[h].e_v > kNoScale && blk[h].e_v < kNanScale;
-            d[h] = has ? max(blk[h].e_v - e_base, kDeepest) : 0;
-            deepest = min(deepest, d[h]);
             cs[h] = fmaxf(q8::mul_exact(c_row, blk[h].k_scale), 1e-37f);     // (-inf of a masked key times 0 would be NaN)
-            odd |= !(blk[h].k_scale == blk[h].k_scale) || blk[h].e_v == kNanScale || (has && blk[h].e_v - e_base < kDeepest);
+            odd |= !(blk[h].k_scale == blk[h].k_scale) || blk[h].e_v == kNanScale;
           }
           odd = __any_sync(0xFFFFFFFFu, odd || c_nan);
         }
-        const int e_now = e_ref == kNoScale ? 0 : e_ref;
 #pragma unroll 1
-        for (int h = 0; h < 2; ++h, back = 1.f) {
-          const int see = h ? seen[1] : seen[0], dv = h ? d[1] : d[0];
+        for (int h = 0; h < 2; ++h) {
+          const int see = h ? seen[1] : seen[0], e_v = h ? blk[1].e_v : blk[0].e_v;
           const bool all = h ? all_seen[1] : all_seen[0];
-          const float c = h ? cs[1] : cs[0], ev = (float)(e_now + dv);
+          // (a block without an exponent has no keys or NaN values: any will do)
+          const float c = h ? cs[1] : cs[0], ev = e_v > kNoScale && e_v < kNanScale ? (float)e_v : 0.f;
           uint32_t w[32];
           bounded_wait_warp(&bar_s[group][h], (n >> 1) & 1, gave_up);
           tc_fence_after();
-          float sum = 0.f;
+          float sum = 0.f, up = 0.f;
 #pragma unroll 1
           for (bool again = false;; again = true) {
             if (again) {
-              // the row's largest score: a new reference where it is above the old one
+              // the row's largest score: new references where it is above the old ones (whole numbers, so that what follows from
+              // them is exact)
               float top = -INFINITY;
 #pragma unroll 1
               for (int j0 = 0; j0 < kBlockN; j0 += 16) {
@@ -414,43 +398,48 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                   if (j0 + j < see) top = fmaxf(top, __uint_as_float(x[j]));
               }
               const float k_scale = h ? blk[1].k_scale : blk[0].k_scale;
-              top = c_nan || !(k_scale == k_scale) ? -INFINITY : fmaf(top, c, ev);
-              float f = back;
-              if (top - m > kFirst) {
-                const float g = m == kUnset ? 0.f : ex2(m - (top - kFirst));
-                f *= g;
-                l = l > 0.f ? l * g : l;
-                m = top - kFirst;
+              top = c_nan || !(k_scale == k_scale) ? -INFINITY : top * c;
+              float f = 1.f;
+              if (top > -INFINITY && (m == kUnset || top - ref > kApart)) {
+                const float now = floorf(top - kFirst);
+                l = l > 0.f ? l * ex2(ref - now) : l;
+                ref = now;
+              }
+              if (top + ev - m > kFirst) {
+                const float now = floorf(top + ev - kFirst);
+                f = m == kUnset ? 0.f : ex2(m - now);
+                m = now;
               }
               __syncwarp();
               if (begun) rescale(f, n, h);
             }
-            sum = weights(my_s + kBlockN * h, w, c, ev - m, all, see);
-            if (again || !(__any_sync(0xFFFFFFFFu, !(sum <= kMost) || back != 1.f) || odd)) break;
+            // 2^-t: the block's sum in units of the row's; past 2^kDeep the block's values are too small to matter, and its
+            // weights are taken to be larger than they are, so that the keys still count in l
+            const float t = m - ref - ev;
+            up = fminf(t, kDeep);
+            sum = weights(my_s + kBlockN * h, w, c, -(ref + up), all, see);
+            if (again || !(__any_sync(0xFFFFFFFFu, !(sum <= (t > kDeep ? kLeast : kMost))) || odd)) break;
           }
           if (odd) {
             const float k_scale = h ? blk[1].k_scale : blk[0].k_scale;
-            const int e_v = h ? blk[1].e_v : blk[0].e_v;
             const bool nan_key = c_nan || !(k_scale == k_scale), nan_value = e_v == kNanScale;
-            const bool none = e_v > kNoScale && !nan_value && e_v - e_now < kDeepest;
             if (nan_key) sum = see > 0 ? NAN : 0.f;
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
               const uint32_t here = (2 * j < see ? 0xFFFFu : 0u) | (2 * j + 1 < see ? 0xFFFF0000u : 0u);
               if (nan_key || nan_value) w[j] = here & 0x7FFF7FFFu;
-              else if (none) w[j] = 0u;
             }
           }
           begun = true;
           tmem_st32(my_s + kBlockN * h, w);
-          l += sum * ex2((float)-dv);
+          l += sum * ex2(up);
           tmem_wait_st();
           tc_fence_before();
           mbar_arrive_warp(&bar_p[group][h]);
         }
       }
       s_top[group][r] = m;
-      s_lse[group][r] = l == 0.f ? -INFINITY : m - (float)(e_ref == kNoScale ? 0 : e_ref) + lg2(l);
+      s_lse[group][r] = l == 0.f ? -INFINITY : ref + lg2(l);
       // the next item's query, while the last products run (every S of this item has been read)
       next_item(item + 1);
       if (next.units > 0) write_query(next);

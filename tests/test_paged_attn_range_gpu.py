@@ -85,3 +85,39 @@ def test_masks_of_many_blocks(new, causal):
         check(got, q, k, v, cu_q, lens, table, causal, lists)
     everything = torch.full_like(mask, -1)
     check(attend(q, cache, cu_q, max(new), lens, table, causal=causal, block_mask=everything), q, k, v, cu_q, lens, table, causal)
+
+
+def check_underflow(got, q, k, v, cu_q, lens, table, causal, lists):
+    """`check`, for results that may be subnormal.  fp32 arithmetic may give 0 for any number below 2^-126: for the result of a
+    piece of a tile, for what it adds to the row's sum, and for the row's result.  A tile of these lengths (units of 128 keys, two
+    for its start, at least three a share) has four pieces at most: nine such numbers, 2^-122.8 at most."""
+    out, lse = (t.cpu() for t in got)
+    ref, ref_lse, size, reach = paged.attend(q, k, v, cu_q.tolist(), lens, table, causal, lists)
+    slack = q.double().abs().amax(-1) * float(k[~k.isnan()].abs().max()) * 128 ** 0.5 * 2.0 ** -18 + (reach + 1) * 2.0 ** -20
+    none = ref_lse == torch.inf
+    assert torch.equal(none, lse == torch.inf) and bool((out[none] == 0).all())
+    assert bool(((lse.double() - ref_lse).abs() <= slack + 2.0 ** -21 * ref_lse.abs())[~none].all())
+    tol = 2.0 ** -8 * ref.abs() + size * (2.0 ** -9 + 2.0 ** -11) * 1.125 + size * (2 * slack)[..., None] + _floor(v, size) + 9 * 2.0 ** -126
+    err = (out.double() - ref).abs()
+    assert bool((err <= tol)[~none].all()), (float((err / tol)[~none].max()), (err > tol).nonzero()[:4].tolist())
+
+
+@pytest.mark.parametrize("dtype", [E4M3, E5M2])
+@pytest.mark.parametrize("new", [3, 9])
+@pytest.mark.parametrize("order", [0, 1, 2, 3])
+def test_values_of_every_size(dtype, new, order):
+    """Values whose blocks are up to 2^227 apart, in blocks that the tokens of a tile select for themselves: a token's sums and its
+    result are those of its own blocks, whatever the others' are."""
+    logs = [[60, -120, 60, 60, -120, 100], [-118, 0, 100, -118, 100, -118], [100, -100, 0, -118, 60, -60], [0, 55, -80, -118, 57, 30]][order]
+    logs = torch.tensor(logs * 2, dtype=torch.float64)
+    length = 64 * len(logs) - 5
+    cache, table, k, v = make([length], 1, 64, dtype, 101, 1.0, lambda p: torch.pow(2.0, logs[p // 64]))
+    n = 150 if new == 1 else 60
+    table, lens, cu_q = table.expand(n, -1).contiguous(), [length] * n, cu([new] * n)
+    q = queries([new] * n, 1, 102)
+    g = torch.Generator().manual_seed(103 + order)
+    lists = torch.stack([torch.randperm(len(logs), generator=g)[:3].sort().values for _ in range(new * n)]).to(torch.int32)[None]
+    few = torch.arange(4 * new)
+    for some in (lists, None):
+        out, lse = attend(q, cache, cu_q, new, lens, table, causal=False, **({} if some is None else dict(topk_idx=some.to(DEV))))
+        check_underflow((out[few], lse[few]), q[few], k, v, cu([new] * 4), lens[:4], table[:4], False, None if some is None else some[:, few])
