@@ -112,7 +112,7 @@ struct __align__(16) Block {
   float k_scale;                                   // 2^eK, or NaN
   int e_v;                                         // eV; kNoScale without keys, kNanScale: NaN block
   int valid;                                       // keys (0: the block only fills a unit), and kPlain
-  int e_unit;                                      // largest (low half) and least (high) eV of the unit's two blocks
+  int e_unit;                                      // largest eV of the unit's two blocks
   int pos;                                         // position of its first key
   uint32_t tokens;                                 // tokens that attend it
   uint32_t pad[2];
@@ -503,9 +503,8 @@ __device__ __forceinline__ void fetch(const AttnParams& p, const CUtensorMap* k_
           r.k_scale = q8::scale_value(kb);
           r.e_v = r.valid == 0 ? kNoScale : vb == kNanByte ? kNanScale : vb - 127;
           const bool has = r.e_v != kNanScale && r.e_v != kNoScale;
-          const int e_most = has ? r.e_v : kNoScale, e_least = has ? r.e_v : -kNoScale;
-          r.e_unit = (max(e_most, __shfl_xor_sync(0xFFFFFFFFu, e_most, 1)) & 0xFFFF) |
-                     min(e_least, __shfl_xor_sync(0xFFFFFFFFu, e_least, 1)) << 16;
+          const int e_most = has ? r.e_v : kNoScale;
+          r.e_unit = max(e_most, __shfl_xor_sync(0xFFFFFFFFu, e_most, 1));
           // (all lanes of a pair have the same)
           const bool plain = r.valid == kBlockN && has && r.k_scale == r.k_scale && r.tokens == (1u << tokens) - 1 &&
                              (!p.causal || r.pos + kBlockN <= reach - (tokens - 1));

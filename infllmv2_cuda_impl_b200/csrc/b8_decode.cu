@@ -24,6 +24,7 @@ namespace {
 using namespace b8;
 
 constexpr int kThreads = 192, kSoftmax = 128;
+constexpr float kMostSum = 100.f;                // log2 of the largest part of a sum after a move
 
 template <int kT>
 struct Shape {
@@ -73,7 +74,7 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   __shared__ Common<kT, kStages> s;
   __shared__ uint64_t bar_s[2], bar_sfree[2], bar_p, bar_pv, bar_q, bar_drain;
-  __shared__ __align__(16) float s_c[kN], s_mu[kN], s_fl[kN], s_fo[kN], s_red[4][kN];
+  __shared__ __align__(16) float s_c[kN], s_mu[kN], s_fl[kN], s_fo[kN], s_red[4][kN], s_most[4][kN];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   __shared__ int s_cost[kThreads / 32];
   volatile int* gave_up = &s.gave_up;
@@ -210,14 +211,14 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
 #pragma unroll
       for (int i = 0; i < kN; ++i) l[i] = 0.f;
       if (stid < kN) s_mu[stid] = kUnset;
-      int e_ref = kNoScale, deepest = 0;           // E; least eV - E of the blocks so far
+      int e_ref = kNoScale;                        // E
 #pragma unroll 1
       for (int i = 0; i < t.units; ++i, ++n) {
         const int stage = n % kStages;
         bounded_wait_warp(&s.full[stage], (n / kStages) & 1, gave_up);
         const Block* blk = &s.block[stage][r >> 6];
         const float k_scale = blk->k_scale;
-        const int e_v = blk->e_v, valid = blk->valid & 0xFF, e_unit = blk->e_unit, e_most = (int16_t)e_unit;
+        const int e_v = blk->e_v, valid = blk->valid & 0xFF, e_most = blk->e_unit;
         // E of this unit: none is chosen before a block has one (NaN values are taken to be at E, whatever it becomes)
         const int e_new = e_ref != kNoScale && e_most - e_ref <= kHighest ? e_ref : e_most;
         // which columns' tokens see the thread's key: the last token those below `valid`, the ones before it fewer if causal
@@ -251,8 +252,6 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
           if (moves && !settled) {
             // new references: the largest x + eV of each column, and E
             const int delta = e_ref == kNoScale ? 0 : e_new - e_ref;
-            const int bump = max(kDeepest - (deepest - delta), 0);
-            deepest = max(deepest - delta, kDeepest);
             const float up = (float)dv_ref;
 #pragma unroll
             for (int j = 0; j < kN; ++j) {
@@ -261,6 +260,14 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
             }
             const int first = reduce_columns<true, kN>(w, lane);
             s_red[quad][first] = w[0];             // (16 columns: two lanes, one value)
+            if (i > 0) {                           // the largest part of each column's sum
+#pragma unroll
+              for (int j = 0; j < kN; ++j) {
+                float most = l[j];
+                asm("redux.sync.max.f32 %0, %0, 0xFFFFFFFF;" : "+f"(most));
+                if (lane == 0) s_most[quad][j] = most;
+              }
+            }
             named_sync<kSoftmax>();
             if (stid < kN) {
               const float top = fmaxf(fmaxf(s_red[0][stid], s_red[1][stid]), fmaxf(s_red[2][stid], s_red[3][stid]));
@@ -269,9 +276,11 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
               if (was == kUnset) {
                 if (top > -INFINITY) now = top - kTop;
               } else {
-                now = was + (float)(bump - delta);
+                now = was - (float)delta;          // (M stays; further up where the sum, of blocks far below E, would leave fp32's range)
                 if (top - now > kRoom) now = top - kTop;
-                fl = ex2(was - now);
+                const float most_l = fmaxf(fmaxf(s_most[0][stid], s_most[1][stid]), fmaxf(s_most[2][stid], s_most[3][stid]));
+                if (most_l > 0.f) now = fmaxf(now, was + lg2(most_l) - kMostSum);
+                fl = ex2(0.5f * (was - now));      // (twice: l may hold 2^100 of blocks far below E, and their part in it counts)
                 fo = ex2(was - now - (float)delta);
               }
               s_mu[stid] = now;
@@ -280,7 +289,7 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
             }
             named_sync<kSoftmax>();
 #pragma unroll
-            for (int j = 0; j < kN; ++j) l[j] = l[j] > 0.f ? l[j] * s_fl[j] : l[j];
+            for (int j = 0; j < kN; ++j) l[j] = l[j] > 0.f ? l[j] * s_fl[j] * s_fl[j] : l[j];
             if (i > 0) {                           // what is in O so far
               bounded_wait_warp(&bar_pv, (n - 1) & 1, gave_up);
               tc_fence_after();
@@ -323,7 +332,6 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
         tc_fence_before();
         mbar_arrive_warp(&bar_sfree[n & 1]);
         e_ref = e_new;
-        deepest = max(min(deepest, (e_unit >> 16) - e_ref), kDeepest);
         // the one buffer of weights is free again when the product before has been made
         if (n > 0) bounded_wait_warp(&bar_pv, (n - 1) & 1, gave_up);
 #pragma unroll
