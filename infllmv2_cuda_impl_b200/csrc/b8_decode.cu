@@ -70,6 +70,8 @@ __global__ void __launch_bounds__(kThreads, 2)
 b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const AttnParams p) {
   using S = Shape<kT>;
   constexpr int kN = S::kN, kStages = S::kStages;
+  // an E for every token where tokens select blocks: one's values may be far from those of a block that another selects
+  constexpr int kE = kSelected ? kT : 1;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   __shared__ Common<kT, kStages> s;
@@ -211,16 +213,31 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
 #pragma unroll
       for (int i = 0; i < kN; ++i) l[i] = 0.f;
       if (stid < kN) s_mu[stid] = kUnset;
-      int e_ref = kNoScale;                        // E
+      int e_ref[kE];                               // E
+#pragma unroll
+      for (int e = 0; e < kE; ++e) e_ref[e] = kNoScale;
 #pragma unroll 1
       for (int i = 0; i < t.units; ++i, ++n) {
         const int stage = n % kStages;
         bounded_wait_warp(&s.full[stage], (n / kStages) & 1, gave_up);
         const Block* blk = &s.block[stage][r >> 6];
         const float k_scale = blk->k_scale;
-        const int e_v = blk->e_v, valid = blk->valid & 0xFF, e_most = blk->e_unit;
+        const int e_v = blk->e_v, valid = blk->valid & 0xFF;
         // E of this unit: none is chosen before a block has one (NaN values are taken to be at E, whatever it becomes)
-        const int e_new = e_ref != kNoScale && e_most - e_ref <= kHighest ? e_ref : e_most;
+        int e_new[kE];
+#pragma unroll
+        for (int e = 0; e < kE; ++e) {
+          int e_most = blk->e_unit;
+          if (kE > 1) {                            // the largest of the blocks that the token selects
+            e_most = kNoScale;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const Block* b = &s.block[stage][i];
+              if (((b->tokens >> e) & 1) && b->e_v != kNanScale) e_most = max(e_most, b->e_v);
+            }
+          }
+          e_new[e] = e_ref[e] != kNoScale && e_most - e_ref[e] <= kHighest ? e_ref[e] : e_most;
+        }
         // which columns' tokens see the thread's key: the last token those below `valid`, the ones before it fewer if causal
         const int left = valid - (r & 63);         // > 0: a key
         uint32_t sees = left > 0 ? (1u << kT) - 1 : 0u;
@@ -233,8 +250,16 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
         }
         const bool all = __all_sync(0xFFFFFFFFu, sees == (1u << kT) - 1);
         // eV - E; a NaN block's weights are NaN, those of a block far below the others' nothing
-        const int dv = e_v == kNanScale ? 0 : e_v - e_new, dv_ref = max(dv, kDeepest);
-        const float v_ref = pow2i(dv_ref), v_scale = e_v == kNanScale ? NAN : dv < kDeepest ? 0.f : v_ref;
+        int dv[kE];
+        float v_ref[kE], v_scale[kE];
+#pragma unroll
+        for (int e = 0; e < kE; ++e) {
+          // (a token that does not select the block has weights of 0, for which its exponent may be any)
+          const bool any = e_v == kNanScale || (kE > 1 && !((blk->tokens >> e) & 1));
+          dv[e] = any ? 0 : e_v - e_new[e];
+          v_ref[e] = pow2i(max(dv[e], kDeepest));
+          v_scale[e] = e_v == kNanScale ? NAN : dv[e] < kDeepest ? 0.f : v_ref[e];
+        }
         bounded_wait_warp(&bar_s[n & 1], (n >> 1) & 1, gave_up);
         tc_fence_after();
         float w[kN];
@@ -251,11 +276,9 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
           const uint64_t scale2 = pack_f32x2(k_scale, k_scale);
           if (moves && !settled) {
             // new references: the largest x + eV of each column, and E
-            const int delta = e_ref == kNoScale ? 0 : e_new - e_ref;
-            const float up = (float)dv_ref;
 #pragma unroll
             for (int j = 0; j < kN; ++j) {
-              w[j] = fmaf(__uint_as_float(x[j]), q8::mul_exact(k_scale, s_c[j]), up);
+              w[j] = fmaf(__uint_as_float(x[j]), q8::mul_exact(k_scale, s_c[j]), (float)max(dv[kE > 1 ? j / kGroup : 0], kDeepest));
               if (!((sees >> (j / kGroup)) & 1) || !(w[j] == w[j])) w[j] = -INFINITY;
             }
             const int first = reduce_columns<true, kN>(w, lane);
@@ -270,6 +293,8 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
             }
             named_sync<kSoftmax>();
             if (stid < kN) {
+              int delta = e_ref[0] == kNoScale ? 0 : e_new[0] - e_ref[0];
+              if (kE > 1 && stid >= kGroup) delta = e_ref[kE - 1] == kNoScale ? 0 : e_new[kE - 1] - e_ref[kE - 1];
               const float top = fmaxf(fmaxf(s_red[0][stid], s_red[1][stid]), fmaxf(s_red[2][stid], s_red[3][stid]));
               const float was = s_mu[stid];
               float now = was, fl = 0.f, fo = 0.f;
@@ -322,27 +347,34 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
               if (!((sees >> (j / kGroup)) & 1)) w[j] = 0.f;
           }
           if (settled) break;
-          float most = w[0];
+          bool far = false;
 #pragma unroll
-          for (int j = 1; j < kN; j += 2) most = fmaxf(fmaxf(most, w[j]), w[j + 1 < kN ? j + 1 : j]);
+          for (int e = 0; e < kE; ++e) {
+            constexpr int kOf = kN / kE;           // columns of an E
+            float most = w[e * kOf];
+#pragma unroll
+            for (int j = 1; j < kOf; j += 2) most = fmaxf(fmaxf(most, w[e * kOf + j]), w[e * kOf + (j + 1 < kOf ? j + 1 : j)]);
+            far |= e_new[e] != e_ref[e] || most * v_ref[e] > 32768.f;
+          }
           // (one vote decides for all warps, whatever each has read: a wait that gave up must not part them)
-          moves = named_any<kSoftmax>(e_new != e_ref || most * v_ref > 32768.f);
+          moves = named_any<kSoftmax>(far);
           if (!moves) break;
         }
         tc_fence_before();
         mbar_arrive_warp(&bar_sfree[n & 1]);
-        e_ref = e_new;
+#pragma unroll
+        for (int e = 0; e < kE; ++e) e_ref[e] = e_new[e];
         // the one buffer of weights is free again when the product before has been made
         if (n > 0) bounded_wait_warp(&bar_pv, (n - 1) & 1, gave_up);
 #pragma unroll
         for (int j = 0; j < kN; ++j) l[j] += w[j];
-        if (!all && !(v_scale == v_scale)) {       // (only the columns that see the key are NaN)
+        if (!all && !(v_scale[0] == v_scale[0])) {       // (only the columns that see the key are NaN)
 #pragma unroll
           for (int j = 0; j < kN; ++j)
             if ((sees >> (j / kGroup)) & 1) w[j] = NAN;
         } else {
 #pragma unroll
-          for (int j = 0; j < kN; ++j) w[j] *= v_scale;
+          for (int j = 0; j < kN; ++j) w[j] *= v_scale[kE > 1 ? j / kGroup : 0];
         }
 #pragma unroll
         for (int tok = 0; tok < kT; ++tok) {
@@ -387,11 +419,12 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
       tc_fence_after();
       named_sync<kSoftmax>();
       const bool lost = *gave_up;
-      // 2^E; a block's smallest exponent is -127
-      const float e_scale = lost ? NAN : e_ref == -127 ? __uint_as_float(1u << 22) : pow2i(e_ref > kNoScale ? e_ref : 0);
 #pragma unroll
       for (int tok = 0; tok < kT; ++tok) {
         if (tok >= t.tokens) continue;
+        // 2^E; a block's smallest exponent is -127
+        const int e = e_ref[kE > 1 ? tok : 0];
+        const float e_scale = lost ? NAN : e == -127 ? __uint_as_float(1u << 22) : pow2i(e > kNoScale ? e : 0);
         uint32_t o[3][16];
         if (t.units > 0) {
 #pragma unroll
