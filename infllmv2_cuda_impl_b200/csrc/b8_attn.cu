@@ -154,9 +154,10 @@ __global__ void __launch_bounds__(kJoinThreads) b8_join_kernel(const AttnParams 
     for (int u = 0; u < kAtOnce; ++u) w[u] = p.part_lse[piece(min(i + u * kStep, pieces - 1))];
 #pragma unroll
     for (int u = 0; u < kAtOnce; ++u) {
-      w[u] = i + u * kStep < pieces ? ex2(w[u] - ref) : 0.f;           // (NaN: the sum is, and all that it divides)
-      sum += w[u];
-      acc.x += w[u] * o[u].x, acc.y += w[u] * o[u].y, acc.z += w[u] * o[u].z, acc.w += w[u] * o[u].w;
+      // its square root, so that a small part of large values is not lost below 2^-126 (NaN: the sum is, and all that it divides)
+      const float f = i + u * kStep < pieces ? ex2(0.5f * (w[u] - ref)) : 0.f;
+      sum += f * f;
+      acc.x += f * (f * o[u].x), acc.y += f * (f * o[u].y), acc.z += f * (f * o[u].z), acc.w += f * (f * o[u].w);
     }
     if (i + kAtOnce * kStep < pieces) load(i + kAtOnce * kStep);
   }

@@ -1,5 +1,7 @@
 """GPU: attention over 8-bit blocks at the edges of its arithmetic: queries and keys of the largest and smallest sizes, scores that
 move the references, walks of many selected blocks.  Tolerances: tests/test_paged_attn_gpu.py, and `check_exact`."""
+import math
+
 import pytest
 import torch
 
@@ -87,17 +89,17 @@ def test_masks_of_many_blocks(new, causal):
     check(attend(q, cache, cu_q, max(new), lens, table, causal=causal, block_mask=everything), q, k, v, cu_q, lens, table, causal)
 
 
-def check_underflow(got, q, k, v, cu_q, lens, table, causal, lists):
+def check_underflow(got, q, k, v, cu_q, lens, table, causal, lists, pieces=4):
     """`check`, for results that may be subnormal.  fp32 arithmetic may give 0 for any number below 2^-126: for the result of a
-    piece of a tile, for what it adds to the row's sum, and for the row's result.  A tile of these lengths (units of 128 keys, two
-    for its start, at least three a share) has four pieces at most: nine such numbers, 2^-122.8 at most."""
+    piece of a tile, for what it adds to the row's sum, and for the row's result.  A share is three units of 128 keys at least, and
+    a tile's start counts as two, so that 1536 keys have four pieces at most."""
     out, lse = (t.cpu() for t in got)
     ref, ref_lse, size, reach = paged.attend(q, k, v, cu_q.tolist(), lens, table, causal, lists)
     slack = q.double().abs().amax(-1) * float(k[~k.isnan()].abs().max()) * 128 ** 0.5 * 2.0 ** -18 + (reach + 1) * 2.0 ** -20
     none = ref_lse == torch.inf
     assert torch.equal(none, lse == torch.inf) and bool((out[none] == 0).all())
     assert bool(((lse.double() - ref_lse).abs() <= slack + 2.0 ** -21 * ref_lse.abs())[~none].all())
-    tol = 2.0 ** -8 * ref.abs() + size * (2.0 ** -9 + 2.0 ** -11) * 1.125 + size * (2 * slack)[..., None] + _floor(v, size) + 9 * 2.0 ** -126
+    tol = 2.0 ** -8 * ref.abs() + size * (2.0 ** -9 + 2.0 ** -11) * 1.125 + size * (2 * slack)[..., None] + _floor(v, size) + (2 * pieces + 1) * 2.0 ** -126
     err = (out.double() - ref).abs()
     assert bool((err <= tol)[~none].all()), (float((err / tol)[~none].max()), (err > tol).nonzero()[:4].tolist())
 
@@ -122,3 +124,31 @@ def test_values_of_every_size(dtype, new, order):
     for some in (lists, None):
         out, lse = attend(q, cache, cu_q, new, lens, table, causal=False, **({} if some is None else dict(topk_idx=some.to(DEV))))
         check_underflow((out[few], lse[few]), q[few], k, v, cu([new] * 4), lens[:4], table[:4], False, None if some is None else some[:, few])
+
+
+@pytest.mark.parametrize("dtype", [E4M3, E5M2])
+@pytest.mark.parametrize("new", [3, 9])
+@pytest.mark.parametrize("high_first", [False, True])
+def test_pieces_far_apart(dtype, new, high_first):
+    """Half of the keys score 2^128 times the others and have values 2^-128 of theirs, so that both halves count alike, in pieces
+    of one tile that are joined."""
+    length, hk = 64 * 60, 1
+    q = torch.full((new, 16, 128), 0.5, dtype=torch.bfloat16)
+    high = (torch.arange(length) < length // 2) == high_first
+    size = 128 * math.log(2.0) / (0.5 * 128 ** 0.5)                # what every feature of a high key is: 128 log(2) = 128 q k 128^-1/2
+    k = torch.where(high, size, 0.0).double()[:, None, None].expand(length, hk, 128).to(torch.bfloat16)
+    g = torch.Generator().manual_seed(105)
+    v = (torch.randn(length, hk, 128, generator=g, dtype=torch.float64) * torch.where(high, 2.0 ** -108, 2.0 ** 20).double()[:, None, None]).to(torch.bfloat16)
+    cache = [c.view(torch.uint8) for c in infllm_v2.b8_cache(60, 64, hk, dtype, "cpu")]
+    codes = []
+    for i, x in ((0, k), (1, v)):
+        y, e = paged.write(x, cache[i].view(dtype), cache[2 + i], torch.arange(length))
+        codes.append(y.float().to(dtype)), cache[2 + i].copy_(e)
+    cache = codes + [c.view(torch.float8_e8m0fnu) for c in cache[2:]]
+    kk, vv = (paged.numbers(cache[i], cache[2 + i].view(torch.uint8)) for i in (0, 1))
+    table, cu_q = torch.arange(60, dtype=torch.int32)[None], cu([new])
+    got = attend(q, [c.to(DEV) for c in cache], cu_q, new, [length], table, causal=False)
+    _, _, size, _ = paged.attend(q, kk, vv, cu_q.tolist(), [length], table, False)
+    _, _, low, _ = paged.attend(q, kk, torch.where(high.view(60, 64)[:, None, :, None], 0.0, vv), cu_q.tolist(), [length], table, False)
+    assert float((low / size).mean()) > 2.0 ** -4                  # (the low half counts)
+    check_underflow(got, q, kk, vv, cu_q, [length], table, False, None, pieces=11)
