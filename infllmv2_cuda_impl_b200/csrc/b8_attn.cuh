@@ -112,10 +112,10 @@ struct __align__(16) Block {
   float k_scale;                                   // 2^eK, or NaN
   int e_v;                                         // eV; kNoScale without keys, kNanScale: NaN block
   int valid;                                       // keys (0: the block only fills a unit), and kPlain
-  int e_unit;                                      // largest eV of the unit's two blocks
+  int e_unit[2];                                   // largest eV of the unit's two blocks; in tiles of two tokens, of each one's
   int pos;                                         // position of its first key
   uint32_t tokens;                                 // tokens that attend it
-  uint32_t pad[2];
+  float ev;                                        // eV, or 0 where it has none (no keys, or NaN values)
 };
 // A CTA's part of a tile.
 struct __align__(16) Item {
@@ -503,8 +503,12 @@ __device__ __forceinline__ void fetch(const AttnParams& p, const CUtensorMap* k_
           r.k_scale = q8::scale_value(kb);
           r.e_v = r.valid == 0 ? kNoScale : vb == kNanByte ? kNanScale : vb - 127;
           const bool has = r.e_v != kNanScale && r.e_v != kNoScale;
-          const int e_most = has ? r.e_v : kNoScale;
-          r.e_unit = max(e_most, __shfl_xor_sync(0xFFFFFFFFu, e_most, 1));
+          r.ev = has ? (float)r.e_v : 0.f;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const int e = has && (kT != 2 || ((r.tokens >> t) & 1)) ? r.e_v : kNoScale;
+            r.e_unit[t] = max(e, __shfl_xor_sync(0xFFFFFFFFu, e, 1));
+          }
           // (all lanes of a pair have the same)
           const bool plain = r.valid == kBlockN && has && r.k_scale == r.k_scale && r.tokens == (1u << tokens) - 1 &&
                              (!p.causal || r.pos + kBlockN <= reach - (tokens - 1));

@@ -76,7 +76,7 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   __shared__ Common<kT, kStages> s;
   __shared__ uint64_t bar_s[2], bar_sfree[2], bar_p, bar_pv, bar_q, bar_drain;
-  __shared__ __align__(16) float s_c[kN], s_mu[kN], s_fl[kN], s_fo[kN], s_red[4][kN], s_most[4][kN];
+  __shared__ __align__(16) float s_c[kN], s_mu[kN], s_fl[kN], s_fo[kN], s_red[4][kN], s_most[4][kE];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   __shared__ int s_cost[kThreads / 32];
   volatile int* gave_up = &s.gave_up;
@@ -227,15 +227,7 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
         int e_new[kE];
 #pragma unroll
         for (int e = 0; e < kE; ++e) {
-          int e_most = blk->e_unit;
-          if (kE > 1) {                            // the largest of the blocks that the token selects
-            e_most = kNoScale;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const Block* b = &s.block[stage][i];
-              if (((b->tokens >> e) & 1) && b->e_v != kNanScale) e_most = max(e_most, b->e_v);
-            }
-          }
+          const int e_most = kE == kT ? blk->e_unit[e] : max(blk->e_unit[0], blk->e_unit[1]);
           e_new[e] = e_ref[e] != kNoScale && e_most - e_ref[e] <= kHighest ? e_ref[e] : e_most;
         }
         // which columns' tokens see the thread's key: the last token those below `valid`, the ones before it fewer if causal
@@ -283,13 +275,14 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
             }
             const int first = reduce_columns<true, kN>(w, lane);
             s_red[quad][first] = w[0];             // (16 columns: two lanes, one value)
-            if (i > 0) {                           // the largest part of each column's sum
+            // the largest part of the sums so far (of one number for all columns of an E: a number for each costs every call 0.7 us)
 #pragma unroll
-              for (int j = 0; j < kN; ++j) {
-                float most = l[j];
-                asm("redux.sync.max.f32 %0, %0, 0xFFFFFFFF;" : "+f"(most));
-                if (lane == 0) s_most[quad][j] = most;
-              }
+            for (int e = 0; e < kE; ++e) {
+              float most = 0.f;
+#pragma unroll
+              for (int j = 0; j < kN / kE; ++j) most = fmaxf(most, l[e * (kN / kE) + j]);
+              asm("redux.sync.max.f32 %0, %0, 0xFFFFFFFF;" : "+f"(most));
+              if (lane == 0) s_most[quad][e] = most;
             }
             named_sync<kSoftmax>();
             if (stid < kN) {
@@ -303,8 +296,9 @@ b8_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
               } else {
                 now = was - (float)delta;          // (M stays; further up where the sum, of blocks far below E, would leave fp32's range)
                 if (top - now > kRoom) now = top - kTop;
-                const float most_l = fmaxf(fmaxf(s_most[0][stid], s_most[1][stid]), fmaxf(s_most[2][stid], s_most[3][stid]));
-                if (most_l > 0.f) now = fmaxf(now, was + lg2(most_l) - kMostSum);
+                const int e = kE > 1 ? stid / kGroup : 0;
+                const float most_l = fmaxf(fmaxf(s_most[0][e], s_most[1][e]), fmaxf(s_most[2][e], s_most[3][e]));
+                if (delta > 0 && most_l > 0.f) now = fmaxf(now, was + lg2(most_l) - kMostSum);
                 fl = ex2(0.5f * (was - now));      // (twice: l may hold 2^100 of blocks far below E, and their part in it counts)
                 fo = ex2(was - now - (float)delta);
               }
