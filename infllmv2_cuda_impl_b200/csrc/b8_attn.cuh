@@ -115,7 +115,7 @@ struct __align__(16) Block {
   int e_unit[2];                                   // largest eV of the unit's two blocks; in tiles of two tokens, of each one's
   int pos;                                         // position of its first key
   uint32_t tokens;                                 // tokens that attend it
-  float ev;                                        // eV, or 0 where it has none (no keys, or NaN values)
+  uint32_t pad;
 };
 // A CTA's part of a tile.
 struct __align__(16) Item {
@@ -503,7 +503,6 @@ __device__ __forceinline__ void fetch(const AttnParams& p, const CUtensorMap* k_
           r.k_scale = q8::scale_value(kb);
           r.e_v = r.valid == 0 ? kNoScale : vb == kNanByte ? kNanScale : vb - 127;
           const bool has = r.e_v != kNanScale && r.e_v != kNoScale;
-          r.ev = has ? (float)r.e_v : 0.f;
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             const int e = has && (kT != 2 || ((r.tokens >> t) & 1)) ? r.e_v : kNoScale;

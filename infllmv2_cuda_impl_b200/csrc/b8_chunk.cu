@@ -374,17 +374,14 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
         }
 #pragma unroll 1
         for (int h = 0; h < 2; ++h) {
-          const int see = h ? seen[1] : seen[0];
+          const int see = h ? seen[1] : seen[0], e_v = h ? blk[1].e_v : blk[0].e_v;
           const bool all = h ? all_seen[1] : all_seen[0];
-          // (a block without an exponent has no keys or NaN values: 0 will do)
-          const float c = h ? cs[1] : cs[0], ev = h ? blk[1].ev : blk[0].ev;
-          // What the block's sum is multiplied by is 2^up.  Past 2^kDeep its values are too small to matter, and its weights are taken
-          // to be larger than they are, so that the keys still count in l.
-          float t = m - ref - ev, up = fminf(t, kDeep);
+          // (a block without an exponent has no keys or NaN values: any will do)
+          const float c = h ? cs[1] : cs[0], ev = e_v > kNoScale && e_v < kNanScale ? (float)e_v : 0.f;
           uint32_t w[32];
           bounded_wait_warp(&bar_s[group][h], (n >> 1) & 1, gave_up);
           tc_fence_after();
-          float sum = 0.f;
+          float sum = 0.f, up = 0.f;
 #pragma unroll 1
           for (bool again = false;; again = true) {
             if (again) {
@@ -413,16 +410,19 @@ b8_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                 f = m == kUnset ? 0.f : ex2(m - now);
                 m = now;
               }
-              t = m - ref - ev, up = fminf(t, kDeep);
               __syncwarp();
               if (begun) rescale(f, n, h);
             }
+            // 2^-t: the block's sum in units of the row's; past 2^kDeep the block's values are too small to matter, and its
+            // weights are taken to be larger than they are, so that the keys still count in l
+            const float t = m - ref - ev;
+            up = fminf(t, kDeep);
             sum = weights(my_s + kBlockN * h, w, c, -(ref + up), all, see);
             if (again || !(__any_sync(0xFFFFFFFFu, !(sum <= (t > kDeep ? kLeast : kMost))) || odd)) break;
           }
           if (odd) {
             const float k_scale = h ? blk[1].k_scale : blk[0].k_scale;
-            const bool nan_key = c_nan || !(k_scale == k_scale), nan_value = (h ? blk[1].e_v : blk[0].e_v) == kNanScale;
+            const bool nan_key = c_nan || !(k_scale == k_scale), nan_value = e_v == kNanScale;
             if (nan_key) sum = see > 0 ? NAN : 0.f;
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
