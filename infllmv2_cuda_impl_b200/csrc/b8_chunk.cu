@@ -18,8 +18,9 @@
 //
 // What bounds it: a unit takes 2150 clocks.  Its exponentials need 1024 of them in the special-function units, its products 1024
 // in the tensor cores, and shared memory 1660 (scores of 64 keys read the query again; values are read, written as fp16 and
-// read by the product).  A chunk of 4096 tokens over 32768: 1.88 ms, 1.1 PFLOP/s of the attention's own FLOPs (a third of the
-// products serves the query's second term).  Tried and slower: scores of whole units; 16 softmax warps, two to a row's 32 keys
+// read by the product).  A chunk of 4096 tokens over 32768: 1.85 ms (2.0 under the power cap), 1.1 PFLOP/s of the attention's own
+// FLOPs (a third of the products serves the query's second term).  Where tokens select blocks a tile walks the union of theirs, and
+// every warp takes the exponentials of all of it: 2048 tokens over 65536, 64 blocks each, 345 us where the selected pairs' FLOPs take 82.  Tried and slower: scores of whole units; 16 softmax warps, two to a row's 32 keys
 // each (1880 -> 2167 us: the vote that holds them together); scores fetched from TMEM in halves; masked and unmasked
 // forms of the weights' code.
 #include "b8_attn.cuh"

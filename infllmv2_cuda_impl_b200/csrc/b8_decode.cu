@@ -12,8 +12,10 @@
 // What bounds it is memory, and at both ends latency.  64 sequences of 16000 tokens, 2 KV heads: 87 us with the join, 6.1 TB/s,
 // 93 % of the copy bandwidth.  64 selected blocks of 64 sequences, 135 MB: 34-36 us where the bytes take 21: 5 us until the first
 // unit is there (lengths, list, page, tile: each a trip to memory of 0.7 us), CTAs that end some us apart, and the join.  Short
-// sequences pay for the start and end of tiles: 4096 of 200 tokens 164 us where the bytes take 65.
-// Registers decide: with the columns' factors and references in them 30 words were spilled, and every call took 5 us more.
+// sequences pay for the start and end of tiles: 4096 of 200 tokens 169 us where the bytes take 65.  Two tokens, 64 sequences of
+// 16000: 130 us.
+// Registers decide: with the columns' factors and references in them 30 words were spilled, and every call took 5 us more.  (The
+// two-token forms still spill: four words, eight where blocks are selected.)
 // Tried and slower or equal: four sequences per lane in the deal (one sequence +0.6 us, 256 sequences -1.2), joins that
 // work the cuts out instead of reading them (+1 to +4 us), going through the join's code once over zeros while it waits (+0.3).
 #include "b8_attn.cuh"
