@@ -9,7 +9,7 @@ using namespace b8;
 
 constexpr int kPlanThreads = 1024, kJoinThreads = 128;
 // Blocks that a token's mask row is taken to select: how many CTAs get a share follows from it.  A count would be a pass over the
-// masks in front.  Where tokens are many it does not matter (64 sequences of 32768 tokens, 16 / 64 / 256 / 512 blocks each: 21.4 / 36.3 /
+// masks in front.  Where sequences are many it matters little (64 sequences of 32768 tokens, 16 / 64 / 256 / 512 blocks each: 21.4 / 36.3 /
 // 95.0 / 177 us, as lists, whose length is known, 15.7 / 34.3 / 99.0 / 180); one token alone walks masks of more blocks in few CTAs (131072
 // tokens, 64 / 256 / 512 / 2048 blocks: 13.5 / 23.8 / 37.3 / 118 us, as lists 12.0 / 15.8 / 18.1 / 57.6, without a selection 30).
 constexpr int kUsualBlocks = 64;

@@ -201,7 +201,7 @@ def infllmv2_attn_paged_b8(
     refused (slots -1) mean nothing.  Blocks are selected among at most 524288 keys of capacity.  Weights are rounded to 9 bits
     (2^-9 + 2^-11 of each) where max_seqlen_q is 1 or 2, to fp16 (2^-11) elsewhere, queries to 2^-17.8 of the row's largest
     element; scores must stay in fp32's range.  Where max_seqlen_q is 1 or 2, values of a block that are more than 2^90 below
-    the largest block's of those that the token attends count as 0.
+    the largest block's of those that the token attends (without a selection: the sequence's tokens) count as 0.
     Returns out (total_q, nheads, 128) [, softmax_lse (total_q, nheads) fp32].  Forward only."""
     what = "infllmv2_attn_paged_b8"
     pages, hk, length, code, dev = _check_b8(what, k_cache, v_cache, k_scale, v_scale)
